@@ -141,6 +141,91 @@ int sq_argmax(void *stream, const float *logits, size_t n, int64_t *out_index);
 #define SQ_ARGMAX_NOALLOC_MAX_N (1u << 24)
 int sq_argmax_noalloc(void *stream, const float *logits, size_t n, int64_t *out_index);
 
+/* ---- paged 8-bit KV cache (device pointers; async on stream) ----------------- */
+/* No counterpart in the reference, whose cache is one f32 sequence
+ * (models/common/kv_cache.rs:8-78). Batched serving: sequences of different lengths
+ * share one pool of fixed-size pages, held in 8 bits. A step appends the new tokens
+ * of every sequence (any number each, none included), then attends to the cache.
+ *
+ * Page p, kv head g, position offset i, dimension d:
+ *     value = (k[((p * n_kv_heads + g) * page + i) * head_dim + d] - 128) * k_scale[p * n_kv_heads + g]
+ * page: 16, 32, 64, 128 or 256 positions; head_dim: 32, 64, 128 or 256. */
+typedef struct {
+    uint8_t *k, *v;          /* [n_pages][n_kv_heads][page][head_dim], 16-byte aligned */
+    float *k_scale, *v_scale; /* [n_pages][n_kv_heads] */
+    int n_pages, n_kv_heads, page, head_dim;
+} sq_paged_cache;
+
+/* One step of n_seqs sequences, the same for every layer. Row t of a step's q / k / v /
+ * output is new token t; sequence b has the rows q_start[b] .. q_start[b + 1] - 1, which
+ * are its last positions: kv_len[b] counts what it holds WITH them. The page table names
+ * the page of each `page` positions; entries past kv_len are not read. The arrays are
+ * device memory and are read by the kernels (a captured graph replays with new
+ * contents); n_tokens and max_new bound what they may say. */
+typedef struct {
+    const int32_t *q_start;    /* [n_seqs + 1], ascending from 0 to n_tokens */
+    const int32_t *kv_len;     /* [n_seqs] */
+    const int32_t *page_table; /* [n_seqs][pages_per_seq] */
+    int n_seqs, n_tokens;
+    int max_new;               /* most new tokens of one sequence */
+    int pages_per_seq;
+} sq_paged_batch;
+
+/* What the kernels found wrong in a batch's arrays on the current device since the
+ * record was last cleared (a page id outside the cache, lengths beyond the page table,
+ * rows out of order, positions outside the rotation table; such entries are skipped,
+ * never read through): SQ_OK, SQ_ERR_ARG with a message that says what, or
+ * SQ_ERR_TIMEOUT when a bounded wait expired. Call after synchronizing the stream;
+ * `clear` != 0 resets the record. */
+int sq_paged_status(int clear);
+
+/* Rotate and append. k and v rows (n_kv_heads * head_dim elements of dtype SQ_F32 or
+ * SQ_BF16, `stride` elements apart) go to their sequence's pages; k is rotated to its
+ * position on the way (interleaved pairs, rope_cos / rope_sin [rope_rows][head_dim / 2]
+ * f32). A page and head's scale is the largest magnitude it has been given / 127: a new
+ * token that needs more raises it and the page's earlier codes are rounded to the new
+ * scale; the first token of a page starts it anew. NaN is stored as 0, an infinity as
+ * the page's largest value. q, if not NULL, is rotated into q_out (may be q) in the
+ * same launch (rows of n_heads * head_dim). Rows are 16-byte aligned. A page that gets
+ * new tokens must belong to one sequence only. */
+int sq_paged_append(void *stream, const sq_paged_cache *c, const sq_paged_batch *b, int dtype,
+                    const void *k, long long k_stride, const void *v, long long v_stride,
+                    const float *rope_cos, const float *rope_sin, int rope_rows,
+                    const void *q, long long q_stride, int n_heads, void *q_out, long long q_out_stride);
+
+/* Causal grouped attention of the new tokens over the cache (the step appended before):
+ * head h reads kv head h / (n_heads / n_kv_heads); the query at position p sees the
+ * positions <= p, with window > 0 only those > p - window and the first `sinks` ones.
+ * out = softmax(scale * q.k) v; a query that sees nothing gets zeros. q, out: rows of
+ * n_heads * head_dim elements of dtype. ws: sq_paged_attention_workspace() bytes of
+ * device memory, 256-byte aligned, zero-filled once before its first use; calls that
+ * share it must be ordered on the device. */
+int sq_paged_attention(void *stream, const sq_paged_cache *c, const sq_paged_batch *b, int dtype,
+                       const void *q, long long q_stride, int n_heads, float scale, int window, int sinks,
+                       void *out, long long out_stride, void *ws, size_t ws_bytes);
+int sq_paged_attention_workspace(const sq_paged_cache *c, const sq_paged_batch *b, int n_heads, size_t *bytes);
+
+/* Values read back: k_out / v_out [n_seqs][count][n_kv_heads * head_dim] of dtype, row i
+ * of sequence b = position first[b] + i, zeros from kv_len[b] on (and before 0). */
+int sq_paged_read(void *stream, const sq_paged_cache *c, const sq_paged_batch *b, const int32_t *first, int count,
+                  int dtype, void *k_out, void *v_out);
+
+/* Speculative decoding: verification of drafted tokens from given random numbers.
+ * Sequence b has n_draft[b] <= max_draft drafted tokens (n_draft NULL: max_draft each).
+ * target: rows [n_seqs][max_draft + 1] of `vocab` f32 probabilities, target_stride
+ * elements apart; draft: rows [n_seqs][max_draft], or NULL when the draft was certain of
+ * its tokens. Token i is accepted while uniform[b][i] * draft(token) < target(token).
+ * At the first rejection the next token is drawn from max(target - draft, 0), after the
+ * last draft from the target, with uniform[b][max_draft]: the lowest index whose
+ * cumulated weight exceeds the uniform's share of the total, weights being the
+ * probabilities in units of 2^-38 (whole numbers: the result does not depend on the
+ * order of the sum) and the uniform's first 24 bits counting. A remainder without mass
+ * falls back to the target, a target without mass gives -1. out_tokens
+ * [n_seqs][max_draft + 1]: the accepted tokens, the drawn one, then -1. */
+int sq_verify_drafts(void *stream, const float *target, long long target_stride, const float *draft,
+                     long long draft_stride, const int32_t *tokens, const int32_t *n_draft, const float *uniform,
+                     int n_seqs, int max_draft, int vocab, int32_t *n_accepted, int32_t *out_tokens);
+
 /* ---- model level (host pointers) ------------------------------------------------ */
 
 typedef struct sq_model sq_model;

@@ -44,7 +44,17 @@ class LlamaConfig(C.Structure):
         ("rope_orig_ctx", C.c_float)]
 
 
-_vp, _i, _sz, _f = C.c_void_p, C.c_int, C.c_size_t, C.c_float
+class PagedCacheDesc(C.Structure):
+    _fields_ = [(n, C.c_void_p) for n in ("k", "v", "k_scale", "v_scale")] + [
+        (n, C.c_int) for n in ("n_pages", "n_kv_heads", "page", "head_dim")]
+
+
+class PagedBatchDesc(C.Structure):
+    _fields_ = [(n, C.c_void_p) for n in ("q_start", "kv_len", "page_table")] + [
+        (n, C.c_int) for n in ("n_seqs", "n_tokens", "max_new", "pages_per_seq")]
+
+
+_vp, _i, _sz, _f, _ll = C.c_void_p, C.c_int, C.c_size_t, C.c_float, C.c_longlong
 SIGNATURES = {
     "sq_last_error": (C.c_char_p, []),
     "sq_version": (C.c_char_p, []),
@@ -64,6 +74,14 @@ SIGNATURES = {
     "sq_dequantize": (_i, [_vp, _vp, _i, _sz, _vp]),
     "sq_argmax": (_i, [_vp, _vp, _sz, _vp]),
     "sq_argmax_noalloc": (_i, [_vp, _vp, _sz, _vp]),
+    "sq_paged_status": (_i, [_i]),
+    "sq_paged_append": (_i, [_vp, C.POINTER(PagedCacheDesc), C.POINTER(PagedBatchDesc), _i, _vp, _ll, _vp, _ll, _vp,
+                             _vp, _i, _vp, _ll, _i, _vp, _ll]),
+    "sq_paged_attention": (_i, [_vp, C.POINTER(PagedCacheDesc), C.POINTER(PagedBatchDesc), _i, _vp, _ll, _i, _f, _i,
+                                _i, _vp, _ll, _vp, _sz]),
+    "sq_paged_attention_workspace": (_i, [C.POINTER(PagedCacheDesc), C.POINTER(PagedBatchDesc), _i, C.POINTER(_sz)]),
+    "sq_paged_read": (_i, [_vp, C.POINTER(PagedCacheDesc), C.POINTER(PagedBatchDesc), _vp, _i, _i, _vp, _vp]),
+    "sq_verify_drafts": (_i, [_vp, _vp, _ll, _vp, _ll, _vp, _vp, _vp, _i, _i, _i, _vp, _vp]),
     "sq_model_create": (_i, [C.POINTER(LlamaConfig), _i, _i, C.POINTER(_vp)]),
     "sq_model_upload_tensor": (_i, [_vp, C.c_char_p, _i, C.POINTER(C.c_uint64), _i, _vp, _sz]),
     "sq_model_finalize": (_i, [_vp]),

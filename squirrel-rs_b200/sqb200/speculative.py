@@ -1,0 +1,52 @@
+"""Speculative decoding over the C ABI: verification of drafted tokens from given random
+numbers. No counterpart in the reference, whose generation takes one greedy token a step
+(text_generator.rs:38-101)."""
+import torch
+
+from . import lib
+from .lib import KernelError, _check, _stream
+
+_SHAPE, _TYPE, _ARG = 1, 2, 5
+
+
+def _array(t, shape, dtype, what):
+    if t.shape != shape or not t.is_contiguous():
+        raise KernelError(_SHAPE, f"{what}: a contiguous {tuple(shape)} tensor is wanted")
+    if t.dtype != dtype:
+        raise KernelError(_TYPE, f"{what}: {dtype} is wanted")
+    if not t.is_cuda:
+        raise KernelError(_ARG, f"{what}: a CUDA tensor is wanted")
+    return t.data_ptr()
+
+
+def _probs(t, n, rows, vocab, what):
+    """[n, rows, vocab] float32 whose rows lie one stride apart (a slice of wider rows)."""
+    if t.shape != (n, rows, vocab) or t.numel() and ((vocab > 1 and t.stride(2) != 1) or
+                                                    (n > 1 and t.stride(0) != rows * t.stride(1))):
+        raise KernelError(_SHAPE, f"{what}: [{n}, {rows}, {vocab}] with one stride between rows is wanted")
+    if t.dtype != torch.float32:
+        raise KernelError(_TYPE, f"{what}: probabilities are float32")
+    if not t.is_cuda:
+        raise KernelError(_ARG, f"{what}: a CUDA tensor is wanted")
+    return t.data_ptr(), max(t.stride(1), vocab)
+
+
+def verify_drafts(target, draft, tokens, uniform, n_draft=None):
+    """target [n, K + 1, vocab]: the target's probabilities at each drafted token and after
+    the last; draft [n, K, vocab]: the drafting distribution, or None when it was certain of
+    its tokens; tokens [n, K] int32; uniform [n, K + 1] in [0, 1); n_draft [n] int32: tokens
+    drafted for each sequence (None: K). Returns (accepted [n], tokens [n, K + 1]) int32:
+    the accepted drafts, the token drawn after them, then -1."""
+    if tokens.dim() != 2 or target.dim() != 3:
+        raise KernelError(_SHAPE, "tokens are [n, K], target is [n, K + 1, vocab]")
+    n, k = tokens.shape
+    vocab = target.shape[2]
+    tp, ts = _probs(target, n, k + 1, vocab, "target")
+    dp, ds = _probs(draft, n, k, vocab, "draft") if draft is not None else (None, 0)
+    accepted = torch.empty(n, dtype=torch.int32, device=target.device)
+    out = torch.empty((n, k + 1), dtype=torch.int32, device=target.device)
+    _check(lib.load().sq_verify_drafts(
+        _stream(), tp, ts, dp, ds, _array(tokens, (n, k), torch.int32, "tokens"),
+        _array(n_draft, (n,), torch.int32, "n_draft") if n_draft is not None else None,
+        _array(uniform, (n, k + 1), torch.float32, "uniform"), n, k, vocab, accepted.data_ptr(), out.data_ptr()))
+    return accepted, out
