@@ -1,4 +1,30 @@
-// paged_attention.cu — causal grouped attention over the paged 8-bit cache.
+// paged_attention.cu — causal grouped attention over the paged 8-bit cache, for few query
+// rows a kv head (single tokens, drafted tokens): bound by reading the cache.
+//
+// out = softmax(scale * q.k) v over the keys a query sees, in one pass with a running
+// maximum and sum. A row is one query token of one head; the rows of a kv head share its
+// keys, so every code is read and converted once for all of them.
+//
+// The products run on mma.sync m16n8k16 (f16 in, f32 sums) rather than tcgen05: with at
+// most 32 rows the tensor work is small, and the register fragments let a warp convert
+// the codes it needs where it needs them, with no second pass through shared memory.
+//   scores:  S[16 keys][8 columns]   = K[16 keys][dims] Q^T      (keys in the M rows)
+//   output:  O[16 dims][8 columns]  += V^T[16 dims][keys] P      (dimensions in the M rows)
+// Dimensions and keys are numbered inside the products so that a lane's K fragment is 16
+// consecutive bytes of a key and its V fragment consecutive bytes of four keys; P goes
+// from the scores' layout to the operand's by movmatrix.
+//
+// Precision. Codes are whole numbers up to 127: exact in f16. Query rows are scaled by a
+// power of two; an f32 row takes two f16 terms (22 bits) in two columns of the same tile, a bf16
+// row is exact in one. Weights, at most 2^10 (the maximum's), likewise: two terms for f32
+// rows, one (11 bits, under the output's 8) for bf16 rows. The V scale of a page goes
+// into the weights relative to the largest met so far, so f16 never overflows.
+//
+// Work is split evenly over the grid: the (sequence, kv head, row tile, key tile) space is
+// one line, every block takes an equal piece of it, the four warps of a block take its key
+// tiles in turn. A row tile cut by a block's end leaves partial results in the workspace
+// and the last block to arrive joins them, in block order (equal bits every call).
+#include <float.h>
 #include <math.h>
 
 #include <string>
@@ -10,6 +36,15 @@ namespace sq {
 namespace paged {
 namespace {
 
+constexpr int WARPS = 4, THREADS = WARPS * 32, STAGES = 2;
+constexpr int BLOCKS_PER_SM = 3;
+constexpr int MAX_BLOCKS = 160 * BLOCKS_PER_SM;
+constexpr int MIN_TILES = WARPS;  // key tiles a block takes at least
+constexpr int SLOT_FLOATS = 2112;  // partial results of one row tile: rows x (head_dim + 2), 32 x 66 at most
+constexpr size_t PARTIAL_BYTES = (size_t)MAX_BLOCKS * 2 * SLOT_FLOATS * 4;
+constexpr float LOG2E = 1.4426950408889634f;
+constexpr float WEIGHT_EXP = 10.f;  // weights are 2^(s - max + 10)
+
 template <typename T>
 struct AttnArgs {
   Cache c;
@@ -18,63 +53,619 @@ struct AttnArgs {
   T *out;
   long long qs, os;
   int n_heads, group;
-  float scale;
+  float scale;  // of the scores, times log2(e)
   int window, sinks;
+  float *part;
+  int *count;  // blocks that have left their part of a row tile; zero between calls
+  int max_row_tiles;
 };
 
-__device__ __forceinline__ float to_f(float x) { return x; }
-__device__ __forceinline__ float to_f(__nv_bfloat16 x) { return __bfloat162float(x); }
-__device__ __forceinline__ void put(float *p, float x) { *p = x; }
-__device__ __forceinline__ void put(__nv_bfloat16 *p, float x) { *p = __float2bfloat16_rn(x); }
+__device__ __forceinline__ long long warp_sum_ll(long long v) {
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+  return v;
+}
+__device__ __forceinline__ uint32_t smem_addr(const void *p) { return (uint32_t)__cvta_generic_to_shared(p); }
+__device__ __forceinline__ void cp16(uint32_t dst, const void *src) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
+}
+__device__ __forceinline__ void cp_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int N>
+__device__ __forceinline__ void cp_wait() {
+  asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
+}
+__device__ __forceinline__ uint2 lds64(uint32_t a) {
+  uint2 v;
+  asm volatile("ld.shared.v2.u32 {%0, %1}, [%2];" : "=r"(v.x), "=r"(v.y) : "r"(a));
+  return v;
+}
+__device__ __forceinline__ float ex2(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+__device__ __forceinline__ uint32_t sub1152(uint32_t x) {  // two f16: 1024 + code -> code - 128
+  uint32_t y;
+  asm("sub.f16x2 %0, %1, %2;" : "=r"(y) : "r"(x), "r"(0x64806480u));
+  return y;
+}
+// Codes (bytes 0, 1) and (2, 3) of a word as f16 pairs.
+__device__ __forceinline__ uint32_t codes_lo(uint32_t w) { return sub1152(__byte_perm(w, 0x64646464u, 0x4140)); }
+__device__ __forceinline__ uint32_t codes_hi(uint32_t w) { return sub1152(__byte_perm(w, 0x64646464u, 0x4342)); }
+__device__ __forceinline__ uint32_t pack(float lo, float hi) {
+  const __half2 h = __floats2half2_rn(lo, hi);
+  return *reinterpret_cast<const uint32_t *>(&h);
+}
+__device__ __forceinline__ float2 unpack(uint32_t x) { return __half22float2(*reinterpret_cast<const __half2 *>(&x)); }
+__device__ __forceinline__ uint32_t transpose8x8(uint32_t x) {
+  uint32_t y;
+  asm("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(y) : "r"(x));
+  return y;
+}
+__device__ __forceinline__ void mma(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+  asm volatile(
+      "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
+      : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+      : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
 
-// One warp a query row and head; lanes share the dimensions, keys come one at a time.
-template <typename T, int HD>
-__global__ void __launch_bounds__(32) k_paged_attention(const AttnArgs<T> a) {
-  constexpr int DPL = HD / 32;
-  const int t = blockIdx.x, h = blockIdx.y, g = h / a.group, lane = threadIdx.x;
-  const int b = seq_of_token(a.b, t);
-  const Seq s = load_seq(a.b, a.c, b);
-  const int pos = s.len - s.n + (t - s.first);
-  float q[DPL], acc[DPL], m = -INFINITY, l = 0.f;
-  for (int i = 0; i < DPL; i++) {
-    q[i] = to_f(a.q[t * a.qs + h * HD + lane * DPL + i]) * a.scale;
-    acc[i] = 0.f;
+template <typename T, int HD_, int NT_>
+struct Cfg {
+  static constexpr int HD = HD_, NT = NT_;
+  static constexpr bool SPLIT = sizeof(T) == 4;          // two f16 terms a row
+  static constexpr int ROWS_NT = SPLIT ? 4 : 8;          // rows of an 8-column tile (columns 4..7: second terms)
+  static constexpr int ROWS = NT * ROWS_NT;
+  static constexpr int TK = HD <= 64 ? 64 : 4096 / HD;   // keys a tile
+  static constexpr int NG = TK / 16;                     // groups of 16 keys: each within one page
+  static constexpr int TILE = TK * HD;                   // bytes of one operand's tile
+  static constexpr int KS = HD / 16;                     // 16-dimension steps
+  static constexpr int SMEM = WARPS * STAGES * 2 * TILE;
+  static_assert(ROWS * (HD + 2) <= SLOT_FLOATS, "a row tile's partial results fit a slot");
+  static_assert(WARPS * ROWS * (HD + 2) * 4 <= SMEM, "the warps' results fit the ring");
+};
+
+// Byte offset of 16-byte chunk c of key r in a group of 16 keys. Chunks are permuted
+// within 128-byte lines so that both fragment loads (K: 8 lanes on 2 keys, V: lanes on
+// keys 0, 2, 4, 6) touch every bank once.
+template <int HD>
+__device__ __forceinline__ int chunk_at(int r, int c) {
+  if constexpr (HD >= 128) {
+    const int x = (r & 6) ^ ((r & 1) << 2);
+    return r * HD + (c ^ x) * 16;  // x < 8 permutes inside lines of 8 chunks
+  } else if constexpr (HD == 64) {
+    const int line = r >> 1, i = (r & 1) * 4 + c;
+    return line * 128 + (i ^ (2 * (line & 3))) * 16;
+  } else {
+    const int line = r >> 2, i = (r & 3) * 2 + c;
+    return line * 128 + (i ^ (2 * (line & 1))) * 16;
   }
-  for (int j = 0; j <= pos && j < s.len; j++) {
-    if (a.window && j <= pos - a.window && j >= a.sinks) {
-      j = pos - a.window;
-      continue;
+}
+
+// A sequence's key tiles: those of the first `sinks` positions, then from the window's
+// start (all of them without a window). A sequence with new tokens has one at least, seen
+// or not, so that every row is written.
+struct Span {
+  int n;      // key tiles
+  int n_sink;  // the first ones, counted from tile 0
+  int skip;   // tile number minus index after them
+};
+template <int TK>
+__device__ __forceinline__ Span key_span(const Seq &s, int window, int sinks) {
+  Span p = {max((s.len + TK - 1) / TK, 1), 0, 0};
+  if (window) {
+    const int lo = max(s.len - s.n - window + 1, 0) / TK;  // tile of the first position in a window
+    p.n_sink = min((min(sinks, s.len) + TK - 1) / TK, lo);
+    p.skip = lo - p.n_sink;
+    p.n -= p.skip;
+  }
+  return p;
+}
+
+template <class C, typename T>
+__global__ void __launch_bounds__(THREADS, C::NT <= 2 ? BLOCKS_PER_SM : 2) k_paged_few(const AttnArgs<T> a) {
+  constexpr int HD = C::HD, NT = C::NT, TK = C::TK, NG = C::NG, KS = C::KS, ROWS = C::ROWS, RN = C::ROWS_NT;
+  constexpr int MT = HD / 16;  // 16-dimension tiles of the output
+  extern __shared__ __align__(128) uint8_t ring[];
+  __shared__ long long s_scan[WARPS + 1];
+  __shared__ int s_last;
+  const int tid = threadIdx.x, lane = tid & 31, wid = tid >> 5, g = lane >> 2, t = lane & 3;
+  const Cache &c = a.c;
+  const int rows_of_token = a.group;
+
+  auto tiles_of = [&](const Seq &s) -> long long {
+    if (!s.n) return 0;
+    const int rt = (s.n * rows_of_token + ROWS - 1) / ROWS;
+    return (long long)key_span<TK>(s, a.window, a.sinks).n * rt * c.kv_heads;
+  };
+  // This block's piece [at, end) of the line of all tiles, and the sequence it starts in.
+  long long total = 0;
+  for (int b = tid; b < a.b.n_seqs; b += THREADS) total += tiles_of(load_seq(a.b, c, b));
+  total = warp_sum_ll(total);
+  if (lane == 0) s_scan[wid] = total;
+  __syncthreads();
+  total = 0;
+#pragma unroll
+  for (int w = 0; w < WARPS; w++) total += s_scan[w];
+  const long long per = max((total + gridDim.x - 1) / gridDim.x, (long long)MIN_TILES);
+  long long at = per * blockIdx.x;
+  const long long end = min(at + per, total);
+  if (at >= end) return;
+  int b = 0;
+  long long b_start = 0;  // first tile of sequence b
+  for (int b0 = 0; b0 < a.b.n_seqs; b0 += THREADS) {
+    const long long n = b0 + tid < a.b.n_seqs ? tiles_of(load_seq(a.b, c, b0 + tid)) : 0;
+    long long run = n;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const long long y = __shfl_up_sync(0xffffffffu, run, o);
+      if (lane >= o) run += y;
     }
-    const int page = load_page(a.b, a.c, b, j);
-    if (page < 0) continue;
-    const long long slot = (long long)page * a.c.kv_heads + g;
-    const long long at = (slot * a.c.page + (j & (a.c.page - 1))) * HD + lane * DPL;
-    float d = 0.f;
-    for (int i = 0; i < DPL; i++) d = fmaf(q[i], (float)a.c.k[at + i] - 128.f, d);
-    d = warp_sum(d) * a.c.ks[slot];
-    const float mn = fmaxf(m, d), corr = expf(m - mn), p = expf(d - mn);
-    l = l * corr + p;
-    for (int i = 0; i < DPL; i++) acc[i] = acc[i] * corr + p * a.c.vs[slot] * ((float)a.c.v[at + i] - 128.f);
-    m = mn;
+    __syncthreads();
+    if (lane == 31) s_scan[wid] = run;
+    __syncthreads();
+    long long before = b_start;
+    for (int w = 0; w < wid; w++) before += s_scan[w];
+    run += before;
+    if (at >= run - n && at < run) {  // one thread at most
+      s_last = b0 + tid;
+      s_scan[WARPS] = run - n;
+    }
+    long long all = b_start;
+    for (int w = 0; w < WARPS; w++) all += s_scan[w];
+    __syncthreads();
+    if (at < all) {
+      b = s_last;
+      b_start = s_scan[WARPS];
+      break;
+    }
+    b_start = all;
   }
-  for (int i = 0; i < DPL; i++) put(a.out + t * a.os + h * HD + lane * DPL + i, l == 0.f ? 0.f : acc[i] / l);
+
+  const uint32_t my_ring = smem_addr(ring) + wid * (STAGES * 2 * C::TILE);
+  while (at < end) {
+    Seq s = load_seq(a.b, c, b);
+    long long n_b = tiles_of(s);
+    while (at >= b_start + n_b) {  // sequences without new tokens or positions hold no tiles
+      b_start += n_b;
+      s = load_seq(a.b, c, ++b);
+      n_b = tiles_of(s);
+    }
+    const Span span = key_span<TK>(s, a.window, a.sinks);
+    const int row_tiles = (s.n * rows_of_token + ROWS - 1) / ROWS;
+    const int job = (int)((at - b_start) / span.n), head = job / row_tiles, rt = job - head * row_tiles;
+    const long long job_start = b_start + (long long)job * span.n;
+    const int t0 = (int)(at - job_start), t1 = (int)min((long long)span.n, end - job_start);
+    const int pos0 = s.len - s.n;  // position of the first new token
+
+    // ---- query fragments: column g of tile nt = row nt * RN + g % RN, term g / RN
+    uint32_t qf[NT][KS][2];
+    float cf[NT][2];   // factor of the lane's two columns' scores
+    int pos[NT][2];    // and their rows' positions (-1: no such row)
+#pragma unroll
+    for (int nt = 0; nt < NT; nt++) {
+      const int r = rt * ROWS + nt * RN + (g & (RN - 1)), tok = r / rows_of_token, h = r - tok * rows_of_token;
+      const bool ok = tok < s.n;
+      const T *src = a.q + (s.first + (ok ? tok : 0)) * a.qs + (head * rows_of_token + (ok ? h : 0)) * HD;
+      float x[KS * 4];  // the lane's dimensions: 16 consecutive ones of each 64 (8 of 32)
+      float top = 0.f;
+      bool finite = true;
+#pragma unroll
+      for (int i = 0; i < KS; i++) {
+        const int d = HD >= 64 ? (i >> 2) * 64 + t * 16 + (i & 3) * 4 : t * 8 + i * 4;
+        const float4 v = ok ? load4(src + d) : make_float4(0.f, 0.f, 0.f, 0.f);
+        x[4 * i] = v.x, x[4 * i + 1] = v.y, x[4 * i + 2] = v.z, x[4 * i + 3] = v.w;
+#pragma unroll
+        for (int j = 0; j < 4; j++) {
+          top = fmaxf(top, fabsf(x[4 * i + j]));
+          finite &= fabsf(x[4 * i + j]) <= FLT_MAX;
+        }
+      }
+      top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
+      top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
+      finite = (__ballot_sync(0xffffffffu, finite) >> (lane & 28) & 15) == 15;  // of the row's four lanes
+      // the largest element becomes 2^10 .. 2^11; a row with NaN or infinity is NaN as a whole
+      const int e = top > 0.f ? min(10 - ((int)(__float_as_uint(top) >> 23) - 127), 127) : 0;
+      const float up = finite ? __uint_as_float((uint32_t)(e + 127) << 23) : __int_as_float(0x7fffffff);
+      const float down = scalbnf(a.scale, -e);
+#pragma unroll
+      for (int i = 0; i < KS; i++) {
+#pragma unroll
+        for (int j = 0; j < 2; j++) {
+          const float u = x[4 * i + 2 * j] * up, v = x[4 * i + 2 * j + 1] * up;
+          uint32_t f = pack(u, v);
+          if (C::SPLIT && g >= RN) {
+            const float2 hi = unpack(f);
+            f = pack(u - hi.x, v - hi.y);
+          }
+          qf[nt][i][j] = f;
+        }
+      }
+#pragma unroll
+      for (int j = 0; j < 2; j++) {  // column 2t + j is row (2t + j) % RN: held by lanes of that g
+        const int from = ((2 * t + j) & (RN - 1)) * 4;
+        cf[nt][j] = __shfl_sync(0xffffffffu, down, from);
+        const int p = __shfl_sync(0xffffffffu, ok ? pos0 + tok : -1, from);
+        pos[nt][j] = p;
+      }
+    }
+    const int last_row = min((rt + 1) * ROWS, s.n * rows_of_token) - 1;
+    const int min_pos = pos0 + rt * ROWS / rows_of_token, max_pos = pos0 + last_row / rows_of_token;
+
+    float o[MT][NT][4], m[NT][2], l[NT][2], unit = 0.f;
+#pragma unroll
+    for (int nt = 0; nt < NT; nt++) {
+#pragma unroll
+      for (int j = 0; j < 2; j++) m[nt][j] = -INFINITY, l[nt][j] = 0.f;
+#pragma unroll
+      for (int mt = 0; mt < MT; mt++)
+#pragma unroll
+        for (int i = 0; i < 4; i++) o[mt][nt][i] = 0.f;
+    }
+
+    // ---- this warp's key tiles t0 + wid, + WARPS, ...
+    auto tile_key = [&](int i) { return (i < span.n_sink ? i : i + span.skip) * TK; };
+    // Lane j < NG holds group j's page (-1: none) and, once loaded, its scales.
+    auto page_of = [&](int i) {
+      const int key = tile_key(i) + 16 * lane;
+      return i < t1 && lane < NG && key < s.len ? load_page(a.b, c, b, key) : -1;
+    };
+    auto load_tile = [&](int i, int page, int stage, float &ks, float &vs) {
+      ks = vs = 0.f;
+      if (i < t1) {
+        if (page >= 0) {
+          ks = c.ks[(long long)page * c.kv_heads + head];
+          vs = c.vs[(long long)page * c.kv_heads + head];
+        }
+        const int key0 = tile_key(i);
+        const uint32_t dst = my_ring + stage * (2 * C::TILE);
+#pragma unroll
+        for (int j = 0; j < NG; j++) {
+          const int p = __shfl_sync(0xffffffffu, page, j);
+          if (p < 0) continue;
+          const long long src = (((long long)p * c.kv_heads + head) * c.page + ((key0 + 16 * j) & (c.page - 1))) * HD;
+#pragma unroll
+          for (int k = 0; k < HD / 32; k++) {
+            const int q = k * 32 + lane;
+            const uint32_t d = dst + j * 16 * HD + chunk_at<HD>(q / (HD / 16), q % (HD / 16));
+            cp16(d, c.k + src + q * 16);
+            cp16(d + C::TILE, c.v + src + q * 16);
+          }
+        }
+      }
+      cp_commit();
+    };
+    float ks[STAGES], vs[STAGES];
+    int page[STAGES];
+    int i = t0 + wid;
+#pragma unroll
+    for (int st = 0; st < STAGES; st++) {
+      page[st] = page_of(i + st * WARPS);
+      load_tile(i + st * WARPS, page[st], st, ks[st], vs[st]);
+    }
+    int next_page = page_of(i + STAGES * WARPS);
+#pragma unroll 1
+    for (int st = 0; i < t1; i += WARPS, st ^= 1) {
+      cp_wait<STAGES - 1>();
+      __syncwarp();
+      const uint32_t kt = my_ring + st * (2 * C::TILE), vt = kt + C::TILE;
+      const float tks = st ? ks[1] : ks[0], tvs = st ? vs[1] : vs[0];
+      const int tpage = st ? page[1] : page[0];
+      const int key0 = tile_key(i);
+
+      // scores
+      float sc[NG][NT][4];
+#pragma unroll
+      for (int j = 0; j < NG; j++) {
+#pragma unroll
+        for (int nt = 0; nt < NT; nt++)
+#pragma unroll
+          for (int x = 0; x < 4; x++) sc[j][nt][x] = 0.f;
+        const uint32_t base = kt + j * 16 * HD;
+        if constexpr (HD >= 64) {
+#pragma unroll
+          for (int ch = 0; ch < HD / 64; ch++) {
+            const uint4 u = lds128(base + chunk_at<HD>(g, ch * 4 + t)), w = lds128(base + chunk_at<HD>(g + 8, ch * 4 + t));
+            const uint32_t uu[4] = {u.x, u.y, u.z, u.w}, ww[4] = {w.x, w.y, w.z, w.w};
+#pragma unroll
+            for (int k = 0; k < 4; k++) {
+              const uint32_t f[4] = {codes_lo(uu[k]), codes_lo(ww[k]), codes_hi(uu[k]), codes_hi(ww[k])};
+#pragma unroll
+              for (int nt = 0; nt < NT; nt++) mma(sc[j][nt], f, qf[nt][ch * 4 + k][0], qf[nt][ch * 4 + k][1]);
+            }
+          }
+        } else {
+          const uint2 u = lds64(base + chunk_at<HD>(g, t >> 1) + (t & 1) * 8);
+          const uint2 w = lds64(base + chunk_at<HD>(g + 8, t >> 1) + (t & 1) * 8);
+          const uint32_t uu[2] = {u.x, u.y}, ww[2] = {w.x, w.y};
+#pragma unroll
+          for (int k = 0; k < 2; k++) {
+            const uint32_t f[4] = {codes_lo(uu[k]), codes_lo(ww[k]), codes_hi(uu[k]), codes_hi(ww[k])};
+#pragma unroll
+            for (int nt = 0; nt < NT; nt++) mma(sc[j][nt], f, qf[nt][k][0], qf[nt][k][1]);
+          }
+        }
+      }
+      // in log2 units, the second terms' columns added to the first's (both then hold the sum)
+#pragma unroll
+      for (int j = 0; j < NG; j++) {
+        const float gks = __shfl_sync(0xffffffffu, tks, j);
+#pragma unroll
+        for (int nt = 0; nt < NT; nt++) {
+          const float f0 = cf[nt][0] * gks, f1 = cf[nt][1] * gks;
+#pragma unroll
+          for (int x = 0; x < 4; x++) {
+            if (C::SPLIT) sc[j][nt][x] += __shfl_xor_sync(0xffffffffu, sc[j][nt][x], 2);
+            sc[j][nt][x] *= x & 1 ? f1 : f0;
+          }
+        }
+      }
+      const unsigned paged_groups = __ballot_sync(0xffffffffu, tpage >= 0);
+      if (key0 + TK - 1 > min_pos || (a.window && key0 <= max_pos - a.window && key0 + TK > a.sinks) ||
+          (paged_groups & ((1u << NG) - 1)) != (1u << NG) - 1) {
+#pragma unroll
+        for (int j = 0; j < NG; j++)
+#pragma unroll
+          for (int x = 0; x < 4; x++) {
+            const int key = key0 + 16 * j + g + (x >> 1) * 8;
+#pragma unroll
+            for (int nt = 0; nt < NT; nt++) {
+              const int p = pos[nt][x & 1];
+              const bool seen = key <= p && (!a.window || key > p - a.window || key < a.sinks) && (paged_groups >> j & 1);
+              if (!seen) sc[j][nt][x] = -INFINITY;
+            }
+          }
+      }
+      // running maximum; the rows' earlier results move to it and to the largest V scale
+      const float top_vs = lane < NG ? tvs : 0.f;
+      float new_unit = top_vs;
+#pragma unroll
+      for (int x = 1; x < NG; x <<= 1) new_unit = fmaxf(new_unit, __shfl_xor_sync(0xffffffffu, new_unit, x));
+      new_unit = fmaxf(unit, __shfl_sync(0xffffffffu, new_unit, 0));
+      const float per_unit = new_unit > 0.f ? 1.f / new_unit : 0.f;
+      const float unit_corr = unit * per_unit;
+      unit = new_unit;
+      const float share = tvs * per_unit;  // of group `lane`
+      float corr[NT][2], ref[NT][2];
+      bool moved = unit_corr != 1.f;
+#pragma unroll
+      for (int nt = 0; nt < NT; nt++)
+#pragma unroll
+        for (int j = 0; j < 2; j++) {
+          float mx = m[nt][j];
+#pragma unroll
+          for (int k = 0; k < NG; k++) mx = fmaxf(mx, fmaxf(sc[k][nt][j], sc[k][nt][2 + j]));
+#pragma unroll
+          for (int x = 4; x < 32; x <<= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, x));
+          ref[nt][j] = mx == -INFINITY ? 0.f : mx - WEIGHT_EXP;
+          corr[nt][j] = ex2(m[nt][j] - WEIGHT_EXP - ref[nt][j]);  // 0 while nothing was seen
+          if (mx == m[nt][j]) corr[nt][j] = 1.f;
+          moved |= corr[nt][j] != 1.f;
+          l[nt][j] *= corr[nt][j];
+          m[nt][j] = mx;
+        }
+      if (__any_sync(0xffffffffu, moved)) {
+#pragma unroll
+        for (int nt = 0; nt < NT; nt++) {
+          const float f0 = corr[nt][0] * unit_corr, f1 = corr[nt][1] * unit_corr;
+#pragma unroll
+          for (int mt = 0; mt < MT; mt++) {
+            o[mt][nt][0] *= f0, o[mt][nt][1] *= f1, o[mt][nt][2] *= f0, o[mt][nt][3] *= f1;
+          }
+        }
+      }
+      // weights, as the operand of the second product
+      uint32_t pf[NG][NT][2];
+#pragma unroll
+      for (int j = 0; j < NG; j++) {
+        const float gshare = __shfl_sync(0xffffffffu, share, j);
+#pragma unroll
+        for (int nt = 0; nt < NT; nt++)
+#pragma unroll
+          for (int x = 0; x < 2; x++) {
+            float u = ex2(sc[j][nt][2 * x] - ref[nt][0]), v = ex2(sc[j][nt][2 * x + 1] - ref[nt][1]);
+            l[nt][0] += u;
+            l[nt][1] += v;
+            u *= gshare;
+            v *= gshare;
+            uint32_t f = pack(u, v);
+            if (C::SPLIT) {
+              const float2 hi = unpack(f);
+              const uint32_t lo = pack(u - hi.x, v - hi.y);
+              f = t < 2 ? f : lo;
+            }
+            pf[j][nt][x] = transpose8x8(f);
+          }
+      }
+      // output
+#pragma unroll
+      for (int j = 0; j < NG; j++) {
+        const uint32_t base = vt + j * 16 * HD;
+        constexpr int CH = HD >= 128 ? HD / 128 : 1;  // 16-byte pieces of the lane's dimensions
+#pragma unroll
+        for (int ch = 0; ch < CH; ch++) {
+          constexpr int W = HD >= 128 ? 4 : HD / 32;  // words of a piece
+          uint32_t w[4][W];  // keys 2t, 2t + 1, 2t + 8, 2t + 9
+#pragma unroll
+          for (int k = 0; k < 4; k++) {
+            const int r = 2 * t + (k & 1) + (k >> 1) * 8;
+            if constexpr (HD >= 128) {
+              const uint4 u = lds128(base + chunk_at<HD>(r, ch * 8 + g));
+              w[k][0] = u.x, w[k][1] = u.y, w[k][2] = u.z, w[k][3] = u.w;
+            } else if constexpr (HD == 64) {
+              const uint2 u = lds64(base + chunk_at<HD>(r, g >> 1) + (g & 1) * 8);
+              w[k][0] = u.x, w[k][1] = u.y;
+            } else {
+              w[k][0] = lds32(base + chunk_at<HD>(r, g >> 2) + (g & 3) * 4);
+            }
+          }
+#pragma unroll
+          for (int x = 0; x < W; x++)
+#pragma unroll
+            for (int y = 0; y < 2; y++) {  // dimensions 4x + 2y, 4x + 2y + 1 of the piece
+              const uint32_t u = __byte_perm(w[0][x], w[1][x], y ? 0x7362 : 0x5140);
+              const uint32_t v = __byte_perm(w[2][x], w[3][x], y ? 0x7362 : 0x5140);
+              const uint32_t f[4] = {codes_lo(u), codes_hi(u), codes_lo(v), codes_hi(v)};
+#pragma unroll
+              for (int nt = 0; nt < NT; nt++) mma(o[ch * 2 * W + 2 * x + y][nt], f, pf[j][nt][0], pf[j][nt][1]);
+            }
+        }
+      }
+      __syncwarp();  // every lane has read the stage that is loaded next
+      float nks, nvs;
+      const int np = next_page;
+      load_tile(i + STAGES * WARPS, np, st, nks, nvs);
+      next_page = page_of(i + (STAGES + 1) * WARPS);
+      if (st) ks[1] = nks, vs[1] = nvs, page[1] = np;
+      else ks[0] = nks, vs[0] = nvs, page[0] = np;
+    }
+    cp_wait<0>();
+    __syncthreads();
+
+    // ---- the warps' results joined: [warp][row]: maximum, sum, head_dim outputs
+    float *mine = reinterpret_cast<float *>(ring) + wid * ROWS * (HD + 2);
+#pragma unroll
+    for (int nt = 0; nt < NT; nt++)
+#pragma unroll
+      for (int j = 0; j < 2; j++) {
+        float sum = l[nt][j];
+#pragma unroll
+        for (int x = 4; x < 32; x <<= 1) sum += __shfl_xor_sync(0xffffffffu, sum, x);
+        const int col = 2 * t + j, row = nt * RN + (col & (RN - 1));
+        float *dst = mine + row * (HD + 2);
+        if (g == 0 && col < RN) {
+          dst[0] = m[nt][j];
+          dst[1] = sum;
+        }
+#pragma unroll
+        for (int mt = 0; mt < MT; mt++)
+#pragma unroll
+          for (int x = 0; x < 2; x++) {
+            float v = o[mt][nt][2 * x + j];
+            if (C::SPLIT) v += __shfl_xor_sync(0xffffffffu, v, 2);
+            const int d = HD >= 128 ? (mt / 8) * 128 + g * 16 + (mt % 8) * 2 + x : g * (HD / 8) + mt * 2 + x;
+            if (col < RN) dst[2 + d] = v * unit;
+          }
+      }
+    __syncthreads();
+    const bool whole = t0 == 0 && t1 == span.n;
+    const int rows = last_row + 1 - rt * ROWS;
+    auto put = [&](int row, int d, float v) {
+      const int r = rt * ROWS + row, tok = r / rows_of_token, h = r - tok * rows_of_token;
+      T *p = a.out + (s.first + tok) * a.os + (head * rows_of_token + h) * HD + d;
+      if constexpr (C::SPLIT) *p = v;
+      else *p = __float2bfloat16_rn(v);
+    };
+    float *slot = a.part + (size_t)(2 * blockIdx.x + (job_start > per * blockIdx.x ? 1 : 0)) * SLOT_FLOATS;
+    for (int e = tid; e < rows * HD; e += THREADS) {
+      const int row = e / HD, d = e % HD;
+      const float *src = reinterpret_cast<const float *>(ring) + row * (HD + 2);
+      float top = -INFINITY, sum = 0.f, v = 0.f;
+#pragma unroll
+      for (int w = 0; w < WARPS; w++) top = fmaxf(top, src[w * ROWS * (HD + 2)]);
+      const float at0 = top == -INFINITY ? 0.f : top;
+#pragma unroll
+      for (int w = 0; w < WARPS; w++) {
+        const float *x = src + w * ROWS * (HD + 2);
+        const float f = ex2(x[0] - at0);
+        sum = fmaf(x[1], f, sum);
+        v = fmaf(x[2 + d], f, v);
+      }
+      if (whole) {
+        put(row, d, sum == 0.f ? 0.f : v / sum);
+      } else {
+        slot[row * (HD + 2) + 2 + d] = v;
+        if (d == 0) {
+          slot[row * (HD + 2)] = top;
+          slot[row * (HD + 2) + 1] = sum;
+        }
+      }
+    }
+    if (!whole) {  // the last block to arrive joins all parts, in block order
+      const long long first = job_start / per, parts = (job_start + span.n - 1) / per - first + 1;
+      int *count = a.count + ((long long)b * c.kv_heads + head) * a.max_row_tiles + rt;
+      __threadfence();
+      __syncthreads();
+      if (tid == 0) s_last = atomicAdd(count, 1) == (int)parts - 1;
+      __syncthreads();
+      if (s_last) {
+        __threadfence();
+        auto part = [&](long long i) {  // the first part may be its block's second row tile
+          return a.part + (size_t)(2 * (first + i) + (i == 0 && job_start > per * first ? 1 : 0)) * SLOT_FLOATS;
+        };
+        for (int e = tid; e < rows * HD; e += THREADS) {
+          const int row = e / HD, d = e % HD;
+          float top = -INFINITY, sum = 0.f, v = 0.f;
+#pragma unroll 8
+          for (int i = 0; i < (int)parts; i++) top = fmaxf(top, __ldcg(part(i) + row * (HD + 2)));
+          const float at0 = top == -INFINITY ? 0.f : top;
+#pragma unroll 8
+          for (int i = 0; i < (int)parts; i++) {
+            const float *x = part(i) + row * (HD + 2);
+            const float f = ex2(__ldcg(x) - at0);
+            sum = fmaf(__ldcg(x + 1), f, sum);
+            v = fmaf(__ldcg(x + 2 + d), f, v);
+          }
+          put(row, d, sum == 0.f ? 0.f : v / sum);
+        }
+        if (tid == 0) *count = 0;
+      }
+    }
+    at = job_start + t1;
+    __syncthreads();  // the ring is free again
+  }
+}
+
+template <class C, typename T>
+cudaError_t launch(cudaStream_t s, AttnArgs<T> &a) {
+  static int blocks[64] = {};
+  int dev = 0;
+  cudaError_t e = cudaGetDevice(&dev);
+  if (e != cudaSuccess) return e;
+  if (dev >= 64) return cudaErrorInvalidDevice;
+  if (!blocks[dev]) {
+    int sms = 0, per_sm = 0;
+    if ((e = cudaFuncSetAttribute(k_paged_few<C, T>, cudaFuncAttributeMaxDynamicSharedMemorySize, C::SMEM)) !=
+            cudaSuccess ||
+        (e = cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev)) != cudaSuccess ||
+        (e = cudaOccupancyMaxActiveBlocksPerMultiprocessor(&per_sm, k_paged_few<C, T>, THREADS, C::SMEM)) !=
+            cudaSuccess)
+      return e;
+    blocks[dev] = min(sms * max(per_sm, 1), MAX_BLOCKS);
+  }
+  a.max_row_tiles = (a.b.max_new * a.group + C::ROWS - 1) / C::ROWS;
+  k_paged_few<C, T><<<blocks[dev], THREADS, C::SMEM, s>>>(a);
+  return cudaGetLastError();
+}
+
+// The narrowest tile that takes all rows of a kv head, up to what the registers hold.
+template <typename T, int HD>
+cudaError_t launch_few(cudaStream_t s, AttnArgs<T> &a) {
+  const int rows = a.b.max_new * a.group;
+  if (rows <= Cfg<T, HD, 1>::ROWS || HD == 256) return launch<Cfg<T, HD, 1>>(s, a);
+  if constexpr (HD <= 128) {
+    if (rows <= Cfg<T, HD, 2>::ROWS || HD == 128) return launch<Cfg<T, HD, 2>>(s, a);
+  }
+  if constexpr (HD <= 64) return launch<Cfg<T, HD, 4>>(s, a);
+  return cudaErrorInvalidValue;
+}
+
+size_t workspace_bytes(const Batch &b, const Cache &c, int n_heads) {
+  const long long tiles = ((long long)b.max_new * (n_heads / c.kv_heads) + 3) / 4;  // narrowest row tile: 4 rows
+  return PARTIAL_BYTES + (size_t)b.n_seqs * c.kv_heads * tiles * sizeof(int);
 }
 
 template <typename T>
 cudaError_t attention(cudaStream_t s, const Cache &c, const Batch &b, const void *q, long long qs, int n_heads,
-                      float scale, int window, int sinks, void *out, long long os) {
-  const AttnArgs<T> a = {c, b, (const T *)q, (T *)out, qs, os, n_heads, n_heads / c.kv_heads, scale, window, sinks};
-  const dim3 grid(b.n_tokens, n_heads);
+                      float scale, int window, int sinks, void *out, long long os, void *ws) {
+  AttnArgs<T> a = {c,  b,      (const T *)q, (T *)out,     qs, os, n_heads, n_heads / c.kv_heads, scale * LOG2E,
+                   window, sinks, (float *)ws, (int *)((uint8_t *)ws + PARTIAL_BYTES), 0};
   switch (c.hd) {
-    case 32: k_paged_attention<T, 32><<<grid, 32, 0, s>>>(a); break;
-    case 64: k_paged_attention<T, 64><<<grid, 32, 0, s>>>(a); break;
-    case 128: k_paged_attention<T, 128><<<grid, 32, 0, s>>>(a); break;
-    default: k_paged_attention<T, 256><<<grid, 32, 0, s>>>(a); break;
+    case 32: return launch_few<T, 32>(s, a);
+    case 64: return launch_few<T, 64>(s, a);
+    case 128: return launch_few<T, 128>(s, a);
+    default: return launch_few<T, 256>(s, a);
   }
-  return cudaGetLastError();
 }
-
-size_t workspace_bytes(const Batch &, const Cache &, int) { return 256; }
 
 int check_heads(const Cache &c, int n_heads, const char *what) {
   if (n_heads <= 0 || n_heads % c.kv_heads)
@@ -113,6 +704,7 @@ extern "C" int sq_paged_attention(void *stream, const sq_paged_cache *cache, con
   if (dtype != SQ_F32 && dtype != SQ_BF16)
     return fail(SQ_ERR_INVALID_TYPE, "paged_attention: rows must be F32 or BF16");
   if (window < 0 || sinks < 0) return fail(SQ_ERR_SHAPE, "paged_attention: negative window or sinks");
+  if ((long long)b.n_tokens * n_heads > INT32_MAX) return fail(SQ_ERR_SHAPE, "paged_attention: too many query rows");
   if (!b.n_tokens) return SQ_OK;
   const long long width = (long long)n_heads * c.hd;
   st = paged::check_rows(q, q_stride, width, dtype, "paged_attention: q");
@@ -123,6 +715,6 @@ extern "C" int sq_paged_attention(void *stream, const sq_paged_cache *cache, con
   if ((uintptr_t)ws & 255) return fail(SQ_ERR_ALIGN, "paged_attention: the workspace must be 256-byte aligned");
   if (!(b.err = paged::err_ptr())) return fail(SQ_ERR_CUDA, "paged_attention: no current CUDA device");
   const auto run = dtype == SQ_F32 ? paged::attention<float> : paged::attention<__nv_bfloat16>;
-  cudaError_t e = run((cudaStream_t)stream, c, b, q, q_stride, n_heads, scale, window, sinks, out, out_stride);
+  cudaError_t e = run((cudaStream_t)stream, c, b, q, q_stride, n_heads, scale, window, sinks, out, out_stride, ws);
   return e == cudaSuccess ? SQ_OK : cuda_fail(e, "sq_paged_attention");
 }
