@@ -29,8 +29,7 @@
 
 #include <string>
 
-#include "common.cuh"
-#include "paged.cuh"
+#include "paged_attention.cuh"
 
 namespace sq {
 namespace paged {
@@ -42,61 +41,13 @@ constexpr int MAX_BLOCKS = 160 * BLOCKS_PER_SM;
 constexpr int MIN_TILES = WARPS;  // key tiles a block takes at least
 constexpr int SLOT_FLOATS = 2112;  // partial results of one row tile: rows x (head_dim + 2), 32 x 66 at most
 constexpr size_t PARTIAL_BYTES = (size_t)MAX_BLOCKS * 2 * SLOT_FLOATS * 4;
-constexpr float LOG2E = 1.4426950408889634f;
 constexpr float WEIGHT_EXP = 10.f;  // weights are 2^(s - max + 10)
 
-template <typename T>
-struct AttnArgs {
-  Cache c;
-  Batch b;
-  const T *q;
-  T *out;
-  long long qs, os;
-  int n_heads, group;
-  float scale;  // of the scores, times log2(e)
-  int window, sinks;
-  float *part;
-  int *count;  // blocks that have left their part of a row tile; zero between calls
-  int max_row_tiles;
-};
-
-__device__ __forceinline__ long long warp_sum_ll(long long v) {
-#pragma unroll
-  for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
-  return v;
-}
-__device__ __forceinline__ uint32_t smem_addr(const void *p) { return (uint32_t)__cvta_generic_to_shared(p); }
-__device__ __forceinline__ void cp16(uint32_t dst, const void *src) {
-  asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
-}
-__device__ __forceinline__ void cp_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
-template <int N>
-__device__ __forceinline__ void cp_wait() {
-  asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
-}
 __device__ __forceinline__ uint2 lds64(uint32_t a) {
   uint2 v;
   asm volatile("ld.shared.v2.u32 {%0, %1}, [%2];" : "=r"(v.x), "=r"(v.y) : "r"(a));
   return v;
 }
-__device__ __forceinline__ float ex2(float x) {
-  float y;
-  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
-  return y;
-}
-__device__ __forceinline__ uint32_t sub1152(uint32_t x) {  // two f16: 1024 + code -> code - 128
-  uint32_t y;
-  asm("sub.f16x2 %0, %1, %2;" : "=r"(y) : "r"(x), "r"(0x64806480u));
-  return y;
-}
-// Codes (bytes 0, 1) and (2, 3) of a word as f16 pairs.
-__device__ __forceinline__ uint32_t codes_lo(uint32_t w) { return sub1152(__byte_perm(w, 0x64646464u, 0x4140)); }
-__device__ __forceinline__ uint32_t codes_hi(uint32_t w) { return sub1152(__byte_perm(w, 0x64646464u, 0x4342)); }
-__device__ __forceinline__ uint32_t pack(float lo, float hi) {
-  const __half2 h = __floats2half2_rn(lo, hi);
-  return *reinterpret_cast<const uint32_t *>(&h);
-}
-__device__ __forceinline__ float2 unpack(uint32_t x) { return __half22float2(*reinterpret_cast<const __half2 *>(&x)); }
 __device__ __forceinline__ uint32_t transpose8x8(uint32_t x) {
   uint32_t y;
   asm("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(y) : "r"(x));
@@ -173,7 +124,7 @@ __global__ void __launch_bounds__(THREADS, C::NT <= 2 ? BLOCKS_PER_SM : 2) k_pag
   const int rows_of_token = a.group;
 
   auto tiles_of = [&](const Seq &s) -> long long {
-    if (!s.n) return 0;
+    if (!s.n || s.n * rows_of_token > a.few_rows) return 0;
     const int rt = (s.n * rows_of_token + ROWS - 1) / ROWS;
     return (long long)key_span<TK>(s, a.window, a.sinks).n * rt * c.kv_heads;
   };
@@ -263,9 +214,8 @@ __global__ void __launch_bounds__(THREADS, C::NT <= 2 ? BLOCKS_PER_SM : 2) k_pag
       top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
       top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
       finite = (__ballot_sync(0xffffffffu, finite) >> (lane & 28) & 15) == 15;  // of the row's four lanes
-      // the largest element becomes 2^10 .. 2^11; a row with NaN or infinity is NaN as a whole
-      const int e = top > 0.f ? min(10 - ((int)(__float_as_uint(top) >> 23) - 127), 127) : 0;
-      const float up = finite ? __uint_as_float((uint32_t)(e + 127) << 23) : __int_as_float(0x7fffffff);
+      const int e = row_exp(top);
+      const float up = row_factor(e, finite);
       const float down = scalbnf(a.scale, -e);
 #pragma unroll
       for (int i = 0; i < KS; i++) {
@@ -632,7 +582,7 @@ cudaError_t launch(cudaStream_t s, AttnArgs<T> &a) {
       return e;
     blocks[dev] = min(sms * max(per_sm, 1), MAX_BLOCKS);
   }
-  a.max_row_tiles = (a.b.max_new * a.group + C::ROWS - 1) / C::ROWS;
+  a.max_row_tiles = (min(a.b.max_new * a.group, a.few_rows) + C::ROWS - 1) / C::ROWS;
   k_paged_few<C, T><<<blocks[dev], THREADS, C::SMEM, s>>>(a);
   return cudaGetLastError();
 }
@@ -640,7 +590,7 @@ cudaError_t launch(cudaStream_t s, AttnArgs<T> &a) {
 // The narrowest tile that takes all rows of a kv head, up to what the registers hold.
 template <typename T, int HD>
 cudaError_t launch_few(cudaStream_t s, AttnArgs<T> &a) {
-  const int rows = a.b.max_new * a.group;
+  const int rows = min(a.b.max_new * a.group, a.few_rows);
   if (rows <= Cfg<T, HD, 1>::ROWS || HD == 256) return launch<Cfg<T, HD, 1>>(s, a);
   if constexpr (HD <= 128) {
     if (rows <= Cfg<T, HD, 2>::ROWS || HD == 128) return launch<Cfg<T, HD, 2>>(s, a);
@@ -649,16 +599,47 @@ cudaError_t launch_few(cudaStream_t s, AttnArgs<T> &a) {
   return cudaErrorInvalidValue;
 }
 
-size_t workspace_bytes(const Batch &b, const Cache &c, int n_heads) {
-  const long long tiles = ((long long)b.max_new * (n_heads / c.kv_heads) + 3) / 4;  // narrowest row tile: 4 rows
-  return PARTIAL_BYTES + (size_t)b.n_seqs * c.kv_heads * tiles * sizeof(int);
+// Rows a kv head up to which a sequence is this file's: beyond, the products cost more than
+// the reading of the cache.
+constexpr int FEW_ROWS = 64;
+
+bool goes_many(const Cache &c, int max_new, int group) {
+  return (long long)max_new * group > FEW_ROWS && many_supported(c, group);
+}
+
+// Partial results of both kernels, then the counters of both.
+struct Workspace {
+  size_t many_part, few_count, many_count, bytes;
+};
+Workspace workspace(const Batch &b, const Cache &c, int n_heads) {
+  const int group = n_heads / c.kv_heads;
+  const bool many = goes_many(c, b.max_new, group);
+  const size_t jobs = (size_t)b.n_seqs * c.kv_heads;
+  const long long rows = many ? FEW_ROWS : (long long)b.max_new * group;
+  Workspace w;
+  w.many_part = PARTIAL_BYTES;
+  w.few_count = w.many_part + (many ? many_partial_bytes(c.hd) : 0);
+  w.many_count = w.few_count + jobs * ((rows + 3) / 4) * sizeof(int);  // row tiles have 4 rows at least
+  w.bytes = w.many_count + (many ? jobs * many_row_tiles(b.max_new, group) * sizeof(int) : 0);
+  return w;
 }
 
 template <typename T>
 cudaError_t attention(cudaStream_t s, const Cache &c, const Batch &b, const void *q, long long qs, int n_heads,
                       float scale, int window, int sinks, void *out, long long os, void *ws) {
-  AttnArgs<T> a = {c,  b,      (const T *)q, (T *)out,     qs, os, n_heads, n_heads / c.kv_heads, scale * LOG2E,
-                   window, sinks, (float *)ws, (int *)((uint8_t *)ws + PARTIAL_BYTES), 0};
+  const Workspace w = workspace(b, c, n_heads);
+  uint8_t *p = (uint8_t *)ws;
+  AttnArgs<T> a = {c,      b,     (const T *)q, (T *)out,  qs,      os, n_heads, n_heads / c.kv_heads, scale * LOG2E,
+                   window, sinks, INT32_MAX,    (float *)p, (int *)(p + w.few_count), 0};
+  if (goes_many(c, b.max_new, a.group)) {
+    AttnArgs<T> m = a;
+    a.few_rows = m.few_rows = FEW_ROWS;
+    m.part = (float *)(p + w.many_part);
+    m.count = (int *)(p + w.many_count);
+    const cudaError_t e = launch_many(s, m);
+    // all sequences bring as many tokens as the longest: none is left for the other kernel
+    if (e != cudaSuccess || (long long)b.max_new * b.n_seqs == b.n_tokens) return e;
+  }
   switch (c.hd) {
     case 32: return launch_few<T, 32>(s, a);
     case 64: return launch_few<T, 64>(s, a);
@@ -688,7 +669,7 @@ extern "C" int sq_paged_attention_workspace(const sq_paged_cache *cache, const s
   if (!st && !bytes) st = fail(SQ_ERR_ARG, "paged_attention_workspace: null pointer");
   if (!st) st = paged::check_heads(c, n_heads, "paged_attention_workspace");
   if (st) return st;
-  *bytes = paged::workspace_bytes(b, c, n_heads);
+  *bytes = paged::workspace(b, c, n_heads).bytes;
   return SQ_OK;
 }
 
@@ -710,7 +691,7 @@ extern "C" int sq_paged_attention(void *stream, const sq_paged_cache *cache, con
   st = paged::check_rows(q, q_stride, width, dtype, "paged_attention: q");
   if (!st) st = paged::check_rows(out, out_stride, width, dtype, "paged_attention: out");
   if (st) return st;
-  if (!ws || ws_bytes < paged::workspace_bytes(b, c, n_heads))
+  if (!ws || ws_bytes < paged::workspace(b, c, n_heads).bytes)
     return fail(SQ_ERR_ARG, "paged_attention: the workspace is smaller than paged_attention_workspace says");
   if ((uintptr_t)ws & 255) return fail(SQ_ERR_ALIGN, "paged_attention: the workspace must be 256-byte aligned");
   if (!(b.err = paged::err_ptr())) return fail(SQ_ERR_CUDA, "paged_attention: no current CUDA device");
