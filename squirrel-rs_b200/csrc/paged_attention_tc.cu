@@ -5,15 +5,19 @@
 // A block works on 256 query rows of one kv head (row = token * group + head of the
 // group), two tiles X of 128 that share every key block, so that a code is converted once
 // for 256 rows:
-//   warps 8-10  codes of a block of keys to shared memory (cp.async, each thread its own
+//   warps 8-11  codes of a block of keys to shared memory (cp.async, each thread its own
 //               chunks), converted to f16 (exact: whole numbers up to 127) into the
 //               128-byte swizzled tiles of K [keys][dims] and V [keys][dims]; two stages
-//   warp 11     one thread issues the products, f32 sums in tensor memory:
+//   warp 12     one thread issues the products, f32 sums in tensor memory:
 //               S_X = Q_X K^T (K-major operands), O_X (+)= P_X V (V read MN-major as it
 //               lies, P from tensor memory). Order: P V of one tile, its next S, then the
 //               other tile: one tile's softmax runs under the other's products
-//   warps 0-7   one thread a row (= tensor-memory lane): its scores to registers, running
-//               maximum, weights back to the columns the scores left, sum
+//   warp 13     walks this block's share of the work and hands it out piece by piece
+//   warps 0-7   one thread a row (= tensor-memory lane): running maximum of its scores,
+//               weights over the columns the scores leave, sum. The scores are read twice
+//               from tensor memory, 64 at a time in a rolled loop: with 128 held and the
+//               loops unrolled the kernel was 200 KB of code, and every role spent its
+//               time waiting for instructions (2,048-token chunk: 412 us)
 // Products issued by one thread complete in order, so a tile's S being done says that its
 // last P V is done too: no further barriers between them.
 //
@@ -32,6 +36,7 @@
 // copies finish, frees its tensor memory and returns.
 #include <cuda.h>
 #include <float.h>
+#include <limits.h>
 
 #include "paged_attention.cuh"
 #include "tc.cuh"
@@ -42,15 +47,16 @@ namespace {
 
 using namespace tc;
 
-constexpr int SOFTMAX_WARPS = 8, LOAD_WARPS = 3, WARPS = SOFTMAX_WARPS + LOAD_WARPS + 1;
+constexpr int SOFTMAX_WARPS = 8, LOAD_WARPS = 4, MMA_WARP = SOFTMAX_WARPS + LOAD_WARPS;
+constexpr int WARPS = 16;  // whole warpgroups: registers are shared out by them (warps 13-15 only take part in barriers)
 constexpr int THREADS = WARPS * 32, LOADERS = LOAD_WARPS * 32;
 constexpr int TILE_ROWS = 128, ROWS = 2 * TILE_ROWS;
 constexpr int STAGES = 2, SCALE_STAGES = 4;
 constexpr int MAX_BLOCKS = 160;
 constexpr int MIN_BLOCKS = 2;  // key blocks a thread block takes at least
 constexpr float WEIGHT_EXP = 3.f, REF_LAG = 6.f, UNIT_LAG = 64.f;
-// Registers a thread: launched with 168 (384 x 168 = 64,512), then 256 x 208 + 128 x 88.
-constexpr int SOFTMAX_REGS = 208, OTHER_REGS = 88;
+// Registers a thread: launched with 128 (512 x 128 = 65,536), then 256 x 184 + 128 x 80 + 128 x 64.
+constexpr int SOFTMAX_REGS = 184, LOAD_REGS = 80, MMA_REGS = 64;
 
 template <typename T, int HD_>
 struct Cfg {
@@ -62,9 +68,10 @@ struct Cfg {
   static constexpr int PANELS = HD / 64;                    // 64 dimensions = 128 bytes of f16
   static constexpr int Q_PANEL = TILE_ROWS * 128, KV_PANEL = BK * 128;
   static constexpr int Q_TILE = PANELS * Q_PANEL, KV_TILE = PANELS * KV_PANEL;
-  static constexpr int CHUNKS = BK * HD / 16;                     // 16-code chunks of a block
-  static constexpr int PER_LOADER = (CHUNKS + LOADERS - 1) / LOADERS;
-  static constexpr int RAW = PER_LOADER * LOADERS * 16;
+  static constexpr int ROW_CHUNKS = HD / 16;                      // 16-code chunks of a key
+  static constexpr int STEP_ROWS = LOADERS / ROW_CHUNKS;          // keys the loading threads take at once: 16 or 32
+  static constexpr int STEPS = BK / STEP_ROWS;
+  static constexpr int RAW = BK * HD;
   static constexpr int OFF_Q = 0, OFF_K = OFF_Q + 2 * TERMS * Q_TILE, OFF_V = OFF_K + STAGES * KV_TILE,
                        OFF_RAW = OFF_V + STAGES * KV_TILE, OFF_SCALE = OFF_RAW + 2 * RAW,
                        OFF_BAR = OFF_SCALE + SCALE_STAGES * 4 * 8 * 4;
@@ -94,9 +101,15 @@ enum : int {
   B_P = 15,      // [2 tiles] weights written
   B_O = 17,      // [2 tiles] the piece's last P V done
   B_FIN = 19,
-  N_BARS = 20
+  B_PIECE = 20,  // [4] a piece handed out
+  B_DONE = 24,   // a piece's rows written
+  N_BARS = 25
 };
-constexpr uint32_t TM_O = 256, TM_COLS = 512;  // S / P of tile X at X * BK, O at 256 + 128 X
+// Columns of tile X: S at X * BK, the first terms of P over its first half; O at 256 + 128 X;
+// second terms of P at 320 + 128 X (head_dim 64) or 128 + 64 X.
+constexpr uint32_t TM_O = 256, TM_COLS = 512;
+template <class C>
+__host__ __device__ constexpr uint32_t tm_lo(int x) { return C::HD == 64 ? 320 + 128 * x : 128 + 64 * x; }
 
 // f16 operands, f32 sums; B K-major or (bit 16) MN-major.
 constexpr uint32_t idesc_f16(int M, int N, bool b_mn) {
@@ -123,6 +136,16 @@ __device__ __forceinline__ void tmem_ld32(uint32_t a, float *v) {
 #pragma unroll
   for (int i = 0; i < 32; i++) v[i] = __uint_as_float(r[i]);
 }
+__device__ __forceinline__ void tmem_st32(uint32_t a, const uint32_t *r) {
+  asm volatile(
+      "tcgen05.st.sync.aligned.32x32b.x32.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, "
+      "%16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31, %32};" ::"r"(a),
+      "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]),
+      "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15]), "r"(r[16]), "r"(r[17]), "r"(r[18]),
+      "r"(r[19]), "r"(r[20]), "r"(r[21]), "r"(r[22]), "r"(r[23]), "r"(r[24]), "r"(r[25]), "r"(r[26]), "r"(r[27]),
+      "r"(r[28]), "r"(r[29]), "r"(r[30]), "r"(r[31])
+      : "memory");
+}
 // Orders the uses of N loaded registers after the wait for them.
 template <int N>
 __device__ __forceinline__ void tmem_ready(float *v) {
@@ -134,27 +157,26 @@ __device__ __forceinline__ void sts128(uint32_t a, uint32_t x, uint32_t y, uint3
   asm volatile("st.shared.v4.u32 [%0], {%1, %2, %3, %4};" ::"r"(a), "r"(x), "r"(y), "r"(z), "r"(w) : "memory");
 }
 
-// Sum over i < n of floor((a i + b) / m), by Euclid's steps.
-__device__ __forceinline__ long long floor_sum(long long n, int m, int a, long long b) {
-  long long sum = 0;
-  unsigned mm = m, aa = a;
-  unsigned long long bb = b;
-  while (n > 0) {
-    if (aa >= mm) {
-      sum += (n - 1) * n / 2 * (aa / mm);
-      aa %= mm;
+// Sum over i < n of floor((a i + b) / m), by Euclid's steps. The host refuses calls whose
+// line of key blocks would not be below 2^31.
+__device__ __forceinline__ int floor_sum(unsigned n, unsigned m, unsigned a, unsigned b) {
+  unsigned sum = 0;
+  while (n) {
+    if (a >= m) {
+      sum += n * (n - 1) / 2 * (a / m);
+      a %= m;
     }
-    if (bb >= mm) {
-      sum += n * (long long)(bb / mm);
-      bb %= mm;
+    if (b >= m) {
+      sum += n * (b / m);
+      b %= m;
     }
-    const unsigned long long y = (unsigned long long)aa * n + bb;
-    if (y < mm) break;
-    n = y / mm;
-    bb = y % mm;
-    const unsigned x = mm;
-    mm = aa;
-    aa = x;
+    const unsigned y = a * n + b;
+    if (y < m) break;
+    n = y / m;
+    b = y % m;
+    const unsigned x = m;
+    m = a;
+    a = x;
   }
   return sum;
 }
@@ -176,93 +198,106 @@ struct Line {
     if (window && window < s.len)
       flat = min((min(sinks, s.len) + BK - 1) / BK + (window + tokens + BK - 3) / BK + 1, (s.len + BK - 1) / BK);
   }
-  __device__ __forceinline__ long long before(int rt) const {  // key blocks of row tiles 0 .. rt - 1
-    if (flat) return (long long)rt * flat;
+  __device__ __forceinline__ int before(int rt) const {  // key blocks of row tiles 0 .. rt - 1
+    if (flat) return rt * flat;
     return rt + floor_sum(rt, BK, tokens, pos0 + tokens - 1);
   }
   __device__ __forceinline__ int of(int rt) const {
-    return flat ? flat : (int)((pos0 + (long long)(rt + 1) * tokens - 1) / BK) + 1;
+    return flat ? flat : (pos0 + (rt + 1) * tokens - 1) / BK + 1;
   }
 };
 
 // One block's part of a row tile.
-template <int BK>
 struct Piece {
-  int b, head, rt;
-  Seq s;
-  int first_tok, n_rows;     // tokens from first_tok on, rows in use
-  int t0, n;                 // key blocks t0 .. t0 + n - 1 of the tile (n may be 0)
-  int n_sink, skip;          // tile index to block number, as in the few-row kernel
-  bool whole;
-  int slot;                  // of the partial results
-  long long first;           // blocks first .. first + parts - 1 share the tile
-  int parts;
-  bool late;                 // block `first` began another tile before this one: its second slot
-  __device__ __forceinline__ int block(int i) const { return i < n_sink ? i : i + skip; }
+  int b, head;
+  int row0, n_rows;     // first token's row of the step, query rows in use (token * group + head of the group)
+  int pos0, len;        // first token's position; positions held
+  int t0, n;            // key blocks t0 .. t0 + n - 1 of the tile (n may be 0; -1: no more pieces)
+  int n_sink, skip;     // tile index to block number, as in the few-row kernel
+  int whole;
+  int slot;             // of the partial results
+  int first, parts;     // thread blocks first .. first + parts - 1 share the tile
+  int late;             // block `first` began another tile before this one: its second slot
+  int counter;
+  __device__ __forceinline__ int block(int i) const { return t0 + i + (t0 + i < n_sink ? 0 : skip); }
 };
+constexpr int PIECES = 4;
 
-// Walks this thread block's piece of the line; every warp does so on its own.
+// Walks this thread block's piece of the line.
 template <int BK>
 struct Walk {
-  long long at, end, per;
-  long long seq_start;  // of sequence b on the line
-  int b;
+  int at, end, per;
+  int seq_start;   // of sequence b on the line
+  int tile_start;  // of the row tile (head, rt)
+  int b, head, rt;
+  bool found;  // the first row tile is looked up, the others follow
   Line<BK> line;
   Seq s;
-  long long per_head;
+  int per_head;
 
   template <typename T>
-  __device__ __forceinline__ void load(const AttnArgs<T> &a) {
-    s = load_seq(a.b, a.c, b);
-    line.set(s, a.group, a.window, a.sinks, a.few_rows);
-    per_head = line.before(line.row_tiles);
-  }
-  template <typename T>
-  __device__ __forceinline__ bool next(const AttnArgs<T> &a, Piece<BK> &p) {
+  __device__ __forceinline__ bool next(const AttnArgs<T> &a, Piece &p) {
     if (at >= end) return false;
-    while (at >= seq_start + per_head * a.c.kv_heads) {
-      seq_start += per_head * a.c.kv_heads;
-      b++;
-      load(a);
+    bool other = !found;
+    if (found && ++rt == line.row_tiles) {
+      rt = 0;
+      if (++head == a.c.kv_heads) {
+        head = 0;
+        other = true;
+        b++;
+      }
     }
-    const long long in_seq = at - seq_start;
-    p.head = (int)(in_seq / per_head);
-    const long long in_head = in_seq - p.head * per_head;
-    // the row tile that holds in_head: 32 candidates at a time
-    int lo = 0, width = line.row_tiles;
-    while (width > 1) {
-      const int step = (width + 31) / 32, mine = lo + (threadIdx.x & 31) * step;
-      const unsigned le = __ballot_sync(0xffffffffu, mine < lo + width && line.before(mine) <= in_head);
-      const int k = 31 - __clz(le);  // lane 0 always holds
-      lo += k * step;
-      width = min(step, width - k * step);
+    if (other) {
+#pragma unroll 1
+      for (;; b++) {  // at < end: a sequence with row tiles follows
+        s = load_seq(a.b, a.c, b);
+        line.set(s, a.group, a.window, a.sinks, a.few_rows);
+        if (line.row_tiles) break;
+      }
     }
-    p.rt = lo;
+    if (!found) {
+      per_head = line.before(line.row_tiles);
+      head = (at - seq_start) / per_head;
+      const int in_head = at - seq_start - head * per_head;
+      // the row tile that holds in_head: 32 candidates at a time
+      rt = 0;
+#pragma unroll 1
+      for (int width = line.row_tiles; width > 1;) {
+        const int step = (width + 31) / 32, mine = rt + (threadIdx.x & 31) * step;
+        const unsigned le = __ballot_sync(0xffffffffu, mine < rt + width && line.before(mine) <= in_head);
+        const int k = 31 - __clz(le);  // lane 0 always holds
+        rt += k * step;
+        width = min(step, width - k * step);
+      }
+      tile_start = seq_start + head * per_head + line.before(rt);
+      found = true;
+    }
+    const int slots = line.of(rt), first_tok = rt * line.tokens, toks = min(line.tokens, s.n - first_tok);
     p.b = b;
-    p.s = s;
-    const int slots = line.of(lo);
-    const long long tile_start = seq_start + p.head * per_head + line.before(lo);
-    p.first_tok = lo * line.tokens;
-    const int toks = min(line.tokens, s.n - p.first_tok);
+    p.head = head;
+    p.row0 = s.first + first_tok;
     p.n_rows = toks * a.group;
-    const int min_pos = s.len - s.n + p.first_tok, max_pos = max(min_pos + toks - 1, 0);
-    int real = max_pos / BK + 1;
+    p.pos0 = s.len - s.n + first_tok;
+    p.len = s.len;
+    int real = max(p.pos0 + toks - 1, 0) / BK + 1;
     p.n_sink = p.skip = 0;
     if (line.flat) {
-      const int low = max(min_pos - a.window + 1, 0) / BK;
+      const int low = max(p.pos0 - a.window + 1, 0) / BK;
       p.n_sink = min((min(a.sinks, s.len) + BK - 1) / BK, low);
       p.skip = low - p.n_sink;
       real -= p.skip;
     }
-    p.t0 = (int)(at - tile_start);
-    const int t1 = (int)min((long long)slots, end - tile_start);
+    p.t0 = at - tile_start;
+    const int t1 = min(slots, end - tile_start);
     p.n = max(min(t1, real) - p.t0, 0);
     p.whole = p.t0 == 0 && t1 == slots;
-    p.slot = 2 * blockIdx.x + (tile_start > per * blockIdx.x ? 1 : 0);
     p.first = tile_start / per;
-    p.parts = (int)((tile_start + slots - 1) / per - p.first) + 1;
+    p.parts = (tile_start + slots - 1) / per - p.first + 1;
     p.late = tile_start > per * p.first;
+    p.slot = 2 * blockIdx.x + (tile_start > per * (int)blockIdx.x ? 1 : 0);
+    p.counter = (b * a.c.kv_heads + head) * a.max_row_tiles + rt;
     at = tile_start + t1;
+    tile_start += slots;
     return true;
   }
 };
@@ -272,9 +307,10 @@ __global__ void __launch_bounds__(THREADS, 1) k_paged_many(const AttnArgs<T> a) 
   constexpr int HD = C::HD, BK = C::BK, NG = C::NG, TERMS = C::TERMS;
   constexpr bool SPLIT = C::SPLIT;
   extern __shared__ uint8_t smem_raw[];
-  __shared__ long long s_scan[WARPS + 2];
+  __shared__ int s_scan[WARPS + 2];
   __shared__ int s_seq, s_abort, s_last;
   __shared__ uint32_t s_tmem;
+  __shared__ Piece s_pieces[PIECES];
   const uint32_t base = (smem_addr(smem_raw) + 1023u) & ~1023u;
   uint8_t *gen = smem_raw + (base - smem_addr(smem_raw));
   Scales *scales = reinterpret_cast<Scales *>(gen + C::OFF_SCALE);
@@ -283,37 +319,37 @@ __global__ void __launch_bounds__(THREADS, 1) k_paged_many(const AttnArgs<T> a) 
   const Cache &c = a.c;
 
   // ---- this block's piece of the line
-  auto blocks_of = [&](int b) -> long long {
+  auto blocks_of = [&](int b) -> int {
     Line<BK> l;
     l.set(load_seq(a.b, c, b), a.group, a.window, a.sinks, a.few_rows);
     return l.before(l.row_tiles) * c.kv_heads;
   };
-  long long total = 0;
+  int total = 0;
   for (int b = tid; b < a.b.n_seqs; b += THREADS) total += blocks_of(b);
-  total = warp_sum_ll(total);
+  total = __reduce_add_sync(0xffffffffu, total);
   if (lane == 0) s_scan[warp] = total;
   __syncthreads();
   total = 0;
   for (int w = 0; w < WARPS; w++) total += s_scan[w];
   Walk<BK> walk;
-  walk.per = max((total + gridDim.x - 1) / gridDim.x, (long long)MIN_BLOCKS);
+  walk.per = max((total + (int)gridDim.x - 1) / (int)gridDim.x, MIN_BLOCKS);
+  if (walk.per * (long long)blockIdx.x >= total) return;
   walk.at = walk.per * blockIdx.x;
   walk.end = min(walk.at + walk.per, total);
-  if (walk.at >= walk.end) return;
   walk.b = 0;
   walk.seq_start = 0;
   for (int b0 = 0; b0 < a.b.n_seqs; b0 += THREADS) {
-    const long long n = b0 + tid < a.b.n_seqs ? blocks_of(b0 + tid) : 0;
-    long long run = n;
+    const int n = b0 + tid < a.b.n_seqs ? blocks_of(b0 + tid) : 0;
+    int run = n;
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
-      const long long y = __shfl_up_sync(0xffffffffu, run, o);
+      const int y = __shfl_up_sync(0xffffffffu, run, o);
       if (lane >= o) run += y;
     }
     __syncthreads();
     if (lane == 31) s_scan[warp] = run;
     __syncthreads();
-    long long all = walk.seq_start;
+    int all = walk.seq_start;
     for (int w = 0; w < WARPS; w++) {
       if (w == warp) run += all;
       all += s_scan[w];
@@ -330,11 +366,11 @@ __global__ void __launch_bounds__(THREADS, 1) k_paged_many(const AttnArgs<T> a) 
     }
     walk.seq_start = all;
   }
-  walk.load(a);
+  walk.found = false;
 
   if (tid == 0) {
     for (int i = 0; i < N_BARS; i++) {
-      const unsigned count = i == B_Q                          ? SOFTMAX_WARPS
+      const unsigned count = i == B_Q || i == B_DONE           ? SOFTMAX_WARPS
                              : i >= B_P && i < B_P + 2         ? SOFTMAX_WARPS / 2
                              : i >= B_K && i < B_K + 2         ? LOAD_WARPS
                              : i >= B_V && i < B_V + 2         ? LOAD_WARPS
@@ -345,7 +381,7 @@ __global__ void __launch_bounds__(THREADS, 1) k_paged_many(const AttnArgs<T> a) 
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   }
   __syncwarp();
-  if (warp == WARPS - 1) tmem_alloc(smem_addr(&s_tmem), TM_COLS);
+  if (warp == MMA_WARP) tmem_alloc(smem_addr(&s_tmem), TM_COLS);
   fence_before();
   __syncthreads();
   fence_after();
@@ -374,83 +410,199 @@ __global__ void __launch_bounds__(THREADS, 1) k_paged_many(const AttnArgs<T> a) 
     return ok;
   };
 
-  Piece<BK> p;
-  if (warp >= SOFTMAX_WARPS) {
-    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(OTHER_REGS));
-    if (warp < SOFTMAX_WARPS + LOAD_WARPS) {
-      // ---------------- codes to f16 tiles ----------------
-      const int me = tid - SOFTMAX_WARPS * 32;
-      constexpr int ROW_CHUNKS = HD / 16;
-      unsigned done = 0;  // blocks so far
-      bool ok = true;
-      while (ok && walk.next(a, p)) {
-        float unit = 0.f;
-        // Lane j < NG: page and scales of group j of a block.
-        auto page_of = [&](int i) {
-          const int key = p.block(p.t0 + i) * BK + 16 * lane;
-          return i < p.n && lane < NG && key < p.s.len ? load_page(a.b, c, p.b, key) : -1;
-        };
-        auto fetch = [&](int i, int page, const uint8_t *codes, int raw) {
-          if (i < p.n) {
-            const int key0 = p.block(p.t0 + i) * BK;
+  if (warp >= MMA_WARP) {
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(MMA_REGS));
+    if (warp == MMA_WARP + 1) {
+      // ---------------- pieces ----------------
+      bool more = true;
+#pragma unroll 1
+      for (unsigned k = 0; more; k++) {
+        Piece p;
+        more = walk.next(a, p);
+        if (!more) p.n = -1;
+        if (k >= PIECES && !wait_warp(B_DONE, k - PIECES)) break;  // its place is free
+        if (lane == 0) {
+          s_pieces[k % PIECES] = p;
+          bar_arrive(bar(B_PIECE + k % PIECES));
+        }
+        __syncwarp();
+      }
+    } else if (warp == MMA_WARP) {
+      // ---------------- products ----------------
+      if (lane == 0) {
+        unsigned done = 0, tile_done[2] = {0, 0};
+        bool ok = true;
+#pragma unroll 1
+        for (unsigned k = 0; ok; k++) {
+          if (!(ok = wait(B_PIECE + k % PIECES, k / PIECES))) break;
+          const int n = s_pieces[k % PIECES].n, tiles = s_pieces[k % PIECES].n_rows > TILE_ROWS ? 2 : 1;
+          if (n < 0) break;
+          // An operand's place is the low bits of its descriptor, in units of 16 bytes: every one is a base and a sum.
+          const uint64_t qd = sw128_desc(base + C::OFF_Q), kd = sw128_desc(base + C::OFF_K);
+          const uint64_t vd = mn_desc(base + C::OFF_V, C::KV_PANEL);
+          auto scores = [&](int x, int st) {
+            const uint64_t q = qd + (uint32_t)(x * (TERMS * C::Q_TILE >> 4)), k = kd + (uint32_t)(st * (C::KV_TILE >> 4));
+            const uint32_t d = tmem + x * BK;
 #pragma unroll
-            for (int k = 0; k < C::PER_LOADER; k++) {
-              const int q = me + k * LOADERS, r = q / ROW_CHUNKS;
-              const int pg = __shfl_sync(0xffffffffu, page, min(r >> 4, NG - 1));  // a warp's 32 chunks: one group
-              if (q < C::CHUNKS && pg >= 0) {
-                const long long at = (((long long)pg * c.kv_heads + p.head) * c.page + ((key0 + r) & (c.page - 1))) * HD;
-                cp16(base + C::OFF_RAW + raw * C::RAW + q * 16, codes + at + (q % ROW_CHUNKS) * 16);
+            for (int t = 0; t < TERMS; t++)
+#pragma unroll
+              for (int i = 0; i < HD / 16; i++)
+                mma_bf16(d, q + ((t * C::Q_TILE + (i >> 2) * C::Q_PANEL + (i & 3) * 32) >> 4),
+                         k + (((i >> 2) * C::KV_PANEL + (i & 3) * 32) >> 4), idesc_f16(TILE_ROWS, BK, false),
+                         t || i ? 1u : 0u);
+            mma_commit(bar(B_S + x));
+          };
+          auto output = [&](int x, int st, bool first) {
+            const uint64_t v = vd + (uint32_t)(st * (C::KV_TILE >> 4));
+            const uint32_t d = tmem + TM_O + x * 128, hi = tmem + x * BK, lo = tmem + tm_lo<C>(x);
+#pragma unroll
+            for (int t = 0; t < TERMS; t++)
+#pragma unroll
+              for (int i = 0; i < BK / 16; i++)
+                mma_bf16_ts(d, (t ? lo : hi) + i * 8, v + (i * 2048 >> 4), idesc_f16(TILE_ROWS, HD, true),
+                            t || i ? 1u : (SPLIT || first ? 0u : 1u));
+          };
+          ok = wait(B_Q, k);
+#pragma unroll 1
+          for (int i = 0; ok && i < n; i++, done++) {
+            const int st = done % STAGES, st1 = (done + 1) % STAGES;
+#pragma unroll 1
+            for (int x = i ? 0 : -tiles; x < tiles; x++) {  // the piece's first scores, then each tile's turn
+              if (x < 0) {
+                if (x == -tiles && !(ok = wait(B_K + st, done / STAGES))) break;
+                fence_after();
+                scores(x + tiles, st);
+                if (x == -1) mma_commit(bar(B_K_FREE + st));
+                continue;
+              }
+              if (!(ok = wait(B_P + x, x ? tile_done[1]++ : tile_done[0]++))) break;
+              if (x == 0 && !(ok = wait(B_V + st, done / STAGES))) break;
+              fence_after();
+              output(x, st, i == 0);
+              if (i + 1 < n) {
+                if (x == 0 && !(ok = wait(B_K + st1, (done + 1) / STAGES))) break;
+                fence_after();
+                scores(x, st1);
+              } else {
+                mma_commit(bar(B_O + x));
               }
             }
+            if (!ok) break;
+            mma_commit(bar(B_V_FREE + st));
+            if (i + 1 < n) mma_commit(bar(B_K_FREE + st1));
           }
-          cp_commit();
-        };
-        // Own chunks: raw codes -> f16 in the swizzled tile; groups not in `present` become zeros.
-        auto convert = [&](uint32_t present, int raw, uint32_t tile) {
+        }
+        // every product done before the columns are freed
+        mma_commit(bar(B_FIN));
+        bar_drain(bar(B_FIN), 0u);
+      }
+      __syncwarp();
+    }
+  } else if (warp >= SOFTMAX_WARPS) {
+    // ---------------- codes to f16 tiles ----------------
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(LOAD_REGS));
+    const int me = tid - SOFTMAX_WARPS * 32, r0 = me / C::ROW_CHUNKS, ch = me % C::ROW_CHUNKS;
+    constexpr int STEP_GROUPS = C::STEP_ROWS / 16;  // groups of a step: a warp's keys are of one
+    const int my_group = r0 >> 4;
+    // Own chunks: raw codes at raw + 2048 k; in the tile row r0 + STEP_ROWS k, 16-byte pieces 2 ch and 2 ch + 1
+    // of the row's dimensions. With two panels a row's upper lanes start with their second piece, so that
+    // eight lanes meet every bank once.
+    const uint32_t raw = base + C::OFF_RAW + me * 16;
+    const bool swap = HD == 128 && (ch & 4);
+    const uint32_t row = (ch >> 2) * C::KV_PANEL + r0 * 128;
+    const uint32_t piece0 = row + ((((ch & 3) * 2) + swap) ^ (r0 & 7)) * 16;
+    const uint32_t piece1 = row + ((((ch & 3) * 2) + !swap) ^ (r0 & 7)) * 16;
+    unsigned done = 0;  // blocks so far
+    bool ok = true;
+#pragma unroll 1
+    for (unsigned k = 0; ok; k++) {
+      if (!(ok = wait_warp(B_PIECE + k % PIECES, k / PIECES))) break;
+      const Piece p = s_pieces[k % PIECES];
+      if (p.n < 0) break;
+      // Lane j < NG: page (-1: none) and scales of group j of a block.
+      struct Group {
+        int page;
+        float ks, vs;
+      };
+      auto entry_of = [&](int i) {  // of the page table, looked up a block ahead of its use; INT_MIN: no such group
+        if (i >= p.n || lane >= NG) return INT_MIN;
+        const int key = p.block(i) * BK + 16 * lane;
+        return key < p.len ? a.b.table[(long long)p.b * a.b.table_row + (key >> c.page_shift)] : INT_MIN;
+      };
+      auto checked = [&](int entry) {
+        if ((unsigned)entry < (unsigned)c.n_pages) return entry;
+        if (entry != INT_MIN) flag(a.b.err, BAD_PAGE);
+        return -1;
+      };
+      auto scales_of = [&](int page) {
+        Group g = {page, 0.f, 0.f};
+        if (page >= 0) {
+          g.ks = c.ks[(long long)page * c.kv_heads + p.head];
+          g.vs = c.vs[(long long)page * c.kv_heads + p.head];
+        }
+        return g;
+      };
+      auto fetch = [&](int i, int page, const uint8_t *codes, int which) {
+        if (i < p.n) {
+          const int key0 = p.block(i) * BK + (r0 & 15);
 #pragma unroll
-          for (int k = 0; k < C::PER_LOADER; k++) {
-            const int q = me + k * LOADERS, r = q / ROW_CHUNKS, ch = q % ROW_CHUNKS;
-            if (q >= C::CHUNKS) break;
-            uint4 u = lds128(base + C::OFF_RAW + raw * C::RAW + q * 16);
-            if (!(present >> (r >> 4) & 1)) u = make_uint4(0x80808080u, 0x80808080u, 0x80808080u, 0x80808080u);
-            const uint32_t row = tile + (ch >> 2) * C::KV_PANEL + r * 128;
-            const int at = (ch & 3) * 2;
-            const bool swap = HD == 128 && (ch & 4);  // the second panel's lanes start with their odd chunk: no bank twice
-            uint4 lo = make_uint4(codes_lo(u.x), codes_hi(u.x), codes_lo(u.y), codes_hi(u.y));
-            uint4 hi = make_uint4(codes_lo(u.z), codes_hi(u.z), codes_lo(u.w), codes_hi(u.w));
-            if (swap) {
-              const uint4 x = lo;
-              lo = hi;
-              hi = x;
+          for (int k = 0; k < C::STEPS; k++) {
+            const int g = k * STEP_GROUPS + my_group, pg = __shfl_sync(0xffffffffu, page, g);
+            if (pg >= 0) {
+              const long long at = (((long long)pg * c.kv_heads + p.head) * c.page + ((key0 + 16 * g) & (c.page - 1))) * HD;
+              cp16(raw + which * C::RAW + k * (LOADERS * 16), codes + at + ch * 16);
             }
-            sts128(row + ((at + swap) ^ (r & 7)) * 16, lo.x, lo.y, lo.z, lo.w);
-            sts128(row + ((at + !swap) ^ (r & 7)) * 16, hi.x, hi.y, hi.z, hi.w);
           }
-        };
-        int page = page_of(0);
-        fetch(0, page, c.k, 0);
-        fetch(0, page, c.v, 1);
-        int next = page_of(1);
-        for (int i = 0; i < p.n; i++, done++) {
-          const int st = done % STAGES;
-          const uint32_t present = __ballot_sync(0xffffffffu, page >= 0);
-          float ks = 0.f, vs = 0.f;
-          if (page >= 0) {
-            ks = c.ks[(long long)page * c.kv_heads + p.head];
-            vs = c.vs[(long long)page * c.kv_heads + p.head];
-          }
-          float top = vs;
+        }
+        cp_commit();
+      };
+      auto convert = [&](uint32_t present, int which, uint32_t tile) {  // groups not present become zeros
+        uint4 u[C::STEPS];
 #pragma unroll
-          for (int o = 1; o < NG; o <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
-          top = __shfl_sync(0xffffffffu, top, 0);
-          if (SPLIT || top > unit * UNIT_LAG || unit == 0.f) unit = top;
-          // the scales' slot was read out when P of block done - 2 was written, before this stage was freed
-          if (done >= STAGES && !(ok = wait_warp(B_K_FREE + st, done / STAGES - 1))) break;
-          if (warp == SOFTMAX_WARPS) {
+        for (int k = 0; k < C::STEPS; k++) u[k] = lds128(raw + which * C::RAW + k * (LOADERS * 16));
+        if (present != (1u << NG) - 1) {
+#pragma unroll
+          for (int k = 0; k < C::STEPS; k++)
+            if (!(present >> (k * STEP_GROUPS + my_group) & 1))
+              u[k] = make_uint4(0x80808080u, 0x80808080u, 0x80808080u, 0x80808080u);
+        }
+#pragma unroll
+        for (int k = 0; k < C::STEPS; k++) {
+          if (swap) {
+            const uint4 x = u[k];
+            u[k] = make_uint4(x.z, x.w, x.x, x.y);
+          }
+          const uint32_t to = tile + k * (C::STEP_ROWS * 128);
+          sts128(to + piece0, codes_lo(u[k].x), codes_hi(u[k].x), codes_lo(u[k].y), codes_hi(u[k].y));
+          sts128(to + piece1, codes_lo(u[k].z), codes_hi(u[k].z), codes_lo(u[k].w), codes_hi(u[k].w));
+        }
+      };
+      float unit = 0.f;
+      int later = entry_of(1);
+      Group now = scales_of(checked(entry_of(0)));
+      fetch(0, now.page, c.k, 0);
+      fetch(0, now.page, c.v, 1);
+      Group next = scales_of(checked(later));
+      later = entry_of(2);
+#pragma unroll 1
+      for (int i = 0; ok && i < p.n; i++, done++) {
+        const int st = done % STAGES;
+        const uint32_t present = __ballot_sync(0xffffffffu, now.page >= 0);
+        const uint32_t with_v = __ballot_sync(0xffffffffu, now.page >= 0 && now.vs > 0.f);
+        float top = now.vs;
+#pragma unroll
+        for (int o = 1; o < NG; o <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+        top = __shfl_sync(0xffffffffu, top, 0);
+        if (SPLIT || top > unit * UNIT_LAG || unit == 0.f) unit = top;
+#pragma unroll 1
+        for (int v = 0; v < 2; v++) {  // K, then V
+          if (done >= STAGES && !(ok = wait_warp((v ? B_V_FREE : B_K_FREE) + st, done / STAGES - 1))) break;
+          // Scores of block done - 2 are done, so weights of done - 3 and before: the scales of done - 4 have been read.
+          if (!v && warp == SOFTMAX_WARPS) {
             Scales &sc = scales[done % SCALE_STAGES];
             if (lane < NG) {
-              const float share = vs > 0.f ? vs / unit : 0.f;
-              sc.ks[lane] = ks;
+              const float share = now.vs > 0.f ? now.vs / unit : 0.f;
+              sc.ks[lane] = now.ks;
               if (SPLIT) {
                 sc.share[lane] = share;
               } else {  // as an exponent; below 2^-100 of the unit: as good as none
@@ -467,90 +619,17 @@ __global__ void __launch_bounds__(THREADS, 1) k_paged_many(const AttnArgs<T> a) 
             if (lane == 0) bar_arrive(bar(B_SCALE + done % SCALE_STAGES));
           }
           cp_wait<1>();
-          convert(present, 0, base + C::OFF_K + st * C::KV_TILE);
-          fetch(i + 1, next, c.k, 0);
-          fence_proxy_async();
+          convert(v ? with_v : present, v, base + (v ? C::OFF_V : C::OFF_K) + st * C::KV_TILE);
+          fence_proxy_async();  // before the next copies: it would wait for them
           __syncwarp();
-          if (lane == 0) bar_arrive(bar(B_K + st));
-          if (done >= STAGES && !(ok = wait_warp(B_V_FREE + st, done / STAGES - 1))) break;
-          cp_wait<1>();
-          convert(present & __ballot_sync(0xffffffffu, vs > 0.f), 1, base + C::OFF_V + st * C::KV_TILE);
-          fetch(i + 1, next, c.v, 1);
-          fence_proxy_async();
-          __syncwarp();
-          if (lane == 0) bar_arrive(bar(B_V + st));
-          page = next;
-          next = page_of(i + 2);
+          if (lane == 0) bar_arrive(bar((v ? B_V : B_K) + st));
+          fetch(i + 1, next.page, v ? c.v : c.k, v);
         }
-        cp_wait<0>();
+        now = next;
+        next = scales_of(checked(later));
+        later = entry_of(i + 3);
       }
-    } else {
-      // ---------------- products ----------------
-      unsigned done = 0, pieces = 0, tile_done[2] = {0, 0};
-      bool ok = true;
-      while (ok && walk.next(a, p)) {
-        if (lane == 0) {
-          const int tiles = p.n_rows > TILE_ROWS ? 2 : 1;
-          auto scores = [&](int x, int st) {
-            uint32_t acc = 0;
-#pragma unroll
-            for (int t = 0; t < TERMS; t++)
-#pragma unroll
-              for (int k = 0; k < HD / 16; k++, acc = 1)
-                mma_bf16(tmem + x * BK,
-                         sw128_desc(base + C::OFF_Q + (x * TERMS + t) * C::Q_TILE + (k >> 2) * C::Q_PANEL + (k & 3) * 32),
-                         sw128_desc(base + C::OFF_K + st * C::KV_TILE + (k >> 2) * C::KV_PANEL + (k & 3) * 32),
-                         idesc_f16(TILE_ROWS, BK, false), acc);
-            mma_commit(bar(B_S + x));
-          };
-          auto output = [&](int x, int st, bool first) {
-            uint32_t acc = SPLIT || first ? 0 : 1;
-#pragma unroll
-            for (int t = 0; t < TERMS; t++)
-#pragma unroll
-              for (int k = 0; k < BK / 16; k++, acc = 1)
-                mma_bf16_ts(tmem + TM_O + x * 128, tmem + x * BK + t * (BK / 2) + k * 8,
-                            mn_desc(base + C::OFF_V + st * C::KV_TILE + k * 2048, C::KV_PANEL),
-                            idesc_f16(TILE_ROWS, HD, true), acc);
-          };
-          ok = wait(B_Q, pieces);
-          for (int i = 0; ok && i < p.n; i++, done++) {
-            const int st = done % STAGES;
-            if (i == 0) {
-              if (!(ok = wait(B_K + st, done / STAGES))) break;
-              fence_after();
-              for (int x = 0; x < tiles; x++) scores(x, st);
-              mma_commit(bar(B_K_FREE + st));
-            }
-            const int st1 = (done + 1) % STAGES;
-            for (int x = 0; x < tiles; x++) {
-              if (!(ok = wait(B_P + x, tile_done[x]))) break;
-              tile_done[x]++;
-              if (x == 0 && !(ok = wait(B_V + st, done / STAGES))) break;
-              fence_after();
-              output(x, st, i == 0);
-              if (i + 1 < p.n) {
-                if (x == 0 && !(ok = wait(B_K + st1, (done + 1) / STAGES))) break;
-                fence_after();
-                scores(x, st1);
-              } else {
-                mma_commit(bar(B_O + x));
-              }
-            }
-            if (!ok) break;
-            mma_commit(bar(B_V_FREE + st));
-            if (i + 1 < p.n) mma_commit(bar(B_K_FREE + st1));
-          }
-          pieces++;
-        }
-        ok = __shfl_sync(0xffffffffu, ok, 0);
-        __syncwarp();
-      }
-      if (lane == 0) {  // every product done before the columns are freed
-        mma_commit(bar(B_FIN));
-        bar_drain(bar(B_FIN), 0u);
-      }
-      __syncwarp();
+      cp_wait<0>();
     }
   } else {
     // ---------------- softmax and output: one thread a row ----------------
@@ -571,55 +650,83 @@ __global__ void __launch_bounds__(THREADS, 1) k_paged_many(const AttnArgs<T> a) 
       return res != 0;
     };
     unsigned done = 0, tile_done = 0, outs = 0;
-    while (walk.next(a, p)) {
+#pragma unroll 1
+    for (unsigned k = 0;; k++) {
+      bool ok = wait_warp(B_PIECE + k % PIECES, k / PIECES);
+      const Piece &piece = s_pieces[k % PIECES];
+      const int n = ok ? piece.n : -1;
+      if (ok && n < 0) break;
       // ---- the row's query as f16 terms in the swizzled tile
-      const int tok = p.first_tok + row / a.group, h = p.head * a.group + row % a.group;
-      const bool live = row < p.n_rows;
-      const T *src = a.q + (long long)(p.s.first + (live ? tok : 0)) * a.qs + (live ? h : 0) * HD;
-      const float sign = a.scale < 0.f ? -1.f : 1.f;  // the factor of the scores is then not negative: maxima commute
+      const int n_rows = piece.n_rows, tok = row / a.group, h = piece.head * a.group + row % a.group;
+      const bool live = ok && row < n_rows, active = x == 0 || n_rows > TILE_ROWS;
+      const T *src = a.q + (long long)(piece.row0 + (live ? tok : 0)) * a.qs + (live ? h : 0) * HD;
       float top = 0.f;
       bool finite = true;
-#pragma unroll 8
-      for (int d = 0; d < HD; d += 4) {
-        const float4 v = live ? load4(src + d) : make_float4(0.f, 0.f, 0.f, 0.f);
-        const float m4 = fmaxf(fmaxf(fabsf(v.x), fabsf(v.y)), fmaxf(fabsf(v.z), fabsf(v.w)));
-        top = fmaxf(top, m4);
-        finite &= fabsf(v.x) <= FLT_MAX && fabsf(v.y) <= FLT_MAX && fabsf(v.z) <= FLT_MAX && fabsf(v.w) <= FLT_MAX;
+      constexpr int PER16 = 16 / sizeof(T), PART = 8 * PER16;  // elements held at once: 128 bytes
+      uint4 raw[8];
+      auto get = [&](int d0) {
+#pragma unroll
+        for (int j = 0; j < 8; j++)
+          raw[j] = live ? __ldg(reinterpret_cast<const uint4 *>(src + d0 + j * PER16)) : make_uint4(0, 0, 0, 0);
+      };
+      auto pair = [&](int j) {  // elements 2 j, 2 j + 1 of those held
+        const uint4 u = raw[2 * j / PER16];
+        if constexpr (SPLIT) {
+          return j & 1 ? make_float2(__uint_as_float(u.z), __uint_as_float(u.w))
+                       : make_float2(__uint_as_float(u.x), __uint_as_float(u.y));
+        } else {
+          const uint32_t w = (j & 3) == 0 ? u.x : (j & 3) == 1 ? u.y : (j & 3) == 2 ? u.z : u.w;
+          return make_float2(__uint_as_float(w << 16), __uint_as_float(w & 0xFFFF0000u));
+        }
+      };
+#pragma unroll 1
+      for (int d0 = 0; d0 < HD; d0 += PART) {
+        get(d0);
+#pragma unroll
+        for (int j = 0; j < PART / 2; j++) {
+          const float2 v = pair(j);
+          top = fmaxf(top, fmaxf(fabsf(v.x), fabsf(v.y)));
+          finite &= fabsf(v.x) <= FLT_MAX && fabsf(v.y) <= FLT_MAX;
+        }
       }
       const int e = row_exp(top);
-      const float up = row_factor(e, finite) * sign, cf = scalbnf(fabsf(a.scale), -e);
-#pragma unroll 4
-      for (int d = 0; d < HD; d += 8) {
-        const float4 v = live ? load4(src + d) : make_float4(0.f, 0.f, 0.f, 0.f);
-        const float4 w = live ? load4(src + d + 4) : make_float4(0.f, 0.f, 0.f, 0.f);
-        const float y[8] = {v.x * up, v.y * up, v.z * up, v.w * up, w.x * up, w.y * up, w.z * up, w.w * up};
-        uint32_t f[4], g[4];
+      // the sign of the scale goes into the row: the factor of its scores is then not negative and maxima commute
+      const float up = row_factor(e, finite) * (a.scale < 0.f ? -1.f : 1.f), cf = scalbnf(fabsf(a.scale), -e);
+#pragma unroll 1
+      for (int d0 = 0; d0 < HD; d0 += PART) {
+        get(d0);
 #pragma unroll
-        for (int j = 0; j < 4; j++) {
-          f[j] = pack(y[2 * j], y[2 * j + 1]);
-          const float2 hi = unpack(f[j]);
-          g[j] = pack(y[2 * j] - hi.x, y[2 * j + 1] - hi.y);
+        for (int d = 0; d < PART; d += 8) {
+          uint32_t f[4], g[4];
+#pragma unroll
+          for (int j = 0; j < 4; j++) {
+            const float2 v = pair(d / 2 + j);
+            const float y0 = v.x * up, y1 = v.y * up;
+            f[j] = pack(y0, y1);
+            const float2 hi = unpack(f[j]);
+            g[j] = pack(y0 - hi.x, y1 - hi.y);
+          }
+          const uint32_t dst = base + C::OFF_Q + x * TERMS * C::Q_TILE + ((d0 + d) >> 6) * C::Q_PANEL + r * 128 +
+                               ((((d0 + d) >> 3) & 7) ^ (r & 7)) * 16;
+          sts128(dst, f[0], f[1], f[2], f[3]);
+          if (SPLIT) sts128(dst + C::Q_TILE, g[0], g[1], g[2], g[3]);
         }
-        const uint32_t dst = base + C::OFF_Q + x * TERMS * C::Q_TILE + (d >> 6) * C::Q_PANEL + r * 128 +
-                             (((d >> 3) & 7) ^ (r & 7)) * 16;
-        sts128(dst, f[0], f[1], f[2], f[3]);
-        if (SPLIT) sts128(dst + C::Q_TILE, g[0], g[1], g[2], g[3]);
       }
       fence_proxy_async();
       __syncwarp();
       if (lane == 0) bar_arrive(bar(B_Q));
 
-      const bool active = x == 0 || p.n_rows > TILE_ROWS;
-      const int pos = live ? p.s.len - p.s.n + tok : -1;
+      const int pos0 = piece.pos0, t0 = piece.t0, n_sink = piece.n_sink, skip = piece.skip;
+      const int pos = live ? pos0 + tok : -1;
+      const int low = a.window ? pos - a.window : -1;  // seen: low < key <= pos, or key < sinks
+      const int sinks = a.window ? a.sinks : 0;
       const int warp_row = x * TILE_ROWS + 32 * (warp & 3);  // rows of the warp: for the test whether to mask
-      const int min_pos = p.s.len - p.s.n + p.first_tok + warp_row / a.group;
-      const int max_pos = p.s.len - p.s.n + p.first_tok + (warp_row + 31) / a.group;
+      const int min_pos = pos0 + warp_row / a.group, max_pos = pos0 + (warp_row + 31) / a.group;
       float o[SPLIT ? HD : 1], ref = -INFINITY, l = 0.f, unit = 0.f;
       if constexpr (SPLIT) {
 #pragma unroll
         for (int d = 0; d < HD; d++) o[d] = 0.f;
       }
-      bool ok = true;
       auto add_output = [&]() {  // f32 rows: o += unit * O of the last block
         if constexpr (SPLIT) {
 #pragma unroll
@@ -632,37 +739,59 @@ __global__ void __launch_bounds__(THREADS, 1) k_paged_many(const AttnArgs<T> a) 
           }
         }
       };
-      for (int i = 0; i < p.n; i++, done++) {
-        if (!active) continue;
-        if (!(ok = wait_warp(B_SCALE + done % SCALE_STAGES, done / SCALE_STAGES))) break;
+      // The last turn (i = n) takes the last block's output.
+#pragma unroll 1
+      for (int i = 0; ok && active && i <= n && n; i++) {
+        if (i == n) {
+          ok = wait_warp(B_O + x, outs++);
+          fence_after();
+          if (ok) add_output();
+          break;
+        }
+        const Scales &sc = scales[(done + i) % SCALE_STAGES];
+        if (!(ok = wait_warp(B_SCALE + (done + i) % SCALE_STAGES, (done + i) / SCALE_STAGES))) break;
         if (!(ok = wait_warp(B_S + x, tile_done))) break;
         tile_done++;
         fence_after();
         if (SPLIT && i) add_output();
-        const Scales &sc = scales[done % SCALE_STAGES];
-        float s[BK];
-#pragma unroll
-        for (int k = 0; k < BK; k += 32) tmem_ld32(s_col + k, s + k);
-        tmem_ready<BK>(s);
-        const int key0 = p.block(p.t0 + i) * BK;
+        const int key0 = (t0 + i + (t0 + i < n_sink ? 0 : skip)) * BK;
         const uint32_t present = sc.present;
-        if (key0 + BK - 1 > min_pos || (a.window && key0 <= max_pos - a.window && key0 + BK > a.sinks) ||
-            (present & ((1u << NG) - 1)) != (1u << NG) - 1) {
-          const int low = a.window ? pos - a.window : -1;  // seen: low < key <= pos, or a sink
+        const bool hide = key0 + BK - 1 > min_pos || (a.window && key0 <= max_pos - a.window && key0 + BK > a.sinks) ||
+                          present != (1u << NG) - 1;
+        auto load64 = [&](int k0, float (&v)[64]) {  // scores of keys k0 .. k0 + 63 of the block
+          tmem_ld32(s_col + k0, v);
+          tmem_ld32(s_col + k0 + 32, v + 32);
+          tmem_ready<64>(v);
+          if (hide) {
+            const int q = key0 + k0;  // bits: keys q .. q + 63
+            auto upto = [&](int end) -> uint64_t {  // keys < end
+              const int m = min(max(end - q, 0), 64);
+              return m == 64 ? ~0ull : (1ull << m) - 1;
+            };
+            uint64_t see = upto(pos + 1) & (~upto(low + 1) | upto(sinks));
 #pragma unroll
-          for (int k = 0; k < BK; k++) {
-            const int key = key0 + k;
-            if (key > pos || (key <= low && key >= a.sinks) || !(present >> (k >> 4) & 1)) s[k] = -INFINITY;
+            for (int g = 0; g < 4; g++)
+              if (!(present >> (k0 / 16 + g) & 1)) see &= ~(0xffffull << (16 * g));
+            const uint32_t s0 = (uint32_t)see, s1 = (uint32_t)(see >> 32);
+#pragma unroll
+            for (int j = 0; j < 32; j++) {
+              v[j] = s0 >> j & 1 ? v[j] : -INFINITY;
+              v[32 + j] = s1 >> j & 1 ? v[32 + j] : -INFINITY;
+            }
           }
-        }
+        };
         float mx = -INFINITY;
+#pragma unroll 1
+        for (int k0 = 0; k0 < BK; k0 += 64) {
+          float v[64];
+          load64(k0, v);
 #pragma unroll
-        for (int g = 0; g < NG; g++) {
-          float m2[2] = {s[16 * g], s[16 * g + 1]};
+          for (int g = 0; g < 4; g++) {
+            float m1 = v[16 * g];
 #pragma unroll
-          for (int k = 2; k < 16; k++) m2[k & 1] = fmaxf(m2[k & 1], s[16 * g + k]);
-          const float m1 = fmaxf(m2[0], m2[1]);
-          mx = fmaxf(mx, m1 == -INFINITY ? m1 : m1 * (cf * sc.ks[g]));
+            for (int j = 1; j < 16; j++) m1 = fmaxf(m1, v[16 * g + j]);
+            mx = fmaxf(mx, m1 == -INFINITY ? m1 : m1 * (cf * sc.ks[k0 / 16 + g]));
+          }
         }
         // the reference follows the maximum, the unit the block's: earlier results move along
         float alpha = 1.f;
@@ -693,101 +822,96 @@ __global__ void __launch_bounds__(THREADS, 1) k_paged_many(const AttnArgs<T> a) 
           }
         }
         const float shift = ref == -INFINITY ? 0.f : WEIGHT_EXP - ref;
-        // weights into the columns that held the scores (this thread has read them all)
-        float sum[2] = {0.f, 0.f};
+        // weights, the first terms into columns whose scores this thread has read
+        float sum = 0.f;
+#pragma unroll 1
+        for (int k0 = 0; k0 < BK; k0 += 64) {
+          float v[64];
+          load64(k0, v);
+          uint32_t hi[32], lo[SPLIT ? 32 : 1];
 #pragma unroll
-        for (int g = 0; g < NG; g++) {
-          const float f = fmaxf(cf * sc.ks[g], FLT_MIN), share = sc.share[g];  // not 0: hidden scores are -infinity
-          uint32_t hi[8], lo[8];
-          if constexpr (SPLIT) {
-#pragma unroll
-            for (int k = 0; k < 8; k++) {
-              float u = ex2(fmaf(s[16 * g + 2 * k], f, shift)), v = ex2(fmaf(s[16 * g + 2 * k + 1], f, shift));
-              sum[0] += u;
-              sum[1] += v;
-              u *= share;
-              v *= share;
-              hi[k] = pack(u, v);
-              const float2 w = unpack(hi[k]);
-              lo[k] = pack(u - w.x, v - w.y);
-            }
-            tmem_st8(s_col + 8 * g, hi);
-            tmem_st8(s_col + BK / 2 + 8 * g, lo);
-          } else {
-            const float sh = shift + share;
+          for (int g = 0; g < 4; g++) {
+            const float f = fmaxf(cf * sc.ks[k0 / 16 + g], FLT_MIN);  // not 0: hidden scores are -infinity
+            const float share = sc.share[k0 / 16 + g], sh = SPLIT ? shift : shift + share;
             float gs[2] = {0.f, 0.f};
 #pragma unroll
-            for (int k = 0; k < 8; k++) {
-              const float u = ex2(fmaf(s[16 * g + 2 * k], f, sh)), v = ex2(fmaf(s[16 * g + 2 * k + 1], f, sh));
+            for (int j = 0; j < 8; j++) {
+              float u = ex2(fmaf(v[16 * g + 2 * j], f, sh)), w = ex2(fmaf(v[16 * g + 2 * j + 1], f, sh));
               gs[0] += u;
-              gs[1] += v;
-              hi[k] = pack(u, v);
+              gs[1] += w;
+              if constexpr (SPLIT) u *= share, w *= share;
+              hi[8 * g + j] = pack(u, w);
+              if constexpr (SPLIT) {
+                const float2 h2 = unpack(hi[8 * g + j]);
+                lo[8 * g + j] = pack(u - h2.x, w - h2.y);
+              }
             }
-            sum[0] = fmaf(gs[0] + gs[1], sc.inv[g], sum[0]);
-            tmem_st8(s_col + 8 * g, hi);
+            if constexpr (SPLIT) sum += gs[0] + gs[1];
+            else sum = fmaf(gs[0] + gs[1], sc.inv[k0 / 16 + g], sum);
           }
+          tmem_st32(s_col + k0 / 2, hi);
+          if constexpr (SPLIT) tmem_st32(tmem + lanes + tm_lo<C>(x) + k0 / 2, lo);
         }
-        l += sum[0] + sum[1];
+        l += sum;
         tmem_wait_st();
         fence_before();
         __syncwarp();
         if (lane == 0) bar_arrive(bar(B_P + x));
       }
-      // ---- the last block's output
-      if (ok && active && p.n) {
-        ok = wait_warp(B_O + x, outs);
-        outs++;
-        fence_after();
-        if (ok) add_output();
-      }
       if (!all_ok(ok)) break;
-      const bool none = !active || !p.n;  // nothing was computed: l = 0, O is not the tile's
-      T *dst = a.out + (long long)(p.s.first + tok) * a.os + h * HD;
+      done += n;
+      const bool none = !active || !n;  // nothing was computed: l = 0, O is not the tile's
+      const bool whole = piece.whole;
+      T *dst = a.out + (long long)(piece.row0 + tok) * a.os + h * HD;
+      float *slot = a.part + (size_t)piece.slot * C::SLOT + row;  // [head_dim][rows], maxima, sums
+      const float inv = l == 0.f ? 0.f : 1.f / l;
       auto write = [&](int d, const float *v) {  // 32 values
         if (!live) return;
 #pragma unroll
         for (int j = 0; j < 32; j += 4) store4(dst + d + j, make_float4(v[j], v[j + 1], v[j + 2], v[j + 3]));
       };
-      float *slot = a.part + (size_t)p.slot * C::SLOT;  // [head_dim][rows], maxima, sums
-      const float inv = l == 0.f ? 0.f : 1.f / l;
-#pragma unroll
-      for (int d = 0; d < HD; d += 32) {
-        float v[32];
-        if constexpr (SPLIT) {
-#pragma unroll
-          for (int j = 0; j < 32; j++) v[j] = o[d + j];
-        } else {
-          tmem_ld32(o_col + d, v);
-          tmem_ready<32>(v);
-#pragma unroll
-          for (int j = 0; j < 32; j++) v[j] = none ? 0.f : v[j] * unit;
-        }
-        if (p.whole) {
+      auto put = [&](int d, float *v) {
+        if (whole) {
 #pragma unroll
           for (int j = 0; j < 32; j++) v[j] = l == 0.f ? 0.f : v[j] * inv;
           write(d, v);
         } else {
 #pragma unroll
-          for (int j = 0; j < 32; j++) slot[(d + j) * ROWS + row] = v[j];
+          for (int j = 0; j < 32; j++) slot[(d + j) * ROWS] = v[j];
+        }
+      };
+      if constexpr (SPLIT) {
+#pragma unroll
+        for (int d = 0; d < HD; d += 32) put(d, o + d);
+      } else {
+#pragma unroll 1
+        for (int d = 0; d < HD; d += 32) {
+          float v[32];
+          tmem_ld32(o_col + d, v);
+          tmem_ready<32>(v);
+#pragma unroll
+          for (int j = 0; j < 32; j++) v[j] = none ? 0.f : v[j] * unit;
+          put(d, v);
         }
       }
-      if (!p.whole) {  // the last block to arrive joins all parts, in block order
-        slot[HD * ROWS + row] = ref;
-        slot[(HD + 1) * ROWS + row] = l;
-        int *count = a.count + ((long long)p.b * c.kv_heads + p.head) * a.max_row_tiles + p.rt;
-        const int parts = p.parts;
+      if (!whole) {  // the last block to arrive joins all parts, in block order
+        slot[HD * ROWS] = ref;
+        slot[(HD + 1) * ROWS] = l;
+        int *count = a.count + piece.counter;
+        const int parts = piece.parts, first = piece.first, late = piece.late;
         __threadfence();
         all_ok(true);
         if (tid == 0) s_last = atomicAdd(count, 1) == parts - 1;
         all_ok(true);
         if (s_last) {
           __threadfence();
-          auto part = [&](int i) {
-            return a.part + (size_t)(2 * (p.first + i) + (i == 0 && p.late ? 1 : 0)) * C::SLOT + row;
-          };
-          float top = -INFINITY, sum = 0.f;
+          auto part = [&](int i) { return a.part + (size_t)(2 * (first + i) + (i == 0 ? late : 0)) * C::SLOT + row; };
+          top = -INFINITY;
+          float sum = 0.f;
+#pragma unroll 1
           for (int i = 0; i < parts; i++) top = fmaxf(top, __ldcg(part(i) + HD * ROWS));
           const float at0 = top == -INFINITY ? 0.f : top;
+#pragma unroll 1
           for (int i = 0; i < parts; i++)
             sum = fmaf(__ldcg(part(i) + (HD + 1) * ROWS), ex2(__ldcg(part(i) + HD * ROWS) - at0), sum);
           const float all_inv = sum == 0.f ? 0.f : 1.f / sum;
@@ -796,11 +920,12 @@ __global__ void __launch_bounds__(THREADS, 1) k_paged_many(const AttnArgs<T> a) 
             float v[32];
 #pragma unroll
             for (int j = 0; j < 32; j++) v[j] = 0.f;
+#pragma unroll 1
             for (int i = 0; i < parts; i++) {
-              const float *x0 = part(i);
-              const float f = ex2(__ldcg(x0 + HD * ROWS) - at0);
+              const float *src = part(i);
+              const float f = ex2(__ldcg(src + HD * ROWS) - at0);
 #pragma unroll
-              for (int j = 0; j < 32; j++) v[j] = fmaf(__ldcg(x0 + (d + j) * ROWS), f, v[j]);
+              for (int j = 0; j < 32; j++) v[j] = fmaf(__ldcg(src + (d + j) * ROWS), f, v[j]);
             }
 #pragma unroll
             for (int j = 0; j < 32; j++) v[j] = sum == 0.f ? 0.f : v[j] * all_inv;
@@ -809,11 +934,13 @@ __global__ void __launch_bounds__(THREADS, 1) k_paged_many(const AttnArgs<T> a) 
           if (tid == 0) *count = 0;
         }
       }
+      __syncwarp();
+      if (lane == 0) bar_arrive(bar(B_DONE));
     }
   }
   fence_before();
   __syncthreads();
-  if (warp == WARPS - 1) {
+  if (warp == MMA_WARP) {
     fence_after();
     tmem_dealloc(tmem, TM_COLS);
   }
