@@ -146,6 +146,31 @@ __device__ __forceinline__ void tmem_st32(uint32_t a, const uint32_t *r) {
       "r"(r[28]), "r"(r[29]), "r"(r[30]), "r"(r[31])
       : "memory");
 }
+__device__ __forceinline__ bool elect_one() {
+  uint32_t r;
+  asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.u32 %0, 1, 0, p;\n\t}" : "=r"(r));
+  return r != 0;
+}
+// D[tmem] (+)= A B with A from shared memory, or from tensor memory (_ts).
+__device__ __forceinline__ void mma_f16(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, bool add) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
+      "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(d),
+      "l"(a), "l"(b), "r"(idesc), "r"((uint32_t)add)
+      : "memory");
+}
+__device__ __forceinline__ void mma_f16_ts(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, bool add) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
+      "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}" ::"r"(d),
+      "r"(a), "l"(b), "r"(idesc), "r"((uint32_t)add)
+      : "memory");
+}
+__device__ __forceinline__ float max3(float a, float b, float c) {
+  float d;
+  asm("max.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
+  return d;
+}
 // Orders the uses of N loaded registers after the wait for them.
 template <int N>
 __device__ __forceinline__ void tmem_ready(float *v) {
@@ -402,6 +427,9 @@ __global__ void __launch_bounds__(THREADS, 1) k_paged_many(const AttnArgs<T> a) 
     }
     return true;
   };
+  auto wait_all = [&](int i, unsigned phase) -> bool {  // every lane waits; the warp goes on together
+    return __all_sync(0xffffffffu, wait(i, phase));
+  };
   auto wait_warp = [&](int i, unsigned phase) -> bool {  // lane 0 waits, the warp follows
     int ok = 1;
     if (lane == 0) ok = wait(i, phase);
@@ -429,73 +457,81 @@ __global__ void __launch_bounds__(THREADS, 1) k_paged_many(const AttnArgs<T> a) 
       }
     } else if (warp == MMA_WARP) {
       // ---------------- products ----------------
-      if (lane == 0) {
-        unsigned done = 0, tile_done[2] = {0, 0};
-        bool ok = true;
+      // The whole warp walks the loop, so that addresses and descriptors are uniform values; one elected thread
+      // issues (with a single thread in the loop each product took 100 to 150 clocks to issue, twice its own time).
+      const bool leader = elect_one();
+      const uint32_t tm = __shfl_sync(0xffffffffu, tmem, 0);
+      auto commit = [&](int i) {
+        if (leader) mma_commit(bar(i));
+      };
+      unsigned done = 0, tile_done[2] = {0, 0};
+      bool ok = true;
 #pragma unroll 1
-        for (unsigned k = 0; ok; k++) {
-          if (!(ok = wait(B_PIECE + k % PIECES, k / PIECES))) break;
-          const int n = s_pieces[k % PIECES].n, tiles = s_pieces[k % PIECES].n_rows > TILE_ROWS ? 2 : 1;
-          if (n < 0) break;
-          // An operand's place is the low bits of its descriptor, in units of 16 bytes: every one is a base and a sum.
-          const uint64_t qd = sw128_desc(base + C::OFF_Q), kd = sw128_desc(base + C::OFF_K);
-          const uint64_t vd = mn_desc(base + C::OFF_V, C::KV_PANEL);
-          auto scores = [&](int x, int st) {
-            const uint64_t q = qd + (uint32_t)(x * (TERMS * C::Q_TILE >> 4)), k = kd + (uint32_t)(st * (C::KV_TILE >> 4));
-            const uint32_t d = tmem + x * BK;
+      for (unsigned k = 0; ok; k++) {
+        if (!(ok = wait_all(B_PIECE + k % PIECES, k / PIECES))) break;
+        const int n = __shfl_sync(0xffffffffu, s_pieces[k % PIECES].n, 0);
+        const int tiles = __shfl_sync(0xffffffffu, s_pieces[k % PIECES].n_rows, 0) > TILE_ROWS ? 2 : 1;
+        if (n < 0) break;
+        // An operand's place is the low bits of its descriptor, in units of 16 bytes: every one is a base and a sum.
+        const uint64_t qd = sw128_desc(base + C::OFF_Q), kd = sw128_desc(base + C::OFF_K);
+        const uint64_t vd = mn_desc(base + C::OFF_V, C::KV_PANEL);
+        auto scores = [&](int x, int st) {
+          const uint64_t q = qd + (uint32_t)(x * (TERMS * C::Q_TILE >> 4)), kk = kd + (uint32_t)(st * (C::KV_TILE >> 4));
+          const uint32_t d = tm + x * BK;
+          if (leader) {
 #pragma unroll
             for (int t = 0; t < TERMS; t++)
 #pragma unroll
               for (int i = 0; i < HD / 16; i++)
-                mma_bf16(d, q + ((t * C::Q_TILE + (i >> 2) * C::Q_PANEL + (i & 3) * 32) >> 4),
-                         k + (((i >> 2) * C::KV_PANEL + (i & 3) * 32) >> 4), idesc_f16(TILE_ROWS, BK, false),
-                         t || i ? 1u : 0u);
+                mma_f16(d, q + ((t * C::Q_TILE + (i >> 2) * C::Q_PANEL + (i & 3) * 32) >> 4),
+                        kk + (((i >> 2) * C::KV_PANEL + (i & 3) * 32) >> 4), idesc_f16(TILE_ROWS, BK, false), t || i);
             mma_commit(bar(B_S + x));
-          };
-          auto output = [&](int x, int st, bool first) {
-            const uint64_t v = vd + (uint32_t)(st * (C::KV_TILE >> 4));
-            const uint32_t d = tmem + TM_O + x * 128, hi = tmem + x * BK, lo = tmem + tm_lo<C>(x);
+          }
+        };
+        auto output = [&](int x, int st, bool add) {
+          const uint64_t v = vd + (uint32_t)(st * (C::KV_TILE >> 4));
+          const uint32_t d = tm + TM_O + x * 128, hi = tm + x * BK, lo = tm + tm_lo<C>(x);
+          if (leader) {
 #pragma unroll
             for (int t = 0; t < TERMS; t++)
 #pragma unroll
               for (int i = 0; i < BK / 16; i++)
-                mma_bf16_ts(d, (t ? lo : hi) + i * 8, v + (i * 2048 >> 4), idesc_f16(TILE_ROWS, HD, true),
-                            t || i ? 1u : (SPLIT || first ? 0u : 1u));
-          };
-          ok = wait(B_Q, k);
-#pragma unroll 1
-          for (int i = 0; ok && i < n; i++, done++) {
-            const int st = done % STAGES, st1 = (done + 1) % STAGES;
-#pragma unroll 1
-            for (int x = i ? 0 : -tiles; x < tiles; x++) {  // the piece's first scores, then each tile's turn
-              if (x < 0) {
-                if (x == -tiles && !(ok = wait(B_K + st, done / STAGES))) break;
-                fence_after();
-                scores(x + tiles, st);
-                if (x == -1) mma_commit(bar(B_K_FREE + st));
-                continue;
-              }
-              if (!(ok = wait(B_P + x, x ? tile_done[1]++ : tile_done[0]++))) break;
-              if (x == 0 && !(ok = wait(B_V + st, done / STAGES))) break;
-              fence_after();
-              output(x, st, i == 0);
-              if (i + 1 < n) {
-                if (x == 0 && !(ok = wait(B_K + st1, (done + 1) / STAGES))) break;
-                fence_after();
-                scores(x, st1);
-              } else {
-                mma_commit(bar(B_O + x));
-              }
-            }
-            if (!ok) break;
-            mma_commit(bar(B_V_FREE + st));
-            if (i + 1 < n) mma_commit(bar(B_K_FREE + st1));
+                mma_f16_ts(d, (t ? lo : hi) + i * 8, v + (i * 2048 >> 4), idesc_f16(TILE_ROWS, HD, true), t || i || add);
           }
+        };
+        if (!(ok = wait_all(B_Q, k))) break;
+#pragma unroll 1
+        for (int i = 0; ok && i < n; i++, done++) {
+          const int st = done % STAGES, st1 = (done + 1) % STAGES;
+#pragma unroll 1
+          for (int x = i ? 0 : -tiles; x < tiles; x++) {  // the piece's first scores, then each tile's turn
+            if (x < 0) {
+              if (x == -tiles && !(ok = wait_all(B_K + st, done / STAGES))) break;
+              fence_after();
+              scores(x + tiles, st);
+              if (x == -1) commit(B_K_FREE + st);
+              continue;
+            }
+            if (!(ok = wait_all(B_P + x, x ? tile_done[1]++ : tile_done[0]++))) break;
+            if (x == 0 && !(ok = wait_all(B_V + st, done / STAGES))) break;
+            fence_after();
+            output(x, st, !SPLIT && i);
+            if (i + 1 < n) {
+              if (x == 0 && !(ok = wait_all(B_K + st1, (done + 1) / STAGES))) break;
+              fence_after();
+              scores(x, st1);
+            } else {
+              commit(B_O + x);
+            }
+          }
+          if (!ok) break;
+          commit(B_V_FREE + st);
+          if (i + 1 < n) commit(B_K_FREE + st1);
         }
-        // every product done before the columns are freed
-        mma_commit(bar(B_FIN));
-        bar_drain(bar(B_FIN), 0u);
       }
+      // every product done before the columns are freed
+      commit(B_FIN);
+      bar_drain(bar(B_FIN), 0u);
       __syncwarp();
     }
   } else if (warp >= SOFTMAX_WARPS) {
@@ -542,16 +578,18 @@ __global__ void __launch_bounds__(THREADS, 1) k_paged_many(const AttnArgs<T> a) 
         }
         return g;
       };
-      auto fetch = [&](int i, int page, const uint8_t *codes, int which) {
-        if (i < p.n) {
-          const int key0 = p.block(i) * BK + (r0 & 15);
+      // Place of lane's group in the codes, in groups of 16 keys (-1: none).
+      auto place_of = [&](int i, int page) {
+        const int key = p.block(i) * BK + 16 * lane;
+        return page < 0 ? -1 : ((page * c.kv_heads + p.head) << (c.page_shift - 4)) + ((key & (c.page - 1)) >> 4);
+      };
+      auto fetch = [&](bool any, int place, const uint8_t *codes, int which) {
+        if (any) {
+          const uint8_t *mine = codes + (r0 & 15) * HD + ch * 16;
 #pragma unroll
           for (int k = 0; k < C::STEPS; k++) {
-            const int g = k * STEP_GROUPS + my_group, pg = __shfl_sync(0xffffffffu, page, g);
-            if (pg >= 0) {
-              const long long at = (((long long)pg * c.kv_heads + p.head) * c.page + ((key0 + 16 * g) & (c.page - 1))) * HD;
-              cp16(raw + which * C::RAW + k * (LOADERS * 16), codes + at + ch * 16);
-            }
+            const int at = __shfl_sync(0xffffffffu, place, k * STEP_GROUPS + my_group);
+            if (at >= 0) cp16(raw + which * C::RAW + k * (LOADERS * 16), mine + (long long)at * (16 * HD));
           }
         }
         cp_commit();
@@ -580,8 +618,8 @@ __global__ void __launch_bounds__(THREADS, 1) k_paged_many(const AttnArgs<T> a) 
       float unit = 0.f;
       int later = entry_of(1);
       Group now = scales_of(checked(entry_of(0)));
-      fetch(0, now.page, c.k, 0);
-      fetch(0, now.page, c.v, 1);
+#pragma unroll 1
+      for (int v = 0; v < 2; v++) fetch(p.n > 0, place_of(0, now.page), v ? c.v : c.k, v);
       Group next = scales_of(checked(later));
       later = entry_of(2);
 #pragma unroll 1
@@ -594,6 +632,7 @@ __global__ void __launch_bounds__(THREADS, 1) k_paged_many(const AttnArgs<T> a) 
         for (int o = 1; o < NG; o <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
         top = __shfl_sync(0xffffffffu, top, 0);
         if (SPLIT || top > unit * UNIT_LAG || unit == 0.f) unit = top;
+        const int place = place_of(i + 1, next.page);
 #pragma unroll 1
         for (int v = 0; v < 2; v++) {  // K, then V
           if (done >= STAGES && !(ok = wait_warp((v ? B_V_FREE : B_K_FREE) + st, done / STAGES - 1))) break;
@@ -623,7 +662,7 @@ __global__ void __launch_bounds__(THREADS, 1) k_paged_many(const AttnArgs<T> a) 
           fence_proxy_async();  // before the next copies: it would wait for them
           __syncwarp();
           if (lane == 0) bar_arrive(bar((v ? B_V : B_K) + st));
-          fetch(i + 1, next.page, v ? c.v : c.k, v);
+          fetch(i + 1 < p.n, place, v ? c.v : c.k, v);
         }
         now = next;
         next = scales_of(checked(later));
@@ -787,9 +826,13 @@ __global__ void __launch_bounds__(THREADS, 1) k_paged_many(const AttnArgs<T> a) 
           load64(k0, v);
 #pragma unroll
           for (int g = 0; g < 4; g++) {
-            float m1 = v[16 * g];
+            float m1 = fmaxf(v[16 * g], v[16 * g + 1]), m2 = fmaxf(v[16 * g + 2], v[16 * g + 3]);
 #pragma unroll
-            for (int j = 1; j < 16; j++) m1 = fmaxf(m1, v[16 * g + j]);
+            for (int j = 4; j < 16; j += 4) {
+              m1 = max3(m1, v[16 * g + j], v[16 * g + j + 1]);
+              m2 = max3(m2, v[16 * g + j + 2], v[16 * g + j + 3]);
+            }
+            m1 = fmaxf(m1, m2);
             mx = fmaxf(mx, m1 == -INFINITY ? m1 : m1 * (cf * sc.ks[k0 / 16 + g]));
           }
         }
@@ -833,21 +876,24 @@ __global__ void __launch_bounds__(THREADS, 1) k_paged_many(const AttnArgs<T> a) 
           for (int g = 0; g < 4; g++) {
             const float f = fmaxf(cf * sc.ks[k0 / 16 + g], FLT_MIN);  // not 0: hidden scores are -infinity
             const float share = sc.share[k0 / 16 + g], sh = SPLIT ? shift : shift + share;
-            float gs[2] = {0.f, 0.f};
+            const f2x f2 = pk2(f, f), sh2 = pk2(sh, sh), share2 = pk2(share, share);
+            f2x gs = 0ull;
 #pragma unroll
             for (int j = 0; j < 8; j++) {
-              float u = ex2(fmaf(v[16 * g + 2 * j], f, sh)), w = ex2(fmaf(v[16 * g + 2 * j + 1], f, sh));
-              gs[0] += u;
-              gs[1] += w;
-              if constexpr (SPLIT) u *= share, w *= share;
-              hi[8 * g + j] = pack(u, w);
+              const float2 y = up2(ffma2(pk2(v[16 * g + 2 * j], v[16 * g + 2 * j + 1]), f2, sh2));
+              f2x w = pk2(ex2(y.x), ex2(y.y));
+              gs = fadd2(gs, w);
+              if constexpr (SPLIT) w = fmul2(w, share2);
+              const float2 z = up2(w);
+              hi[8 * g + j] = pack(z.x, z.y);
               if constexpr (SPLIT) {
                 const float2 h2 = unpack(hi[8 * g + j]);
-                lo[8 * g + j] = pack(u - h2.x, w - h2.y);
+                lo[8 * g + j] = pack(z.x - h2.x, z.y - h2.y);
               }
             }
-            if constexpr (SPLIT) sum += gs[0] + gs[1];
-            else sum = fmaf(gs[0] + gs[1], sc.inv[k0 / 16 + g], sum);
+            const float2 z = up2(gs);
+            if constexpr (SPLIT) sum += z.x + z.y;
+            else sum = fmaf(z.x + z.y, sc.inv[k0 / 16 + g], sum);
           }
           tmem_st32(s_col + k0 / 2, hi);
           if constexpr (SPLIT) tmem_st32(tmem + lanes + tm_lo<C>(x) + k0 / 2, lo);
