@@ -685,7 +685,11 @@ extern "C" int sq_paged_attention(void *stream, const sq_paged_cache *cache, con
   if (dtype != SQ_F32 && dtype != SQ_BF16)
     return fail(SQ_ERR_INVALID_TYPE, "paged_attention: rows must be F32 or BF16");
   if (window < 0 || sinks < 0) return fail(SQ_ERR_SHAPE, "paged_attention: negative window or sinks");
-  if ((long long)b.n_tokens * n_heads > INT32_MAX) return fail(SQ_ERR_SHAPE, "paged_attention: too many query rows");
+  {  // both kernels number the (row tile, key tile) pairs of a call in 31 bits: row tiles of 4 rows, key tiles of 16
+    const double rows = (double)b.n_tokens * n_heads / 4 + (double)b.n_seqs * c.kv_heads;
+    if (rows * ((double)b.table_row * c.page / 16 + 16) >= INT32_MAX / 2.0)
+      return fail(SQ_ERR_SHAPE, "paged_attention: too many query rows for so long a page table in one call");
+  }
   if (!b.n_tokens) return SQ_OK;
   const long long width = (long long)n_heads * c.hd;
   st = paged::check_rows(q, q_stride, width, dtype, "paged_attention: q");

@@ -3,23 +3,22 @@
 // 64 and 128.
 //
 // A block works on 256 query rows of one kv head (row = token * group + head of the
-// group), two tiles X of 128 that share every key block, so that a code is converted once
-// for 256 rows:
+// group), two tiles X of 128 that share every block of 64 keys, so that a code is
+// converted once for 256 rows:
 //   warps 8-11  codes of a block of keys to shared memory (cp.async, each thread its own
 //               chunks), converted to f16 (exact: whole numbers up to 127) into the
-//               128-byte swizzled tiles of K [keys][dims] and V [keys][dims]; two stages
-//   warp 12     one thread issues the products, f32 sums in tensor memory:
+//               128-byte swizzled tiles of K [keys][dims] and V [keys][dims]
+//   warp 12     issues the products, f32 sums in tensor memory:
 //               S_X = Q_X K^T (K-major operands), O_X (+)= P_X V (V read MN-major as it
-//               lies, P from tensor memory). Order: P V of one tile, its next S, then the
-//               other tile: one tile's softmax runs under the other's products
-//   warp 13     walks this block's share of the work and hands it out piece by piece
+//               lies, P from tensor memory). A tile's scores have two buffers: those of
+//               block j + 2 are issued right after P V of block j, so the softmax finds
+//               the next block's scores ready
+//   warp 13     walks this block's share of the work, handed out piece by piece
+//   warp 14     looks up pages and scales, eight blocks of keys at a time
 //   warps 0-7   one thread a row (= tensor-memory lane): running maximum of its scores,
-//               weights over the columns the scores leave, sum. The scores are read twice
-//               from tensor memory, 64 at a time in a rolled loop: with 128 held and the
-//               loops unrolled the kernel was 200 KB of code, and every role spent its
-//               time waiting for instructions (2,048-token chunk: 412 us)
-// Products issued by one thread complete in order, so a tile's S being done says that its
-// last P V is done too: no further barriers between them.
+//               weights over the columns the scores leave, sum
+// Loops are rolled where registers allow: with blocks of 128 keys in unrolled code (200
+// KB) every role spent its time waiting for instructions.
 //
 // Precision, as in the few-row kernel: query rows scaled by powers of two, two f16 terms
 // for f32 rows, one (exact) for bf16 rows. Weights are 2^(s - ref + 3); ref follows the
@@ -36,7 +35,6 @@
 // copies finish, frees its tensor memory and returns.
 #include <cuda.h>
 #include <float.h>
-#include <limits.h>
 
 #include "paged_attention.cuh"
 #include "tc.cuh"
@@ -48,10 +46,10 @@ namespace {
 using namespace tc;
 
 constexpr int SOFTMAX_WARPS = 8, LOAD_WARPS = 4, MMA_WARP = SOFTMAX_WARPS + LOAD_WARPS;
-constexpr int WARPS = 16;  // whole warpgroups: registers are shared out by them (warps 13-15 only take part in barriers)
+constexpr int WARPS = 16;  // whole warpgroups: registers are shared out by them (warp 15 only takes part in barriers)
 constexpr int THREADS = WARPS * 32, LOADERS = LOAD_WARPS * 32;
 constexpr int TILE_ROWS = 128, ROWS = 2 * TILE_ROWS;
-constexpr int STAGES = 2, SCALE_STAGES = 4;
+constexpr int BATCH = 8, BATCHES = 2;  // blocks of keys looked up at once, and how many such batches are held
 constexpr int MAX_BLOCKS = 160;
 constexpr int MIN_BLOCKS = 2;  // key blocks a thread block takes at least
 constexpr float WEIGHT_EXP = 3.f, REF_LAG = 6.f, UNIT_LAG = 64.f;
@@ -63,7 +61,8 @@ struct Cfg {
   static constexpr int HD = HD_;
   static constexpr bool SPLIT = sizeof(T) == 4;
   static constexpr int TERMS = SPLIT ? 2 : 1;
-  static constexpr int BK = SPLIT && HD == 128 ? 64 : 128;  // keys a block; 64: two stages fit beside Q's two terms
+  static constexpr int BK = 64;                             // keys a block
+  static constexpr int STAGES = SPLIT && HD == 128 ? 2 : 4;  // of K and V each
   static constexpr int NG = BK / 16;                        // groups of 16 keys: each within one page
   static constexpr int PANELS = HD / 64;                    // 64 dimensions = 128 bytes of f16
   static constexpr int Q_PANEL = TILE_ROWS * 128, KV_PANEL = BK * 128;
@@ -74,42 +73,44 @@ struct Cfg {
   static constexpr int RAW = BK * HD;
   static constexpr int OFF_Q = 0, OFF_K = OFF_Q + 2 * TERMS * Q_TILE, OFF_V = OFF_K + STAGES * KV_TILE,
                        OFF_RAW = OFF_V + STAGES * KV_TILE, OFF_SCALE = OFF_RAW + 2 * RAW,
-                       OFF_BAR = OFF_SCALE + SCALE_STAGES * 4 * 8 * 4;
-  static constexpr int SMEM = 1024 + OFF_BAR + 256;
+                       OFF_BAR = OFF_SCALE + BATCHES * BATCH * 96;
+  static constexpr int SMEM = 1024 + OFF_BAR + 320;
   static constexpr int SLOT = ROWS * (HD + 2);  // floats of a cut row tile's partial result
   static_assert(SMEM <= 232448 - 256, "shared memory of a block");
 };
 
-// A block's scales, read by the softmax threads: [group] K scale, V share, 1 / V share
-// (bf16: log2 of the share), and in the last row: bit mask of present groups, unit.
-struct Scales {
-  float ks[8], share[8], inv[8];
-  uint32_t present;
+// What is looked up for a block of 64 keys: of its four groups of 16 the place in the
+// codes (in groups of 16 keys; -1: none), the K scale, the V scale relative to the unit
+// (f32 rows: the ratio; bf16 rows: its log2, and 1 / ratio).
+struct Plan {
+  int place[4];
+  float ks[4], share[4], inv[4];
+  uint32_t present, with_v;  // bit masks of groups: there at all; with a V scale that is not 0
   float unit;
-  float pad[6];
+  float pad[5];
 };
-static_assert(sizeof(Scales) == 128, "four rows of eight words");
+static_assert(sizeof(Plan) == 96, "room in shared memory");
 
+constexpr int MAX_STAGES = 4;
 enum : int {
-  B_Q = 0,       // both tiles' queries written
-  B_K = 1,       // [2] a stage's K written
-  B_K_FREE = 3,  // [2] S of both tiles done
-  B_V = 5,       // [2]
-  B_V_FREE = 7,  // [2]
-  B_SCALE = 9,   // [4] a block's scales written
-  B_S = 13,      // [2 tiles] scores done (and the tile's last P V)
-  B_P = 15,      // [2 tiles] weights written
-  B_O = 17,      // [2 tiles] the piece's last P V done
-  B_FIN = 19,
-  B_PIECE = 20,  // [4] a piece handed out
-  B_DONE = 24,   // a piece's rows written
-  N_BARS = 25
+  B_Q = 0,        // both tiles' queries written
+  B_K = 1,        // [stages] K written
+  B_K_FREE = 5,   // [stages] scores of both tiles done
+  B_V = 9,        // [stages]
+  B_V_FREE = 13,  // [stages]
+  B_S = 17,       // [2 tiles][2 buffers] scores done
+  B_P = 21,       // [2 tiles][2 buffers] weights written
+  B_PV = 25,      // [2 tiles] a block's P V done
+  B_PIECE = 27,   // [4] a piece handed out
+  B_DONE = 31,    // a piece's rows written
+  B_PLAN = 32,    // [2] a batch of blocks looked up
+  B_PLAN_FREE = 34,
+  B_FIN = 36,
+  N_BARS = 37
 };
-// Columns of tile X: S at X * BK, the first terms of P over its first half; O at 256 + 128 X;
-// second terms of P at 320 + 128 X (head_dim 64) or 128 + 64 X.
+// Columns: S, and P over it, of tile X and buffer B at 128 X + 64 B (P: first terms in 32, second terms
+// in the next 32); O at 256 + 128 X.
 constexpr uint32_t TM_O = 256, TM_COLS = 512;
-template <class C>
-__host__ __device__ constexpr uint32_t tm_lo(int x) { return C::HD == 64 ? 320 + 128 * x : 128 + 64 * x; }
 
 // f16 operands, f32 sums; B K-major or (bit 16) MN-major.
 constexpr uint32_t idesc_f16(int M, int N, bool b_mn) {
@@ -170,6 +171,10 @@ __device__ __forceinline__ float max3(float a, float b, float c) {
   float d;
   asm("max.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
   return d;
+}
+__device__ __forceinline__ uint32_t bf16_pair(float a, float b) {
+  const __nv_bfloat162 x = __floats2bfloat162_rn(a, b);
+  return *reinterpret_cast<const uint32_t *>(&x);
 }
 // Orders the uses of N loaded registers after the wait for them.
 template <int N>
@@ -338,7 +343,8 @@ __global__ void __launch_bounds__(THREADS, 1) k_paged_many(const AttnArgs<T> a) 
   __shared__ Piece s_pieces[PIECES];
   const uint32_t base = (smem_addr(smem_raw) + 1023u) & ~1023u;
   uint8_t *gen = smem_raw + (base - smem_addr(smem_raw));
-  Scales *scales = reinterpret_cast<Scales *>(gen + C::OFF_SCALE);
+  Plan *plans = reinterpret_cast<Plan *>(gen + C::OFF_SCALE);  // [batch][block]
+  constexpr int STAGES = C::STAGES;
   auto bar = [&](int i) { return base + C::OFF_BAR + 8u * (uint32_t)i; };
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const Cache &c = a.c;
@@ -395,11 +401,10 @@ __global__ void __launch_bounds__(THREADS, 1) k_paged_many(const AttnArgs<T> a) 
 
   if (tid == 0) {
     for (int i = 0; i < N_BARS; i++) {
-      const unsigned count = i == B_Q || i == B_DONE           ? SOFTMAX_WARPS
-                             : i >= B_P && i < B_P + 2         ? SOFTMAX_WARPS / 2
-                             : i >= B_K && i < B_K + 2         ? LOAD_WARPS
-                             : i >= B_V && i < B_V + 2         ? LOAD_WARPS
-                                                               : 1;
+      const unsigned count = i == B_Q || i == B_DONE                                         ? SOFTMAX_WARPS
+                             : i >= B_P && i < B_P + 4                                       ? SOFTMAX_WARPS / 2
+                             : (i >= B_K && i < B_K + MAX_STAGES) || (i >= B_V && i < B_V + MAX_STAGES) ? LOAD_WARPS
+                                                                                             : 1;
       bar_init(bar(i), count);
     }
     s_abort = 0;
@@ -455,6 +460,62 @@ __global__ void __launch_bounds__(THREADS, 1) k_paged_many(const AttnArgs<T> a) 
         }
         __syncwarp();
       }
+    } else if (warp == MMA_WARP + 2) {
+      // ---------------- pages and scales ----------------
+      unsigned batch = 0;
+      bool ok = true;
+#pragma unroll 1
+      for (unsigned k = 0; ok; k++) {
+        if (!(ok = wait_warp(B_PIECE + k % PIECES, k / PIECES))) break;
+        const Piece p = s_pieces[k % PIECES];
+        if (p.n < 0) break;
+        float unit = 0.f;
+        const int j = lane & 3;  // lane: group j of block i
+#pragma unroll 1
+        for (int i0 = 0; i0 < p.n; i0 += BATCH, batch++) {
+          const int i = i0 + (lane >> 2), key = p.block(i) * BK + 16 * j;
+          const bool in = i < p.n;
+          int page = -1;
+          if (in && key < p.len) page = load_page(a.b, c, p.b, key);
+          float ks = 0.f, vs = 0.f;
+          if (page >= 0) {
+            ks = c.ks[(long long)page * c.kv_heads + p.head];
+            vs = c.vs[(long long)page * c.kv_heads + p.head];
+          }
+          float top = fmaxf(vs, __shfl_xor_sync(0xffffffffu, vs, 1));
+          top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
+          float my_unit = top;
+          if (!SPLIT) {  // outputs stay in the unit of the first block until a much larger scale comes
+#pragma unroll 1
+            for (int q = 0; q < BATCH; q++) {
+              const float t = __shfl_sync(0xffffffffu, top, 4 * q);
+              if (t > unit * UNIT_LAG || unit == 0.f) unit = t;
+              if (lane >> 2 == q) my_unit = unit;
+            }
+          }
+          const uint32_t present = __ballot_sync(0xffffffffu, page >= 0) >> (lane & 28) & 15;
+          const uint32_t with_v = __ballot_sync(0xffffffffu, vs > 0.f) >> (lane & 28) & 15;
+          if (batch >= BATCHES && !(ok = wait_warp(B_PLAN_FREE + batch % BATCHES, batch / BATCHES - 1))) break;
+          Plan &plan = plans[batch % BATCHES * BATCH + (lane >> 2)];
+          const float share = vs > 0.f ? vs / my_unit : 0.f;
+          plan.place[j] = page < 0 ? -1 : ((page * c.kv_heads + p.head) << (c.page_shift - 4)) + ((key & (c.page - 1)) >> 4);
+          plan.ks[j] = ks;
+          if (SPLIT) {
+            plan.share[j] = share;
+          } else {  // as an exponent; below 2^-100 of the unit: as good as none
+            const float e = share > 0.f ? fmaxf(log2f(share), -100.f) : 0.f;
+            plan.share[j] = e;
+            plan.inv[j] = share > 0.f ? exp2f(-e) : 1.f;
+          }
+          if (j == 0) {
+            plan.present = present;
+            plan.with_v = with_v;
+            plan.unit = my_unit;
+          }
+          __syncwarp();
+          if (lane == 0) bar_arrive(bar(B_PLAN + batch % BATCHES));
+        }
+      }
     } else if (warp == MMA_WARP) {
       // ---------------- products ----------------
       // The whole warp walks the loop, so that addresses and descriptors are uniform values; one elected thread
@@ -464,7 +525,7 @@ __global__ void __launch_bounds__(THREADS, 1) k_paged_many(const AttnArgs<T> a) 
       auto commit = [&](int i) {
         if (leader) mma_commit(bar(i));
       };
-      unsigned done = 0, tile_done[2] = {0, 0};
+      unsigned done = 0, batch = 0, tile_done[2] = {0, 0};  // blocks in all, batches, blocks of each tile
       bool ok = true;
 #pragma unroll 1
       for (unsigned k = 0; ok; k++) {
@@ -475,9 +536,9 @@ __global__ void __launch_bounds__(THREADS, 1) k_paged_many(const AttnArgs<T> a) 
         // An operand's place is the low bits of its descriptor, in units of 16 bytes: every one is a base and a sum.
         const uint64_t qd = sw128_desc(base + C::OFF_Q), kd = sw128_desc(base + C::OFF_K);
         const uint64_t vd = mn_desc(base + C::OFF_V, C::KV_PANEL);
-        auto scores = [&](int x, int st) {
+        auto scores = [&](int x, int buf, int st) {
           const uint64_t q = qd + (uint32_t)(x * (TERMS * C::Q_TILE >> 4)), kk = kd + (uint32_t)(st * (C::KV_TILE >> 4));
-          const uint32_t d = tm + x * BK;
+          const uint32_t d = tm + x * 128 + buf * 64;
           if (leader) {
 #pragma unroll
             for (int t = 0; t < TERMS; t++)
@@ -485,49 +546,54 @@ __global__ void __launch_bounds__(THREADS, 1) k_paged_many(const AttnArgs<T> a) 
               for (int i = 0; i < HD / 16; i++)
                 mma_f16(d, q + ((t * C::Q_TILE + (i >> 2) * C::Q_PANEL + (i & 3) * 32) >> 4),
                         kk + (((i >> 2) * C::KV_PANEL + (i & 3) * 32) >> 4), idesc_f16(TILE_ROWS, BK, false), t || i);
-            mma_commit(bar(B_S + x));
+            mma_commit(bar(B_S + 2 * x + buf));
           }
         };
-        auto output = [&](int x, int st, bool add) {
+        auto output = [&](int x, int buf, int st, bool add) {
           const uint64_t v = vd + (uint32_t)(st * (C::KV_TILE >> 4));
-          const uint32_t d = tm + TM_O + x * 128, hi = tm + x * BK, lo = tm + tm_lo<C>(x);
+          const uint32_t d = tm + TM_O + x * 128, w = tm + x * 128 + buf * 64;
           if (leader) {
 #pragma unroll
             for (int t = 0; t < TERMS; t++)
 #pragma unroll
               for (int i = 0; i < BK / 16; i++)
-                mma_f16_ts(d, (t ? lo : hi) + i * 8, v + (i * 2048 >> 4), idesc_f16(TILE_ROWS, HD, true), t || i || add);
+                mma_f16_ts(d, w + t * 32 + i * 8, v + (i * 2048 >> 4), idesc_f16(TILE_ROWS, HD, true), t || i || add);
+            mma_commit(bar(B_PV + x));
           }
         };
         if (!(ok = wait_all(B_Q, k))) break;
+        // Turn i: P V of block i, then the scores of block i + 2 (turns -2 and -1: the first scores alone).
 #pragma unroll 1
-        for (int i = 0; ok && i < n; i++, done++) {
-          const int st = done % STAGES, st1 = (done + 1) % STAGES;
+        for (int i = -2; ok && i < n; i++) {
+          const unsigned now = done + i, ahead = now + 2;
+          const int st = now % STAGES, st2 = ahead % STAGES;
+          const bool more = i + 2 < n;
 #pragma unroll 1
-          for (int x = i ? 0 : -tiles; x < tiles; x++) {  // the piece's first scores, then each tile's turn
-            if (x < 0) {
-              if (x == -tiles && !(ok = wait_all(B_K + st, done / STAGES))) break;
+          for (int x = 0; x < tiles; x++) {
+            const unsigned t = (x ? tile_done[1] : tile_done[0]) + i;  // of this tile: buffer t % 2, its turn t / 2
+            const int buf = t & 1;
+            if (i >= 0) {
+              if (!(ok = wait_all(B_P + 2 * x + buf, t / 2))) break;
+              if (x == 0 && !(ok = wait_all(B_V + st, now / STAGES))) break;
               fence_after();
-              scores(x + tiles, st);
-              if (x == -1) commit(B_K_FREE + st);
-              continue;
+              output(x, buf, st, !SPLIT && i);
             }
-            if (!(ok = wait_all(B_P + x, x ? tile_done[1]++ : tile_done[0]++))) break;
-            if (x == 0 && !(ok = wait_all(B_V + st, done / STAGES))) break;
-            fence_after();
-            output(x, st, !SPLIT && i);
-            if (i + 1 < n) {
-              if (x == 0 && !(ok = wait_all(B_K + st1, (done + 1) / STAGES))) break;
+            if (more) {
+              if (x == 0 && !(ok = wait_all(B_K + st2, ahead / STAGES))) break;
               fence_after();
-              scores(x, st1);
-            } else {
-              commit(B_O + x);
+              scores(x, buf, st2);
             }
           }
           if (!ok) break;
-          commit(B_V_FREE + st);
-          if (i + 1 < n) commit(B_K_FREE + st1);
+          if (more) commit(B_K_FREE + st2);
+          if (i >= 0) {
+            commit(B_V_FREE + st);
+            if (i % BATCH == BATCH - 1 || i == n - 1) commit(B_PLAN_FREE + batch++ % BATCHES);
+          }
         }
+        done += n;
+        tile_done[0] += n;
+        if (tiles == 2) tile_done[1] += n;
       }
       // every product done before the columns are freed
       commit(B_FIN);
@@ -548,134 +614,81 @@ __global__ void __launch_bounds__(THREADS, 1) k_paged_many(const AttnArgs<T> a) 
     const uint32_t row = (ch >> 2) * C::KV_PANEL + r0 * 128;
     const uint32_t piece0 = row + ((((ch & 3) * 2) + swap) ^ (r0 & 7)) * 16;
     const uint32_t piece1 = row + ((((ch & 3) * 2) + !swap) ^ (r0 & 7)) * 16;
-    unsigned done = 0;  // blocks so far
+    unsigned done = 0, batch = 0;  // blocks and batches so far
     bool ok = true;
+    auto fetch = [&](const Plan *plan, const uint8_t *codes, int v) {
+      if (plan) {
+        const uint8_t *mine = codes + (r0 & 15) * HD + ch * 16;
+#pragma unroll
+        for (int k = 0; k < C::STEPS; k++) {
+          const int at = plan->place[k * STEP_GROUPS + my_group];
+          if (at >= 0) cp16(raw + v * C::RAW + k * (LOADERS * 16), mine + (long long)at * (16 * HD));
+        }
+      }
+      cp_commit();
+    };
+    auto convert = [&](uint32_t present, int v, uint32_t tile) {  // groups not present become zeros
+      uint4 u[C::STEPS];
+#pragma unroll
+      for (int k = 0; k < C::STEPS; k++) u[k] = lds128(raw + v * C::RAW + k * (LOADERS * 16));
+      if (present != (1u << NG) - 1) {
+#pragma unroll
+        for (int k = 0; k < C::STEPS; k++)
+          if (!(present >> (k * STEP_GROUPS + my_group) & 1))
+            u[k] = make_uint4(0x80808080u, 0x80808080u, 0x80808080u, 0x80808080u);
+      }
+#pragma unroll
+      for (int k = 0; k < C::STEPS; k++) {
+        if (swap) {
+          const uint4 x = u[k];
+          u[k] = make_uint4(x.z, x.w, x.x, x.y);
+        }
+        const uint32_t to = tile + k * (C::STEP_ROWS * 128);
+        sts128(to + piece0, codes_lo(u[k].x), codes_hi(u[k].x), codes_lo(u[k].y), codes_hi(u[k].y));
+        sts128(to + piece1, codes_lo(u[k].z), codes_hi(u[k].z), codes_lo(u[k].w), codes_hi(u[k].w));
+      }
+    };
+    // Turn i: block i is converted, block i + 1 fetched (turn -1: the first is fetched).
 #pragma unroll 1
     for (unsigned k = 0; ok; k++) {
       if (!(ok = wait_warp(B_PIECE + k % PIECES, k / PIECES))) break;
-      const Piece p = s_pieces[k % PIECES];
-      if (p.n < 0) break;
-      // Lane j < NG: page (-1: none) and scales of group j of a block.
-      struct Group {
-        int page;
-        float ks, vs;
-      };
-      auto entry_of = [&](int i) {  // of the page table, looked up a block ahead of its use; INT_MIN: no such group
-        if (i >= p.n || lane >= NG) return INT_MIN;
-        const int key = p.block(i) * BK + 16 * lane;
-        return key < p.len ? a.b.table[(long long)p.b * a.b.table_row + (key >> c.page_shift)] : INT_MIN;
-      };
-      auto checked = [&](int entry) {
-        if ((unsigned)entry < (unsigned)c.n_pages) return entry;
-        if (entry != INT_MIN) flag(a.b.err, BAD_PAGE);
-        return -1;
-      };
-      auto scales_of = [&](int page) {
-        Group g = {page, 0.f, 0.f};
-        if (page >= 0) {
-          g.ks = c.ks[(long long)page * c.kv_heads + p.head];
-          g.vs = c.vs[(long long)page * c.kv_heads + p.head];
-        }
-        return g;
-      };
-      // Place of lane's group in the codes, in groups of 16 keys (-1: none).
-      auto place_of = [&](int i, int page) {
-        const int key = p.block(i) * BK + 16 * lane;
-        return page < 0 ? -1 : ((page * c.kv_heads + p.head) << (c.page_shift - 4)) + ((key & (c.page - 1)) >> 4);
-      };
-      auto fetch = [&](bool any, int place, const uint8_t *codes, int which) {
-        if (any) {
-          const uint8_t *mine = codes + (r0 & 15) * HD + ch * 16;
-#pragma unroll
-          for (int k = 0; k < C::STEPS; k++) {
-            const int at = __shfl_sync(0xffffffffu, place, k * STEP_GROUPS + my_group);
-            if (at >= 0) cp16(raw + which * C::RAW + k * (LOADERS * 16), mine + (long long)at * (16 * HD));
-          }
-        }
-        cp_commit();
-      };
-      auto convert = [&](uint32_t present, int which, uint32_t tile) {  // groups not present become zeros
-        uint4 u[C::STEPS];
-#pragma unroll
-        for (int k = 0; k < C::STEPS; k++) u[k] = lds128(raw + which * C::RAW + k * (LOADERS * 16));
-        if (present != (1u << NG) - 1) {
-#pragma unroll
-          for (int k = 0; k < C::STEPS; k++)
-            if (!(present >> (k * STEP_GROUPS + my_group) & 1))
-              u[k] = make_uint4(0x80808080u, 0x80808080u, 0x80808080u, 0x80808080u);
-        }
-#pragma unroll
-        for (int k = 0; k < C::STEPS; k++) {
-          if (swap) {
-            const uint4 x = u[k];
-            u[k] = make_uint4(x.z, x.w, x.x, x.y);
-          }
-          const uint32_t to = tile + k * (C::STEP_ROWS * 128);
-          sts128(to + piece0, codes_lo(u[k].x), codes_hi(u[k].x), codes_lo(u[k].y), codes_hi(u[k].y));
-          sts128(to + piece1, codes_lo(u[k].z), codes_hi(u[k].z), codes_lo(u[k].w), codes_hi(u[k].w));
-        }
-      };
-      float unit = 0.f;
-      int later = entry_of(1);
-      Group now = scales_of(checked(entry_of(0)));
+      const int n = s_pieces[k % PIECES].n;
+      if (n < 0) break;
+      const Plan *now = nullptr, *next = nullptr;
 #pragma unroll 1
-      for (int v = 0; v < 2; v++) fetch(p.n > 0, place_of(0, now.page), v ? c.v : c.k, v);
-      Group next = scales_of(checked(later));
-      later = entry_of(2);
-#pragma unroll 1
-      for (int i = 0; ok && i < p.n; i++, done++) {
-        const int st = done % STAGES;
-        const uint32_t present = __ballot_sync(0xffffffffu, now.page >= 0);
-        const uint32_t with_v = __ballot_sync(0xffffffffu, now.page >= 0 && now.vs > 0.f);
-        float top = now.vs;
-#pragma unroll
-        for (int o = 1; o < NG; o <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
-        top = __shfl_sync(0xffffffffu, top, 0);
-        if (SPLIT || top > unit * UNIT_LAG || unit == 0.f) unit = top;
-        const int place = place_of(i + 1, next.page);
+      for (int i = -1; ok && i < n; i++) {
+        now = next;
+        next = nullptr;
+        if (i + 1 < n) {
+          const unsigned t = batch + (i + 1) / BATCH;
+          if ((i + 1) % BATCH == 0 && !(ok = wait_warp(B_PLAN + t % BATCHES, t / BATCHES))) break;
+          next = plans + t % BATCHES * BATCH + (i + 1) % BATCH;
+        }
+        const unsigned at = done + i;
+        const int st = at % STAGES;
 #pragma unroll 1
         for (int v = 0; v < 2; v++) {  // K, then V
-          if (done >= STAGES && !(ok = wait_warp((v ? B_V_FREE : B_K_FREE) + st, done / STAGES - 1))) break;
-          // Scores of block done - 2 are done, so weights of done - 3 and before: the scales of done - 4 have been read.
-          if (!v && warp == SOFTMAX_WARPS) {
-            Scales &sc = scales[done % SCALE_STAGES];
-            if (lane < NG) {
-              const float share = now.vs > 0.f ? now.vs / unit : 0.f;
-              sc.ks[lane] = now.ks;
-              if (SPLIT) {
-                sc.share[lane] = share;
-              } else {  // as an exponent; below 2^-100 of the unit: as good as none
-                const float e = share > 0.f ? fmaxf(log2f(share), -100.f) : 0.f;
-                sc.share[lane] = e;
-                sc.inv[lane] = share > 0.f ? exp2f(-e) : 1.f;
-              }
-            }
-            if (lane == 0) {
-              sc.present = present;
-              sc.unit = unit;
-            }
+          if (now) {
+            if (at >= STAGES && !(ok = wait_warp((v ? B_V_FREE : B_K_FREE) + st, at / STAGES - 1))) break;
+            cp_wait<1>();
+            convert(v ? now->with_v : now->present, v, base + (v ? C::OFF_V : C::OFF_K) + st * C::KV_TILE);
+            fence_proxy_async();  // before the next copies: it would wait for them
             __syncwarp();
-            if (lane == 0) bar_arrive(bar(B_SCALE + done % SCALE_STAGES));
+            if (lane == 0) bar_arrive(bar((v ? B_V : B_K) + st));
           }
-          cp_wait<1>();
-          convert(v ? with_v : present, v, base + (v ? C::OFF_V : C::OFF_K) + st * C::KV_TILE);
-          fence_proxy_async();  // before the next copies: it would wait for them
-          __syncwarp();
-          if (lane == 0) bar_arrive(bar((v ? B_V : B_K) + st));
-          fetch(i + 1 < p.n, place, v ? c.v : c.k, v);
+          fetch(next, v ? c.v : c.k, v);
         }
-        now = next;
-        next = scales_of(checked(later));
-        later = entry_of(i + 3);
       }
       cp_wait<0>();
+      done += n;
+      batch += (n + BATCH - 1) / BATCH;
     }
   } else {
     // ---------------- softmax and output: one thread a row ----------------
     asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(SOFTMAX_REGS));
     const int x = warp >> 2, r = tid & (TILE_ROWS - 1), row = x * TILE_ROWS + r;
     const uint32_t lanes = (uint32_t)(32 * (warp & 3)) << 16;
-    const uint32_t s_col = tmem + lanes + x * BK, o_col = tmem + lanes + TM_O + x * 128;
+    const uint32_t s_tile = tmem + lanes + x * 128, o_col = tmem + lanes + TM_O + x * 128;
     auto all_ok = [&](bool v) -> bool {  // of the eight warps; also their barrier
       unsigned res;
       asm volatile(
@@ -688,7 +701,7 @@ __global__ void __launch_bounds__(THREADS, 1) k_paged_many(const AttnArgs<T> a) 
           : "memory");
       return res != 0;
     };
-    unsigned done = 0, tile_done = 0, outs = 0;
+    unsigned batch = 0, tile_done = 0;  // batches so far, blocks of this tile
 #pragma unroll 1
     for (unsigned k = 0;; k++) {
       bool ok = wait_warp(B_PIECE + k % PIECES, k / PIECES);
@@ -766,7 +779,8 @@ __global__ void __launch_bounds__(THREADS, 1) k_paged_many(const AttnArgs<T> a) 
 #pragma unroll
         for (int d = 0; d < HD; d++) o[d] = 0.f;
       }
-      auto add_output = [&]() {  // f32 rows: o += unit * O of the last block
+      // f32 rows: o += unit * O of the last block
+      auto add_output = [&](float unit) {
         if constexpr (SPLIT) {
 #pragma unroll
           for (int d = 0; d < HD; d += 32) {
@@ -778,63 +792,60 @@ __global__ void __launch_bounds__(THREADS, 1) k_paged_many(const AttnArgs<T> a) 
           }
         }
       };
-      // The last turn (i = n) takes the last block's output.
+      // Turn i = n only takes the last block's output.
 #pragma unroll 1
-      for (int i = 0; ok && active && i <= n && n; i++) {
+      for (int i = 0; ok && active && n && i <= n; i++) {
         if (i == n) {
-          ok = wait_warp(B_O + x, outs++);
+          ok = wait_warp(B_PV + x, tile_done + n - 1);
           fence_after();
-          if (ok) add_output();
+          if (ok) add_output(unit);
           break;
         }
-        const Scales &sc = scales[(done + i) % SCALE_STAGES];
-        if (!(ok = wait_warp(B_SCALE + (done + i) % SCALE_STAGES, (done + i) / SCALE_STAGES))) break;
-        if (!(ok = wait_warp(B_S + x, tile_done))) break;
-        tile_done++;
+        const unsigned t = tile_done + i, bt = batch + i / BATCH;
+        const uint32_t s_col = s_tile + (t & 1) * 64;
+        const Plan &plan = plans[bt % BATCHES * BATCH + i % BATCH];
+        if (i % BATCH == 0 && !(ok = wait_warp(B_PLAN + bt % BATCHES, bt / BATCHES))) break;
+        if (!(ok = wait_warp(B_S + 2 * x + (t & 1), t / 2))) break;
         fence_after();
-        if (SPLIT && i) add_output();
+        float v[64];
+        tmem_ld32(s_col, v);
+        tmem_ld32(s_col + 32, v + 32);
         const int key0 = (t0 + i + (t0 + i < n_sink ? 0 : skip)) * BK;
-        const uint32_t present = sc.present;
-        const bool hide = key0 + BK - 1 > min_pos || (a.window && key0 <= max_pos - a.window && key0 + BK > a.sinks) ||
-                          present != (1u << NG) - 1;
-        auto load64 = [&](int k0, float (&v)[64]) {  // scores of keys k0 .. k0 + 63 of the block
-          tmem_ld32(s_col + k0, v);
-          tmem_ld32(s_col + k0 + 32, v + 32);
-          tmem_ready<64>(v);
-          if (hide) {
-            const int q = key0 + k0;  // bits: keys q .. q + 63
-            auto upto = [&](int end) -> uint64_t {  // keys < end
-              const int m = min(max(end - q, 0), 64);
-              return m == 64 ? ~0ull : (1ull << m) - 1;
-            };
-            uint64_t see = upto(pos + 1) & (~upto(low + 1) | upto(sinks));
+        const uint32_t present = plan.present;
+        const float4 ks = *reinterpret_cast<const float4 *>(plan.ks), share4 = *reinterpret_cast<const float4 *>(plan.share);
+        // the factors of the groups' scores; not 0, because hidden scores are -infinity
+        const float f[4] = {fmaxf(cf * ks.x, FLT_MIN), fmaxf(cf * ks.y, FLT_MIN), fmaxf(cf * ks.z, FLT_MIN),
+                            fmaxf(cf * ks.w, FLT_MIN)};
+        const float share[4] = {share4.x, share4.y, share4.z, share4.w};
+        const float new_unit = plan.unit;
+        tmem_ready<64>(v);
+        if (key0 + BK - 1 > min_pos || (a.window && key0 <= max_pos - a.window && key0 + BK > a.sinks) ||
+            present != (1u << NG) - 1) {
+          auto upto = [&](int end) -> uint64_t {  // bits of the block's keys < end
+            const int m = min(max(end - key0, 0), 64);
+            return m == 64 ? ~0ull : (1ull << m) - 1;
+          };
+          uint64_t see = upto(pos + 1) & (~upto(low + 1) | upto(sinks));
 #pragma unroll
-            for (int g = 0; g < 4; g++)
-              if (!(present >> (k0 / 16 + g) & 1)) see &= ~(0xffffull << (16 * g));
-            const uint32_t s0 = (uint32_t)see, s1 = (uint32_t)(see >> 32);
+          for (int g = 0; g < NG; g++)
+            if (!(present >> g & 1)) see &= ~(0xffffull << (16 * g));
+          const uint32_t s0 = (uint32_t)see, s1 = (uint32_t)(see >> 32);
 #pragma unroll
-            for (int j = 0; j < 32; j++) {
-              v[j] = s0 >> j & 1 ? v[j] : -INFINITY;
-              v[32 + j] = s1 >> j & 1 ? v[32 + j] : -INFINITY;
-            }
+          for (int j = 0; j < 32; j++) {
+            v[j] = s0 >> j & 1 ? v[j] : -INFINITY;
+            v[32 + j] = s1 >> j & 1 ? v[32 + j] : -INFINITY;
           }
-        };
+        }
         float mx = -INFINITY;
-#pragma unroll 1
-        for (int k0 = 0; k0 < BK; k0 += 64) {
-          float v[64];
-          load64(k0, v);
 #pragma unroll
-          for (int g = 0; g < 4; g++) {
-            float m1 = fmaxf(v[16 * g], v[16 * g + 1]), m2 = fmaxf(v[16 * g + 2], v[16 * g + 3]);
+        for (int g = 0; g < NG; g++) {
+          float m1 = fmaxf(v[16 * g], v[16 * g + 1]), m2 = fmaxf(v[16 * g + 2], v[16 * g + 3]);
 #pragma unroll
-            for (int j = 4; j < 16; j += 4) {
-              m1 = max3(m1, v[16 * g + j], v[16 * g + j + 1]);
-              m2 = max3(m2, v[16 * g + j + 2], v[16 * g + j + 3]);
-            }
-            m1 = fmaxf(m1, m2);
-            mx = fmaxf(mx, m1 == -INFINITY ? m1 : m1 * (cf * sc.ks[k0 / 16 + g]));
+          for (int j = 4; j < 16; j += 4) {
+            m1 = max3(m1, v[16 * g + j], v[16 * g + j + 1]);
+            m2 = max3(m2, v[16 * g + j + 2], v[16 * g + j + 3]);
           }
+          mx = fmaxf(mx, fmaxf(m1, m2) * f[g]);
         }
         // the reference follows the maximum, the unit the block's: earlier results move along
         float alpha = 1.f;
@@ -842,70 +853,69 @@ __global__ void __launch_bounds__(THREADS, 1) k_paged_many(const AttnArgs<T> a) 
           alpha = ex2(ref - mx);
           ref = mx;
         }
-        float move = alpha;
-        if (!SPLIT && unit != sc.unit) move *= sc.unit > 0.f ? unit / sc.unit : 0.f;
-        unit = sc.unit;
-        l *= alpha;
-        if (i && __any_sync(0xffffffffu, move != 1.f)) {
-          if constexpr (SPLIT) {
+        const float shift = ref == -INFINITY ? 0.f : WEIGHT_EXP - ref;
+        // weights, over the scores
+        float sum = 0.f;
+        uint32_t hi[32], lo[SPLIT ? 32 : 1];
 #pragma unroll
-            for (int d = 0; d < HD; d++) o[d] *= move;
-          } else {
-#pragma unroll 1
-            for (int d = 0; d < HD; d += 32) {
-              float v[32];
-              tmem_ld32(o_col + d, v);
-              tmem_ready<32>(v);
-              uint32_t u[32];
+        for (int g = 0; g < NG; g++) {
+          const float sh = SPLIT ? shift : shift + share[g];
+          const f2x f2 = pk2(f[g], f[g]), sh2 = pk2(sh, sh), share2 = pk2(share[g], share[g]);
+          f2x gs = 0ull;
 #pragma unroll
-              for (int j = 0; j < 32; j++) u[j] = __float_as_uint(v[j] * move);
-#pragma unroll
-              for (int j = 0; j < 32; j += 8) tmem_st8(o_col + d + j, u + j);
+          for (int j = 0; j < 8; j++) {
+            const float2 y = up2(ffma2(pk2(v[16 * g + 2 * j], v[16 * g + 2 * j + 1]), f2, sh2));
+            f2x w = pk2(ex2(y.x), ex2(y.y));
+            gs = fadd2(gs, w);
+            if constexpr (SPLIT) w = fmul2(w, share2);
+            const float2 z = up2(w);
+            hi[8 * g + j] = pack(z.x, z.y);
+            if constexpr (SPLIT) {
+              const float2 h2 = unpack(hi[8 * g + j]);
+              lo[8 * g + j] = pack(z.x - h2.x, z.y - h2.y);
             }
           }
+          const float2 z = up2(gs);
+          if constexpr (SPLIT) sum += z.x + z.y;
+          else sum = fmaf(z.x + z.y, plan.inv[g], sum);
         }
-        const float shift = ref == -INFINITY ? 0.f : WEIGHT_EXP - ref;
-        // weights, the first terms into columns whose scores this thread has read
-        float sum = 0.f;
+        tmem_st32(s_col, hi);
+        if constexpr (SPLIT) tmem_st32(s_col + 32, lo);
+        l = fmaf(l, alpha, sum);
+        float move = alpha;
+        if (!SPLIT && unit != new_unit) move *= new_unit > 0.f ? unit / new_unit : 0.f;
+        const bool any = i && __any_sync(0xffffffffu, move != 1.f);
+        if (i && (SPLIT || any)) {  // the last block's P V is done before its output is read or moved
+          if (!(ok = wait_warp(B_PV + x, t - 1))) break;
+          fence_after();
+          add_output(unit);
+          if (any) {
+            if constexpr (SPLIT) {
+#pragma unroll
+              for (int d = 0; d < HD; d++) o[d] *= move;
+            } else {
 #pragma unroll 1
-        for (int k0 = 0; k0 < BK; k0 += 64) {
-          float v[64];
-          load64(k0, v);
-          uint32_t hi[32], lo[SPLIT ? 32 : 1];
+              for (int d = 0; d < HD; d += 32) {
+                float y[32];
+                tmem_ld32(o_col + d, y);
+                tmem_ready<32>(y);
+                uint32_t u[32];
 #pragma unroll
-          for (int g = 0; g < 4; g++) {
-            const float f = fmaxf(cf * sc.ks[k0 / 16 + g], FLT_MIN);  // not 0: hidden scores are -infinity
-            const float share = sc.share[k0 / 16 + g], sh = SPLIT ? shift : shift + share;
-            const f2x f2 = pk2(f, f), sh2 = pk2(sh, sh), share2 = pk2(share, share);
-            f2x gs = 0ull;
-#pragma unroll
-            for (int j = 0; j < 8; j++) {
-              const float2 y = up2(ffma2(pk2(v[16 * g + 2 * j], v[16 * g + 2 * j + 1]), f2, sh2));
-              f2x w = pk2(ex2(y.x), ex2(y.y));
-              gs = fadd2(gs, w);
-              if constexpr (SPLIT) w = fmul2(w, share2);
-              const float2 z = up2(w);
-              hi[8 * g + j] = pack(z.x, z.y);
-              if constexpr (SPLIT) {
-                const float2 h2 = unpack(hi[8 * g + j]);
-                lo[8 * g + j] = pack(z.x - h2.x, z.y - h2.y);
+                for (int j = 0; j < 32; j++) u[j] = __float_as_uint(y[j] * move);
+                tmem_st32(o_col + d, u);
               }
             }
-            const float2 z = up2(gs);
-            if constexpr (SPLIT) sum += z.x + z.y;
-            else sum = fmaf(z.x + z.y, sc.inv[k0 / 16 + g], sum);
           }
-          tmem_st32(s_col + k0 / 2, hi);
-          if constexpr (SPLIT) tmem_st32(tmem + lanes + tm_lo<C>(x) + k0 / 2, lo);
         }
-        l += sum;
+        unit = new_unit;
         tmem_wait_st();
         fence_before();
         __syncwarp();
-        if (lane == 0) bar_arrive(bar(B_P + x));
+        if (lane == 0) bar_arrive(bar(B_P + 2 * x + (t & 1)));
       }
       if (!all_ok(ok)) break;
-      done += n;
+      if (active) tile_done += n;
+      batch += (n + BATCH - 1) / BATCH;
       const bool none = !active || !n;  // nothing was computed: l = 0, O is not the tile's
       const bool whole = piece.whole;
       T *dst = a.out + (long long)(piece.row0 + tok) * a.os + h * HD;
@@ -913,8 +923,16 @@ __global__ void __launch_bounds__(THREADS, 1) k_paged_many(const AttnArgs<T> a) 
       const float inv = l == 0.f ? 0.f : 1.f / l;
       auto write = [&](int d, const float *v) {  // 32 values
         if (!live) return;
+        if constexpr (SPLIT) {
 #pragma unroll
-        for (int j = 0; j < 32; j += 4) store4(dst + d + j, make_float4(v[j], v[j + 1], v[j + 2], v[j + 3]));
+          for (int j = 0; j < 32; j += 4) store4(dst + d + j, make_float4(v[j], v[j + 1], v[j + 2], v[j + 3]));
+        } else {
+#pragma unroll
+          for (int j = 0; j < 32; j += 8)
+            *reinterpret_cast<uint4 *>(dst + d + j) =
+                make_uint4(bf16_pair(v[j], v[j + 1]), bf16_pair(v[j + 2], v[j + 3]), bf16_pair(v[j + 4], v[j + 5]),
+                           bf16_pair(v[j + 6], v[j + 7]));
+        }
       };
       auto put = [&](int d, float *v) {
         if (whole) {
