@@ -607,6 +607,17 @@ bool goes_many(const Cache &c, int max_new, int group) {
   return (long long)max_new * group > FEW_ROWS && many_supported(c, group);
 }
 
+// Whether the (row tile, key tile) pairs of a call can be numbered in 31 bits by both kernels: 128 rows or
+// more a tile and 64 keys for the many-row one, 4 rows and 16 keys at least for the other.
+bool countable(const Batch &b, const Cache &c, int n_heads) {
+  const int group = n_heads / c.kv_heads;
+  const bool many = goes_many(c, b.max_new, group);
+  const double keys = (double)b.table_row * c.page, tokens = b.n_tokens, seqs = b.n_seqs;
+  const double few = many ? seqs * (FEW_ROWS / 4) : tokens * group / 4 + seqs;
+  const double rest = many ? (tokens * group / 128 + seqs) * (keys / 64 + 8) : 0;
+  return few * c.kv_heads * (keys / 16 + 2) < INT32_MAX && rest * c.kv_heads < INT32_MAX;
+}
+
 // Partial results of both kernels, then the counters of both.
 struct Workspace {
   size_t many_part, few_count, many_count, bytes;
@@ -685,11 +696,8 @@ extern "C" int sq_paged_attention(void *stream, const sq_paged_cache *cache, con
   if (dtype != SQ_F32 && dtype != SQ_BF16)
     return fail(SQ_ERR_INVALID_TYPE, "paged_attention: rows must be F32 or BF16");
   if (window < 0 || sinks < 0) return fail(SQ_ERR_SHAPE, "paged_attention: negative window or sinks");
-  {  // both kernels number the (row tile, key tile) pairs of a call in 31 bits: row tiles of 4 rows, key tiles of 16
-    const double rows = (double)b.n_tokens * n_heads / 4 + (double)b.n_seqs * c.kv_heads;
-    if (rows * ((double)b.table_row * c.page / 16 + 16) >= INT32_MAX / 2.0)
-      return fail(SQ_ERR_SHAPE, "paged_attention: too many query rows for so long a page table in one call");
-  }
+  if (!paged::countable(b, c, n_heads))
+    return fail(SQ_ERR_SHAPE, "paged_attention: too many query rows for so long a page table in one call");
   if (!b.n_tokens) return SQ_OK;
   const long long width = (long long)n_heads * c.hd;
   st = paged::check_rows(q, q_stride, width, dtype, "paged_attention: q");

@@ -5,8 +5,8 @@
 // A block works on 256 query rows of one kv head (row = token * group + head of the
 // group), two tiles X of 128 that share every block of 64 keys, so that a code is
 // converted once for 256 rows:
-//   warps 8-11  codes of a block of keys to shared memory (cp.async, each thread its own
-//               chunks), converted to f16 (exact: whole numbers up to 127) into the
+//   warps 8-11  codes of a block of keys, loaded a block ahead to registers and converted
+//               to f16 (exact: whole numbers up to 127) into the
 //               128-byte swizzled tiles of K [keys][dims] and V [keys][dims]
 //   warp 12     issues the products, f32 sums in tensor memory:
 //               S_X = Q_X K^T (K-major operands), O_X (+)= P_X V (V read MN-major as it
@@ -70,9 +70,8 @@ struct Cfg {
   static constexpr int ROW_CHUNKS = HD / 16;                      // 16-code chunks of a key
   static constexpr int STEP_ROWS = LOADERS / ROW_CHUNKS;          // keys the loading threads take at once: 16 or 32
   static constexpr int STEPS = BK / STEP_ROWS;
-  static constexpr int RAW = BK * HD;
   static constexpr int OFF_Q = 0, OFF_K = OFF_Q + 2 * TERMS * Q_TILE, OFF_V = OFF_K + STAGES * KV_TILE,
-                       OFF_RAW = OFF_V + STAGES * KV_TILE, OFF_SCALE = OFF_RAW + 2 * RAW,
+                       OFF_SCALE = OFF_V + STAGES * KV_TILE,
                        OFF_BAR = OFF_SCALE + BATCHES * BATCH * 96;
   static constexpr int SMEM = 1024 + OFF_BAR + 320;
   static constexpr int SLOT = ROWS * (HD + 2);  // floats of a cut row tile's partial result
@@ -182,6 +181,9 @@ __device__ __forceinline__ void tmem_ready(float *v) {
   asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
 #pragma unroll
   for (int i = 0; i < N; i++) asm volatile("" : "+f"(v[i]));
+}
+__device__ __forceinline__ void sts64(uint32_t a, uint32_t x, uint32_t y) {
+  asm volatile("st.shared.v2.u32 [%0], {%1, %2};" ::"r"(a), "r"(x), "r"(y) : "memory");
 }
 __device__ __forceinline__ void sts128(uint32_t a, uint32_t x, uint32_t y, uint32_t z, uint32_t w) {
   asm volatile("st.shared.v4.u32 [%0], {%1, %2, %3, %4};" ::"r"(a), "r"(x), "r"(y), "r"(z), "r"(w) : "memory");
@@ -417,30 +419,20 @@ __global__ void __launch_bounds__(THREADS, 1) k_paged_many(const AttnArgs<T> a) 
   fence_after();
   const uint32_t tmem = s_tmem;
   volatile int *abort_flag = &s_abort;
-  // Bounded: false once any wait of the block has expired.
+  // Every lane waits; bounded (about two seconds): false for the whole warp once any wait of the block has expired.
   auto wait = [&](int i, unsigned phase) -> bool {
     const uint32_t b = bar(i);
-    if (bar_try_wait(b, phase & 1u)) return true;
-    const long long t0 = clock64();
-    while (!bar_try_wait_sleep(b, phase & 1u, 20000u)) {
-      if (*abort_flag) return false;
-      if (clock64() - t0 > WAIT_LIMIT) {
+    bool ok = bar_try_wait(b, phase & 1u);
+    if (!ok) {
+      const unsigned t0 = (unsigned)clock();
+      do ok = bar_try_wait_sleep(b, phase & 1u, 20000u);
+      while (!ok && !*abort_flag && (unsigned)clock() - t0 < 4000000000u);
+      if (!ok && !*abort_flag) {
         flag(a.b.err, BAD_WAIT);
         *abort_flag = 1;
-        return false;
       }
     }
-    return true;
-  };
-  auto wait_all = [&](int i, unsigned phase) -> bool {  // every lane waits; the warp goes on together
-    return __all_sync(0xffffffffu, wait(i, phase));
-  };
-  auto wait_warp = [&](int i, unsigned phase) -> bool {  // lane 0 waits, the warp follows
-    int ok = 1;
-    if (lane == 0) ok = wait(i, phase);
-    ok = __shfl_sync(0xffffffffu, ok, 0);
-    __syncwarp();
-    return ok;
+    return __all_sync(0xffffffffu, ok);
   };
 
   if (warp >= MMA_WARP) {
@@ -453,7 +445,7 @@ __global__ void __launch_bounds__(THREADS, 1) k_paged_many(const AttnArgs<T> a) 
         Piece p;
         more = walk.next(a, p);
         if (!more) p.n = -1;
-        if (k >= PIECES && !wait_warp(B_DONE, k - PIECES)) break;  // its place is free
+        if (k >= PIECES && !wait(B_DONE, k - PIECES)) break;  // its place is free
         if (lane == 0) {
           s_pieces[k % PIECES] = p;
           bar_arrive(bar(B_PIECE + k % PIECES));
@@ -466,7 +458,7 @@ __global__ void __launch_bounds__(THREADS, 1) k_paged_many(const AttnArgs<T> a) 
       bool ok = true;
 #pragma unroll 1
       for (unsigned k = 0; ok; k++) {
-        if (!(ok = wait_warp(B_PIECE + k % PIECES, k / PIECES))) break;
+        if (!(ok = wait(B_PIECE + k % PIECES, k / PIECES))) break;
         const Piece p = s_pieces[k % PIECES];
         if (p.n < 0) break;
         float unit = 0.f;
@@ -495,7 +487,7 @@ __global__ void __launch_bounds__(THREADS, 1) k_paged_many(const AttnArgs<T> a) 
           }
           const uint32_t present = __ballot_sync(0xffffffffu, page >= 0) >> (lane & 28) & 15;
           const uint32_t with_v = __ballot_sync(0xffffffffu, vs > 0.f) >> (lane & 28) & 15;
-          if (batch >= BATCHES && !(ok = wait_warp(B_PLAN_FREE + batch % BATCHES, batch / BATCHES - 1))) break;
+          if (batch >= BATCHES && !(ok = wait(B_PLAN_FREE + batch % BATCHES, batch / BATCHES - 1))) break;
           Plan &plan = plans[batch % BATCHES * BATCH + (lane >> 2)];
           const float share = vs > 0.f ? vs / my_unit : 0.f;
           plan.place[j] = page < 0 ? -1 : ((page * c.kv_heads + p.head) << (c.page_shift - 4)) + ((key & (c.page - 1)) >> 4);
@@ -529,7 +521,7 @@ __global__ void __launch_bounds__(THREADS, 1) k_paged_many(const AttnArgs<T> a) 
       bool ok = true;
 #pragma unroll 1
       for (unsigned k = 0; ok; k++) {
-        if (!(ok = wait_all(B_PIECE + k % PIECES, k / PIECES))) break;
+        if (!(ok = wait(B_PIECE + k % PIECES, k / PIECES))) break;
         const int n = __shfl_sync(0xffffffffu, s_pieces[k % PIECES].n, 0);
         const int tiles = __shfl_sync(0xffffffffu, s_pieces[k % PIECES].n_rows, 0) > TILE_ROWS ? 2 : 1;
         if (n < 0) break;
@@ -561,7 +553,7 @@ __global__ void __launch_bounds__(THREADS, 1) k_paged_many(const AttnArgs<T> a) 
             mma_commit(bar(B_PV + x));
           }
         };
-        if (!(ok = wait_all(B_Q, k))) break;
+        if (!(ok = wait(B_Q, k))) break;
         // Turn i: P V of block i, then the scores of block i + 2 (turns -2 and -1: the first scores alone).
 #pragma unroll 1
         for (int i = -2; ok && i < n; i++) {
@@ -573,13 +565,13 @@ __global__ void __launch_bounds__(THREADS, 1) k_paged_many(const AttnArgs<T> a) 
             const unsigned t = (x ? tile_done[1] : tile_done[0]) + i;  // of this tile: buffer t % 2, its turn t / 2
             const int buf = t & 1;
             if (i >= 0) {
-              if (!(ok = wait_all(B_P + 2 * x + buf, t / 2))) break;
-              if (x == 0 && !(ok = wait_all(B_V + st, now / STAGES))) break;
+              if (!(ok = wait(B_P + 2 * x + buf, t / 2))) break;
+              if (x == 0 && !(ok = wait(B_V + st, now / STAGES))) break;
               fence_after();
               output(x, buf, st, !SPLIT && i);
             }
             if (more) {
-              if (x == 0 && !(ok = wait_all(B_K + st2, ahead / STAGES))) break;
+              if (x == 0 && !(ok = wait(B_K + st2, ahead / STAGES))) break;
               fence_after();
               scores(x, buf, st2);
             }
@@ -606,37 +598,27 @@ __global__ void __launch_bounds__(THREADS, 1) k_paged_many(const AttnArgs<T> a) 
     const int me = tid - SOFTMAX_WARPS * 32, r0 = me / C::ROW_CHUNKS, ch = me % C::ROW_CHUNKS;
     constexpr int STEP_GROUPS = C::STEP_ROWS / 16;  // groups of a step: a warp's keys are of one
     const int my_group = r0 >> 4;
-    // Own chunks: raw codes at raw + 2048 k; in the tile row r0 + STEP_ROWS k, 16-byte pieces 2 ch and 2 ch + 1
-    // of the row's dimensions. With two panels a row's upper lanes start with their second piece, so that
-    // eight lanes meet every bank once.
-    const uint32_t raw = base + C::OFF_RAW + me * 16;
+    // Own chunks: keys r0 + STEP_ROWS k, codes 16 ch .. of the row; in the tile that row's 16-byte pieces 2 ch and
+    // 2 ch + 1. With two panels a row's upper lanes start with their second piece, so that eight lanes meet
+    // every bank once.
     const bool swap = HD == 128 && (ch & 4);
     const uint32_t row = (ch >> 2) * C::KV_PANEL + r0 * 128;
     const uint32_t piece0 = row + ((((ch & 3) * 2) + swap) ^ (r0 & 7)) * 16;
     const uint32_t piece1 = row + ((((ch & 3) * 2) + !swap) ^ (r0 & 7)) * 16;
     unsigned done = 0, batch = 0;  // blocks and batches so far
     bool ok = true;
-    auto fetch = [&](const Plan *plan, const uint8_t *codes, int v) {
-      if (plan) {
-        const uint8_t *mine = codes + (r0 & 15) * HD + ch * 16;
+    // Groups that are not there (or, for V, have a scale of 0) become zeros.
+    auto fetch = [&](uint4 (&u)[C::STEPS], const int4 &place, uint32_t present, const uint8_t *codes) {
+      const int at[4] = {place.x, place.y, place.z, place.w};
 #pragma unroll
-        for (int k = 0; k < C::STEPS; k++) {
-          const int at = plan->place[k * STEP_GROUPS + my_group];
-          if (at >= 0) cp16(raw + v * C::RAW + k * (LOADERS * 16), mine + (long long)at * (16 * HD));
-        }
+      for (int k = 0; k < C::STEPS; k++) {
+        const int g0 = k * STEP_GROUPS, at_k = STEP_GROUPS == 1 ? at[g0] : (my_group ? at[(g0 + 1) & 3] : at[g0]);
+        u[k] = make_uint4(0x80808080u, 0x80808080u, 0x80808080u, 0x80808080u);
+        if (present >> (g0 + my_group) & 1)
+          u[k] = __ldg(reinterpret_cast<const uint4 *>(codes + (long long)at_k * (16 * HD)));
       }
-      cp_commit();
     };
-    auto convert = [&](uint32_t present, int v, uint32_t tile) {  // groups not present become zeros
-      uint4 u[C::STEPS];
-#pragma unroll
-      for (int k = 0; k < C::STEPS; k++) u[k] = lds128(raw + v * C::RAW + k * (LOADERS * 16));
-      if (present != (1u << NG) - 1) {
-#pragma unroll
-        for (int k = 0; k < C::STEPS; k++)
-          if (!(present >> (k * STEP_GROUPS + my_group) & 1))
-            u[k] = make_uint4(0x80808080u, 0x80808080u, 0x80808080u, 0x80808080u);
-      }
+    auto convert = [&](uint4 (&u)[C::STEPS], uint32_t tile) {
 #pragma unroll
       for (int k = 0; k < C::STEPS; k++) {
         if (swap) {
@@ -648,38 +630,45 @@ __global__ void __launch_bounds__(THREADS, 1) k_paged_many(const AttnArgs<T> a) 
         sts128(to + piece1, codes_lo(u[k].z), codes_hi(u[k].z), codes_lo(u[k].w), codes_hi(u[k].w));
       }
     };
+    const uint8_t *my_k = c.k + (r0 & 15) * HD + ch * 16, *my_v = c.v + (r0 & 15) * HD + ch * 16;
     // Turn i: block i is converted, block i + 1 fetched (turn -1: the first is fetched).
 #pragma unroll 1
     for (unsigned k = 0; ok; k++) {
-      if (!(ok = wait_warp(B_PIECE + k % PIECES, k / PIECES))) break;
+      if (!(ok = wait(B_PIECE + k % PIECES, k / PIECES))) break;
       const int n = s_pieces[k % PIECES].n;
       if (n < 0) break;
-      const Plan *now = nullptr, *next = nullptr;
+      uint4 ku[C::STEPS], vu[C::STEPS];
 #pragma unroll 1
       for (int i = -1; ok && i < n; i++) {
-        now = next;
-        next = nullptr;
+        int4 place = {0, 0, 0, 0};
+        uint32_t present = 0, with_v = 0;
         if (i + 1 < n) {
           const unsigned t = batch + (i + 1) / BATCH;
-          if ((i + 1) % BATCH == 0 && !(ok = wait_warp(B_PLAN + t % BATCHES, t / BATCHES))) break;
-          next = plans + t % BATCHES * BATCH + (i + 1) % BATCH;
+          if ((i + 1) % BATCH == 0 && !(ok = wait(B_PLAN + t % BATCHES, t / BATCHES))) break;
+          const Plan &plan = plans[t % BATCHES * BATCH + (i + 1) % BATCH];
+          place = *reinterpret_cast<const int4 *>(plan.place);
+          present = plan.present;
+          with_v = plan.with_v;
         }
         const unsigned at = done + i;
         const int st = at % STAGES;
-#pragma unroll 1
-        for (int v = 0; v < 2; v++) {  // K, then V
-          if (now) {
-            if (at >= STAGES && !(ok = wait_warp((v ? B_V_FREE : B_K_FREE) + st, at / STAGES - 1))) break;
-            cp_wait<1>();
-            convert(v ? now->with_v : now->present, v, base + (v ? C::OFF_V : C::OFF_K) + st * C::KV_TILE);
-            fence_proxy_async();  // before the next copies: it would wait for them
-            __syncwarp();
-            if (lane == 0) bar_arrive(bar((v ? B_V : B_K) + st));
-          }
-          fetch(next, v ? c.v : c.k, v);
+        if (i >= 0) {
+          if (at >= STAGES && !(ok = wait(B_K_FREE + st, at / STAGES - 1))) break;
+          convert(ku, base + C::OFF_K + st * C::KV_TILE);
+          fence_proxy_async();
+          __syncwarp();
+          if (lane == 0) bar_arrive(bar(B_K + st));
         }
+        if (i + 1 < n) fetch(ku, place, present, my_k);
+        if (i >= 0) {
+          if (at >= STAGES && !(ok = wait(B_V_FREE + st, at / STAGES - 1))) break;
+          convert(vu, base + C::OFF_V + st * C::KV_TILE);
+          fence_proxy_async();
+          __syncwarp();
+          if (lane == 0) bar_arrive(bar(B_V + st));
+        }
+        if (i + 1 < n) fetch(vu, place, with_v, my_v);
       }
-      cp_wait<0>();
       done += n;
       batch += (n + BATCH - 1) / BATCH;
     }
@@ -704,64 +693,71 @@ __global__ void __launch_bounds__(THREADS, 1) k_paged_many(const AttnArgs<T> a) 
     unsigned batch = 0, tile_done = 0;  // batches so far, blocks of this tile
 #pragma unroll 1
     for (unsigned k = 0;; k++) {
-      bool ok = wait_warp(B_PIECE + k % PIECES, k / PIECES);
+      bool ok = wait(B_PIECE + k % PIECES, k / PIECES);
       const Piece &piece = s_pieces[k % PIECES];
       const int n = ok ? piece.n : -1;
       if (ok && n < 0) break;
-      // ---- the row's query as f16 terms in the swizzled tile
-      const int n_rows = piece.n_rows, tok = row / a.group, h = piece.head * a.group + row % a.group;
+      const int n_rows = piece.n_rows, row0 = piece.row0, h0 = piece.head * a.group, tok = row / a.group;
       const bool live = ok && row < n_rows, active = x == 0 || n_rows > TILE_ROWS;
-      const T *src = a.q + (long long)(piece.row0 + (live ? tok : 0)) * a.qs + (live ? h : 0) * HD;
-      float top = 0.f;
-      bool finite = true;
-      constexpr int PER16 = 16 / sizeof(T), PART = 8 * PER16;  // elements held at once: 128 bytes
-      uint4 raw[8];
-      auto get = [&](int d0) {
-#pragma unroll
-        for (int j = 0; j < 8; j++)
-          raw[j] = live ? __ldg(reinterpret_cast<const uint4 *>(src + d0 + j * PER16)) : make_uint4(0, 0, 0, 0);
+      const int warp_row = x * TILE_ROWS + 32 * (warp & 3);  // first of the warp's 32 rows
+      // Rows of the warp move in and out ROW_LANES lanes a row, 16 bytes a lane.
+      constexpr int ROW_LANES = HD * (int)sizeof(T) / 16, AT_ONCE = 32 / ROW_LANES, PER16 = 16 / (int)sizeof(T);
+      const int sub = lane / ROW_LANES, piece16 = lane % ROW_LANES;
+      auto row_at = [&](const auto *rows, long long stride, int i) {  // the lane's part of the warp's row i
+        const int q = warp_row + i, t = q / a.group;
+        return rows + (long long)(row0 + t) * stride + (h0 + q - t * a.group) * HD + piece16 * PER16;
       };
-      auto pair = [&](int j) {  // elements 2 j, 2 j + 1 of those held
-        const uint4 u = raw[2 * j / PER16];
-        if constexpr (SPLIT) {
-          return j & 1 ? make_float2(__uint_as_float(u.z), __uint_as_float(u.w))
-                       : make_float2(__uint_as_float(u.x), __uint_as_float(u.y));
-        } else {
-          const uint32_t w = (j & 3) == 0 ? u.x : (j & 3) == 1 ? u.y : (j & 3) == 2 ? u.z : u.w;
-          return make_float2(__uint_as_float(w << 16), __uint_as_float(w & 0xFFFF0000u));
-        }
+      auto stage = [&](int i, int at) {  // 16-byte chunk `at` of the warp's row i, over the row's bytes in the query tile
+        return base + C::OFF_Q + x * TERMS * C::Q_TILE + (at >> 3) * C::Q_PANEL + (32 * (warp & 3) + i) * 128 +
+               ((at ^ i) & 7) * 16;
       };
+      // ---- the queries: fetched into their tile, then replaced by their f16 terms row by row
 #pragma unroll 1
-      for (int d0 = 0; d0 < HD; d0 += PART) {
-        get(d0);
-#pragma unroll
-        for (int j = 0; j < PART / 2; j++) {
-          const float2 v = pair(j);
-          top = fmaxf(top, fmaxf(fabsf(v.x), fabsf(v.y)));
-          finite &= fabsf(v.x) <= FLT_MAX && fabsf(v.y) <= FLT_MAX;
-        }
+      for (int i = sub; i < 32; i += AT_ONCE) {
+        if (ok && warp_row + i < n_rows) cp16(stage(i, piece16), row_at(a.q, a.qs, i));
+        else sts128(stage(i, piece16), 0, 0, 0, 0);
       }
-      const int e = row_exp(top);
-      // the sign of the scale goes into the row: the factor of its scores is then not negative and maxima commute
-      const float up = row_factor(e, finite) * (a.scale < 0.f ? -1.f : 1.f), cf = scalbnf(fabsf(a.scale), -e);
+      cp_commit();
+      cp_wait<0>();
+      __syncwarp();
+      float cf = 0.f;  // factor of the row's scores
 #pragma unroll 1
-      for (int d0 = 0; d0 < HD; d0 += PART) {
-        get(d0);
+      for (int i = sub; i < 32; i += AT_ONCE) {
+        const uint4 u = lds128(stage(i, piece16));
+        const uint32_t w[4] = {u.x, u.y, u.z, u.w};
+        float v[PER16], top = 0.f;
+        bool finite = true;
 #pragma unroll
-        for (int d = 0; d < PART; d += 8) {
-          uint32_t f[4], g[4];
+        for (int e = 0; e < PER16; e++) {
+          v[e] = SPLIT ? __uint_as_float(w[e % 4]) : __uint_as_float(e & 1 ? w[e / 2] & 0xFFFF0000u : w[e / 2] << 16);
+          top = fmaxf(top, fabsf(v[e]));
+          finite &= fabsf(v[e]) <= FLT_MAX;
+        }
+        if (!finite) top = INFINITY;
 #pragma unroll
-          for (int j = 0; j < 4; j++) {
-            const float2 v = pair(d / 2 + j);
-            const float y0 = v.x * up, y1 = v.y * up;
-            f[j] = pack(y0, y1);
-            const float2 hi = unpack(f[j]);
-            g[j] = pack(y0 - hi.x, y1 - hi.y);
-          }
-          const uint32_t dst = base + C::OFF_Q + x * TERMS * C::Q_TILE + ((d0 + d) >> 6) * C::Q_PANEL + r * 128 +
-                               ((((d0 + d) >> 3) & 7) ^ (r & 7)) * 16;
-          sts128(dst, f[0], f[1], f[2], f[3]);
-          if (SPLIT) sts128(dst + C::Q_TILE, g[0], g[1], g[2], g[3]);
+        for (int o = 1; o < ROW_LANES; o <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+        finite = top <= FLT_MAX;
+        const int e = row_exp(finite ? top : 0.f);
+        // the sign of the scale goes into the row: the factor of its scores is then not negative and maxima commute
+        const float up = row_factor(e, finite) * (a.scale < 0.f ? -1.f : 1.f);
+        const int e_mine = __shfl_sync(0xffffffffu, e, (lane % AT_ONCE) * ROW_LANES);
+        if (lane / AT_ONCE == i / AT_ONCE) cf = scalbnf(fabsf(a.scale), -e_mine);  // lane: row i of the warp
+        uint32_t f[PER16 / 2], g[PER16 / 2];
+#pragma unroll
+        for (int z = 0; z < PER16 / 2; z++) {
+          const float y0 = v[2 * z] * up, y1 = v[2 * z + 1] * up;
+          f[z] = pack(y0, y1);
+          const float2 hi = unpack(f[z]);
+          g[z] = pack(y0 - hi.x, y1 - hi.y);
+        }
+        // the terms of dimensions d .. : 8 elements a chunk, second terms in the panels after the first ones'
+        const int d = piece16 * PER16;
+        if constexpr (SPLIT) {
+          __syncwarp();  // the row has been read
+          sts64(stage(i, d / 8) + (d & 7) * 2, f[0], f[1]);
+          sts64(stage(i, HD / 8 + d / 8) + (d & 7) * 2, g[0], g[1]);
+        } else {
+          sts128(stage(i, piece16), f[0], f[1], f[2], f[3]);
         }
       }
       fence_proxy_async();
@@ -772,7 +768,6 @@ __global__ void __launch_bounds__(THREADS, 1) k_paged_many(const AttnArgs<T> a) 
       const int pos = live ? pos0 + tok : -1;
       const int low = a.window ? pos - a.window : -1;  // seen: low < key <= pos, or key < sinks
       const int sinks = a.window ? a.sinks : 0;
-      const int warp_row = x * TILE_ROWS + 32 * (warp & 3);  // rows of the warp: for the test whether to mask
       const int min_pos = pos0 + warp_row / a.group, max_pos = pos0 + (warp_row + 31) / a.group;
       float o[SPLIT ? HD : 1], ref = -INFINITY, l = 0.f, unit = 0.f;
       if constexpr (SPLIT) {
@@ -796,7 +791,7 @@ __global__ void __launch_bounds__(THREADS, 1) k_paged_many(const AttnArgs<T> a) 
 #pragma unroll 1
       for (int i = 0; ok && active && n && i <= n; i++) {
         if (i == n) {
-          ok = wait_warp(B_PV + x, tile_done + n - 1);
+          ok = wait(B_PV + x, tile_done + n - 1);
           fence_after();
           if (ok) add_output(unit);
           break;
@@ -804,8 +799,8 @@ __global__ void __launch_bounds__(THREADS, 1) k_paged_many(const AttnArgs<T> a) 
         const unsigned t = tile_done + i, bt = batch + i / BATCH;
         const uint32_t s_col = s_tile + (t & 1) * 64;
         const Plan &plan = plans[bt % BATCHES * BATCH + i % BATCH];
-        if (i % BATCH == 0 && !(ok = wait_warp(B_PLAN + bt % BATCHES, bt / BATCHES))) break;
-        if (!(ok = wait_warp(B_S + 2 * x + (t & 1), t / 2))) break;
+        if (i % BATCH == 0 && !(ok = wait(B_PLAN + bt % BATCHES, bt / BATCHES))) break;
+        if (!(ok = wait(B_S + 2 * x + (t & 1), t / 2))) break;
         fence_after();
         float v[64];
         tmem_ld32(s_col, v);
@@ -886,7 +881,7 @@ __global__ void __launch_bounds__(THREADS, 1) k_paged_many(const AttnArgs<T> a) 
         if (!SPLIT && unit != new_unit) move *= new_unit > 0.f ? unit / new_unit : 0.f;
         const bool any = i && __any_sync(0xffffffffu, move != 1.f);
         if (i && (SPLIT || any)) {  // the last block's P V is done before its output is read or moved
-          if (!(ok = wait_warp(B_PV + x, t - 1))) break;
+          if (!(ok = wait(B_PV + x, t - 1))) break;
           fence_after();
           add_output(unit);
           if (any) {
@@ -918,21 +913,29 @@ __global__ void __launch_bounds__(THREADS, 1) k_paged_many(const AttnArgs<T> a) 
       batch += (n + BATCH - 1) / BATCH;
       const bool none = !active || !n;  // nothing was computed: l = 0, O is not the tile's
       const bool whole = piece.whole;
-      T *dst = a.out + (long long)(piece.row0 + tok) * a.os + h * HD;
       float *slot = a.part + (size_t)piece.slot * C::SLOT + row;  // [head_dim][rows], maxima, sums
       const float inv = l == 0.f ? 0.f : 1.f / l;
-      auto write = [&](int d, const float *v) {  // 32 values
-        if (!live) return;
-        if constexpr (SPLIT) {
+      // Results go out through the warp's own rows of the query tile (its products are done; other warps may be at
+      // the next piece's queries): a thread writes its row, then ROW_LANES lanes a row store 16 bytes each.
+      auto write = [&](int d, const float *v) {  // 32 values of the thread's row
 #pragma unroll
-          for (int j = 0; j < 32; j += 4) store4(dst + d + j, make_float4(v[j], v[j + 1], v[j + 2], v[j + 3]));
-        } else {
-#pragma unroll
-          for (int j = 0; j < 32; j += 8)
-            *reinterpret_cast<uint4 *>(dst + d + j) =
-                make_uint4(bf16_pair(v[j], v[j + 1]), bf16_pair(v[j + 2], v[j + 3]), bf16_pair(v[j + 4], v[j + 5]),
-                           bf16_pair(v[j + 6], v[j + 7]));
+        for (int j = 0; j < 32; j += PER16) {
+          const uint32_t dst = stage(lane, (d + j) / PER16);
+          if constexpr (SPLIT)
+            sts128(dst, __float_as_uint(v[j]), __float_as_uint(v[j + 1]), __float_as_uint(v[j + 2]), __float_as_uint(v[j + 3]));
+          else
+            sts128(dst, bf16_pair(v[j], v[j + 1]), bf16_pair(v[j + 2], v[j + 3]), bf16_pair(v[j + 4], v[j + 5]),
+                   bf16_pair(v[j + 6], v[j + 7]));
         }
+      };
+      auto flush = [&]() {
+        __syncwarp();
+#pragma unroll 1
+        for (int i = sub; i < 32; i += AT_ONCE) {
+          const uint4 u = lds128(stage(i, piece16));
+          if (warp_row + i < n_rows) *reinterpret_cast<uint4 *>(const_cast<T *>(row_at(a.out, a.os, i))) = u;
+        }
+        __syncwarp();
       };
       auto put = [&](int d, float *v) {
         if (whole) {
@@ -958,7 +961,9 @@ __global__ void __launch_bounds__(THREADS, 1) k_paged_many(const AttnArgs<T> a) 
           put(d, v);
         }
       }
-      if (!whole) {  // the last block to arrive joins all parts, in block order
+      if (whole) {
+        flush();
+      } else {  // the last block to arrive joins all parts, in block order
         slot[HD * ROWS] = ref;
         slot[(HD + 1) * ROWS] = l;
         int *count = a.count + piece.counter;
@@ -970,8 +975,7 @@ __global__ void __launch_bounds__(THREADS, 1) k_paged_many(const AttnArgs<T> a) 
         if (s_last) {
           __threadfence();
           auto part = [&](int i) { return a.part + (size_t)(2 * (first + i) + (i == 0 ? late : 0)) * C::SLOT + row; };
-          top = -INFINITY;
-          float sum = 0.f;
+          float top = -INFINITY, sum = 0.f;
 #pragma unroll 1
           for (int i = 0; i < parts; i++) top = fmaxf(top, __ldcg(part(i) + HD * ROWS));
           const float at0 = top == -INFINITY ? 0.f : top;
@@ -995,6 +999,7 @@ __global__ void __launch_bounds__(THREADS, 1) k_paged_many(const AttnArgs<T> a) 
             for (int j = 0; j < 32; j++) v[j] = sum == 0.f ? 0.f : v[j] * all_inv;
             write(d, v);
           }
+          flush();
           if (tid == 0) *count = 0;
         }
       }
