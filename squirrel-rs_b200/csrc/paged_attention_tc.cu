@@ -560,21 +560,19 @@ __global__ void __launch_bounds__(THREADS, 1) k_paged_many(const AttnArgs<T> a) 
           const unsigned now = done + i, ahead = now + 2;
           const int st = now % STAGES, st2 = ahead % STAGES;
           const bool more = i + 2 < n;
+          // K of block i + 2 comes after V of block i + 1: one wait for both, well before it is needed
+          if (!(ok = more ? wait(B_K + st2, ahead / STAGES) : i < 0 || wait(B_V + st, now / STAGES))) break;
+          fence_after();
 #pragma unroll 1
           for (int x = 0; x < tiles; x++) {
             const unsigned t = (x ? tile_done[1] : tile_done[0]) + i;  // of this tile: buffer t % 2, its turn t / 2
             const int buf = t & 1;
             if (i >= 0) {
               if (!(ok = wait(B_P + 2 * x + buf, t / 2))) break;
-              if (x == 0 && !(ok = wait(B_V + st, now / STAGES))) break;
               fence_after();
               output(x, buf, st, !SPLIT && i);
             }
-            if (more) {
-              if (x == 0 && !(ok = wait(B_K + st2, ahead / STAGES))) break;
-              fence_after();
-              scores(x, buf, st2);
-            }
+            if (more) scores(x, buf, st2);
           }
           if (!ok) break;
           if (more) commit(B_K_FREE + st2);
@@ -712,7 +710,7 @@ __global__ void __launch_bounds__(THREADS, 1) k_paged_many(const AttnArgs<T> a) 
                ((at ^ i) & 7) * 16;
       };
       // ---- the queries: fetched into their tile, then replaced by their f16 terms row by row
-#pragma unroll 1
+#pragma unroll 4
       for (int i = sub; i < 32; i += AT_ONCE) {
         if (ok && warp_row + i < n_rows) cp16(stage(i, piece16), row_at(a.q, a.qs, i));
         else sts128(stage(i, piece16), 0, 0, 0, 0);
@@ -721,7 +719,7 @@ __global__ void __launch_bounds__(THREADS, 1) k_paged_many(const AttnArgs<T> a) 
       cp_wait<0>();
       __syncwarp();
       float cf = 0.f;  // factor of the row's scores
-#pragma unroll 1
+#pragma unroll 2
       for (int i = sub; i < 32; i += AT_ONCE) {
         const uint4 u = lds128(stage(i, piece16));
         const uint32_t w[4] = {u.x, u.y, u.z, u.w};
@@ -930,7 +928,7 @@ __global__ void __launch_bounds__(THREADS, 1) k_paged_many(const AttnArgs<T> a) 
       };
       auto flush = [&]() {
         __syncwarp();
-#pragma unroll 1
+#pragma unroll 4
         for (int i = sub; i < 32; i += AT_ONCE) {
           const uint4 u = lds128(stage(i, piece16));
           if (warp_row + i < n_rows) *reinterpret_cast<uint4 *>(const_cast<T *>(row_at(a.out, a.os, i))) = u;
