@@ -34,30 +34,32 @@ unsigned *err_ptr() {
 }
 
 int check_cache(const sq_paged_cache *c, Cache *out, const char *what) {
-  const std::string w = std::string(what) + ": ";
-  if (!c || !c->k || !c->v || !c->k_scale || !c->v_scale) return fail(SQ_ERR_ARG, w + "null cache pointer");
-  if (c->n_pages <= 0 || c->n_kv_heads <= 0) return fail(SQ_ERR_SHAPE, w + "a cache has pages and kv heads");
+  auto fail = [&](int code, const char *msg) { return sq::fail(code, std::string(what) + ": " + msg); };
+  if (!c || !c->k || !c->v || !c->k_scale || !c->v_scale) return fail(SQ_ERR_ARG, "null cache pointer");
+  if (c->n_pages <= 0 || c->n_kv_heads <= 0) return fail(SQ_ERR_SHAPE, "a cache has pages and kv heads");
   int shift = 4;
   while (shift < 8 && (1 << shift) != c->page) shift++;
-  if ((1 << shift) != c->page) return fail(SQ_ERR_SHAPE, w + "a page holds 16, 32, 64, 128 or 256 positions");
+  if ((1 << shift) != c->page) return fail(SQ_ERR_SHAPE, "a page holds 16, 32, 64, 128 or 256 positions");
   if (c->head_dim != 32 && c->head_dim != 64 && c->head_dim != 128 && c->head_dim != 256)
-    return fail(SQ_ERR_SHAPE, w + "head_dim must be 32, 64, 128 or 256");
+    return fail(SQ_ERR_SHAPE, "head_dim must be 32, 64, 128 or 256");
+  if ((long long)c->n_pages * c->n_kv_heads * (c->page / 16) > INT32_MAX)
+    return fail(SQ_ERR_SHAPE, "the cache's groups of 16 positions and kv heads must be countable in 31 bits");
   if (((uintptr_t)c->k | (uintptr_t)c->v) & 15 || ((uintptr_t)c->k_scale | (uintptr_t)c->v_scale) & 3)
-    return fail(SQ_ERR_ALIGN, w + "codes must be 16-byte aligned, scales 4-byte");
+    return fail(SQ_ERR_ALIGN, "codes must be 16-byte aligned, scales 4-byte");
   *out = {c->k, c->v, c->k_scale, c->v_scale, c->n_pages, c->n_kv_heads, c->page, shift, c->head_dim};
   return SQ_OK;
 }
 
 int check_batch(const sq_paged_batch *b, Batch *out, const char *what) {
-  const std::string w = std::string(what) + ": ";
-  if (!b || !b->q_start || !b->kv_len || !b->page_table) return fail(SQ_ERR_ARG, w + "null batch pointer");
-  if (b->n_seqs <= 0 || b->n_seqs > 65535) return fail(SQ_ERR_SHAPE, w + "1 to 65535 sequences");
+  auto fail = [&](int code, const char *msg) { return sq::fail(code, std::string(what) + ": " + msg); };
+  if (!b || !b->q_start || !b->kv_len || !b->page_table) return fail(SQ_ERR_ARG, "null batch pointer");
+  if (b->n_seqs <= 0 || b->n_seqs > 65535) return fail(SQ_ERR_SHAPE, "1 to 65535 sequences");
   if (b->n_tokens < 0 || b->max_new < 0 || b->max_new > b->n_tokens || (b->n_tokens && !b->max_new) ||
       (long long)b->max_new * b->n_seqs < b->n_tokens)
-    return fail(SQ_ERR_SHAPE, w + "max_new must be the most new tokens of one sequence");
-  if (b->pages_per_seq <= 0) return fail(SQ_ERR_SHAPE, w + "a page table has columns");
+    return fail(SQ_ERR_SHAPE, "max_new must be the most new tokens of one sequence");
+  if (b->pages_per_seq <= 0) return fail(SQ_ERR_SHAPE, "a page table has columns");
   if (((uintptr_t)b->q_start | (uintptr_t)b->kv_len | (uintptr_t)b->page_table) & 3)
-    return fail(SQ_ERR_ALIGN, w + "batch arrays must be 4-byte aligned");
+    return fail(SQ_ERR_ALIGN, "batch arrays must be 4-byte aligned");
   *out = {b->q_start, b->kv_len, b->page_table, b->n_seqs, b->n_tokens, b->max_new, b->pages_per_seq, nullptr};
   return SQ_OK;
 }

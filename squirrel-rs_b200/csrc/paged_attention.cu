@@ -18,13 +18,19 @@
 // power of two; an f32 row takes two f16 terms (22 bits) in two columns of the same tile, a bf16
 // row is exact in one. Weights, at most 2^10 (the maximum's), likewise: two terms for f32
 // rows, one (11 bits, under the output's 8) for bf16 rows. The V scale of a page goes
-// into the weights relative to the largest met so far, so f16 never overflows.
+// into the weights relative to the largest met so far, so f16 never overflows. K's codes
+// enter as the f16 numbers code * 2^-24 (denormal, exact; one instruction a pair) and
+// their bias leaves with the sum of the row, 128 sum(q): that costs a score two bits of 24
+// at most. V's bias is taken off before the product: an output is an average that may be
+// a thousand times smaller than 128. The tensor core truncates its running sum (2^-25 of it a
+// step on average), so f32 rows move their sums every 16 steps to f32 sums in shared memory.
 //
 // Work is split evenly over the grid: the (sequence, kv head, row tile, key tile) space is
 // one line, every block takes an equal piece of it, the four warps of a block take its key
 // tiles in turn. A row tile cut by a block's end leaves partial results in the workspace
 // and the last block to arrive joins them, in block order (equal bits every call).
 #include <float.h>
+#include <limits.h>
 #include <math.h>
 
 #include <string>
@@ -39,6 +45,7 @@ constexpr int WARPS = 4, THREADS = WARPS * 32, STAGES = 2;
 constexpr int BLOCKS_PER_SM = 3;
 constexpr int MAX_BLOCKS = 160 * BLOCKS_PER_SM;
 constexpr int MIN_TILES = WARPS;  // key tiles a block takes at least
+constexpr int FLUSH_STEPS = 16;   // f32 rows: 16-key products summed on the tensor core at a stretch
 constexpr int SLOT_FLOATS = 2112;  // partial results of one row tile: rows x (head_dim + 2), 32 x 66 at most
 constexpr size_t PARTIAL_BYTES = (size_t)MAX_BLOCKS * 2 * SLOT_FLOATS * 4;
 constexpr float WEIGHT_EXP = 10.f;  // weights are 2^(s - max + 10)
@@ -48,6 +55,9 @@ __device__ __forceinline__ uint2 lds64(uint32_t a) {
   asm volatile("ld.shared.v2.u32 {%0, %1}, [%2];" : "=r"(v.x), "=r"(v.y) : "r"(a));
   return v;
 }
+// Codes (bytes 0, 2) and (1, 3) of a word as pairs of f16 numbers code * 2^-24.
+__device__ __forceinline__ uint32_t codes_02(uint32_t w) { return w & 0x00FF00FFu; }
+__device__ __forceinline__ uint32_t codes_13(uint32_t w) { return __byte_perm(w, 0, 0x4341); }
 __device__ __forceinline__ uint32_t transpose8x8(uint32_t x) {
   uint32_t y;
   asm("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(y) : "r"(x));
@@ -70,9 +80,13 @@ struct Cfg {
   static constexpr int NG = TK / 16;                     // groups of 16 keys: each within one page
   static constexpr int TILE = TK * HD;                   // bytes of one operand's tile
   static constexpr int KS = HD / 16;                     // 16-dimension steps
-  static constexpr int SMEM = WARPS * STAGES * 2 * TILE;
+  static constexpr int RING = WARPS * STAGES * 2 * TILE;
+  static constexpr int SUMS = SPLIT ? WARPS * 32 * (HD / 16) * NT * 4 * 4 : 0;  // f32 rows: a lane's output sums
+  static constexpr int SMEM = RING + SUMS;
+  static constexpr int BATCH = 32 / NG;  // tiles whose pages a warp looks up at once
+  static constexpr int BLOCKS = NT <= 2 && 3 * SMEM <= 223 * 1024 ? BLOCKS_PER_SM : 2;
   static_assert(ROWS * (HD + 2) <= SLOT_FLOATS, "a row tile's partial results fit a slot");
-  static_assert(WARPS * ROWS * (HD + 2) * 4 <= SMEM, "the warps' results fit the ring");
+  static_assert(WARPS * ROWS * (HD + 2) * 4 <= RING, "the warps' results fit the ring");
 };
 
 // Byte offset of 16-byte chunk c of key r in a group of 16 keys. Chunks are permuted
@@ -113,7 +127,7 @@ __device__ __forceinline__ Span key_span(const Seq &s, int window, int sinks) {
 }
 
 template <class C, typename T>
-__global__ void __launch_bounds__(THREADS, C::NT <= 2 ? BLOCKS_PER_SM : 2) k_paged_few(const AttnArgs<T> a) {
+__global__ void __launch_bounds__(THREADS, C::BLOCKS) k_paged_few(const AttnArgs<T> a) {
   constexpr int HD = C::HD, NT = C::NT, TK = C::TK, NG = C::NG, KS = C::KS, ROWS = C::ROWS, RN = C::ROWS_NT;
   constexpr int MT = HD / 16;  // 16-dimension tiles of the output
   extern __shared__ __align__(128) uint8_t ring[];
@@ -190,7 +204,7 @@ __global__ void __launch_bounds__(THREADS, C::NT <= 2 ? BLOCKS_PER_SM : 2) k_pag
 
     // ---- query fragments: column g of tile nt = row nt * RN + g % RN, term g / RN
     uint32_t qf[NT][KS][2];
-    float cf[NT][2];   // factor of the lane's two columns' scores
+    float cf[NT][2], cb[NT][2];  // factor and offset of the lane's two columns' scores
     int pos[NT][2];    // and their rows' positions (-1: no such row)
 #pragma unroll
     for (int nt = 0; nt < NT; nt++) {
@@ -217,25 +231,33 @@ __global__ void __launch_bounds__(THREADS, C::NT <= 2 ? BLOCKS_PER_SM : 2) k_pag
       const int e = row_exp(top);
       const float up = row_factor(e, finite);
       const float down = scalbnf(a.scale, -e);
+      float sum = 0.f;  // of the row's terms, for the bias of the codes
 #pragma unroll
       for (int i = 0; i < KS; i++) {
 #pragma unroll
-        for (int j = 0; j < 2; j++) {
-          const float u = x[4 * i + 2 * j] * up, v = x[4 * i + 2 * j + 1] * up;
+        for (int j = 0; j < 2; j++) {  // dimensions 4 i + j and 4 i + j + 2: bytes of a word two apart
+          const float u = x[4 * i + j] * up, v = x[4 * i + j + 2] * up;
           uint32_t f = pack(u, v);
-          if (C::SPLIT && g >= RN) {
-            const float2 hi = unpack(f);
-            f = pack(u - hi.x, v - hi.y);
+          const float2 hi = unpack(f);
+          sum += hi.x + hi.y;
+          if (C::SPLIT) {
+            const uint32_t lo = pack(u - hi.x, v - hi.y);
+            const float2 l2 = unpack(lo);
+            sum += l2.x + l2.y;
+            if (g >= RN) f = lo;
           }
           qf[nt][i][j] = f;
         }
       }
+      sum += __shfl_xor_sync(0xffffffffu, sum, 1);
+      sum += __shfl_xor_sync(0xffffffffu, sum, 2);
 #pragma unroll
       for (int j = 0; j < 2; j++) {  // column 2t + j is row (2t + j) % RN: held by lanes of that g
         const int from = ((2 * t + j) & (RN - 1)) * 4;
-        cf[nt][j] = __shfl_sync(0xffffffffu, down, from);
-        const int p = __shfl_sync(0xffffffffu, ok ? pos0 + tok : -1, from);
-        pos[nt][j] = p;
+        const float d = __shfl_sync(0xffffffffu, down, from), q = __shfl_sync(0xffffffffu, sum, from);
+        cf[nt][j] = d * 16777216.f;
+        cb[nt][j] = -128.f * q * d;
+        pos[nt][j] = __shfl_sync(0xffffffffu, ok ? pos0 + tok : -1, from);
       }
     }
     const int last_row = min((rt + 1) * ROWS, s.n * rows_of_token) - 1;
@@ -251,56 +273,110 @@ __global__ void __launch_bounds__(THREADS, C::NT <= 2 ? BLOCKS_PER_SM : 2) k_pag
 #pragma unroll
         for (int i = 0; i < 4; i++) o[mt][nt][i] = 0.f;
     }
-
-    // ---- this warp's key tiles t0 + wid, + WARPS, ...
-    auto tile_key = [&](int i) { return (i < span.n_sink ? i : i + span.skip) * TK; };
-    // Lane j < NG holds group j's page (-1: none) and, once loaded, its scales.
-    auto page_of = [&](int i) {
-      const int key = tile_key(i) + 16 * lane;
-      return i < t1 && lane < NG && key < s.len ? load_page(a.b, c, b, key) : -1;
+    // f32 rows: sums[i][lane] += o every few tiles; `late` is what they have still to be multiplied by
+    float *sums = reinterpret_cast<float *>(ring + C::RING) + wid * (32 * MT * NT * 4) + lane;
+    float late[NT][2];
+    if constexpr (C::SPLIT) {
+#pragma unroll
+      for (int nt = 0; nt < NT; nt++) late[nt][0] = late[nt][1] = 1.f;
+#pragma unroll
+      for (int i = 0; i < MT * NT * 4; i++) sums[i * 32] = 0.f;
+    }
+    auto flush = [&]() {
+#pragma unroll
+      for (int mt = 0; mt < MT; mt++)
+#pragma unroll
+        for (int nt = 0; nt < NT; nt++)
+#pragma unroll
+          for (int i = 0; i < 4; i++) {
+            float *p = sums + ((mt * NT + nt) * 4 + i) * 32;
+            *p = fmaf(*p, late[nt][i & 1], o[mt][nt][i]);
+            o[mt][nt][i] = 0.f;
+          }
+#pragma unroll
+      for (int nt = 0; nt < NT; nt++) late[nt][0] = late[nt][1] = 1.f;
     };
-    auto load_tile = [&](int i, int page, int stage, float &ks, float &vs) {
-      ks = vs = 0.f;
-      if (i < t1) {
-        if (page >= 0) {
-          ks = c.ks[(long long)page * c.kv_heads + head];
-          vs = c.vs[(long long)page * c.kv_heads + head];
-        }
-        const int key0 = tile_key(i);
+
+    // ---- this warp's key tiles: the k-th is t0 + wid + k WARPS. Lane NG q + j of a batch of tiles holds the place (in
+    // groups of 16 keys; -1: none) and the scales of group j of its tile q. A batch's table entries are loaded a batch
+    // ahead, its scales half a batch ahead.
+    auto tile_key = [&](int k) {
+      const int i = t0 + wid + k * WARPS;
+      return (i < span.n_sink ? i : i + span.skip) * TK;
+    };
+    const int n_tiles = t1 - t0 > wid ? (t1 - t0 - wid + WARPS - 1) / WARPS : 0;
+    constexpr int BATCH = C::BATCH;
+    auto entry_of = [&](int batch) {  // INT_MIN: no such group
+      const int k = batch * BATCH + lane / NG, key = tile_key(k) + 16 * (lane % NG);
+      return k < n_tiles && key < s.len ? a.b.table[(long long)b * a.b.table_row + (key >> c.page_shift)] : INT_MIN;
+    };
+    auto place_of = [&](int batch, int entry) {
+      if ((unsigned)entry >= (unsigned)c.n_pages) {
+        if (entry != INT_MIN) flag(a.b.err, BAD_PAGE);
+        return -1;
+      }
+      const int key = tile_key(batch * BATCH + lane / NG) + 16 * (lane % NG);
+      return ((entry * c.kv_heads + head) << (c.page_shift - 4)) + ((key & (c.page - 1)) >> 4);
+    };
+    auto scale_of = [&](const float *scales, int place) { return place < 0 ? 0.f : scales[place >> (c.page_shift - 4)]; };
+    // 16-byte pieces of a group of 16 keys: lane + 32 k, at lane_at(k) in the group's room in shared memory.
+    auto lane_at = [&](int k) { return chunk_at<HD>((k * 32 + lane) / (HD / 16), (k * 32 + lane) % (HD / 16)); };
+    const uint8_t *my_k = c.k + lane * 16, *my_v = c.v + lane * 16;
+    auto load_tile = [&](int k, int place, int stage) {  // `place`: of the tile's batch
+      if (k < n_tiles) {
         const uint32_t dst = my_ring + stage * (2 * C::TILE);
 #pragma unroll
         for (int j = 0; j < NG; j++) {
-          const int p = __shfl_sync(0xffffffffu, page, j);
+          const int p = __shfl_sync(0xffffffffu, place, k % BATCH * NG + j);
           if (p < 0) continue;
-          const long long src = (((long long)p * c.kv_heads + head) * c.page + ((key0 + 16 * j) & (c.page - 1))) * HD;
+          const uint8_t *ksrc = my_k + (long long)p * (16 * HD), *vsrc = my_v + (long long)p * (16 * HD);
 #pragma unroll
-          for (int k = 0; k < HD / 32; k++) {
-            const int q = k * 32 + lane;
-            const uint32_t d = dst + j * 16 * HD + chunk_at<HD>(q / (HD / 16), q % (HD / 16));
-            cp16(d, c.k + src + q * 16);
-            cp16(d + C::TILE, c.v + src + q * 16);
+          for (int q = 0; q < HD / 32; q++) {
+            cp16(dst + j * 16 * HD + lane_at(q), ksrc + q * 512);
+            cp16(dst + j * 16 * HD + lane_at(q) + C::TILE, vsrc + q * 512);
           }
         }
       }
       cp_commit();
     };
-    float ks[STAGES], vs[STAGES];
-    int page[STAGES];
-    int i = t0 + wid;
+    int place = place_of(0, entry_of(0)), entry = entry_of(1), next_place = -1;
+    float ks = scale_of(c.ks, place), vs = scale_of(c.vs, place), next_ks = 0.f, next_vs = 0.f, share = 0.f;
+    int st = 0;
+    if constexpr (BATCH >= STAGES) {
 #pragma unroll
-    for (int st = 0; st < STAGES; st++) {
-      page[st] = page_of(i + st * WARPS);
-      load_tile(i + st * WARPS, page[st], st, ks[st], vs[st]);
+      for (int k = 0; k < STAGES; k++) load_tile(k, place, k);
     }
-    int next_page = page_of(i + STAGES * WARPS);
 #pragma unroll 1
-    for (int st = 0; i < t1; i += WARPS, st ^= 1) {
+    for (int k = 0; k < n_tiles; k++, st ^= 1) {
+      const int in_batch = k % BATCH;
+      if (in_batch == 0) {
+        if (k) place = next_place, ks = next_ks, vs = next_vs, entry = entry_of(k / BATCH + 1);
+        // the largest V scale so far: earlier results move to it
+        const float top = __uint_as_float(__reduce_max_sync(0xffffffffu, __float_as_uint(fmaxf(vs, 0.f))));
+        const float new_unit = fmaxf(unit, top), per_unit = new_unit > 0.f ? 1.f / new_unit : 0.f;
+        const float move = unit * per_unit;
+        if (k && move != 1.f) {
+#pragma unroll
+          for (int nt = 0; nt < NT; nt++) {
+            if (C::SPLIT) late[nt][0] *= move, late[nt][1] *= move;
+#pragma unroll
+            for (int mt = 0; mt < MT; mt++)
+#pragma unroll
+              for (int i = 0; i < 4; i++) o[mt][nt][i] *= move;
+          }
+        }
+        unit = new_unit;
+        share = vs * per_unit;
+      }
+      if (in_batch == BATCH / 2) {
+        next_place = place_of(k / BATCH + 1, entry);
+        next_ks = scale_of(c.ks, next_place);
+        next_vs = scale_of(c.vs, next_place);
+      }
       cp_wait<STAGES - 1>();
       __syncwarp();
+      const int key0 = tile_key(k);
       const uint32_t kt = my_ring + st * (2 * C::TILE), vt = kt + C::TILE;
-      const float tks = st ? ks[1] : ks[0], tvs = st ? vs[1] : vs[0];
-      const int tpage = st ? page[1] : page[0];
-      const int key0 = tile_key(i);
 
       // scores
       float sc[NG][NT][4];
@@ -317,10 +393,10 @@ __global__ void __launch_bounds__(THREADS, C::NT <= 2 ? BLOCKS_PER_SM : 2) k_pag
             const uint4 u = lds128(base + chunk_at<HD>(g, ch * 4 + t)), w = lds128(base + chunk_at<HD>(g + 8, ch * 4 + t));
             const uint32_t uu[4] = {u.x, u.y, u.z, u.w}, ww[4] = {w.x, w.y, w.z, w.w};
 #pragma unroll
-            for (int k = 0; k < 4; k++) {
-              const uint32_t f[4] = {codes_lo(uu[k]), codes_lo(ww[k]), codes_hi(uu[k]), codes_hi(ww[k])};
+            for (int x = 0; x < 4; x++) {
+              const uint32_t f[4] = {codes_02(uu[x]), codes_02(ww[x]), codes_13(uu[x]), codes_13(ww[x])};
 #pragma unroll
-              for (int nt = 0; nt < NT; nt++) mma(sc[j][nt], f, qf[nt][ch * 4 + k][0], qf[nt][ch * 4 + k][1]);
+              for (int nt = 0; nt < NT; nt++) mma(sc[j][nt], f, qf[nt][ch * 4 + x][0], qf[nt][ch * 4 + x][1]);
             }
           }
         } else {
@@ -328,30 +404,30 @@ __global__ void __launch_bounds__(THREADS, C::NT <= 2 ? BLOCKS_PER_SM : 2) k_pag
           const uint2 w = lds64(base + chunk_at<HD>(g + 8, t >> 1) + (t & 1) * 8);
           const uint32_t uu[2] = {u.x, u.y}, ww[2] = {w.x, w.y};
 #pragma unroll
-          for (int k = 0; k < 2; k++) {
-            const uint32_t f[4] = {codes_lo(uu[k]), codes_lo(ww[k]), codes_hi(uu[k]), codes_hi(ww[k])};
+          for (int x = 0; x < 2; x++) {
+            const uint32_t f[4] = {codes_02(uu[x]), codes_02(ww[x]), codes_13(uu[x]), codes_13(ww[x])};
 #pragma unroll
-            for (int nt = 0; nt < NT; nt++) mma(sc[j][nt], f, qf[nt][k][0], qf[nt][k][1]);
+            for (int nt = 0; nt < NT; nt++) mma(sc[j][nt], f, qf[nt][x][0], qf[nt][x][1]);
           }
         }
       }
       // in log2 units, the second terms' columns added to the first's (both then hold the sum)
 #pragma unroll
       for (int j = 0; j < NG; j++) {
-        const float gks = __shfl_sync(0xffffffffu, tks, j);
+        const float gks = __shfl_sync(0xffffffffu, ks, in_batch * NG + j);
 #pragma unroll
         for (int nt = 0; nt < NT; nt++) {
-          const float f0 = cf[nt][0] * gks, f1 = cf[nt][1] * gks;
+          const float f0 = cf[nt][0] * gks, f1 = cf[nt][1] * gks, b0 = cb[nt][0] * gks, b1 = cb[nt][1] * gks;
 #pragma unroll
           for (int x = 0; x < 4; x++) {
             if (C::SPLIT) sc[j][nt][x] += __shfl_xor_sync(0xffffffffu, sc[j][nt][x], 2);
-            sc[j][nt][x] *= x & 1 ? f1 : f0;
+            sc[j][nt][x] = fmaf(sc[j][nt][x], x & 1 ? f1 : f0, x & 1 ? b1 : b0);
           }
         }
       }
-      const unsigned paged_groups = __ballot_sync(0xffffffffu, tpage >= 0);
+      const unsigned there = __ballot_sync(0xffffffffu, place >= 0) >> (in_batch * NG);
       if (key0 + TK - 1 > min_pos || (a.window && key0 <= max_pos - a.window && key0 + TK > a.sinks) ||
-          (paged_groups & ((1u << NG) - 1)) != (1u << NG) - 1) {
+          (there & ((1u << NG) - 1)) != (1u << NG) - 1) {
 #pragma unroll
         for (int j = 0; j < NG; j++)
 #pragma unroll
@@ -360,43 +436,34 @@ __global__ void __launch_bounds__(THREADS, C::NT <= 2 ? BLOCKS_PER_SM : 2) k_pag
 #pragma unroll
             for (int nt = 0; nt < NT; nt++) {
               const int p = pos[nt][x & 1];
-              const bool seen = key <= p && (!a.window || key > p - a.window || key < a.sinks) && (paged_groups >> j & 1);
+              const bool seen = key <= p && (!a.window || key > p - a.window || key < a.sinks) && (there >> j & 1);
               if (!seen) sc[j][nt][x] = -INFINITY;
             }
           }
       }
-      // running maximum; the rows' earlier results move to it and to the largest V scale
-      const float top_vs = lane < NG ? tvs : 0.f;
-      float new_unit = top_vs;
-#pragma unroll
-      for (int x = 1; x < NG; x <<= 1) new_unit = fmaxf(new_unit, __shfl_xor_sync(0xffffffffu, new_unit, x));
-      new_unit = fmaxf(unit, __shfl_sync(0xffffffffu, new_unit, 0));
-      const float per_unit = new_unit > 0.f ? 1.f / new_unit : 0.f;
-      const float unit_corr = unit * per_unit;
-      unit = new_unit;
-      const float share = tvs * per_unit;  // of group `lane`
+      // running maximum; the rows' earlier results move to it
       float corr[NT][2], ref[NT][2];
-      bool moved = unit_corr != 1.f;
+      bool moved = false;
 #pragma unroll
       for (int nt = 0; nt < NT; nt++)
 #pragma unroll
         for (int j = 0; j < 2; j++) {
           float mx = m[nt][j];
 #pragma unroll
-          for (int k = 0; k < NG; k++) mx = fmaxf(mx, fmaxf(sc[k][nt][j], sc[k][nt][2 + j]));
+          for (int x = 0; x < NG; x++) mx = fmaxf(mx, fmaxf(sc[x][nt][j], sc[x][nt][2 + j]));
 #pragma unroll
           for (int x = 4; x < 32; x <<= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, x));
           ref[nt][j] = mx == -INFINITY ? 0.f : mx - WEIGHT_EXP;
-          corr[nt][j] = ex2(m[nt][j] - WEIGHT_EXP - ref[nt][j]);  // 0 while nothing was seen
-          if (mx == m[nt][j]) corr[nt][j] = 1.f;
+          corr[nt][j] = mx == m[nt][j] ? 1.f : ex2(m[nt][j] - mx);  // 0 while nothing was seen
           moved |= corr[nt][j] != 1.f;
-          l[nt][j] *= corr[nt][j];
           m[nt][j] = mx;
         }
       if (__any_sync(0xffffffffu, moved)) {
 #pragma unroll
         for (int nt = 0; nt < NT; nt++) {
-          const float f0 = corr[nt][0] * unit_corr, f1 = corr[nt][1] * unit_corr;
+          const float f0 = corr[nt][0], f1 = corr[nt][1];
+          l[nt][0] *= f0, l[nt][1] *= f1;
+          if (C::SPLIT) late[nt][0] *= f0, late[nt][1] *= f1;
 #pragma unroll
           for (int mt = 0; mt < MT; mt++) {
             o[mt][nt][0] *= f0, o[mt][nt][1] *= f1, o[mt][nt][2] *= f0, o[mt][nt][3] *= f1;
@@ -407,7 +474,7 @@ __global__ void __launch_bounds__(THREADS, C::NT <= 2 ? BLOCKS_PER_SM : 2) k_pag
       uint32_t pf[NG][NT][2];
 #pragma unroll
       for (int j = 0; j < NG; j++) {
-        const float gshare = __shfl_sync(0xffffffffu, share, j);
+        const float gshare = __shfl_sync(0xffffffffu, share, in_batch * NG + j);
 #pragma unroll
         for (int nt = 0; nt < NT; nt++)
 #pragma unroll
@@ -461,13 +528,12 @@ __global__ void __launch_bounds__(THREADS, C::NT <= 2 ? BLOCKS_PER_SM : 2) k_pag
         }
       }
       __syncwarp();  // every lane has read the stage that is loaded next
-      float nks, nvs;
-      const int np = next_page;
-      load_tile(i + STAGES * WARPS, np, st, nks, nvs);
-      next_page = page_of(i + (STAGES + 1) * WARPS);
-      if (st) ks[1] = nks, vs[1] = nvs, page[1] = np;
-      else ks[0] = nks, vs[0] = nvs, page[0] = np;
+      load_tile(k + STAGES, (in_batch + STAGES < BATCH ? place : next_place), st);
+      if constexpr (C::SPLIT) {
+        if (k % (FLUSH_STEPS / NG) == FLUSH_STEPS / NG - 1) flush();
+      }
     }
+    if constexpr (C::SPLIT) flush();
     cp_wait<0>();
     __syncthreads();
 
@@ -491,6 +557,7 @@ __global__ void __launch_bounds__(THREADS, C::NT <= 2 ? BLOCKS_PER_SM : 2) k_pag
 #pragma unroll
           for (int x = 0; x < 2; x++) {
             float v = o[mt][nt][2 * x + j];
+            if (C::SPLIT) v = sums[((mt * NT + nt) * 4 + 2 * x + j) * 32];
             if (C::SPLIT) v += __shfl_xor_sync(0xffffffffu, v, 2);
             const int d = HD >= 128 ? (mt / 8) * 128 + g * 16 + (mt % 8) * 2 + x : g * (HD / 8) + mt * 2 + x;
             if (col < RN) dst[2 + d] = v * unit;

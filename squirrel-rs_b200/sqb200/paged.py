@@ -17,7 +17,7 @@ import ctypes as C
 import torch
 
 from . import lib
-from .lib import KernelError, _check, _stream
+from .lib import KernelError, _check
 
 _KINDS = {torch.float32: lib.F32, torch.bfloat16: lib.BF16}
 _SHAPE, _TYPE, _ARG = 1, 2, 5
@@ -30,19 +30,38 @@ def _need(ok, code, what):
 
 def _kind(t):
     kind = _KINDS.get(t.dtype)
-    _need(kind is not None, _TYPE, "rows must be float32 or bfloat16")
+    if kind is None:
+        raise KernelError(_TYPE, "rows must be float32 or bfloat16")
     return kind
 
 
 def _rows(t, rows, width, dtype, what):
-    """A [rows, width] tensor of dtype whose rows may be a slice of wider ones."""
-    if t.dim() != 2 or t.shape[0] != rows or t.shape[1] != width or (width > 1 and t.stride(1) != 1):
-        raise KernelError(_SHAPE, f"{what}: {rows} rows of {width} consecutive elements are wanted")
-    if t.dtype != dtype:
+    """Address and row stride of a [rows, width] tensor of dtype whose rows may be a slice of
+    wider ones."""
+    if t.dtype is not dtype:
         raise KernelError(_TYPE, f"{what}: {dtype} is wanted")
+    if t.shape != (rows, width):
+        raise KernelError(_SHAPE, f"{what}: {rows} rows of {width} elements are wanted")
+    stride, step = t.stride()
+    if step != 1 and width > 1:
+        raise KernelError(_SHAPE, f"{what}: a row's elements must be consecutive")
     if not t.is_cuda:
         raise KernelError(_ARG, f"{what}: a CUDA tensor is wanted")
-    return t.data_ptr(), t.stride(0)
+    return t.data_ptr(), stride if rows > 1 else width  # one row: its stride says nothing
+
+
+# The calls take a microsecond or two of GPU time at their smallest, so the binding keeps
+# what it can: the entry points, the structs' addresses, torch's raw stream lookup.
+_raw_stream = torch._C._cuda_getCurrentRawStream
+_device = torch.cuda.current_device
+_entry = {}
+
+
+def _fn(name):
+    f = _entry.get(name)
+    if f is None:
+        f = _entry[name] = getattr(lib.load(), name)
+    return f
 
 
 class PagedCache:
@@ -61,6 +80,7 @@ class PagedCache:
               "a cache is CUDA tensors of one device")
         self.k, self.v, self.k_scale, self.v_scale = k, v, k_scale, v_scale
         self.n_pages, self.n_kv_heads, self.page, self.head_dim = k.shape
+        self.row, self.half, self.scale = self.n_kv_heads * self.head_dim, self.head_dim // 2, self.head_dim ** -0.5
         self.desc = lib.PagedCacheDesc(k.data_ptr(), v.data_ptr(), k_scale.data_ptr(), v_scale.data_ptr(), *k.shape)
         self.ref = C.pointer(self.desc)
 
@@ -89,8 +109,8 @@ class PagedBatch:
               q_start.shape == (kv_len.shape[0] + 1,), _SHAPE,
               "q_start [n_seqs + 1], kv_len [n_seqs], page_table [n_seqs, pages_per_seq]")
         self.q_start, self.kv_len, self.page_table = q_start, kv_len, page_table
-        self.n_tokens, self.max_new = n_tokens, max_new
-        self.desc = lib.PagedBatchDesc(q_start.data_ptr(), kv_len.data_ptr(), page_table.data_ptr(), kv_len.shape[0],
+        self.n_seqs, self.n_tokens, self.max_new = kv_len.shape[0], n_tokens, max_new
+        self.desc = lib.PagedBatchDesc(q_start.data_ptr(), kv_len.data_ptr(), page_table.data_ptr(), self.n_seqs,
                                        n_tokens, max_new, page_table.shape[1])
         self.ref = C.pointer(self.desc)
         self._workspaces = {}
@@ -100,7 +120,7 @@ class PagedBatch:
         ws = self._workspaces.get(key)
         if ws is None:
             size = C.c_size_t()
-            _check(lib.load().sq_paged_attention_workspace(cache.ref, self.ref, n_heads, C.byref(size)))
+            _check(_fn("sq_paged_attention_workspace")(cache.ref, self.ref, n_heads, C.byref(size)))
             t = torch.zeros(size.value, dtype=torch.uint8, device=cache.k.device)
             ws = self._workspaces[key] = (t, t.data_ptr(), size.value)
         return ws
@@ -110,25 +130,29 @@ def append(cache, batch, k, v, cos, sin, q=None, q_out=None):
     """Rotate k [n_tokens, n_kv_heads * head_dim] to its positions and store it and v in the
     pages; rotate q [n_tokens, n_heads * head_dim], if given, and return it (in q_out, which
     may be q, or a new tensor). cos, sin: [positions, head_dim / 2] float32."""
-    width = cache.n_kv_heads * cache.head_dim
+    n, width, dtype = batch.n_tokens, cache.row, k.dtype
     kind = _kind(k)
-    kp, ks = _rows(k, batch.n_tokens, width, k.dtype, "k")
-    vp, vs = _rows(v, batch.n_tokens, width, k.dtype, "v")
+    kp, ks = _rows(k, n, width, dtype, "k")
+    vp, vs = _rows(v, n, width, dtype, "v")
+    positions = cos.shape[0]
     for t in (cos, sin):
-        _need(t.dim() == 2 and t.shape[1] == cache.head_dim // 2 and t.shape[0] == cos.shape[0] and
-              t.is_contiguous() and t.dtype == torch.float32 and t.is_cuda, _SHAPE,
-              "rotation tables are contiguous float32 [positions, head_dim / 2] on the GPU")
+        if t.shape != (positions, cache.half) or t.dtype is not torch.float32 or not t.is_contiguous() or not t.is_cuda:
+            raise KernelError(_SHAPE, "rotation tables are contiguous float32 [positions, head_dim / 2] on the GPU")
     qp = qop = None
     qs = qos = n_heads = 0
     if q is not None:
-        _need(q.dim() == 2 and q.shape[1] % cache.head_dim == 0, _SHAPE, "q: rows of whole heads are wanted")
-        n_heads = q.shape[1] // cache.head_dim
+        q_width = q.shape[1] if q.dim() == 2 else 0
+        n_heads = q_width // cache.head_dim
+        if n_heads * cache.head_dim != q_width or not n_heads:
+            raise KernelError(_SHAPE, "q: rows of whole heads are wanted")
         if q_out is None:
-            q_out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
-        qp, qs = _rows(q, batch.n_tokens, q.shape[1], k.dtype, "q")
-        qop, qos = _rows(q_out, batch.n_tokens, q.shape[1], k.dtype, "q_out")
-    _check(lib.load().sq_paged_append(_stream(), cache.ref, batch.ref, kind, kp, ks, vp, vs, cos.data_ptr(),
-                                      sin.data_ptr(), cos.shape[0], qp, qs, n_heads, qop, qos))
+            q_out = q.new_empty((n, q_width))
+        qp, qs = _rows(q, n, q_width, dtype, "q")
+        qop, qos = _rows(q_out, n, q_width, dtype, "q_out")
+    st = _fn("sq_paged_append")(_raw_stream(_device()), cache.ref, batch.ref, kind, kp, ks, vp, vs, cos.data_ptr(),
+                                sin.data_ptr(), positions, qp, qs, n_heads, qop, qos)
+    if st:
+        _check(st)
     return q_out
 
 
@@ -136,36 +160,41 @@ def attention(cache, batch, q, window=0, sinks=0, scale=None, out=None):
     """Causal grouped attention of q [n_tokens, n_heads * head_dim] over the cache: the query
     at position p sees the positions <= p, with window > 0 only the last `window` of them
     and the first `sinks` ones. scale: head_dim ** -0.5 unless given."""
-    _need(q.dim() == 2 and q.shape[1] % cache.head_dim == 0, _SHAPE, "q: rows of whole heads are wanted")
-    n_heads = q.shape[1] // cache.head_dim
+    n, dtype = batch.n_tokens, q.dtype
+    width = q.shape[1] if q.dim() == 2 else 0
+    n_heads = width // cache.head_dim
+    if n_heads * cache.head_dim != width or not n_heads:
+        raise KernelError(_SHAPE, "q: rows of whole heads are wanted")
     kind = _kind(q)
-    qp, qs = _rows(q, batch.n_tokens, q.shape[1], q.dtype, "q")
+    qp, qs = _rows(q, n, width, dtype, "q")
     if out is None:
-        out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
-    op, os_ = _rows(out, batch.n_tokens, q.shape[1], q.dtype, "out")
+        out = q.new_empty((n, width))
+    op, os_ = _rows(out, n, width, dtype, "out")
     _, ws, ws_bytes = batch.workspace(cache, n_heads)
-    _check(lib.load().sq_paged_attention(_stream(), cache.ref, batch.ref, kind, qp, qs, n_heads,
-                                         cache.head_dim ** -0.5 if scale is None else scale, window, sinks, op, os_,
-                                         ws, ws_bytes))
+    st = _fn("sq_paged_attention")(_raw_stream(_device()), cache.ref, batch.ref, kind, qp, qs, n_heads,
+                                   cache.scale if scale is None else scale, window, sinks, op, os_, ws, ws_bytes)
+    if st:
+        _check(st)
     return out
 
 
 def read(cache, batch, first, count, dtype=torch.float32):
     """The values of `count` positions of each sequence from first[b] (int32 CUDA tensor) on:
     k, v [n_seqs, count, n_kv_heads * head_dim], zeros past kv_len[b]."""
-    n = batch.kv_len.shape[0]
-    _need(first.shape == (n,) and first.dtype == torch.int32 and first.is_cuda and first.is_contiguous(), _SHAPE,
-          "first: one int32 position of each sequence on the GPU")
-    _need(dtype in _KINDS, _TYPE, "values are read as float32 or bfloat16")
-    shape = (n, count, cache.n_kv_heads * cache.head_dim)
-    k = torch.empty(shape, dtype=dtype, device=cache.k.device)
-    v = torch.empty(shape, dtype=dtype, device=cache.k.device)
-    _check(lib.load().sq_paged_read(_stream(), cache.ref, batch.ref, first.data_ptr(), count, _KINDS[dtype],
-                                    k.data_ptr(), v.data_ptr()))
+    n = batch.n_seqs
+    if first.shape != (n,) or first.dtype is not torch.int32 or not first.is_cuda or not first.is_contiguous():
+        raise KernelError(_SHAPE, "first: one int32 position of each sequence on the GPU")
+    if dtype not in _KINDS:
+        raise KernelError(_TYPE, "values are read as float32 or bfloat16")
+    k, v = (cache.k_scale.new_empty((n, count, cache.row), dtype=dtype) for _ in range(2))
+    st = _fn("sq_paged_read")(_raw_stream(_device()), cache.ref, batch.ref, first.data_ptr(), count, _KINDS[dtype],
+                              k.data_ptr(), v.data_ptr())
+    if st:
+        _check(st)
     return k, v
 
 
 def status(clear=True):
     """sq_paged_status: raise what the kernels found wrong in a batch's arrays (call after
     synchronizing)."""
-    _check(lib.load().sq_paged_status(int(clear)))
+    _check(_fn("sq_paged_status")(int(clear)))

@@ -3,16 +3,16 @@ numbers. No counterpart in the reference, whose generation takes one greedy toke
 (text_generator.rs:38-101)."""
 import torch
 
-from . import lib
-from .lib import KernelError, _check, _stream
+from .lib import KernelError, _check
+from .paged import _device, _fn, _raw_stream
 
 _SHAPE, _TYPE, _ARG = 1, 2, 5
 
 
 def _array(t, shape, dtype, what):
     if t.shape != shape or not t.is_contiguous():
-        raise KernelError(_SHAPE, f"{what}: a contiguous {tuple(shape)} tensor is wanted")
-    if t.dtype != dtype:
+        raise KernelError(_SHAPE, f"{what}: a contiguous {shape} tensor is wanted")
+    if t.dtype is not dtype:
         raise KernelError(_TYPE, f"{what}: {dtype} is wanted")
     if not t.is_cuda:
         raise KernelError(_ARG, f"{what}: a CUDA tensor is wanted")
@@ -43,10 +43,11 @@ def verify_drafts(target, draft, tokens, uniform, n_draft=None):
     vocab = target.shape[2]
     tp, ts = _probs(target, n, k + 1, vocab, "target")
     dp, ds = _probs(draft, n, k, vocab, "draft") if draft is not None else (None, 0)
-    accepted = torch.empty(n, dtype=torch.int32, device=target.device)
-    out = torch.empty((n, k + 1), dtype=torch.int32, device=target.device)
-    _check(lib.load().sq_verify_drafts(
-        _stream(), tp, ts, dp, ds, _array(tokens, (n, k), torch.int32, "tokens"),
+    accepted, out = tokens.new_empty(n), tokens.new_empty((n, k + 1))
+    st = _fn("sq_verify_drafts")(
+        _raw_stream(_device()), tp, ts, dp, ds, _array(tokens, (n, k), torch.int32, "tokens"),
         _array(n_draft, (n,), torch.int32, "n_draft") if n_draft is not None else None,
-        _array(uniform, (n, k + 1), torch.float32, "uniform"), n, k, vocab, accepted.data_ptr(), out.data_ptr()))
+        _array(uniform, (n, k + 1), torch.float32, "uniform"), n, k, vocab, accepted.data_ptr(), out.data_ptr())
+    if st:
+        _check(st)
     return accepted, out
