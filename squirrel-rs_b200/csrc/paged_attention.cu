@@ -8,15 +8,15 @@
 // The products run on mma.sync m16n8k16 (f16 in, f32 sums) rather than tcgen05: with at
 // most 32 rows the tensor work is small, and the register fragments let a warp convert
 // the codes it needs where it needs them, with no second pass through shared memory.
-//   scores:  S[16 keys][8 columns]   = K[16 keys][dims] Q^T      (keys in the M rows)
-//   output:  O[16 dims][8 columns]  += V^T[16 dims][keys] P      (dimensions in the M rows)
+//   scores:  S[16 keys][8 rows]   = K[16 keys][dims] Q^T      (keys in the M rows)
+//   output:  O[16 dims][8 rows]  += V^T[16 dims][keys] P      (dimensions in the M rows)
 // Dimensions and keys are numbered inside the products so that a lane's K fragment is 16
 // consecutive bytes of a key and its V fragment consecutive bytes of four keys; P goes
 // from the scores' layout to the operand's by movmatrix.
 //
 // Precision. Codes are whole numbers up to 127: exact in f16. Query rows are scaled by a
-// power of two; an f32 row takes two f16 terms (22 bits) in two columns of the same tile, a bf16
-// row is exact in one. Weights, at most 2^10 (the maximum's), likewise: two terms for f32
+// power of two; an f32 row takes two f16 terms (22 bits) and so two products, a bf16 row is
+// exact in one. Weights, at most 2^10 (the maximum's), likewise: two terms for f32
 // rows, one (11 bits, under the output's 8) for bf16 rows. The V scale of a page goes
 // into the weights relative to the largest met so far, so f16 never overflows. K's codes
 // enter as the f16 numbers code * 2^-24 (denormal, exact; one instruction a pair) and
@@ -43,10 +43,10 @@ namespace {
 
 constexpr int WARPS = 4, THREADS = WARPS * 32, STAGES = 2;
 constexpr int BLOCKS_PER_SM = 3;
-constexpr int MAX_BLOCKS = 160 * BLOCKS_PER_SM;
+constexpr int MAX_BLOCKS = 160 * BLOCKS_PER_SM;  // and parts of a row tile
 constexpr int MIN_TILES = WARPS;  // key tiles a block takes at least
 constexpr int FLUSH_STEPS = 16;   // f32 rows: 16-key products summed on the tensor core at a stretch
-constexpr int SLOT_FLOATS = 2112;  // partial results of one row tile: rows x (head_dim + 2), 32 x 66 at most
+constexpr int SLOT_FLOATS = 2112;  // partial results of a row tile: 32 x 66 at most: maxima, sums, [row][head_dim]
 constexpr size_t PARTIAL_BYTES = (size_t)MAX_BLOCKS * 2 * SLOT_FLOATS * 4;
 constexpr float WEIGHT_EXP = 10.f;  // weights are 2^(s - max + 10)
 
@@ -73,9 +73,9 @@ __device__ __forceinline__ void mma(float (&d)[4], const uint32_t (&a)[4], uint3
 template <typename T, int HD_, int NT_>
 struct Cfg {
   static constexpr int HD = HD_, NT = NT_;
-  static constexpr bool SPLIT = sizeof(T) == 4;          // two f16 terms a row
-  static constexpr int ROWS_NT = SPLIT ? 4 : 8;          // rows of an 8-column tile (columns 4..7: second terms)
-  static constexpr int ROWS = NT * ROWS_NT;
+  static constexpr bool SPLIT = sizeof(T) == 4;  // two f16 terms a row and weight
+  static constexpr int TERMS = SPLIT ? 2 : 1;
+  static constexpr int ROWS = NT * 8;
   static constexpr int TK = HD <= 64 ? 64 : 4096 / HD;   // keys a tile
   static constexpr int NG = TK / 16;                     // groups of 16 keys: each within one page
   static constexpr int TILE = TK * HD;                   // bytes of one operand's tile
@@ -86,6 +86,7 @@ struct Cfg {
   static constexpr int BATCH = 32 / NG;  // tiles whose pages a warp looks up at once
   static constexpr int BLOCKS = NT <= 2 && 3 * SMEM <= 223 * 1024 ? BLOCKS_PER_SM : 2;
   static_assert(ROWS * (HD + 2) <= SLOT_FLOATS, "a row tile's partial results fit a slot");
+  static_assert((MAX_BLOCKS * 8 + THREADS * 4) * 4 <= RING, "the factors of eight rows' parts fit the ring");
   static_assert(WARPS * ROWS * (HD + 2) * 4 <= RING, "the warps' results fit the ring");
 };
 
@@ -128,11 +129,12 @@ __device__ __forceinline__ Span key_span(const Seq &s, int window, int sinks) {
 
 template <class C, typename T>
 __global__ void __launch_bounds__(THREADS, C::BLOCKS) k_paged_few(const AttnArgs<T> a) {
-  constexpr int HD = C::HD, NT = C::NT, TK = C::TK, NG = C::NG, KS = C::KS, ROWS = C::ROWS, RN = C::ROWS_NT;
+  constexpr int HD = C::HD, NT = C::NT, TK = C::TK, NG = C::NG, KS = C::KS, ROWS = C::ROWS, TERMS = C::TERMS;
   constexpr int MT = HD / 16;  // 16-dimension tiles of the output
   extern __shared__ __align__(128) uint8_t ring[];
   __shared__ long long s_scan[WARPS + 1];
   __shared__ int s_last;
+  __shared__ float s_sum[8];
   const int tid = threadIdx.x, lane = tid & 31, wid = tid >> 5, g = lane >> 2, t = lane & 3;
   const Cache &c = a.c;
   const int rows_of_token = a.group;
@@ -143,8 +145,9 @@ __global__ void __launch_bounds__(THREADS, C::BLOCKS) k_paged_few(const AttnArgs
     return (long long)key_span<TK>(s, a.window, a.sinks).n * rt * c.kv_heads;
   };
   // This block's piece [at, end) of the line of all tiles, and the sequence it starts in.
-  long long total = 0;
-  for (int b = tid; b < a.b.n_seqs; b += THREADS) total += tiles_of(load_seq(a.b, c, b));
+  const long long first_n = tid < a.b.n_seqs ? tiles_of(load_seq(a.b, c, tid)) : 0;
+  long long total = first_n;
+  for (int b = tid + THREADS; b < a.b.n_seqs; b += THREADS) total += tiles_of(load_seq(a.b, c, b));
   total = warp_sum_ll(total);
   if (lane == 0) s_scan[wid] = total;
   __syncthreads();
@@ -157,8 +160,9 @@ __global__ void __launch_bounds__(THREADS, C::BLOCKS) k_paged_few(const AttnArgs
   if (at >= end) return;
   int b = 0;
   long long b_start = 0;  // first tile of sequence b
+#pragma unroll 1
   for (int b0 = 0; b0 < a.b.n_seqs; b0 += THREADS) {
-    const long long n = b0 + tid < a.b.n_seqs ? tiles_of(load_seq(a.b, c, b0 + tid)) : 0;
+    const long long n = !b0 ? first_n : b0 + tid < a.b.n_seqs ? tiles_of(load_seq(a.b, c, b0 + tid)) : 0;
     long long run = n;
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
@@ -168,15 +172,16 @@ __global__ void __launch_bounds__(THREADS, C::BLOCKS) k_paged_few(const AttnArgs
     __syncthreads();
     if (lane == 31) s_scan[wid] = run;
     __syncthreads();
-    long long before = b_start;
-    for (int w = 0; w < wid; w++) before += s_scan[w];
-    run += before;
+    long long all = b_start;
+#pragma unroll
+    for (int w = 0; w < WARPS; w++) {
+      if (w == wid) run += all;
+      all += s_scan[w];
+    }
     if (at >= run - n && at < run) {  // one thread at most
       s_last = b0 + tid;
       s_scan[WARPS] = run - n;
     }
-    long long all = b_start;
-    for (int w = 0; w < WARPS; w++) all += s_scan[w];
     __syncthreads();
     if (at < all) {
       b = s_last;
@@ -202,64 +207,6 @@ __global__ void __launch_bounds__(THREADS, C::BLOCKS) k_paged_few(const AttnArgs
     const int t0 = (int)(at - job_start), t1 = (int)min((long long)span.n, end - job_start);
     const int pos0 = s.len - s.n;  // position of the first new token
 
-    // ---- query fragments: column g of tile nt = row nt * RN + g % RN, term g / RN
-    uint32_t qf[NT][KS][2];
-    float cf[NT][2], cb[NT][2];  // factor and offset of the lane's two columns' scores
-    int pos[NT][2];    // and their rows' positions (-1: no such row)
-#pragma unroll
-    for (int nt = 0; nt < NT; nt++) {
-      const int r = rt * ROWS + nt * RN + (g & (RN - 1)), tok = r / rows_of_token, h = r - tok * rows_of_token;
-      const bool ok = tok < s.n;
-      const T *src = a.q + (s.first + (ok ? tok : 0)) * a.qs + (head * rows_of_token + (ok ? h : 0)) * HD;
-      float x[KS * 4];  // the lane's dimensions: 16 consecutive ones of each 64 (8 of 32)
-      float top = 0.f;
-      bool finite = true;
-#pragma unroll
-      for (int i = 0; i < KS; i++) {
-        const int d = HD >= 64 ? (i >> 2) * 64 + t * 16 + (i & 3) * 4 : t * 8 + i * 4;
-        const float4 v = ok ? load4(src + d) : make_float4(0.f, 0.f, 0.f, 0.f);
-        x[4 * i] = v.x, x[4 * i + 1] = v.y, x[4 * i + 2] = v.z, x[4 * i + 3] = v.w;
-#pragma unroll
-        for (int j = 0; j < 4; j++) {
-          top = fmaxf(top, fabsf(x[4 * i + j]));
-          finite &= fabsf(x[4 * i + j]) <= FLT_MAX;
-        }
-      }
-      top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
-      top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
-      finite = (__ballot_sync(0xffffffffu, finite) >> (lane & 28) & 15) == 15;  // of the row's four lanes
-      const int e = row_exp(top);
-      const float up = row_factor(e, finite);
-      const float down = scalbnf(a.scale, -e);
-      float sum = 0.f;  // of the row's terms, for the bias of the codes
-#pragma unroll
-      for (int i = 0; i < KS; i++) {
-#pragma unroll
-        for (int j = 0; j < 2; j++) {  // dimensions 4 i + j and 4 i + j + 2: bytes of a word two apart
-          const float u = x[4 * i + j] * up, v = x[4 * i + j + 2] * up;
-          uint32_t f = pack(u, v);
-          const float2 hi = unpack(f);
-          sum += hi.x + hi.y;
-          if (C::SPLIT) {
-            const uint32_t lo = pack(u - hi.x, v - hi.y);
-            const float2 l2 = unpack(lo);
-            sum += l2.x + l2.y;
-            if (g >= RN) f = lo;
-          }
-          qf[nt][i][j] = f;
-        }
-      }
-      sum += __shfl_xor_sync(0xffffffffu, sum, 1);
-      sum += __shfl_xor_sync(0xffffffffu, sum, 2);
-#pragma unroll
-      for (int j = 0; j < 2; j++) {  // column 2t + j is row (2t + j) % RN: held by lanes of that g
-        const int from = ((2 * t + j) & (RN - 1)) * 4;
-        const float d = __shfl_sync(0xffffffffu, down, from), q = __shfl_sync(0xffffffffu, sum, from);
-        cf[nt][j] = d * 16777216.f;
-        cb[nt][j] = -128.f * q * d;
-        pos[nt][j] = __shfl_sync(0xffffffffu, ok ? pos0 + tok : -1, from);
-      }
-    }
     const int last_row = min((rt + 1) * ROWS, s.n * rows_of_token) - 1;
     const int min_pos = pos0 + rt * ROWS / rows_of_token, max_pos = pos0 + last_row / rows_of_token;
 
@@ -346,6 +293,62 @@ __global__ void __launch_bounds__(THREADS, C::BLOCKS) k_paged_few(const AttnArgs
 #pragma unroll
       for (int k = 0; k < STAGES; k++) load_tile(k, place, k);
     }
+    // ---- query fragments (the first tiles are on their way): column g of tile nt = row 8 nt + g
+    uint32_t qf[NT][KS][TERMS][2];
+    float cf[NT][2], cb[NT][2];  // factor and offset of the scores of the lane's columns 2t, 2t + 1
+    int pos[NT][2];              // and their rows' positions (-1: no such row)
+#pragma unroll
+    for (int nt = 0; nt < NT; nt++) {
+      const int r = rt * ROWS + nt * 8 + g, tok = r / rows_of_token, h = r - tok * rows_of_token;
+      const bool ok = tok < s.n;
+      const T *src = a.q + (s.first + (ok ? tok : 0)) * a.qs + (head * rows_of_token + (ok ? h : 0)) * HD;
+      float x[KS * 4];  // the lane's dimensions: 16 consecutive ones of each 64 (8 of 32)
+      float top = 0.f;
+      bool finite = true;
+#pragma unroll
+      for (int i = 0; i < KS; i++) {
+        const int d = HD >= 64 ? (i >> 2) * 64 + t * 16 + (i & 3) * 4 : t * 8 + i * 4;
+        const float4 v = ok ? load4(src + d) : make_float4(0.f, 0.f, 0.f, 0.f);
+        x[4 * i] = v.x, x[4 * i + 1] = v.y, x[4 * i + 2] = v.z, x[4 * i + 3] = v.w;
+      }
+#pragma unroll
+      for (int i = 0; i < KS * 4; i++) {
+        top = fmaxf(top, fabsf(x[i]));
+        finite &= fabsf(x[i]) <= FLT_MAX;
+      }
+      top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
+      top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
+      finite = (__ballot_sync(0xffffffffu, finite) >> (lane & 28) & 15) == 15;  // of the row's four lanes
+      const int e = row_exp(top);
+      const float up = row_factor(e, finite);
+      const float down = scalbnf(a.scale, -e);
+      float sum = 0.f;  // of the row's terms, for the bias of the codes
+#pragma unroll
+      for (int i = 0; i < KS; i++) {
+#pragma unroll
+        for (int j = 0; j < 2; j++) {  // dimensions 4 i + j and 4 i + j + 2: bytes of a word two apart
+          const float u = x[4 * i + j] * up, v = x[4 * i + j + 2] * up;
+          qf[nt][i][0][j] = pack(u, v);
+          const float2 hi = unpack(qf[nt][i][0][j]);
+          sum += hi.x + hi.y;
+          if constexpr (C::SPLIT) {
+            qf[nt][i][1][j] = pack(u - hi.x, v - hi.y);
+            const float2 lo = unpack(qf[nt][i][1][j]);
+            sum += lo.x + lo.y;
+          }
+        }
+      }
+      sum += __shfl_xor_sync(0xffffffffu, sum, 1);
+      sum += __shfl_xor_sync(0xffffffffu, sum, 2);
+#pragma unroll
+      for (int j = 0; j < 2; j++) {  // row 2t + j is held by the lanes of g = 2t + j
+        const int from = (2 * t + j) * 4;
+        const float d = __shfl_sync(0xffffffffu, down, from), q = __shfl_sync(0xffffffffu, sum, from);
+        cf[nt][j] = d * 16777216.f;
+        cb[nt][j] = -128.f * q * d;
+        pos[nt][j] = __shfl_sync(0xffffffffu, ok ? pos0 + tok : -1, from);
+      }
+    }
 #pragma unroll 1
     for (int k = 0; k < n_tiles; k++, st ^= 1) {
       const int in_batch = k % BATCH;
@@ -396,7 +399,9 @@ __global__ void __launch_bounds__(THREADS, C::BLOCKS) k_paged_few(const AttnArgs
             for (int x = 0; x < 4; x++) {
               const uint32_t f[4] = {codes_02(uu[x]), codes_02(ww[x]), codes_13(uu[x]), codes_13(ww[x])};
 #pragma unroll
-              for (int nt = 0; nt < NT; nt++) mma(sc[j][nt], f, qf[nt][ch * 4 + x][0], qf[nt][ch * 4 + x][1]);
+              for (int nt = 0; nt < NT; nt++)
+#pragma unroll
+                for (int y = 0; y < TERMS; y++) mma(sc[j][nt], f, qf[nt][ch * 4 + x][y][0], qf[nt][ch * 4 + x][y][1]);
             }
           }
         } else {
@@ -407,11 +412,13 @@ __global__ void __launch_bounds__(THREADS, C::BLOCKS) k_paged_few(const AttnArgs
           for (int x = 0; x < 2; x++) {
             const uint32_t f[4] = {codes_02(uu[x]), codes_02(ww[x]), codes_13(uu[x]), codes_13(ww[x])};
 #pragma unroll
-            for (int nt = 0; nt < NT; nt++) mma(sc[j][nt], f, qf[nt][x][0], qf[nt][x][1]);
+            for (int nt = 0; nt < NT; nt++)
+#pragma unroll
+              for (int y = 0; y < TERMS; y++) mma(sc[j][nt], f, qf[nt][x][y][0], qf[nt][x][y][1]);
           }
         }
       }
-      // in log2 units, the second terms' columns added to the first's (both then hold the sum)
+      // in log2 units
 #pragma unroll
       for (int j = 0; j < NG; j++) {
         const float gks = __shfl_sync(0xffffffffu, ks, in_batch * NG + j);
@@ -419,10 +426,7 @@ __global__ void __launch_bounds__(THREADS, C::BLOCKS) k_paged_few(const AttnArgs
         for (int nt = 0; nt < NT; nt++) {
           const float f0 = cf[nt][0] * gks, f1 = cf[nt][1] * gks, b0 = cb[nt][0] * gks, b1 = cb[nt][1] * gks;
 #pragma unroll
-          for (int x = 0; x < 4; x++) {
-            if (C::SPLIT) sc[j][nt][x] += __shfl_xor_sync(0xffffffffu, sc[j][nt][x], 2);
-            sc[j][nt][x] = fmaf(sc[j][nt][x], x & 1 ? f1 : f0, x & 1 ? b1 : b0);
-          }
+          for (int x = 0; x < 4; x++) sc[j][nt][x] = fmaf(sc[j][nt][x], x & 1 ? f1 : f0, x & 1 ? b1 : b0);
         }
       }
       const unsigned there = __ballot_sync(0xffffffffu, place >= 0) >> (in_batch * NG);
@@ -471,7 +475,7 @@ __global__ void __launch_bounds__(THREADS, C::BLOCKS) k_paged_few(const AttnArgs
         }
       }
       // weights, as the operand of the second product
-      uint32_t pf[NG][NT][2];
+      uint32_t pf[NG][NT][TERMS][2];
 #pragma unroll
       for (int j = 0; j < NG; j++) {
         const float gshare = __shfl_sync(0xffffffffu, share, in_batch * NG + j);
@@ -484,13 +488,12 @@ __global__ void __launch_bounds__(THREADS, C::BLOCKS) k_paged_few(const AttnArgs
             l[nt][1] += v;
             u *= gshare;
             v *= gshare;
-            uint32_t f = pack(u, v);
-            if (C::SPLIT) {
+            const uint32_t f = pack(u, v);
+            pf[j][nt][0][x] = transpose8x8(f);
+            if constexpr (C::SPLIT) {
               const float2 hi = unpack(f);
-              const uint32_t lo = pack(u - hi.x, v - hi.y);
-              f = t < 2 ? f : lo;
+              pf[j][nt][1][x] = transpose8x8(pack(u - hi.x, v - hi.y));
             }
-            pf[j][nt][x] = transpose8x8(f);
           }
       }
       // output
@@ -523,7 +526,10 @@ __global__ void __launch_bounds__(THREADS, C::BLOCKS) k_paged_few(const AttnArgs
               const uint32_t v = __byte_perm(w[2][x], w[3][x], y ? 0x7362 : 0x5140);
               const uint32_t f[4] = {codes_lo(u), codes_hi(u), codes_lo(v), codes_hi(v)};
 #pragma unroll
-              for (int nt = 0; nt < NT; nt++) mma(o[ch * 2 * W + 2 * x + y][nt], f, pf[j][nt][0], pf[j][nt][1]);
+              for (int nt = 0; nt < NT; nt++)
+#pragma unroll
+                for (int z = 0; z < TERMS; z++)
+                  mma(o[ch * 2 * W + 2 * x + y][nt], f, pf[j][nt][z][0], pf[j][nt][z][1]);
             }
         }
       }
@@ -546,9 +552,8 @@ __global__ void __launch_bounds__(THREADS, C::BLOCKS) k_paged_few(const AttnArgs
         float sum = l[nt][j];
 #pragma unroll
         for (int x = 4; x < 32; x <<= 1) sum += __shfl_xor_sync(0xffffffffu, sum, x);
-        const int col = 2 * t + j, row = nt * RN + (col & (RN - 1));
-        float *dst = mine + row * (HD + 2);
-        if (g == 0 && col < RN) {
+        float *dst = mine + (nt * 8 + 2 * t + j) * (HD + 2);
+        if (g == 0) {
           dst[0] = m[nt][j];
           dst[1] = sum;
         }
@@ -556,27 +561,26 @@ __global__ void __launch_bounds__(THREADS, C::BLOCKS) k_paged_few(const AttnArgs
         for (int mt = 0; mt < MT; mt++)
 #pragma unroll
           for (int x = 0; x < 2; x++) {
-            float v = o[mt][nt][2 * x + j];
-            if (C::SPLIT) v = sums[((mt * NT + nt) * 4 + 2 * x + j) * 32];
-            if (C::SPLIT) v += __shfl_xor_sync(0xffffffffu, v, 2);
+            const float v = C::SPLIT ? sums[((mt * NT + nt) * 4 + 2 * x + j) * 32] : o[mt][nt][2 * x + j];
             const int d = HD >= 128 ? (mt / 8) * 128 + g * 16 + (mt % 8) * 2 + x : g * (HD / 8) + mt * 2 + x;
-            if (col < RN) dst[2 + d] = v * unit;
+            dst[2 + d] = v * unit;
           }
       }
     __syncthreads();
     const bool whole = t0 == 0 && t1 == span.n;
     const int rows = last_row + 1 - rt * ROWS;
-    auto put = [&](int row, int d, float v) {
+    auto put = [&](int row, int d, float4 v) {
       const int r = rt * ROWS + row, tok = r / rows_of_token, h = r - tok * rows_of_token;
-      T *p = a.out + (s.first + tok) * a.os + (head * rows_of_token + h) * HD + d;
-      if constexpr (C::SPLIT) *p = v;
-      else *p = __float2bfloat16_rn(v);
+      store4(a.out + (s.first + tok) * a.os + (head * rows_of_token + h) * HD + d, v);
     };
-    float *slot = a.part + (size_t)(2 * blockIdx.x + (job_start > per * blockIdx.x ? 1 : 0)) * SLOT_FLOATS;
-    for (int e = tid; e < rows * HD; e += THREADS) {
-      const int row = e / HD, d = e % HD;
+    auto slot_of = [&](long long block, bool second) { return a.part + (size_t)(2 * block + second) * SLOT_FLOATS; };
+    constexpr int QUADS = HD / 4;
+    float *slot = slot_of(blockIdx.x, job_start > per * blockIdx.x);  // maxima, sums, outputs
+    for (int e = tid; e < rows * QUADS; e += THREADS) {
+      const int row = e / QUADS, d = e % QUADS * 4;
       const float *src = reinterpret_cast<const float *>(ring) + row * (HD + 2);
-      float top = -INFINITY, sum = 0.f, v = 0.f;
+      float top = -INFINITY, sum = 0.f;
+      float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll
       for (int w = 0; w < WARPS; w++) top = fmaxf(top, src[w * ROWS * (HD + 2)]);
       const float at0 = top == -INFINITY ? 0.f : top;
@@ -585,44 +589,80 @@ __global__ void __launch_bounds__(THREADS, C::BLOCKS) k_paged_few(const AttnArgs
         const float *x = src + w * ROWS * (HD + 2);
         const float f = ex2(x[0] - at0);
         sum = fmaf(x[1], f, sum);
-        v = fmaf(x[2 + d], f, v);
+        v.x = fmaf(x[2 + d], f, v.x), v.y = fmaf(x[3 + d], f, v.y);
+        v.z = fmaf(x[4 + d], f, v.z), v.w = fmaf(x[5 + d], f, v.w);
       }
       if (whole) {
-        put(row, d, sum == 0.f ? 0.f : v / sum);
+        const float inv = sum == 0.f ? 0.f : 1.f / sum;
+        put(row, d, sum == 0.f ? make_float4(0.f, 0.f, 0.f, 0.f) : make_float4(v.x * inv, v.y * inv, v.z * inv, v.w * inv));
       } else {
-        slot[row * (HD + 2) + 2 + d] = v;
+        *reinterpret_cast<float4 *>(slot + 2 * ROWS + row * HD + d) = v;
         if (d == 0) {
-          slot[row * (HD + 2)] = top;
-          slot[row * (HD + 2) + 1] = sum;
+          slot[row] = top;
+          slot[ROWS + row] = sum;
         }
       }
     }
-    if (!whole) {  // the last block to arrive joins all parts, in block order
-      const long long first = job_start / per, parts = (job_start + span.n - 1) / per - first + 1;
+    if (!whole) {
+      // The last block to arrive joins all parts, in block order: every part's factors once, to shared memory, then
+      // the threads share out rows, dimensions and (when there are few of those) slices of the parts.
+      const long long first = job_start / per;
+      const int parts = (int)((job_start + span.n - 1) / per - first) + 1;
+      const bool late = job_start > per * first;  // the first part is its block's second row tile
       int *count = a.count + ((long long)b * c.kv_heads + head) * a.max_row_tiles + rt;
       __threadfence();
       __syncthreads();
-      if (tid == 0) s_last = atomicAdd(count, 1) == (int)parts - 1;
+      if (tid == 0) s_last = atomicAdd(count, 1) == parts - 1;
       __syncthreads();
       if (s_last) {
         __threadfence();
-        auto part = [&](long long i) {  // the first part may be its block's second row tile
-          return a.part + (size_t)(2 * (first + i) + (i == 0 && job_start > per * first ? 1 : 0)) * SLOT_FLOATS;
-        };
-        for (int e = tid; e < rows * HD; e += THREADS) {
-          const int row = e / HD, d = e % HD;
-          float top = -INFINITY, sum = 0.f, v = 0.f;
-#pragma unroll 8
-          for (int i = 0; i < (int)parts; i++) top = fmaxf(top, __ldcg(part(i) + row * (HD + 2)));
-          const float at0 = top == -INFINITY ? 0.f : top;
-#pragma unroll 8
-          for (int i = 0; i < (int)parts; i++) {
-            const float *x = part(i) + row * (HD + 2);
-            const float f = ex2(__ldcg(x) - at0);
-            sum = fmaf(__ldcg(x + 1), f, sum);
-            v = fmaf(__ldcg(x + 2 + d), f, v);
+        auto part = [&](int i) { return slot_of(first + i, i == 0 && late); };
+        float *factor = reinterpret_cast<float *>(ring), *share_of = factor + MAX_BLOCKS * 8;  // [row of 8][part]; slices
+        for (int r0 = 0; r0 < rows; r0 += 8) {
+          const int nr = min(8, rows - r0);
+          __syncthreads();
+          for (int e = tid; e < nr * parts; e += THREADS) factor[e] = __ldcg(part(e % parts) + r0 + e / parts);
+          __syncthreads();
+          for (int r = wid; r < nr; r += WARPS) {  // a warp a row: maximum, factors, sum
+            float *f = factor + r * parts, top = -INFINITY, sum = 0.f;
+            for (int i = lane; i < parts; i += 32) top = fmaxf(top, f[i]);
+            top = warp_max(top);
+            const float at0 = top == -INFINITY ? 0.f : top;
+            for (int i = lane; i < parts; i += 32) {
+              const float x = ex2(f[i] - at0);
+              f[i] = x;
+              sum = fmaf(__ldcg(part(i) + ROWS + r0 + r), x, sum);
+            }
+            sum = warp_sum(sum);
+            if (lane == 0) s_sum[r] = sum;
           }
-          put(row, d, sum == 0.f ? 0.f : v / sum);
+          __syncthreads();
+          const int items = nr * QUADS, slices = max(1, THREADS / items);
+          for (int e0 = 0; e0 < items; e0 += THREADS) {
+            const int item = slices > 1 ? tid % items : e0 + tid, slice = slices > 1 ? tid / items : 0;
+            const int row = item / QUADS, d = item % QUADS * 4;
+            float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
+            if (item < items && slice < slices) {
+              const float *f = factor + row * parts;
+#pragma unroll 8
+              for (int i = slice; i < parts; i += slices) {
+                const float4 x = __ldcg(reinterpret_cast<const float4 *>(part(i) + 2 * ROWS + (r0 + row) * HD + d));
+                const float y = f[i];
+                v.x = fmaf(x.x, y, v.x), v.y = fmaf(x.y, y, v.y), v.z = fmaf(x.z, y, v.z), v.w = fmaf(x.w, y, v.w);
+              }
+              if (slice) *reinterpret_cast<float4 *>(share_of + 4 * tid) = v;
+            }
+            if (slices > 1) __syncthreads();
+            if (item < items && slice == 0) {
+              for (int i = 1; i < slices; i++) {
+                const float4 x = *reinterpret_cast<const float4 *>(share_of + 4 * (tid + i * items));
+                v.x += x.x, v.y += x.y, v.z += x.z, v.w += x.w;
+              }
+              const float sum = s_sum[row], inv = sum == 0.f ? 0.f : 1.f / sum;
+              put(r0 + row, d,
+                  sum == 0.f ? make_float4(0.f, 0.f, 0.f, 0.f) : make_float4(v.x * inv, v.y * inv, v.z * inv, v.w * inv));
+            }
+          }
         }
         if (tid == 0) *count = 0;
       }
@@ -654,15 +694,18 @@ cudaError_t launch(cudaStream_t s, AttnArgs<T> &a) {
   return cudaGetLastError();
 }
 
-// The narrowest tile that takes all rows of a kv head, up to what the registers hold.
+// As few row tiles as the registers allow (8 rows and head_dim 256, 16 and 128, 32 below), and those as narrow as
+// takes all rows.
 template <typename T, int HD>
 cudaError_t launch_few(cudaStream_t s, AttnArgs<T> &a) {
   const int rows = min(a.b.max_new * a.group, a.few_rows);
-  if (rows <= Cfg<T, HD, 1>::ROWS || HD == 256) return launch<Cfg<T, HD, 1>>(s, a);
-  if constexpr (HD <= 128) {
-    if (rows <= Cfg<T, HD, 2>::ROWS || HD == 128) return launch<Cfg<T, HD, 2>>(s, a);
+  constexpr int MOST = HD == 256 ? 1 : HD == 128 ? 2 : 4;
+  const int tiles = (rows + 8 * MOST - 1) / (8 * MOST), nt = ((rows + tiles - 1) / tiles + 7) / 8;
+  if (nt == 1) return launch<Cfg<T, HD, 1>>(s, a);
+  if constexpr (MOST >= 2) {
+    if (nt == 2) return launch<Cfg<T, HD, 2>>(s, a);
   }
-  if constexpr (HD <= 64) return launch<Cfg<T, HD, 4>>(s, a);
+  if constexpr (MOST == 4) return nt == 3 ? launch<Cfg<T, HD, 3>>(s, a) : launch<Cfg<T, HD, 4>>(s, a);
   return cudaErrorInvalidValue;
 }
 
@@ -697,7 +740,7 @@ Workspace workspace(const Batch &b, const Cache &c, int n_heads) {
   Workspace w;
   w.many_part = PARTIAL_BYTES;
   w.few_count = w.many_part + (many ? many_partial_bytes(c.hd) : 0);
-  w.many_count = w.few_count + jobs * ((rows + 3) / 4) * sizeof(int);  // row tiles have 4 rows at least
+  w.many_count = w.few_count + jobs * ((rows + 7) / 8) * sizeof(int);  // row tiles have 8 rows at least
   w.bytes = w.many_count + (many ? jobs * many_row_tiles(b.max_new, group) * sizeof(int) : 0);
   return w;
 }
