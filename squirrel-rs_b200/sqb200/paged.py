@@ -50,18 +50,29 @@ def _rows(t, rows, width, dtype, what):
     return t.data_ptr(), stride if rows > 1 else width  # one row: its stride says nothing
 
 
-# The calls take a microsecond or two of GPU time at their smallest, so the binding keeps
-# what it can: the entry points, the structs' addresses, torch's raw stream lookup.
+# The smallest calls take a few microseconds of GPU time, so the binding spends as little as
+# it can: entry points are looked up once, structs are passed by address, streams come from
+# torch's raw lookup, and tensors that this module makes itself are not checked again.
 _raw_stream = torch._C._cuda_getCurrentRawStream
 _device = torch.cuda.current_device
-_entry = {}
+
+
+_entries = {}
+
+
+def _bind(name):
+    """The library's entry point `name`: structs are passed as addresses, and the interpreter
+    lock is kept, for the calls only queue work."""
+    lib.load()
+    f = getattr(C.PyDLL(lib.LIB_PATH), name)
+    f.restype, types = lib.SIGNATURES[name]
+    f.argtypes = [C.c_void_p if issubclass(t, C._Pointer) else t for t in types]
+    _entries[name] = f
+    return f
 
 
 def _fn(name):
-    f = _entry.get(name)
-    if f is None:
-        f = _entry[name] = getattr(lib.load(), name)
-    return f
+    return _entries.get(name) or _bind(name)
 
 
 class PagedCache:
@@ -80,9 +91,11 @@ class PagedCache:
               "a cache is CUDA tensors of one device")
         self.k, self.v, self.k_scale, self.v_scale = k, v, k_scale, v_scale
         self.n_pages, self.n_kv_heads, self.page, self.head_dim = k.shape
+        self.shape_key = (self.n_kv_heads, self.page, self.head_dim)
         self.row, self.half, self.scale = self.n_kv_heads * self.head_dim, self.head_dim // 2, self.head_dim ** -0.5
+        self.like = {t: torch.empty(0, dtype=t, device=k.device) for t in _KINDS}  # for new tensors of these types
         self.desc = lib.PagedCacheDesc(k.data_ptr(), v.data_ptr(), k_scale.data_ptr(), v_scale.data_ptr(), *k.shape)
-        self.ref = C.pointer(self.desc)
+        self.ref = C.addressof(self.desc)
 
     @classmethod
     def empty(cls, n_pages, n_kv_heads, head_dim, page=64, device="cuda"):
@@ -112,15 +125,17 @@ class PagedBatch:
         self.n_seqs, self.n_tokens, self.max_new = kv_len.shape[0], n_tokens, max_new
         self.desc = lib.PagedBatchDesc(q_start.data_ptr(), kv_len.data_ptr(), page_table.data_ptr(), self.n_seqs,
                                        n_tokens, max_new, page_table.shape[1])
-        self.ref = C.pointer(self.desc)
+        self.ref = C.addressof(self.desc)
         self._workspaces = {}
 
     def workspace(self, cache, n_heads):
-        key = (n_heads, cache.n_kv_heads, cache.head_dim, cache.page)
+        """(tensor, address, bytes) for attention over caches of this shape."""
+        key = (cache.shape_key, n_heads)
         ws = self._workspaces.get(key)
         if ws is None:
             size = C.c_size_t()
-            _check(_fn("sq_paged_attention_workspace")(cache.ref, self.ref, n_heads, C.byref(size)))
+            _check(lib.load().sq_paged_attention_workspace(C.pointer(cache.desc), C.pointer(self.desc), n_heads,
+                                                           C.byref(size)))
             t = torch.zeros(size.value, dtype=torch.uint8, device=cache.k.device)
             ws = self._workspaces[key] = (t, t.data_ptr(), size.value)
         return ws
@@ -145,10 +160,12 @@ def append(cache, batch, k, v, cos, sin, q=None, q_out=None):
         n_heads = q_width // cache.head_dim
         if n_heads * cache.head_dim != q_width or not n_heads:
             raise KernelError(_SHAPE, "q: rows of whole heads are wanted")
-        if q_out is None:
-            q_out = q.new_empty((n, q_width))
         qp, qs = _rows(q, n, q_width, dtype, "q")
-        qop, qos = _rows(q_out, n, q_width, dtype, "q_out")
+        if q_out is None:
+            q_out = torch.empty_like(q)
+            qop, qos = q_out.data_ptr(), q_width
+        else:
+            qop, qos = _rows(q_out, n, q_width, dtype, "q_out")
     st = _fn("sq_paged_append")(_raw_stream(_device()), cache.ref, batch.ref, kind, kp, ks, vp, vs, cos.data_ptr(),
                                 sin.data_ptr(), positions, qp, qs, n_heads, qop, qos)
     if st:
@@ -168,8 +185,10 @@ def attention(cache, batch, q, window=0, sinks=0, scale=None, out=None):
     kind = _kind(q)
     qp, qs = _rows(q, n, width, dtype, "q")
     if out is None:
-        out = q.new_empty((n, width))
-    op, os_ = _rows(out, n, width, dtype, "out")
+        out = torch.empty_like(q)
+        op, os_ = out.data_ptr(), width
+    else:
+        op, os_ = _rows(out, n, width, dtype, "out")
     _, ws, ws_bytes = batch.workspace(cache, n_heads)
     st = _fn("sq_paged_attention")(_raw_stream(_device()), cache.ref, batch.ref, kind, qp, qs, n_heads,
                                    cache.scale if scale is None else scale, window, sinks, op, os_, ws, ws_bytes)
@@ -184,10 +203,12 @@ def read(cache, batch, first, count, dtype=torch.float32):
     n = batch.n_seqs
     if first.shape != (n,) or first.dtype is not torch.int32 or not first.is_cuda or not first.is_contiguous():
         raise KernelError(_SHAPE, "first: one int32 position of each sequence on the GPU")
-    if dtype not in _KINDS:
+    kind = _KINDS.get(dtype)
+    if kind is None:
         raise KernelError(_TYPE, "values are read as float32 or bfloat16")
-    k, v = (cache.k_scale.new_empty((n, count, cache.row), dtype=dtype) for _ in range(2))
-    st = _fn("sq_paged_read")(_raw_stream(_device()), cache.ref, batch.ref, first.data_ptr(), count, _KINDS[dtype],
+    like = cache.like[dtype]
+    k, v = like.new_empty((n, count, cache.row)), like.new_empty((n, count, cache.row))
+    st = _fn("sq_paged_read")(_raw_stream(_device()), cache.ref, batch.ref, first.data_ptr(), count, kind,
                               k.data_ptr(), v.data_ptr())
     if st:
         _check(st)
