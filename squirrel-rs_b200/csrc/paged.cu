@@ -14,6 +14,7 @@
 #include <string>
 
 #include "common.cuh"
+#include "ops.cuh"
 #include "paged.cuh"
 
 namespace sq {
@@ -123,6 +124,8 @@ template <typename T>
 __global__ void __launch_bounds__(APPEND_THREADS) k_paged_append(const AppendArgs<T> a) {
   const Cache &c = a.c;
   const int tid = threadIdx.x, half = c.hd / 2;
+  pdl_wait();  // the rows and the batch come from earlier kernels, which may still read the cache
+  pdl_trigger();
   if ((int)blockIdx.x >= a.page_blocks) {
     const int blk = blockIdx.x - a.page_blocks, t = blk / a.q_parts, part = blk % a.q_parts;
     const int b = seq_of_token(a.b, t);
@@ -215,6 +218,8 @@ template <typename T>
 __global__ void __launch_bounds__(READ_THREADS)
     k_paged_read(const Cache c, const Batch b, const int *__restrict__ first, int count, T *__restrict__ k_out,
                  T *__restrict__ v_out) {
+  pdl_wait();
+  pdl_trigger();
   const Seq s = load_seq(b, c, blockIdx.y);
   const int quads = c.kv_heads * c.hd / 4, per_head = c.hd / 4;
   const int pos0 = first[blockIdx.y];
@@ -255,8 +260,7 @@ cudaError_t append(cudaStream_t s, const Cache &c, const Batch &b, const void *k
   const long long blocks = page_blocks + (long long)b.n_tokens * a.q_parts;
   if (blocks > INT32_MAX) return cudaErrorInvalidConfiguration;
   a.page_blocks = (int)page_blocks;
-  k_paged_append<T><<<(unsigned)blocks, APPEND_THREADS, 0, s>>>(a);
-  return cudaGetLastError();
+  return launch_ex(k_paged_append<T>, dim3((unsigned)blocks), dim3(APPEND_THREADS), 0, s, pdl_enabled(), a);
 }
 
 }  // namespace
@@ -327,13 +331,12 @@ extern "C" int sq_paged_read(void *stream, const sq_paged_cache *cache, const sq
   if (!st) st = paged::check_rows(v_out, width, width, dtype, "paged_read: v_out");
   if (st) return st;
   if (!(b.err = paged::err_ptr())) return fail(SQ_ERR_CUDA, "paged_read: no current CUDA device");
-  const dim3 grid((count + paged::READ_ROWS - 1) / paged::READ_ROWS, b.n_seqs);
-  if (dtype == SQ_F32)
-    paged::k_paged_read<float><<<grid, paged::READ_THREADS, 0, (cudaStream_t)stream>>>(c, b, first, count,
-                                                                                     (float *)k_out, (float *)v_out);
-  else
-    paged::k_paged_read<__nv_bfloat16><<<grid, paged::READ_THREADS, 0, (cudaStream_t)stream>>>(
-        c, b, first, count, (__nv_bfloat16 *)k_out, (__nv_bfloat16 *)v_out);
-  SQ_CHECK_LAUNCH("sq_paged_read");
+  const dim3 grid((count + paged::READ_ROWS - 1) / paged::READ_ROWS, b.n_seqs), block(paged::READ_THREADS);
+  const cudaError_t e =
+      dtype == SQ_F32 ? launch_ex(paged::k_paged_read<float>, grid, block, 0, (cudaStream_t)stream, pdl_enabled(), c, b,
+                                  first, count, (float *)k_out, (float *)v_out)
+                      : launch_ex(paged::k_paged_read<__nv_bfloat16>, grid, block, 0, (cudaStream_t)stream, pdl_enabled(),
+                                  c, b, first, count, (__nv_bfloat16 *)k_out, (__nv_bfloat16 *)v_out);
+  if (e != cudaSuccess) return cuda_fail(e, "sq_paged_read");
   return SQ_OK;
 }

@@ -27,14 +27,18 @@
 //
 // Work is split evenly over the grid: the (sequence, kv head, row tile, key tile) space is
 // one line, every block takes an equal piece of it, the four warps of a block take its key
-// tiles in turn. A row tile cut by a block's end leaves partial results in the workspace
-// and the last block to arrive joins them, in block order (equal bits every call).
+// tiles in turn. A piece's ends move to the nearest end of a row tile's keys when that is
+// at most SNAP tiles away: a cut costs about 6 us (partial results, the join, a second
+// start), as long as the whole GPU reads some 20 tiles a block. A row tile that is cut
+// leaves partial results in the workspace and the last block to arrive joins them, in block
+// order (equal bits every call).
 #include <float.h>
 #include <limits.h>
 #include <math.h>
 
 #include <string>
 
+#include "ops.cuh"
 #include "paged_attention.cuh"
 
 namespace sq {
@@ -84,6 +88,7 @@ struct Cfg {
   static constexpr int SUMS = SPLIT ? WARPS * 32 * (HD / 16) * NT * 4 * 4 : 0;  // f32 rows: a lane's output sums
   static constexpr int SMEM = RING + SUMS;
   static constexpr int BATCH = 32 / NG;  // tiles whose pages a warp looks up at once
+  static constexpr int SNAP = NT == 1 ? 16 : 8;  // tiles: 32 x 1,028 positions (bf16) 26 -> 21.5 us, 16 x 5 drafts (f32) 45 -> 38
   static constexpr int BLOCKS = NT <= 2 && 3 * SMEM <= 223 * 1024 ? BLOCKS_PER_SM : 2;
   static_assert(ROWS * (HD + 2) <= SLOT_FLOATS, "a row tile's partial results fit a slot");
   static_assert((MAX_BLOCKS * 8 + THREADS * 4) * 4 <= RING, "the factors of eight rows' parts fit the ring");
@@ -129,72 +134,94 @@ __device__ __forceinline__ Span key_span(const Seq &s, int window, int sinks) {
 
 template <class C, typename T>
 __global__ void __launch_bounds__(THREADS, C::BLOCKS) k_paged_few(const AttnArgs<T> a) {
-  constexpr int HD = C::HD, NT = C::NT, TK = C::TK, NG = C::NG, KS = C::KS, ROWS = C::ROWS, TERMS = C::TERMS;
+  constexpr int HD = C::HD, NT = C::NT, TK = C::TK, NG = C::NG, KS = C::KS, ROWS = C::ROWS, TERMS = C::TERMS, SNAP = C::SNAP;
   constexpr int MT = HD / 16;  // 16-dimension tiles of the output
   extern __shared__ __align__(128) uint8_t ring[];
-  __shared__ long long s_scan[WARPS + 1];
+  __shared__ int s_scan[WARPS + 1];
+  __shared__ int s_end[2];
   __shared__ int s_last;
   __shared__ float s_sum[8];
   const int tid = threadIdx.x, lane = tid & 31, wid = tid >> 5, g = lane >> 2, t = lane & 3;
   const Cache &c = a.c;
   const int rows_of_token = a.group;
+  pdl_wait();  // the batch, q and the cache come from earlier kernels
+  pdl_trigger();
 
-  auto tiles_of = [&](const Seq &s) -> long long {
+  auto tiles_of = [&](const Seq &s) -> int {
     if (!s.n || s.n * rows_of_token > a.few_rows) return 0;
     const int rt = (s.n * rows_of_token + ROWS - 1) / ROWS;
-    return (long long)key_span<TK>(s, a.window, a.sinks).n * rt * c.kv_heads;
+    return key_span<TK>(s, a.window, a.sinks).n * rt * c.kv_heads;
   };
   // This block's piece [at, end) of the line of all tiles, and the sequence it starts in.
-  const long long first_n = tid < a.b.n_seqs ? tiles_of(load_seq(a.b, c, tid)) : 0;
-  long long total = first_n;
+  const int first_n = tid < a.b.n_seqs ? tiles_of(load_seq(a.b, c, tid)) : 0;
+  int total = first_n;
   for (int b = tid + THREADS; b < a.b.n_seqs; b += THREADS) total += tiles_of(load_seq(a.b, c, b));
-  total = warp_sum_ll(total);
+  total = __reduce_add_sync(0xffffffffu, total);
   if (lane == 0) s_scan[wid] = total;
+  if (tid < 2) s_end[tid] = -1;
   __syncthreads();
   total = 0;
 #pragma unroll
   for (int w = 0; w < WARPS; w++) total += s_scan[w];
-  const long long per = max((total + gridDim.x - 1) / gridDim.x, (long long)MIN_TILES);
-  long long at = per * blockIdx.x;
-  const long long end = min(at + per, total);
-  if (at >= end) return;
-  int b = 0;
-  long long b_start = 0;  // first tile of sequence b
+  const int per = max((total + (int)gridDim.x - 1) / (int)gridDim.x, MIN_TILES);
+  if (per * (int)blockIdx.x >= total) return;
+  {
+    int before = 0;  // tiles of the sequences before b0
 #pragma unroll 1
-  for (int b0 = 0; b0 < a.b.n_seqs; b0 += THREADS) {
-    const long long n = !b0 ? first_n : b0 + tid < a.b.n_seqs ? tiles_of(load_seq(a.b, c, b0 + tid)) : 0;
-    long long run = n;
+    for (int b0 = 0; b0 < a.b.n_seqs; b0 += THREADS) {
+      const int b = b0 + tid;
+      int n = first_n, n_span = 0;
+      if (b < a.b.n_seqs) {
+        const Seq s = load_seq(a.b, c, b);
+        n = tiles_of(s);
+        n_span = key_span<TK>(s, a.window, a.sinks).n;
+      } else {
+        n = 0;
+      }
+      int run = n;
 #pragma unroll
-    for (int o = 1; o < 32; o <<= 1) {
-      const long long y = __shfl_up_sync(0xffffffffu, run, o);
-      if (lane >= o) run += y;
-    }
-    __syncthreads();
-    if (lane == 31) s_scan[wid] = run;
-    __syncthreads();
-    long long all = b_start;
+      for (int o = 1; o < 32; o <<= 1) {
+        const int y = __shfl_up_sync(0xffffffffu, run, o);
+        if (lane >= o) run += y;
+      }
+      __syncthreads();
+      if (lane == 31) s_scan[wid] = run;
+      __syncthreads();
 #pragma unroll
-    for (int w = 0; w < WARPS; w++) {
-      if (w == wid) run += all;
-      all += s_scan[w];
-    }
-    if (at >= run - n && at < run) {  // one thread at most
-      s_last = b0 + tid;
-      s_scan[WARPS] = run - n;
+      for (int w = 0; w < WARPS; w++) {
+        if (w == wid) run += before;
+        before += s_scan[w];
+      }
+      const int start = run - n;
+#pragma unroll
+      for (int i = 0; i < 2; i++) {  // this piece's start and the next one's
+        const int x = per * ((int)blockIdx.x + i);
+        if (x >= start && x < run) {  // one thread at most
+          const int in_row_tile = (x - start) % n_span;
+          s_end[i] = in_row_tile <= SNAP && in_row_tile <= n_span - in_row_tile ? x - in_row_tile
+                     : n_span - in_row_tile <= SNAP                             ? x - in_row_tile + n_span
+                                                                                : x;
+          if (i == 0) {
+            s_last = b;
+            s_scan[WARPS] = start;
+          }
+        }
+      }
+      if (before > per * ((int)blockIdx.x + 1)) break;
     }
     __syncthreads();
-    if (at < all) {
-      b = s_last;
-      b_start = s_scan[WARPS];
-      break;
-    }
-    b_start = all;
   }
+  int at = s_end[0];
+  const int end = s_end[1] < 0 ? total : s_end[1];
+  if (at >= end) return;
+  int b = s_last;                      // its sequence, or the one before where `at` moved to its end
+  int b_start = s_scan[WARPS];  // first tile of sequence b
+  __syncthreads();
 
   const uint32_t my_ring = smem_addr(ring) + wid * (STAGES * 2 * C::TILE);
   while (at < end) {
     Seq s = load_seq(a.b, c, b);
-    long long n_b = tiles_of(s);
+    int n_b = tiles_of(s);
     while (at >= b_start + n_b) {  // sequences without new tokens or positions hold no tiles
       b_start += n_b;
       s = load_seq(a.b, c, ++b);
@@ -202,9 +229,9 @@ __global__ void __launch_bounds__(THREADS, C::BLOCKS) k_paged_few(const AttnArgs
     }
     const Span span = key_span<TK>(s, a.window, a.sinks);
     const int row_tiles = (s.n * rows_of_token + ROWS - 1) / ROWS;
-    const int job = (int)((at - b_start) / span.n), head = job / row_tiles, rt = job - head * row_tiles;
-    const long long job_start = b_start + (long long)job * span.n;
-    const int t0 = (int)(at - job_start), t1 = (int)min((long long)span.n, end - job_start);
+    const int job = (at - b_start) / span.n, head = job / row_tiles, rt = job - head * row_tiles;
+    const int job_start = b_start + job * span.n;
+    const int t0 = at - job_start, t1 = min(span.n, end - job_start);
     const int pos0 = s.len - s.n;  // position of the first new token
 
     const int last_row = min((rt + 1) * ROWS, s.n * rows_of_token) - 1;
@@ -297,20 +324,27 @@ __global__ void __launch_bounds__(THREADS, C::BLOCKS) k_paged_few(const AttnArgs
     uint32_t qf[NT][KS][TERMS][2];
     float cf[NT][2], cb[NT][2];  // factor and offset of the scores of the lane's columns 2t, 2t + 1
     int pos[NT][2];              // and their rows' positions (-1: no such row)
+    float4 qx[NT][KS];           // the lane's dimensions: 16 consecutive ones of each 64 (8 of 32)
 #pragma unroll
     for (int nt = 0; nt < NT; nt++) {
       const int r = rt * ROWS + nt * 8 + g, tok = r / rows_of_token, h = r - tok * rows_of_token;
       const bool ok = tok < s.n;
       const T *src = a.q + (s.first + (ok ? tok : 0)) * a.qs + (head * rows_of_token + (ok ? h : 0)) * HD;
-      float x[KS * 4];  // the lane's dimensions: 16 consecutive ones of each 64 (8 of 32)
+#pragma unroll
+      for (int i = 0; i < KS; i++)
+        qx[nt][i] = ok ? load4(src + (HD >= 64 ? (i >> 2) * 64 + t * 16 + (i & 3) * 4 : t * 8 + i * 4))
+                       : make_float4(0.f, 0.f, 0.f, 0.f);
+    }
+#pragma unroll
+    for (int nt = 0; nt < NT; nt++) {
+      const int tok = (rt * ROWS + nt * 8 + g) / rows_of_token;
+      const bool ok = tok < s.n;
+      float x[KS * 4];
       float top = 0.f;
       bool finite = true;
 #pragma unroll
-      for (int i = 0; i < KS; i++) {
-        const int d = HD >= 64 ? (i >> 2) * 64 + t * 16 + (i & 3) * 4 : t * 8 + i * 4;
-        const float4 v = ok ? load4(src + d) : make_float4(0.f, 0.f, 0.f, 0.f);
-        x[4 * i] = v.x, x[4 * i + 1] = v.y, x[4 * i + 2] = v.z, x[4 * i + 3] = v.w;
-      }
+      for (int i = 0; i < KS; i++)
+        x[4 * i] = qx[nt][i].x, x[4 * i + 1] = qx[nt][i].y, x[4 * i + 2] = qx[nt][i].z, x[4 * i + 3] = qx[nt][i].w;
 #pragma unroll
       for (int i = 0; i < KS * 4; i++) {
         top = fmaxf(top, fabsf(x[i]));
@@ -553,18 +587,14 @@ __global__ void __launch_bounds__(THREADS, C::BLOCKS) k_paged_few(const AttnArgs
 #pragma unroll
         for (int x = 4; x < 32; x <<= 1) sum += __shfl_xor_sync(0xffffffffu, sum, x);
         float *dst = mine + (nt * 8 + 2 * t + j) * (HD + 2);
-        if (g == 0) {
-          dst[0] = m[nt][j];
-          dst[1] = sum;
+        if (g == 0) *reinterpret_cast<float2 *>(dst) = make_float2(m[nt][j], sum);
+#pragma unroll
+        for (int mt = 0; mt < MT; mt++) {
+          const float *sm = sums + ((mt * NT + nt) * 4 + j) * 32;
+          const float2 v = C::SPLIT ? make_float2(sm[0], sm[64]) : make_float2(o[mt][nt][j], o[mt][nt][2 + j]);
+          const int d = HD >= 128 ? (mt / 8) * 128 + g * 16 + (mt % 8) * 2 : g * (HD / 8) + mt * 2;
+          *reinterpret_cast<float2 *>(dst + 2 + d) = make_float2(v.x * unit, v.y * unit);
         }
-#pragma unroll
-        for (int mt = 0; mt < MT; mt++)
-#pragma unroll
-          for (int x = 0; x < 2; x++) {
-            const float v = C::SPLIT ? sums[((mt * NT + nt) * 4 + 2 * x + j) * 32] : o[mt][nt][2 * x + j];
-            const int d = HD >= 128 ? (mt / 8) * 128 + g * 16 + (mt % 8) * 2 + x : g * (HD / 8) + mt * 2 + x;
-            dst[2 + d] = v * unit;
-          }
       }
     __syncthreads();
     const bool whole = t0 == 0 && t1 == span.n;
@@ -573,9 +603,10 @@ __global__ void __launch_bounds__(THREADS, C::BLOCKS) k_paged_few(const AttnArgs
       const int r = rt * ROWS + row, tok = r / rows_of_token, h = r - tok * rows_of_token;
       store4(a.out + (s.first + tok) * a.os + (head * rows_of_token + h) * HD + d, v);
     };
-    auto slot_of = [&](long long block, bool second) { return a.part + (size_t)(2 * block + second) * SLOT_FLOATS; };
+    // A block has two cut row tiles at most: the one its piece starts in (slot 0) and the one it ends in (slot 1).
+    auto slot_of = [&](int block, bool first_part) { return a.part + (size_t)(2 * block + first_part) * SLOT_FLOATS; };
     constexpr int QUADS = HD / 4;
-    float *slot = slot_of(blockIdx.x, job_start > per * blockIdx.x);  // maxima, sums, outputs
+    float *slot = slot_of(blockIdx.x, t0 == 0);  // maxima, sums, outputs
     for (int e = tid; e < rows * QUADS; e += THREADS) {
       const int row = e / QUADS, d = e % QUADS * 4;
       const float *src = reinterpret_cast<const float *>(ring) + row * (HD + 2);
@@ -606,17 +637,18 @@ __global__ void __launch_bounds__(THREADS, C::BLOCKS) k_paged_few(const AttnArgs
     if (!whole) {
       // The last block to arrive joins all parts, in block order: every part's factors once, to shared memory, then
       // the threads share out rows, dimensions and (when there are few of those) slices of the parts.
-      const long long first = job_start / per;
-      const int parts = (int)((job_start + span.n - 1) / per - first) + 1;
-      const bool late = job_start > per * first;  // the first part is its block's second row tile
-      int *count = a.count + ((long long)b * c.kv_heads + head) * a.max_row_tiles + rt;
-      __threadfence();
+      // The cuts are the multiples of `per` more than SNAP tiles inside; the part before the first is the block's before.
+      const int first = (job_start + SNAP) / per, parts = (job_start + span.n - SNAP - 1) / per - first + 1;
+      int *count = a.count + (b * c.kv_heads + head) * a.max_row_tiles + rt;
       __syncthreads();
-      if (tid == 0) s_last = atomicAdd(count, 1) == parts - 1;
+      if (tid == 0) {  // the block's stores before its arrival, the other blocks' arrivals before its loads
+        __threadfence();
+        s_last = atomicAdd(count, 1) == parts - 1;
+        __threadfence();
+      }
       __syncthreads();
       if (s_last) {
-        __threadfence();
-        auto part = [&](int i) { return slot_of(first + i, i == 0 && late); };
+        auto part = [&](int i) { return slot_of(first + i, i == 0); };
         float *factor = reinterpret_cast<float *>(ring), *share_of = factor + MAX_BLOCKS * 8;  // [row of 8][part]; slices
         for (int r0 = 0; r0 < rows; r0 += 8) {
           const int nr = min(8, rows - r0);
@@ -690,8 +722,7 @@ cudaError_t launch(cudaStream_t s, AttnArgs<T> &a) {
     blocks[dev] = min(sms * max(per_sm, 1), MAX_BLOCKS);
   }
   a.max_row_tiles = (min(a.b.max_new * a.group, a.few_rows) + C::ROWS - 1) / C::ROWS;
-  k_paged_few<C, T><<<blocks[dev], THREADS, C::SMEM, s>>>(a);
-  return cudaGetLastError();
+  return launch_ex(k_paged_few<C, T>, dim3(blocks[dev]), dim3(THREADS), C::SMEM, s, pdl_enabled(), a);
 }
 
 // As few row tiles as the registers allow (8 rows and head_dim 256, 16 and 128, 32 below), and those as narrow as
@@ -717,7 +748,7 @@ bool goes_many(const Cache &c, int max_new, int group) {
   return (long long)max_new * group > FEW_ROWS && many_supported(c, group);
 }
 
-// Whether the (row tile, key tile) pairs of a call can be numbered in 31 bits by both kernels: 128 rows or
+// Whether the (row tile, key tile) pairs of a call can be numbered in 30 bits by both kernels: 128 rows or
 // more a tile and 64 keys for the many-row one, 4 rows and 16 keys at least for the other.
 bool countable(const Batch &b, const Cache &c, int n_heads) {
   const int group = n_heads / c.kv_heads;
@@ -725,7 +756,7 @@ bool countable(const Batch &b, const Cache &c, int n_heads) {
   const double keys = (double)b.table_row * c.page, tokens = b.n_tokens, seqs = b.n_seqs;
   const double few = many ? seqs * (FEW_ROWS / 4) : tokens * group / 4 + seqs;
   const double rest = many ? (tokens * group / 128 + seqs) * (keys / 64 + 8) : 0;
-  return few * c.kv_heads * (keys / 16 + 2) < INT32_MAX && rest * c.kv_heads < INT32_MAX;
+  return few * c.kv_heads * (keys / 16 + 2) < 1 << 30 && rest * c.kv_heads < 1 << 30;
 }
 
 // Partial results of both kernels, then the counters of both.

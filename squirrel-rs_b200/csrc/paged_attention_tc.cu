@@ -36,6 +36,7 @@
 #include <cuda.h>
 #include <float.h>
 
+#include "ops.cuh"
 #include "paged_attention.cuh"
 #include "tc.cuh"
 
@@ -350,6 +351,8 @@ __global__ void __launch_bounds__(THREADS, 1) k_paged_many(const AttnArgs<T> a) 
   auto bar = [&](int i) { return base + C::OFF_BAR + 8u * (uint32_t)i; };
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const Cache &c = a.c;
+  pdl_wait();  // the batch, q and the cache come from earlier kernels
+  pdl_trigger();
 
   // ---- this block's piece of the line
   auto blocks_of = [&](int b) -> int {
@@ -1029,8 +1032,7 @@ cudaError_t launch(cudaStream_t s, AttnArgs<T> &a) {
     blocks[dev] = min(sms, MAX_BLOCKS);
   }
   a.max_row_tiles = many_row_tiles(a.b.max_new, a.group);
-  k_paged_many<C, T><<<blocks[dev], THREADS, C::SMEM, s>>>(a);
-  return cudaGetLastError();
+  return launch_ex(k_paged_many<C, T>, dim3(blocks[dev]), dim3(THREADS), C::SMEM, s, pdl_enabled(), a);
 }
 
 }  // namespace

@@ -17,6 +17,7 @@
 #include <string>
 
 #include "common.cuh"
+#include "ops.cuh"
 #include "status.h"
 
 namespace sq {
@@ -148,6 +149,8 @@ __global__ void __cluster_dims__(VERIFY_CLUSTER, 1, 1) __launch_bounds__(VERIFY_
   const int rank = cluster.block_rank(), b = blockIdx.x / VERIFY_CLUSTER;
   const int tid = threadIdx.x, lane = tid & 31, wid = tid >> 5;
   const int K = a.max_draft, V = a.vocab;
+  pdl_wait();  // the probabilities come from earlier kernels
+  pdl_trigger();
   const int n = a.n_draft ? min(max(a.n_draft[b], 0), K) : K;
   const int *tok = a.tokens + (long long)b * K;
   const float *u = a.uniform + (long long)b * (K + 1);
@@ -245,7 +248,8 @@ extern "C" int sq_verify_drafts(void *stream, const float *target, long long tar
   if (!n_seqs) return SQ_OK;
   const VerifyArgs a = {target, draft,     uniform, tokens,     n_draft,   target_stride, draft_stride,
                         max_draft, vocab, n_accepted, out_tokens};
-  k_verify<<<n_seqs * VERIFY_CLUSTER, VERIFY_THREADS, 0, (cudaStream_t)stream>>>(a);
-  SQ_CHECK_LAUNCH("sq_verify_drafts");
+  const cudaError_t e = launch_ex(k_verify, dim3(n_seqs * VERIFY_CLUSTER), dim3(VERIFY_THREADS), 0,
+                                  (cudaStream_t)stream, pdl_enabled(), a);
+  if (e != cudaSuccess) return cuda_fail(e, "sq_verify_drafts");
   return SQ_OK;
 }
