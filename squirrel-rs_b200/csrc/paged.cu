@@ -153,7 +153,7 @@ struct AppendArgs {
 
 // Blocks [0, page_blocks): one (sequence, touched page, kv head, K or V) each. The rest: one part of a query row each.
 template <typename T>
-__global__ void __launch_bounds__(512) k_paged_append(const AppendArgs<T> a) {
+__global__ void __launch_bounds__(256) k_paged_append(const AppendArgs<T> a) {
   const Cache &c = a.c;
   const int tid = threadIdx.x, half = c.hd / 2, threads = blockDim.x;
   pdl_wait();  // the rows and the batch come from earlier kernels, which may still read the cache
@@ -332,7 +332,7 @@ cudaError_t append(cudaStream_t s, const Cache &c, const Batch &b, const void *k
   const long long page_blocks = 2LL * b.n_seqs * a.touches * c.kv_heads;
   // as many threads as a page's new rows have chunks for, up to HELD a thread
   const int chunks = std::min(c.page, b.max_new) * c.hd / 8;
-  const int threads = std::min(std::max((chunks + HELD - 1) / HELD + 31 & ~31, 128), 512);
+  const int threads = std::min(std::max((chunks + HELD - 1) / HELD + 31 & ~31, 64), 256);
   a.q_parts = q ? (n_heads * c.hd / 8 + threads * Q_CHUNKS - 1) / (threads * Q_CHUNKS) : 0;
   const long long blocks = page_blocks + (long long)b.n_tokens * a.q_parts;
   if (blocks > INT32_MAX) return cudaErrorInvalidConfiguration;
