@@ -792,7 +792,10 @@ __global__ void __launch_bounds__(THREADS, 1) k_paged_many(const AttnArgs<T> a) 
 #pragma unroll 1
       for (int i = 0; ok && active && n && i <= n; i++) {
         if (i == n) {
-          ok = wait(B_PV + x, tile_done + n - 1);
+          // A wait tells a phase from the one before it only: the scores of block n - 1 came after the products of
+          // block n - 3, so with bf16 rows, which do not wait in every turn, those of block n - 2 are waited for first.
+          if (!SPLIT && n > 1) ok = wait(B_PV + x, tile_done + n - 2);
+          ok = ok && wait(B_PV + x, tile_done + n - 1);
           fence_after();
           if (ok) add_output(unit);
           break;

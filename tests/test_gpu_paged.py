@@ -282,6 +282,20 @@ def test_attention_strided_rows_streams_and_repeats(gpu_lib):
     assert (out[:, :64] == -3).all() and (out[:, 576:] == -3).all()
 
 
+@pytest.mark.parametrize("kind", ["f32", "bf16"])
+@pytest.mark.parametrize("hd", [64, 128])
+def test_attention_long_prompts(gpu_lib, hd, kind):
+    """Many row tiles, most of them cut between thread blocks: the result, and equal bits on every call
+    (the products of a piece's last two key blocks are both done before its rows are written)."""
+    from sqb200 import paged
+    s = Setup(14, 8, hd, 64, [1100, 700], [1300, 700])
+    q = s.rows(32 * hd, kind, 1.5)
+    first = paged.attention(s.dcache, s.batch, dev(q).to(KINDS[kind]))
+    for _ in range(20):
+        assert torch.equal(paged.attention(s.dcache, s.batch, dev(q).to(KINDS[kind])), first)
+    s.check_attention(32, kind, q=q)
+
+
 def test_attention_in_a_graph_follows_the_batch(gpu_lib):
     """A captured step replays with new lengths in the batch's arrays."""
     from sqb200 import paged
