@@ -119,7 +119,7 @@ __device__ __forceinline__ void store8(__nv_bfloat16 *p, const Eight &e) {
   *reinterpret_cast<uint4 *>(p) = make_uint4(w[0], w[1], w[2], w[3]);
 }
 __device__ __forceinline__ void spin8(Eight &e, const float *cos, const float *sin) {
-  const float4 c = __ldg(reinterpret_cast<const float4 *>(cos)), s = __ldg(reinterpret_cast<const float4 *>(sin));
+  const float4 c = *reinterpret_cast<const float4 *>(cos), s = *reinterpret_cast<const float4 *>(sin);
   spin(e.x[0], e.x[1], c.x, s.x);
   spin(e.x[2], e.x[3], c.y, s.y);
   spin(e.x[4], e.x[5], c.z, s.z);
@@ -266,8 +266,8 @@ constexpr int READ_ROWS = 4;
 // 16 bytes stored), all of them on their way before the first is stored.
 template <typename T>
 __global__ void __launch_bounds__(READ_THREADS)
-    k_paged_read(const Cache c, const Batch b, const int *__restrict__ first, int count, T *__restrict__ k_out,
-                 T *__restrict__ v_out) {
+    k_paged_read(const Cache c, const Batch b, const int *first, int count, T *k_out,
+                 T *v_out) {
   constexpr int N = 16 / sizeof(T), WORDS = N / 4;
   pdl_wait();
   pdl_trigger();

@@ -18,12 +18,15 @@
 // power of two; an f32 row takes two f16 terms (22 bits) and so two products, a bf16 row is
 // exact in one. Weights, at most 2^10 (the maximum's), likewise: two terms for f32
 // rows, one (11 bits, under the output's 8) for bf16 rows. The V scale of a page goes
-// into the weights relative to the largest met so far, so f16 never overflows. K's codes
-// enter as the f16 numbers code * 2^-24 (denormal, exact; one instruction a pair) and
-// their bias leaves with the sum of the row, 128 sum(q): that costs a score two bits of 24
-// at most. V's bias is taken off before the product: an output is an average that may be
-// a thousand times smaller than 128. The tensor core truncates its running sum (2^-25 of it a
-// step on average), so f32 rows move their sums every 16 steps to f32 sums in shared memory.
+// into the weights relative to the largest met so far, so f16 never overflows. With bf16
+// rows K's codes enter as the f16 numbers code * 2^-24 (denormal, exact; one instruction a
+// pair) and their bias leaves with the sum of the row, 128 sum(q): that costs a score two
+// bits of 24 at most. With f32 rows the bias is taken off before the product (one
+// instruction a pair more), and V's always is: an output is an average that may be a
+// thousand times smaller than 128. The tensor core truncates its running sum (2^-25 of it a
+// step on average), so f32 rows move their sums every 8 groups of keys to f32 sums in shared
+// memory. Both together, 4 x 131,072 positions: 66 -> 69 us; the error of 25,090 positions
+// (128 dimensions) 1.0e-6 -> 5.6e-7 of the result, of 5 drafts x 4,099 1.2e-6 -> 8.1e-7.
 //
 // Work is split evenly over the grid: the (sequence, kv head, row tile, key tile) space is
 // one line, every block takes an equal piece of it, the four warps of a block take its key
@@ -49,7 +52,7 @@ constexpr int WARPS = 4, THREADS = WARPS * 32, STAGES = 2;
 constexpr int BLOCKS_PER_SM = 3;
 constexpr int MAX_BLOCKS = 160 * BLOCKS_PER_SM;  // and parts of a row tile
 constexpr int MIN_TILES = WARPS;  // key tiles a block takes at least
-constexpr int FLUSH_STEPS = 16;   // f32 rows: 16-key products summed on the tensor core at a stretch
+constexpr int FLUSH_STEPS = 8;    // f32 rows: groups of 16 keys summed on the tensor core at a stretch
 constexpr int SLOT_FLOATS = 2112;  // partial results of a row tile: 32 x 66 at most: maxima, sums, [row][head_dim]
 constexpr size_t PARTIAL_BYTES = (size_t)MAX_BLOCKS * 2 * SLOT_FLOATS * 4;
 constexpr float WEIGHT_EXP = 10.f;  // weights are 2^(s - max + 10)
@@ -59,9 +62,15 @@ __device__ __forceinline__ uint2 lds64(uint32_t a) {
   asm volatile("ld.shared.v2.u32 {%0, %1}, [%2];" : "=r"(v.x), "=r"(v.y) : "r"(a));
   return v;
 }
-// Codes (bytes 0, 2) and (1, 3) of a word as pairs of f16 numbers code * 2^-24.
-__device__ __forceinline__ uint32_t codes_02(uint32_t w) { return w & 0x00FF00FFu; }
-__device__ __forceinline__ uint32_t codes_13(uint32_t w) { return __byte_perm(w, 0, 0x4341); }
+// Codes (bytes 0, 2) and (1, 3) of a word as pairs of f16 numbers: code * 2^-24, or exact code - 128.
+template <bool EXACT>
+__device__ __forceinline__ uint32_t codes_02(uint32_t w) {
+  return EXACT ? sub1152(w & 0x00FF00FFu | 0x64006400u) : w & 0x00FF00FFu;
+}
+template <bool EXACT>
+__device__ __forceinline__ uint32_t codes_13(uint32_t w) {
+  return EXACT ? sub1152(__byte_perm(w, 0x64646464u, 0x4341)) : __byte_perm(w, 0, 0x4341);
+}
 __device__ __forceinline__ uint32_t transpose8x8(uint32_t x) {
   uint32_t y;
   asm("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(y) : "r"(x));
@@ -135,6 +144,7 @@ __device__ __forceinline__ Span key_span(const Seq &s, int window, int sinks) {
 template <class C, typename T>
 __global__ void __launch_bounds__(THREADS, C::BLOCKS) k_paged_few(const AttnArgs<T> a) {
   constexpr int HD = C::HD, NT = C::NT, TK = C::TK, NG = C::NG, KS = C::KS, ROWS = C::ROWS, TERMS = C::TERMS, SNAP = C::SNAP;
+  constexpr bool SPLIT = C::SPLIT;
   constexpr int MT = HD / 16;  // 16-dimension tiles of the output
   extern __shared__ __align__(128) uint8_t ring[];
   __shared__ int s_scan[WARPS + 1];
@@ -250,7 +260,7 @@ __global__ void __launch_bounds__(THREADS, C::BLOCKS) k_paged_few(const AttnArgs
     // f32 rows: sums[i][lane] += o every few tiles; `late` is what they have still to be multiplied by
     float *sums = reinterpret_cast<float *>(ring + C::RING) + wid * (32 * MT * NT * 4) + lane;
     float late[NT][2];
-    if constexpr (C::SPLIT) {
+    if constexpr (SPLIT) {
 #pragma unroll
       for (int nt = 0; nt < NT; nt++) late[nt][0] = late[nt][1] = 1.f;
 #pragma unroll
@@ -356,7 +366,7 @@ __global__ void __launch_bounds__(THREADS, C::BLOCKS) k_paged_few(const AttnArgs
       const int e = row_exp(top);
       const float up = row_factor(e, finite);
       const float down = scalbnf(a.scale, -e);
-      float sum = 0.f;  // of the row's terms, for the bias of the codes
+      float sum = 0.f;  // of the row, for the bias of the codes
 #pragma unroll
       for (int i = 0; i < KS; i++) {
 #pragma unroll
@@ -364,12 +374,8 @@ __global__ void __launch_bounds__(THREADS, C::BLOCKS) k_paged_few(const AttnArgs
           const float u = x[4 * i + j] * up, v = x[4 * i + j + 2] * up;
           qf[nt][i][0][j] = pack(u, v);
           const float2 hi = unpack(qf[nt][i][0][j]);
-          sum += hi.x + hi.y;
-          if constexpr (C::SPLIT) {
-            qf[nt][i][1][j] = pack(u - hi.x, v - hi.y);
-            const float2 lo = unpack(qf[nt][i][1][j]);
-            sum += lo.x + lo.y;
-          }
+          if constexpr (SPLIT) qf[nt][i][1][j] = pack(u - hi.x, v - hi.y);
+          else sum += hi.x + hi.y;
         }
       }
       sum += __shfl_xor_sync(0xffffffffu, sum, 1);
@@ -378,8 +384,8 @@ __global__ void __launch_bounds__(THREADS, C::BLOCKS) k_paged_few(const AttnArgs
       for (int j = 0; j < 2; j++) {  // row 2t + j is held by the lanes of g = 2t + j
         const int from = (2 * t + j) * 4;
         const float d = __shfl_sync(0xffffffffu, down, from), q = __shfl_sync(0xffffffffu, sum, from);
-        cf[nt][j] = d * 16777216.f;
-        cb[nt][j] = -128.f * q * d;
+        cf[nt][j] = SPLIT ? d : d * 16777216.f;
+        cb[nt][j] = SPLIT ? 0.f : -128.f * q * d;
         pos[nt][j] = __shfl_sync(0xffffffffu, ok ? pos0 + tok : -1, from);
       }
     }
@@ -395,7 +401,7 @@ __global__ void __launch_bounds__(THREADS, C::BLOCKS) k_paged_few(const AttnArgs
         if (k && move != 1.f) {
 #pragma unroll
           for (int nt = 0; nt < NT; nt++) {
-            if (C::SPLIT) late[nt][0] *= move, late[nt][1] *= move;
+            if (SPLIT) late[nt][0] *= move, late[nt][1] *= move;
 #pragma unroll
             for (int mt = 0; mt < MT; mt++)
 #pragma unroll
@@ -431,7 +437,7 @@ __global__ void __launch_bounds__(THREADS, C::BLOCKS) k_paged_few(const AttnArgs
             const uint32_t uu[4] = {u.x, u.y, u.z, u.w}, ww[4] = {w.x, w.y, w.z, w.w};
 #pragma unroll
             for (int x = 0; x < 4; x++) {
-              const uint32_t f[4] = {codes_02(uu[x]), codes_02(ww[x]), codes_13(uu[x]), codes_13(ww[x])};
+              const uint32_t f[4] = {codes_02<SPLIT>(uu[x]), codes_02<SPLIT>(ww[x]), codes_13<SPLIT>(uu[x]), codes_13<SPLIT>(ww[x])};
 #pragma unroll
               for (int nt = 0; nt < NT; nt++)
 #pragma unroll
@@ -444,7 +450,7 @@ __global__ void __launch_bounds__(THREADS, C::BLOCKS) k_paged_few(const AttnArgs
           const uint32_t uu[2] = {u.x, u.y}, ww[2] = {w.x, w.y};
 #pragma unroll
           for (int x = 0; x < 2; x++) {
-            const uint32_t f[4] = {codes_02(uu[x]), codes_02(ww[x]), codes_13(uu[x]), codes_13(ww[x])};
+            const uint32_t f[4] = {codes_02<SPLIT>(uu[x]), codes_02<SPLIT>(ww[x]), codes_13<SPLIT>(uu[x]), codes_13<SPLIT>(ww[x])};
 #pragma unroll
             for (int nt = 0; nt < NT; nt++)
 #pragma unroll
@@ -501,7 +507,7 @@ __global__ void __launch_bounds__(THREADS, C::BLOCKS) k_paged_few(const AttnArgs
         for (int nt = 0; nt < NT; nt++) {
           const float f0 = corr[nt][0], f1 = corr[nt][1];
           l[nt][0] *= f0, l[nt][1] *= f1;
-          if (C::SPLIT) late[nt][0] *= f0, late[nt][1] *= f1;
+          if (SPLIT) late[nt][0] *= f0, late[nt][1] *= f1;
 #pragma unroll
           for (int mt = 0; mt < MT; mt++) {
             o[mt][nt][0] *= f0, o[mt][nt][1] *= f1, o[mt][nt][2] *= f0, o[mt][nt][3] *= f1;
@@ -524,7 +530,7 @@ __global__ void __launch_bounds__(THREADS, C::BLOCKS) k_paged_few(const AttnArgs
             v *= gshare;
             const uint32_t f = pack(u, v);
             pf[j][nt][0][x] = transpose8x8(f);
-            if constexpr (C::SPLIT) {
+            if constexpr (SPLIT) {
               const float2 hi = unpack(f);
               pf[j][nt][1][x] = transpose8x8(pack(u - hi.x, v - hi.y));
             }
@@ -569,11 +575,11 @@ __global__ void __launch_bounds__(THREADS, C::BLOCKS) k_paged_few(const AttnArgs
       }
       __syncwarp();  // every lane has read the stage that is loaded next
       load_tile(k + STAGES, (in_batch + STAGES < BATCH ? place : next_place), st);
-      if constexpr (C::SPLIT) {
+      if constexpr (SPLIT) {
         if (k % (FLUSH_STEPS / NG) == FLUSH_STEPS / NG - 1) flush();
       }
     }
-    if constexpr (C::SPLIT) flush();
+    if constexpr (SPLIT) flush();
     cp_wait<0>();
     __syncthreads();
 
@@ -591,7 +597,7 @@ __global__ void __launch_bounds__(THREADS, C::BLOCKS) k_paged_few(const AttnArgs
 #pragma unroll
         for (int mt = 0; mt < MT; mt++) {
           const float *sm = sums + ((mt * NT + nt) * 4 + j) * 32;
-          const float2 v = C::SPLIT ? make_float2(sm[0], sm[64]) : make_float2(o[mt][nt][j], o[mt][nt][2 + j]);
+          const float2 v = SPLIT ? make_float2(sm[0], sm[64]) : make_float2(o[mt][nt][j], o[mt][nt][2 + j]);
           const int d = HD >= 128 ? (mt / 8) * 128 + g * 16 + (mt % 8) * 2 : g * (HD / 8) + mt * 2;
           *reinterpret_cast<float2 *>(dst + 2 + d) = make_float2(v.x * unit, v.y * unit);
         }

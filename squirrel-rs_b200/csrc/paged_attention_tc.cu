@@ -616,7 +616,7 @@ __global__ void __launch_bounds__(THREADS, 1) k_paged_many(const AttnArgs<T> a) 
         const int g0 = k * STEP_GROUPS, at_k = STEP_GROUPS == 1 ? at[g0] : (my_group ? at[(g0 + 1) & 3] : at[g0]);
         u[k] = make_uint4(0x80808080u, 0x80808080u, 0x80808080u, 0x80808080u);
         if (present >> (g0 + my_group) & 1)
-          u[k] = __ldg(reinterpret_cast<const uint4 *>(codes + (long long)at_k * (16 * HD)));
+          u[k] = *reinterpret_cast<const uint4 *>(codes + (long long)at_k * (16 * HD));
       }
     };
     auto convert = [&](uint4 (&u)[C::STEPS], uint32_t tile) {

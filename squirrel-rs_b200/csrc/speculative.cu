@@ -78,16 +78,16 @@ template <bool VEC>
 __device__ __forceinline__ void weights4(const Row &r, int i, int end, Parts (&w)[4]) {
   float x[4] = {0.f, 0.f, 0.f, 0.f};
   if (VEC && i + 4 <= end) {
-    const float4 a = __ldg(reinterpret_cast<const float4 *>(r.p + i));
+    const float4 a = *reinterpret_cast<const float4 *>(r.p + i);
     x[0] = a.x, x[1] = a.y, x[2] = a.z, x[3] = a.w;
     if (r.q) {
-      const float4 b = __ldg(reinterpret_cast<const float4 *>(r.q + i));
+      const float4 b = *reinterpret_cast<const float4 *>(r.q + i);
       x[0] = __fsub_rn(x[0], b.x), x[1] = __fsub_rn(x[1], b.y), x[2] = __fsub_rn(x[2], b.z), x[3] = __fsub_rn(x[3], b.w);
     }
   } else {
 #pragma unroll
     for (int j = 0; j < 4; j++)
-      if (i + j < end) x[j] = r.q ? __fsub_rn(__ldg(r.p + i + j), __ldg(r.q + i + j)) : __ldg(r.p + i + j);
+      if (i + j < end) x[j] = r.q ? __fsub_rn(r.p[i + j], r.q[i + j]) : r.p[i + j];
   }
 #pragma unroll
   for (int j = 0; j < 4; j++) w[j] = parts_of(i + j == r.without ? 0.f : x[j]);
