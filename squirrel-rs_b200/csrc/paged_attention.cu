@@ -24,9 +24,10 @@
 // bits of 24 at most. With f32 rows the bias is taken off before the product (one
 // instruction a pair more), and V's always is: an output is an average that may be a
 // thousand times smaller than 128. The tensor core truncates its running sum (2^-25 of it a
-// step on average), so f32 rows move their sums every 8 groups of keys to f32 sums in shared
-// memory. Both together, 4 x 131,072 positions: 66 -> 69 us; the error of 25,090 positions
-// (128 dimensions) 1.0e-6 -> 5.6e-7 of the result, of 5 drafts x 4,099 1.2e-6 -> 8.1e-7.
+// step on average): the scores of the query's two terms are summed apart, and f32 rows
+// move their output sums every 16 groups of keys to f32 sums in shared memory. Measured
+// with 4 x 131,072 positions of f32 rows: the bias taken off afterwards and one sum 66 us, error
+// 1.4e-6 of the result; as it is 69 us, 1.0e-6; sums moved every 8 groups 69.4 us, 8.4e-7.
 //
 // Work is split evenly over the grid: the (sequence, kv head, row tile, key tile) space is
 // one line, every block takes an equal piece of it, the four warps of a block take its key
@@ -52,7 +53,7 @@ constexpr int WARPS = 4, THREADS = WARPS * 32, STAGES = 2;
 constexpr int BLOCKS_PER_SM = 3;
 constexpr int MAX_BLOCKS = 160 * BLOCKS_PER_SM;  // and parts of a row tile
 constexpr int MIN_TILES = WARPS;  // key tiles a block takes at least
-constexpr int FLUSH_STEPS = 8;    // f32 rows: groups of 16 keys summed on the tensor core at a stretch
+constexpr int FLUSH_STEPS = 16;    // f32 rows: groups of 16 keys summed on the tensor core at a stretch
 constexpr int SLOT_FLOATS = 2112;  // partial results of a row tile: 32 x 66 at most: maxima, sums, [row][head_dim]
 constexpr size_t PARTIAL_BYTES = (size_t)MAX_BLOCKS * 2 * SLOT_FLOATS * 4;
 constexpr float WEIGHT_EXP = 10.f;  // weights are 2^(s - max + 10)
@@ -425,10 +426,11 @@ __global__ void __launch_bounds__(THREADS, C::BLOCKS) k_paged_few(const AttnArgs
       float sc[NG][NT][4];
 #pragma unroll
       for (int j = 0; j < NG; j++) {
+        float second[NT][4];  // of the second terms
 #pragma unroll
         for (int nt = 0; nt < NT; nt++)
 #pragma unroll
-          for (int x = 0; x < 4; x++) sc[j][nt][x] = 0.f;
+          for (int x = 0; x < 4; x++) sc[j][nt][x] = second[nt][x] = 0.f;
         const uint32_t base = kt + j * 16 * HD;
         if constexpr (HD >= 64) {
 #pragma unroll
@@ -441,7 +443,7 @@ __global__ void __launch_bounds__(THREADS, C::BLOCKS) k_paged_few(const AttnArgs
 #pragma unroll
               for (int nt = 0; nt < NT; nt++)
 #pragma unroll
-                for (int y = 0; y < TERMS; y++) mma(sc[j][nt], f, qf[nt][ch * 4 + x][y][0], qf[nt][ch * 4 + x][y][1]);
+                for (int y = 0; y < TERMS; y++) mma(y ? second[nt] : sc[j][nt], f, qf[nt][ch * 4 + x][y][0], qf[nt][ch * 4 + x][y][1]);
             }
           }
         } else {
@@ -454,8 +456,14 @@ __global__ void __launch_bounds__(THREADS, C::BLOCKS) k_paged_few(const AttnArgs
 #pragma unroll
             for (int nt = 0; nt < NT; nt++)
 #pragma unroll
-              for (int y = 0; y < TERMS; y++) mma(sc[j][nt], f, qf[nt][x][y][0], qf[nt][x][y][1]);
+              for (int y = 0; y < TERMS; y++) mma(y ? second[nt] : sc[j][nt], f, qf[nt][x][y][0], qf[nt][x][y][1]);
           }
+        }
+        if constexpr (SPLIT) {
+#pragma unroll
+          for (int nt = 0; nt < NT; nt++)
+#pragma unroll
+            for (int x = 0; x < 4; x++) sc[j][nt][x] += second[nt][x];
         }
       }
       // in log2 units

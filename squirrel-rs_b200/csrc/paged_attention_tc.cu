@@ -536,11 +536,11 @@ __global__ void __launch_bounds__(THREADS, 1) k_paged_many(const AttnArgs<T> a) 
           const uint32_t d = tm + x * 128 + buf * 64;
           if (leader) {
 #pragma unroll
-            for (int t = 0; t < TERMS; t++)
+            for (int t = TERMS - 1; t >= 0; t--)  // second terms first: their sums are small when they are truncated
 #pragma unroll
               for (int i = 0; i < HD / 16; i++)
                 mma_f16(d, q + ((t * C::Q_TILE + (i >> 2) * C::Q_PANEL + (i & 3) * 32) >> 4),
-                        kk + (((i >> 2) * C::KV_PANEL + (i & 3) * 32) >> 4), idesc_f16(TILE_ROWS, BK, false), t || i);
+                        kk + (((i >> 2) * C::KV_PANEL + (i & 3) * 32) >> 4), idesc_f16(TILE_ROWS, BK, false), t < TERMS - 1 || i);
             mma_commit(bar(B_S + 2 * x + buf));
           }
         };
@@ -549,10 +549,10 @@ __global__ void __launch_bounds__(THREADS, 1) k_paged_many(const AttnArgs<T> a) 
           const uint32_t d = tm + TM_O + x * 128, w = tm + x * 128 + buf * 64;
           if (leader) {
 #pragma unroll
-            for (int t = 0; t < TERMS; t++)
+            for (int t = TERMS - 1; t >= 0; t--)
 #pragma unroll
               for (int i = 0; i < BK / 16; i++)
-                mma_f16_ts(d, w + t * 32 + i * 8, v + (i * 2048 >> 4), idesc_f16(TILE_ROWS, HD, true), t || i || add);
+                mma_f16_ts(d, w + t * 32 + i * 8, v + (i * 2048 >> 4), idesc_f16(TILE_ROWS, HD, true), t < TERMS - 1 || i || add);
             mma_commit(bar(B_PV + x));
           }
         };
