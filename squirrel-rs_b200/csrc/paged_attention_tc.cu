@@ -24,9 +24,11 @@
 // for f32 rows, one (exact) for bf16 rows. Weights are 2^(s - ref + 3); ref follows the
 // maximum only when it is passed by 2^6, and the V scales go into the weights relative to
 // a unit, so that f16 never overflows and outputs are seldom rescaled.
-//   f32 rows:  weights in two terms; each block's O is summed on its own in tensor memory and
+//   f32 rows:  weights in two terms; the O of four blocks of keys is summed in tensor memory and
 //              added to f32 registers, because the tensor core truncates its running sum
-//              (2^-25 of it a step: 500 steps would cost 1e-5).
+//              (2^-25 of it a step: 500 steps would cost 1e-5). 2048 x 4,133 positions, 128
+//              dimensions: every block 371 us (error 4.5e-7 of the result), every four 348 us
+//              (7.5e-7), every eight 344 us (1.2e-6).
 //   bf16 rows: weights in one term (11 bits, under the output's 8); O stays in tensor memory.
 //
 // Work is split as in the few-row kernel: one line of (sequence, kv head, row tile, key
@@ -53,6 +55,7 @@ constexpr int TILE_ROWS = 128, ROWS = 2 * TILE_ROWS;
 constexpr int BATCH = 8, BATCHES = 2;  // blocks of keys looked up at once, and how many such batches are held
 constexpr int MAX_BLOCKS = 160;
 constexpr int MIN_BLOCKS = 2;  // key blocks a thread block takes at least
+constexpr int MOVE = 4;        // f32 rows: blocks of keys summed in tensor memory at a stretch
 constexpr float WEIGHT_EXP = 3.f, REF_LAG = 6.f, UNIT_LAG = 64.f;
 // Registers a thread: launched with 128 (512 x 128 = 65,536), then 256 x 184 + 128 x 80 + 128 x 64.
 constexpr int SOFTMAX_REGS = 184, LOAD_REGS = 80, MMA_REGS = 64;
@@ -74,7 +77,7 @@ struct Cfg {
   static constexpr int OFF_Q = 0, OFF_K = OFF_Q + 2 * TERMS * Q_TILE, OFF_V = OFF_K + STAGES * KV_TILE,
                        OFF_SCALE = OFF_V + STAGES * KV_TILE,
                        OFF_BAR = OFF_SCALE + BATCHES * BATCH * 96;
-  static constexpr int SMEM = 1024 + OFF_BAR + 320;
+  static constexpr int SMEM = 1024 + OFF_BAR + 352;
   static constexpr int SLOT = ROWS * (HD + 2);  // floats of a cut row tile's partial result
   static_assert(SMEM <= 232448 - 256, "shared memory of a block");
 };
@@ -92,21 +95,24 @@ struct Plan {
 static_assert(sizeof(Plan) == 96, "room in shared memory");
 
 constexpr int MAX_STAGES = 4;
+// A wait tells a phase from the one before it only. So every barrier is one whose phase before is known to be done
+// when a phase is waited for, and whose phase after cannot be: where a waiter may skip phases or lag behind, there
+// is one for each buffer or place.
 enum : int {
-  B_Q = 0,        // both tiles' queries written
-  B_K = 1,        // [stages] K written
-  B_K_FREE = 5,   // [stages] scores of both tiles done
-  B_V = 9,        // [stages]
-  B_V_FREE = 13,  // [stages]
-  B_S = 17,       // [2 tiles][2 buffers] scores done
-  B_P = 21,       // [2 tiles][2 buffers] weights written
-  B_PV = 25,      // [2 tiles] a block's P V done
-  B_PIECE = 27,   // [4] a piece handed out
-  B_DONE = 31,    // a piece's rows written
-  B_PLAN = 32,    // [2] a batch of blocks looked up
-  B_PLAN_FREE = 34,
-  B_FIN = 36,
-  N_BARS = 37
+  B_Q = 0,        // [2] both tiles' queries of a piece written
+  B_K = 2,        // [stages] K written
+  B_K_FREE = 6,   // [stages] scores of both tiles done
+  B_V = 10,       // [stages]
+  B_V_FREE = 14,  // [stages]
+  B_S = 18,       // [2 tiles][2 buffers] scores done
+  B_P = 22,       // [2 tiles][2 buffers] weights written
+  B_PV = 26,      // [2 tiles][2 buffers] P V done
+  B_PIECE = 30,   // [4] a piece handed out
+  B_DONE = 34,    // [4] a piece's rows written
+  B_PLAN = 38,    // [2] a batch of blocks looked up
+  B_PLAN_FREE = 40,
+  B_FIN = 42,
+  N_BARS = 43
 };
 // Columns: S, and P over it, of tile X and buffer B at 128 X + 64 B (P: first terms in 32, second terms
 // in the next 32); O at 256 + 128 X.
@@ -406,7 +412,7 @@ __global__ void __launch_bounds__(THREADS, 1) k_paged_many(const AttnArgs<T> a) 
 
   if (tid == 0) {
     for (int i = 0; i < N_BARS; i++) {
-      const unsigned count = i == B_Q || i == B_DONE                                         ? SOFTMAX_WARPS
+      const unsigned count = i < B_Q + 2 || (i >= B_DONE && i < B_DONE + PIECES)             ? SOFTMAX_WARPS
                              : i >= B_P && i < B_P + 4                                       ? SOFTMAX_WARPS / 2
                              : (i >= B_K && i < B_K + MAX_STAGES) || (i >= B_V && i < B_V + MAX_STAGES) ? LOAD_WARPS
                                                                                              : 1;
@@ -448,7 +454,7 @@ __global__ void __launch_bounds__(THREADS, 1) k_paged_many(const AttnArgs<T> a) 
         Piece p;
         more = walk.next(a, p);
         if (!more) p.n = -1;
-        if (k >= PIECES && !wait(B_DONE, k - PIECES)) break;  // its place is free
+        if (k >= PIECES && !wait(B_DONE + k % PIECES, k / PIECES - 1)) break;  // its place is free
         if (lane == 0) {
           s_pieces[k % PIECES] = p;
           bar_arrive(bar(B_PIECE + k % PIECES));
@@ -479,14 +485,13 @@ __global__ void __launch_bounds__(THREADS, 1) k_paged_many(const AttnArgs<T> a) 
           }
           float top = fmaxf(vs, __shfl_xor_sync(0xffffffffu, vs, 1));
           top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
-          float my_unit = top;
-          if (!SPLIT) {  // outputs stay in the unit of the first block until a much larger scale comes
+          float my_unit = 0.f;
+          // outputs stay in the unit of the first block (of the stretch) until a much larger scale comes
 #pragma unroll 1
-            for (int q = 0; q < BATCH; q++) {
-              const float t = __shfl_sync(0xffffffffu, top, 4 * q);
-              if (t > unit * UNIT_LAG || unit == 0.f) unit = t;
-              if (lane >> 2 == q) my_unit = unit;
-            }
+          for (int q = 0; q < BATCH; q++) {
+            const float t = __shfl_sync(0xffffffffu, top, 4 * q);
+            if (t > unit * UNIT_LAG || unit == 0.f || (SPLIT && q % MOVE == 0)) unit = t;
+            if (lane >> 2 == q) my_unit = unit;
           }
           const uint32_t present = __ballot_sync(0xffffffffu, page >= 0) >> (lane & 28) & 15;
           const uint32_t with_v = __ballot_sync(0xffffffffu, vs > 0.f) >> (lane & 28) & 15;
@@ -553,10 +558,10 @@ __global__ void __launch_bounds__(THREADS, 1) k_paged_many(const AttnArgs<T> a) 
 #pragma unroll
               for (int i = 0; i < BK / 16; i++)
                 mma_f16_ts(d, w + t * 32 + i * 8, v + (i * 2048 >> 4), idesc_f16(TILE_ROWS, HD, true), t < TERMS - 1 || i || add);
-            mma_commit(bar(B_PV + x));
+            mma_commit(bar(B_PV + 2 * x + buf));
           }
         };
-        if (!(ok = wait(B_Q, k))) break;
+        if (!(ok = wait(B_Q + (k & 1), k / 2))) break;
         // Turn i: P V of block i, then the scores of block i + 2 (turns -2 and -1: the first scores alone).
 #pragma unroll 1
         for (int i = -2; ok && i < n; i++) {
@@ -573,7 +578,7 @@ __global__ void __launch_bounds__(THREADS, 1) k_paged_many(const AttnArgs<T> a) 
             if (i >= 0) {
               if (!(ok = wait(B_P + 2 * x + buf, t / 2))) break;
               fence_after();
-              output(x, buf, st, !SPLIT && i);
+              output(x, buf, st, SPLIT ? i % MOVE : i);
             }
             if (more) scores(x, buf, st2);
           }
@@ -763,7 +768,7 @@ __global__ void __launch_bounds__(THREADS, 1) k_paged_many(const AttnArgs<T> a) 
       }
       fence_proxy_async();
       __syncwarp();
-      if (lane == 0) bar_arrive(bar(B_Q));
+      if (lane == 0) bar_arrive(bar(B_Q + (k & 1)));
 
       const int pos0 = piece.pos0, t0 = piece.t0, n_sink = piece.n_sink, skip = piece.skip;
       const int pos = live ? pos0 + tok : -1;
@@ -775,7 +780,7 @@ __global__ void __launch_bounds__(THREADS, 1) k_paged_many(const AttnArgs<T> a) 
 #pragma unroll
         for (int d = 0; d < HD; d++) o[d] = 0.f;
       }
-      // f32 rows: o += unit * O of the last block
+      // f32 rows: o += unit * O
       auto add_output = [&](float unit) {
         if constexpr (SPLIT) {
 #pragma unroll
@@ -788,14 +793,13 @@ __global__ void __launch_bounds__(THREADS, 1) k_paged_many(const AttnArgs<T> a) 
           }
         }
       };
-      // Turn i = n only takes the last block's output.
+      // Products of the tile's block t (not every turn waits for them; those of t - 2 came before the scores of t).
+      auto products_done = [&](unsigned t) { return wait(B_PV + 2 * x + (t & 1), t / 2); };
+      // Turn i = n only takes the last output.
 #pragma unroll 1
       for (int i = 0; ok && active && n && i <= n; i++) {
         if (i == n) {
-          // A wait tells a phase from the one before it only: the scores of block n - 1 came after the products of
-          // block n - 3, so with bf16 rows, which do not wait in every turn, those of block n - 2 are waited for first.
-          if (!SPLIT && n > 1) ok = wait(B_PV + x, tile_done + n - 2);
-          ok = ok && wait(B_PV + x, tile_done + n - 1);
+          ok = products_done(tile_done + n - 1);
           fence_after();
           if (ok) add_output(unit);
           break;
@@ -882,27 +886,30 @@ __global__ void __launch_bounds__(THREADS, 1) k_paged_many(const AttnArgs<T> a) 
         if constexpr (SPLIT) tmem_st32(s_col + 32, lo);
         l = fmaf(l, alpha, sum);
         float move = alpha;
-        if (!SPLIT && unit != new_unit) move *= new_unit > 0.f ? unit / new_unit : 0.f;
+        if (unit != new_unit) move *= new_unit > 0.f ? unit / new_unit : 0.f;
+        const bool take = SPLIT && i % MOVE == 0;  // the output so far is taken, this block's starts anew
         const bool any = i && __any_sync(0xffffffffu, move != 1.f);
-        if (i && (SPLIT || any)) {  // the last block's P V is done before its output is read or moved
-          if (!(ok = wait(B_PV + x, t - 1))) break;
+        if (i && (take || any)) {  // the last block's P V is done before its output is read or moved
+          if (!(ok = products_done(t - 1))) break;
           fence_after();
-          add_output(unit);
-          if (any) {
-            if constexpr (SPLIT) {
-#pragma unroll
-              for (int d = 0; d < HD; d++) o[d] *= move;
-            } else {
+          if (take) {
+            add_output(unit);
+          } else {
 #pragma unroll 1
-              for (int d = 0; d < HD; d += 32) {
-                float y[32];
-                tmem_ld32(o_col + d, y);
-                tmem_ready<32>(y);
-                uint32_t u[32];
+            for (int d = 0; d < HD; d += 32) {
+              float y[32];
+              tmem_ld32(o_col + d, y);
+              tmem_ready<32>(y);
+              uint32_t u[32];
 #pragma unroll
-                for (int j = 0; j < 32; j++) u[j] = __float_as_uint(y[j] * move);
-                tmem_st32(o_col + d, u);
-              }
+              for (int j = 0; j < 32; j++) u[j] = __float_as_uint(y[j] * move);
+              tmem_st32(o_col + d, u);
+            }
+          }
+          if constexpr (SPLIT) {
+            if (__any_sync(0xffffffffu, alpha != 1.f)) {
+#pragma unroll
+              for (int d = 0; d < HD; d++) o[d] *= alpha;
             }
           }
         }
@@ -1008,7 +1015,7 @@ __global__ void __launch_bounds__(THREADS, 1) k_paged_many(const AttnArgs<T> a) 
         }
       }
       __syncwarp();
-      if (lane == 0) bar_arrive(bar(B_DONE));
+      if (lane == 0) bar_arrive(bar(B_DONE + k % PIECES));
     }
   }
   fence_before();

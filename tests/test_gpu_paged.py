@@ -296,6 +296,13 @@ def test_attention_long_prompts(gpu_lib, hd, kind):
     s.check_attention(32, kind, q=q)
 
 
+@pytest.mark.parametrize("kind", ["f32", "bf16"])
+def test_attention_prompts_among_idle_sequences(gpu_lib, kind):
+    """Short prompts far apart in a long batch: thread blocks finish their rows while the next prompt is looked for."""
+    news, lens = [17 if b % 60 == 7 else 0 for b in range(6000)], [17 + b % 3 for b in range(6000)]
+    Setup(15, 8, 64, 64, news, lens).check_attention(32, kind)
+
+
 def test_attention_in_a_graph_follows_the_batch(gpu_lib):
     """A captured step replays with new lengths in the batch's arrays."""
     from sqb200 import paged
