@@ -159,7 +159,8 @@ typedef struct {
 /* One step of n_seqs sequences, the same for every layer. Row t of a step's q / k / v /
  * output is new token t; sequence b has the rows q_start[b] .. q_start[b + 1] - 1, which
  * are its last positions: kv_len[b] counts what it holds WITH them. The page table names
- * the page of each `page` positions; entries past kv_len are not read. The arrays are
+ * the page of each `page` positions; entries past kv_len, and with a window those of pages
+ * that no new token sees, are not read (such pages may be given away). The arrays are
  * device memory and are read by the kernels (a captured graph replays with new
  * contents); n_tokens and max_new bound what they may say. */
 typedef struct {
@@ -186,7 +187,7 @@ int sq_paged_status(int clear);
  * token that needs more raises it and the page's earlier codes are rounded to the new
  * scale; the first token of a page starts it anew. NaN is stored as 0, an infinity as
  * the page's largest value. q, if not NULL, is rotated into q_out (may be q) in the
- * same launch (rows of n_heads * head_dim). Rows are 16-byte aligned. A page that gets
+ * same launch (rows of n_heads * head_dim). Rows and tables are 16-byte aligned. A page that gets
  * new tokens must belong to one sequence only. */
 int sq_paged_append(void *stream, const sq_paged_cache *c, const sq_paged_batch *b, int dtype,
                     const void *k, long long k_stride, const void *v, long long v_stride,
@@ -198,8 +199,11 @@ int sq_paged_append(void *stream, const sq_paged_cache *c, const sq_paged_batch 
  * positions <= p, with window > 0 only those > p - window and the first `sinks` ones.
  * out = softmax(scale * q.k) v; a query that sees nothing gets zeros. q, out: rows of
  * n_heads * head_dim elements of dtype. ws: sq_paged_attention_workspace() bytes of
- * device memory, 256-byte aligned, zero-filled once before its first use; calls that
- * share it must be ordered on the device. */
+ * device memory, 256-byte aligned, zero-filled once before its first use and again
+ * before it serves another cache shape, n_seqs, max_new or n_heads (its counters' places
+ * follow from them); calls that share it must be ordered on the device. SQ_ERR_SHAPE
+ * also when the step's rows times the page table's positions are too many to count in
+ * 31 bits. */
 int sq_paged_attention(void *stream, const sq_paged_cache *c, const sq_paged_batch *b, int dtype,
                        const void *q, long long q_stride, int n_heads, float scale, int window, int sinks,
                        void *out, long long out_stride, void *ws, size_t ws_bytes);

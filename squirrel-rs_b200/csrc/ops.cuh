@@ -39,7 +39,7 @@ bool matvec_fused_ok(const MvArgs &a, int wtype);
 // pdl: launched with programmatic stream serialization (the kernel streams its first
 // weight tiles while the previous kernel finishes; see pdl_enabled()).
 cudaError_t launch_matvec_fused(cudaStream_t s, const MvArgs &a, int wtype, bool pdl = false);
-// Programmatic dependent launches for the one-row decode step (SQB200_PDL=0 turns them off).
+// Programmatic dependent launches for the one-row decode step and the paged cache (SQB200_PDL=0 turns them off).
 bool pdl_enabled();
 
 // Tensor-core GEMM (gemm_tc.cu) for BF16, Q8_0 and Q4_0 weight rows: the f32

@@ -291,9 +291,10 @@ __global__ void __launch_bounds__(THREADS, C::BLOCKS) k_paged_few(const AttnArgs
     };
     const int n_tiles = t1 - t0 > wid ? (t1 - t0 - wid + WARPS - 1) / WARPS : 0;
     constexpr int BATCH = C::BATCH;
-    auto entry_of = [&](int batch) {  // INT_MIN: no such group
+    const int low = a.window ? min_pos - a.window - 15 : -1;  // groups from there on are in a row's window
+    auto entry_of = [&](int batch) {  // INT_MIN: no such group, or none that a row sees
       const int k = batch * BATCH + lane / NG, key = tile_key(k) + 16 * (lane % NG);
-      return k < n_tiles && key < s.len ? a.b.table[(long long)b * a.b.table_row + (key >> c.page_shift)] : INT_MIN;
+      return k < n_tiles && key < s.len && (key > low || key < a.sinks) ? a.b.table[(long long)b * a.b.table_row + (key >> c.page_shift)] : INT_MIN;
     };
     auto place_of = [&](int batch, int entry) {
       if ((unsigned)entry >= (unsigned)c.n_pages) {

@@ -477,7 +477,8 @@ __global__ void __launch_bounds__(THREADS, 1) k_paged_many(const AttnArgs<T> a) 
           const int i = i0 + (lane >> 2), key = p.block(i) * BK + 16 * j;
           const bool in = i < p.n;
           int page = -1;
-          if (in && key < p.len) page = load_page(a.b, c, p.b, key);
+          const bool seen = !a.window || key > p.pos0 - a.window - 15 || key < a.sinks;  // by a row at all
+          if (in && key < p.len && seen) page = load_page(a.b, c, p.b, key);
           float ks = 0.f, vs = 0.f;
           if (page >= 0) {
             ks = c.ks[(long long)page * c.kv_heads + p.head];

@@ -107,7 +107,8 @@ class PagedCache:
 class PagedBatch:
     """One step: sequence b has rows q_start[b] .. q_start[b + 1] - 1 of the step's tensors,
     the last of the kv_len[b] positions that it holds with them; page_table [n_seqs,
-    pages_per_seq] names its pages (entries past kv_len are not read). The arrays are int32
+    pages_per_seq] names its pages (entries past kv_len, and with a window
+    those of pages that no new token sees, are not read). The arrays are int32
     CUDA tensors and are read by the kernels: their contents may change between calls
     within what n_tokens (rows in all) and max_new (most of one sequence) say. The
     attention's workspace is kept here, so calls with one batch must be ordered on the

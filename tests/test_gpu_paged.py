@@ -215,6 +215,32 @@ def test_attention_window(gpu_lib, case, window, sinks, kind):
 
 
 @pytest.mark.parametrize("kind", ["f32", "bf16"])
+@pytest.mark.parametrize("page", [16, 64])
+def test_attention_pages_left_behind_by_the_window(gpu_lib, page, kind):
+    """Pages that no new token sees may be gone: their entries and scales are not used."""
+    news, lens, window, sinks = [1, 5, 90, 0], [500, 333, 700, 260], 70, 20
+    s = Setup(16, 2, 64, page, news, lens)
+    q = s.rows(8 * 64, kind, 1.5)
+    want, size = P.attention(s.cache, s.q_start, lens, s.table, q, 8, window=window, sinks=sinks)
+    for b, (new, n) in enumerate(zip(news, lens)):
+        for p in range(-(-n // page)):
+            if p * page >= sinks and (p + 1) * page - 1 <= n - new - window:
+                for name in ("ks", "vs"):
+                    s.cache[name][s.table[b, p]] = np.nan
+                s.table[b, p] = -1
+    assert (s.table[2, 3:] == -1).any()
+    s.dcache.k_scale.copy_(dev(s.cache["ks"]))
+    s.dcache.v_scale.copy_(dev(s.cache["vs"]))
+    s.batch.page_table.copy_(dev(s.table))
+    from sqb200 import paged
+    got = paged.attention(s.dcache, s.batch, dev(q).to(KINDS[kind]), window=window, sinks=sinks)
+    torch.cuda.synchronize()
+    paged.status()
+    over = np.abs(got.float().cpu().numpy().reshape(want.shape) - want) / P.bound(want, size, kind)
+    assert over.max() <= 1
+
+
+@pytest.mark.parametrize("kind", ["f32", "bf16"])
 @pytest.mark.parametrize("news,lens", [([4], [2]), ([1, 3], [0, 1]), ([90, 1], [40, 40])])
 def test_attention_rows_that_see_nothing(gpu_lib, news, lens, kind):
     """More rows than positions: the first ones stand before position 0 and get zeros."""
