@@ -756,7 +756,9 @@ cudaError_t launch_few(cudaStream_t s, AttnArgs<T> &a) {
 }
 
 // Rows a kv head up to which a sequence is this file's: beyond, the products cost more than
-// the reading of the cache.
+// the reading of the cache. 12 x 4,096 positions at 64 rows, this kernel against the other:
+// f32 rows 72 / 77 us (64 dimensions) and 82 / 146 us (128), bf16 rows 47 / 58 and 66 / 82 us; at
+// 96 rows the other one is ahead.
 constexpr int FEW_ROWS = 64;
 
 bool goes_many(const Cache &c, int max_new, int group) {
