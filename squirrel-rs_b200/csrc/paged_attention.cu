@@ -772,7 +772,7 @@ bool countable(const Batch &b, const Cache &c, int n_heads) {
   const bool many = goes_many(c, b.max_new, group);
   const double keys = (double)b.table_row * c.page, tokens = b.n_tokens, seqs = b.n_seqs;
   const double few = many ? seqs * (FEW_ROWS / 4) : tokens * group / 4 + seqs;
-  const double rest = many ? (tokens * group / 128 + seqs) * (keys / 64 + 8) : 0;
+  const double rest = many ? (tokens * group / 128 + seqs) * (keys / 64 + 16) : 0;
   return few * c.kv_heads * (keys / 16 + 2) < 1 << 30 && rest * c.kv_heads < 1 << 30;
 }
 

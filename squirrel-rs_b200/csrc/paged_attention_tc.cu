@@ -54,6 +54,10 @@ constexpr int THREADS = WARPS * 32, LOADERS = LOAD_WARPS * 32;
 constexpr int TILE_ROWS = 128, ROWS = 2 * TILE_ROWS;
 constexpr int BATCH = 8, BATCHES = 2;  // blocks of keys looked up at once, and how many such batches are held
 constexpr int MAX_BLOCKS = 160;
+// What a row tile costs besides its key blocks, in blocks (queries in, results out, the pipeline's start and end), when
+// the work is shared out. 0 / 4 / 8 / 12 (bf16, 128 dimensions): 2 x 4,096 rows of 8,000 positions 927 / 831 /
+// 774 / 772 us, 16 x 1,000 rows 348 / 294 / 270 / 271 us, 2,048 rows of 4,133 positions 182 / 173 / 167 / 169 us.
+constexpr int TILE_COST = 8;
 constexpr int MIN_BLOCKS = 2;  // key blocks a thread block takes at least
 constexpr int MOVE = 4;        // f32 rows: blocks of keys summed in tensor memory at a stretch
 constexpr float WEIGHT_EXP = 3.f, REF_LAG = 6.f, UNIT_LAG = 64.f;
@@ -220,9 +224,9 @@ __device__ __forceinline__ int floor_sum(unsigned n, unsigned m, unsigned a, uns
   return sum;
 }
 
-// Key blocks of a sequence's row tiles on the line: without a window the causal count of
-// each (a little over for the last), with one the same for all; what a tile does not
-// have of them is empty.
+// Places of a sequence's row tiles on the line: key blocks, without a window the causal
+// count of each (a little over for the last), with one the same for all, and TILE_COST
+// more; what a tile does not have of them is empty.
 template <int BK>
 struct Line {
   int row_tiles, tokens;  // tokens of a row tile
@@ -238,11 +242,11 @@ struct Line {
       flat = min((min(sinks, s.len) + BK - 1) / BK + (window + tokens + BK - 3) / BK + 1, (s.len + BK - 1) / BK);
   }
   __device__ __forceinline__ int before(int rt) const {  // key blocks of row tiles 0 .. rt - 1
-    if (flat) return rt * flat;
-    return rt + floor_sum(rt, BK, tokens, pos0 + tokens - 1);
+    if (flat) return rt * (flat + TILE_COST);
+    return rt * (1 + TILE_COST) + floor_sum(rt, BK, tokens, pos0 + tokens - 1);
   }
   __device__ __forceinline__ int of(int rt) const {
-    return flat ? flat : (pos0 + (rt + 1) * tokens - 1) / BK + 1;
+    return (flat ? flat : (pos0 + (rt + 1) * tokens - 1) / BK + 1) + TILE_COST;
   }
 };
 
@@ -276,68 +280,71 @@ struct Walk {
 
   template <typename T>
   __device__ __forceinline__ bool next(const AttnArgs<T> &a, Piece &p) {
-    if (at >= end) return false;
-    bool other = !found;
-    if (found && ++rt == line.row_tiles) {
-      rt = 0;
-      if (++head == a.c.kv_heads) {
-        head = 0;
-        other = true;
-        b++;
-      }
-    }
-    if (other) {
 #pragma unroll 1
-      for (;; b++) {  // at < end: a sequence with row tiles follows
-        s = load_seq(a.b, a.c, b);
-        line.set(s, a.group, a.window, a.sinks, a.few_rows);
-        if (line.row_tiles) break;
+    for (;;) {
+      if (at >= end) return false;
+      bool other = !found;
+      if (found && ++rt == line.row_tiles) {
+        rt = 0;
+        if (++head == a.c.kv_heads) {
+          head = 0;
+          other = true;
+          b++;
+        }
       }
-    }
-    if (!found) {
-      per_head = line.before(line.row_tiles);
-      head = (at - seq_start) / per_head;
-      const int in_head = at - seq_start - head * per_head;
-      // the row tile that holds in_head: 32 candidates at a time
-      rt = 0;
+      if (other) {
 #pragma unroll 1
-      for (int width = line.row_tiles; width > 1;) {
-        const int step = (width + 31) / 32, mine = rt + (threadIdx.x & 31) * step;
-        const unsigned le = __ballot_sync(0xffffffffu, mine < rt + width && line.before(mine) <= in_head);
-        const int k = 31 - __clz(le);  // lane 0 always holds
-        rt += k * step;
-        width = min(step, width - k * step);
+        for (;; b++) {  // at < end: a sequence with row tiles follows
+          s = load_seq(a.b, a.c, b);
+          line.set(s, a.group, a.window, a.sinks, a.few_rows);
+          if (line.row_tiles) break;
+        }
       }
-      tile_start = seq_start + head * per_head + line.before(rt);
-      found = true;
+      if (!found) {
+        per_head = line.before(line.row_tiles);
+        head = (at - seq_start) / per_head;
+        const int in_head = at - seq_start - head * per_head;
+        // the row tile that holds in_head: 32 candidates at a time
+        rt = 0;
+#pragma unroll 1
+        for (int width = line.row_tiles; width > 1;) {
+          const int step = (width + 31) / 32, mine = rt + (threadIdx.x & 31) * step;
+          const unsigned le = __ballot_sync(0xffffffffu, mine < rt + width && line.before(mine) <= in_head);
+          const int k = 31 - __clz(le);  // lane 0 always holds
+          rt += k * step;
+          width = min(step, width - k * step);
+        }
+        tile_start = seq_start + head * per_head + line.before(rt);
+        found = true;
+      }
+      const int slots = line.of(rt), first_tok = rt * line.tokens, toks = min(line.tokens, s.n - first_tok);
+      p.b = b;
+      p.head = head;
+      p.row0 = s.first + first_tok;
+      p.n_rows = toks * a.group;
+      p.pos0 = s.len - s.n + first_tok;
+      p.len = s.len;
+      int real = max(p.pos0 + toks - 1, 0) / BK + 1;
+      p.n_sink = p.skip = 0;
+      if (line.flat) {
+        const int low = max(p.pos0 - a.window + 1, 0) / BK;
+        p.n_sink = min((min(a.sinks, s.len) + BK - 1) / BK, low);
+        p.skip = low - p.n_sink;
+        real -= p.skip;
+      }
+      p.t0 = at - tile_start;
+      const int t1 = min(slots, end - tile_start);
+      p.n = min(t1, real) - p.t0;
+      p.whole = p.n == real;
+      p.first = tile_start / per;
+      p.parts = (tile_start + real - 1) / per - p.first + 1;
+      p.late = tile_start > per * p.first;
+      p.slot = 2 * blockIdx.x + (tile_start > per * (int)blockIdx.x ? 1 : 0);
+      p.counter = (b * a.c.kv_heads + head) * a.max_row_tiles + rt;
+      at = tile_start + t1;
+      tile_start += slots;
+      if (p.n > 0) return true;
     }
-    const int slots = line.of(rt), first_tok = rt * line.tokens, toks = min(line.tokens, s.n - first_tok);
-    p.b = b;
-    p.head = head;
-    p.row0 = s.first + first_tok;
-    p.n_rows = toks * a.group;
-    p.pos0 = s.len - s.n + first_tok;
-    p.len = s.len;
-    int real = max(p.pos0 + toks - 1, 0) / BK + 1;
-    p.n_sink = p.skip = 0;
-    if (line.flat) {
-      const int low = max(p.pos0 - a.window + 1, 0) / BK;
-      p.n_sink = min((min(a.sinks, s.len) + BK - 1) / BK, low);
-      p.skip = low - p.n_sink;
-      real -= p.skip;
-    }
-    p.t0 = at - tile_start;
-    const int t1 = min(slots, end - tile_start);
-    p.n = max(min(t1, real) - p.t0, 0);
-    p.whole = p.t0 == 0 && t1 == slots;
-    p.first = tile_start / per;
-    p.parts = (tile_start + slots - 1) / per - p.first + 1;
-    p.late = tile_start > per * p.first;
-    p.slot = 2 * blockIdx.x + (tile_start > per * (int)blockIdx.x ? 1 : 0);
-    p.counter = (b * a.c.kv_heads + head) * a.max_row_tiles + rt;
-    at = tile_start + t1;
-    tile_start += slots;
-    return true;
   }
 };
 
