@@ -705,6 +705,7 @@ __global__ void __launch_bounds__(THREADS, 1) k_paged_many(const AttnArgs<T> a) 
       return res != 0;
     };
     unsigned batch = 0, tile_done = 0;  // batches so far, blocks of this tile
+    const int per_group = (65536 + a.group - 1) / a.group;  // row / group = row * per_group >> 16 for rows < 256
 #pragma unroll 1
     for (unsigned k = 0;; k++) {
       bool ok = wait(B_PIECE + k % PIECES, k / PIECES);
@@ -718,7 +719,7 @@ __global__ void __launch_bounds__(THREADS, 1) k_paged_many(const AttnArgs<T> a) 
       constexpr int ROW_LANES = HD * (int)sizeof(T) / 16, AT_ONCE = 32 / ROW_LANES, PER16 = 16 / (int)sizeof(T);
       const int sub = lane / ROW_LANES, piece16 = lane % ROW_LANES;
       auto row_at = [&](const auto *rows, long long stride, int i) {  // the lane's part of the warp's row i
-        const int q = warp_row + i, t = q / a.group;
+        const int q = warp_row + i, t = q * per_group >> 16;
         return rows + (long long)(row0 + t) * stride + (h0 + q - t * a.group) * HD + piece16 * PER16;
       };
       auto stage = [&](int i, int at) {  // 16-byte chunk `at` of the warp's row i, over the row's bytes in the query tile
