@@ -57,7 +57,7 @@ constexpr int MAX_BLOCKS = 160;
 // What a row tile costs besides its key blocks, in blocks (queries in, results out, the pipeline's start and end), when
 // the work is shared out. 0 / 4 / 8 / 12 (bf16, 128 dimensions): 2 x 4,096 rows of 8,000 positions 927 / 831 /
 // 774 / 772 us, 16 x 1,000 rows 348 / 294 / 270 / 271 us, 2,048 rows of 4,133 positions 182 / 173 / 167 / 169 us.
-constexpr int TILE_COST = 8;
+constexpr int TILE_COST = 5;
 constexpr int MIN_BLOCKS = 2;  // key blocks a thread block takes at least
 constexpr int MOVE = 4;        // f32 rows: blocks of keys summed in tensor memory at a stretch
 constexpr float WEIGHT_EXP = 3.f, REF_LAG = 6.f, UNIT_LAG = 64.f;
@@ -192,9 +192,6 @@ __device__ __forceinline__ void tmem_ready(float *v) {
   asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
 #pragma unroll
   for (int i = 0; i < N; i++) asm volatile("" : "+f"(v[i]));
-}
-__device__ __forceinline__ void sts64(uint32_t a, uint32_t x, uint32_t y) {
-  asm volatile("st.shared.v2.u32 [%0], {%1, %2};" ::"r"(a), "r"(x), "r"(y) : "memory");
 }
 __device__ __forceinline__ void sts128(uint32_t a, uint32_t x, uint32_t y, uint32_t z, uint32_t w) {
   asm volatile("st.shared.v4.u32 [%0], {%1, %2, %3, %4};" ::"r"(a), "r"(x), "r"(y), "r"(z), "r"(w) : "memory");
@@ -726,7 +723,7 @@ __global__ void __launch_bounds__(THREADS, 1) k_paged_many(const AttnArgs<T> a) 
         return base + C::OFF_Q + x * TERMS * C::Q_TILE + (at >> 3) * C::Q_PANEL + (32 * (warp & 3) + i) * 128 +
                ((at ^ i) & 7) * 16;
       };
-      // ---- the queries: fetched into their tile, then replaced by their f16 terms row by row
+      // ---- the queries: fetched into their tile, then replaced by their f16 terms
 #pragma unroll 4
       for (int i = sub; i < 32; i += AT_ONCE) {
         if (ok && warp_row + i < n_rows) cp16(stage(i, piece16), row_at(a.q, a.qs, i));
@@ -735,44 +732,49 @@ __global__ void __launch_bounds__(THREADS, 1) k_paged_many(const AttnArgs<T> a) 
       cp_commit();
       cp_wait<0>();
       __syncwarp();
-      float cf = 0.f;  // factor of the row's scores
-#pragma unroll 2
-      for (int i = sub; i < 32; i += AT_ONCE) {
-        const uint4 u = lds128(stage(i, piece16));
-        const uint32_t w[4] = {u.x, u.y, u.z, u.w};
-        float v[PER16], top = 0.f;
-        bool finite = true;
-#pragma unroll
-        for (int e = 0; e < PER16; e++) {
-          v[e] = SPLIT ? __uint_as_float(w[e % 4]) : __uint_as_float(e & 1 ? w[e / 2] & 0xFFFF0000u : w[e / 2] << 16);
-          top = fmaxf(top, fabsf(v[e]));
-          finite &= fabsf(v[e]) <= FLT_MAX;
-        }
-        if (!finite) top = INFINITY;
-#pragma unroll
-        for (int o = 1; o < ROW_LANES; o <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
-        finite = top <= FLT_MAX;
-        const int e = row_exp(finite ? top : 0.f);
-        // the sign of the scale goes into the row: the factor of its scores is then not negative and maxima commute
-        const float up = row_factor(e, finite) * (a.scale < 0.f ? -1.f : 1.f);
-        const int e_mine = __shfl_sync(0xffffffffu, e, (lane % AT_ONCE) * ROW_LANES);
-        if (lane / AT_ONCE == i / AT_ONCE) cf = scalbnf(fabsf(a.scale), -e_mine);  // lane: row i of the warp
-        uint32_t f[PER16 / 2], g[PER16 / 2];
-#pragma unroll
-        for (int z = 0; z < PER16 / 2; z++) {
-          const float y0 = v[2 * z] * up, y1 = v[2 * z + 1] * up;
-          f[z] = pack(y0, y1);
-          const float2 hi = unpack(f[z]);
-          g[z] = pack(y0 - hi.x, y1 - hi.y);
-        }
-        // the terms of dimensions d .. : 8 elements a chunk, second terms in the panels after the first ones'
-        const int d = piece16 * PER16;
+      // Each thread converts its own row in place: its largest magnitude (of the bits, so that NaN and infinities show),
+      // then the terms, 8 elements a chunk, second terms in the panels after the first ones'.
+      uint32_t most = 0;
+#pragma unroll 8
+      for (int j = 0; j < HD / PER16; j++) {
+        const uint4 u = lds128(stage(lane, j));
         if constexpr (SPLIT) {
-          __syncwarp();  // the row has been read
-          sts64(stage(i, d / 8) + (d & 7) * 2, f[0], f[1]);
-          sts64(stage(i, HD / 8 + d / 8) + (d & 7) * 2, g[0], g[1]);
+          most = max(max(most, max(u.x & 0x7FFFFFFFu, u.y & 0x7FFFFFFFu)), max(u.z & 0x7FFFFFFFu, u.w & 0x7FFFFFFFu));
         } else {
-          sts128(stage(i, piece16), f[0], f[1], f[2], f[3]);
+          most = __vmaxu2(most, __vmaxu2(__vmaxu2(u.x & 0x7FFF7FFFu, u.y & 0x7FFF7FFFu),
+                                         __vmaxu2(u.z & 0x7FFF7FFFu, u.w & 0x7FFF7FFFu)));
+        }
+      }
+      if (!SPLIT) most = max(most << 16, most & 0xFFFF0000u);
+      const bool finite = most < 0x7F800000u;
+      const int e = row_exp(finite ? __uint_as_float(most) : 0.f);
+      // the sign of the scale goes into the row: the factor of its scores is then not negative and maxima commute
+      const float up = row_factor(e, finite) * (a.scale < 0.f ? -1.f : 1.f), cf = scalbnf(fabsf(a.scale), -e);
+      if constexpr (SPLIT) {
+        uint32_t g[HD / 2];
+#pragma unroll
+        for (int j = 0; j < HD / 8; j++) {
+          const uint4 u = lds128(stage(lane, 2 * j)), w = lds128(stage(lane, 2 * j + 1));
+          const uint32_t x[8] = {u.x, u.y, u.z, u.w, w.x, w.y, w.z, w.w};
+          uint32_t f[4];
+#pragma unroll
+          for (int z = 0; z < 4; z++) {
+            const float y0 = __uint_as_float(x[2 * z]) * up, y1 = __uint_as_float(x[2 * z + 1]) * up;
+            f[z] = pack(y0, y1);
+            const float2 hi = unpack(f[z]);
+            g[4 * j + z] = pack(y0 - hi.x, y1 - hi.y);
+          }
+          sts128(stage(lane, j), f[0], f[1], f[2], f[3]);
+        }
+#pragma unroll
+        for (int j = 0; j < HD / 8; j++)
+          sts128(stage(lane, HD / 8 + j), g[4 * j], g[4 * j + 1], g[4 * j + 2], g[4 * j + 3]);
+      } else {
+#pragma unroll 4
+        for (int j = 0; j < HD / 8; j++) {
+          const uint4 u = lds128(stage(lane, j));
+          auto two = [&](uint32_t w) { return pack(__uint_as_float(w << 16) * up, __uint_as_float(w & 0xFFFF0000u) * up); };
+          sts128(stage(lane, j), two(u.x), two(u.y), two(u.z), two(u.w));
         }
       }
       fence_proxy_async();
