@@ -8,7 +8,8 @@
 //   warps 8-11  codes of a block of keys, loaded a block ahead to registers and converted
 //               to f16 (exact: whole numbers up to 127) into the
 //               128-byte swizzled tiles of K [keys][dims] and V [keys][dims]
-//   warp 12     issues the products, f32 sums in tensor memory:
+//   warps 12, 15 issue the products of tile 0 and 1, f32 sums in tensor memory (one warp for both spent
+//               a third of its time on waits and commits between them):
 //               S_X = Q_X K^T (K-major operands), O_X (+)= P_X V (V read MN-major as it
 //               lies, P from tensor memory). A tile's scores have two buffers: those of
 //               block j + 2 are issued right after P V of block j, so the softmax finds
@@ -49,7 +50,7 @@ namespace {
 using namespace tc;
 
 constexpr int SOFTMAX_WARPS = 8, LOAD_WARPS = 4, MMA_WARP = SOFTMAX_WARPS + LOAD_WARPS;
-constexpr int WARPS = 16;  // whole warpgroups: registers are shared out by them (warp 15 only takes part in barriers)
+constexpr int WARPS = 16;  // whole warpgroups: registers are shared out by them
 constexpr int THREADS = WARPS * 32, LOADERS = LOAD_WARPS * 32;
 constexpr int TILE_ROWS = 128, ROWS = 2 * TILE_ROWS;
 constexpr int BATCH = 8, BATCHES = 2;  // blocks of keys looked up at once, and how many such batches are held
@@ -416,10 +417,13 @@ __global__ void __launch_bounds__(THREADS, 1) k_paged_many(const AttnArgs<T> a) 
 
   if (tid == 0) {
     for (int i = 0; i < N_BARS; i++) {
-      const unsigned count = i < B_Q + 2 || (i >= B_DONE && i < B_DONE + PIECES)             ? SOFTMAX_WARPS
-                             : i >= B_P && i < B_P + 4                                       ? SOFTMAX_WARPS / 2
-                             : (i >= B_K && i < B_K + MAX_STAGES) || (i >= B_V && i < B_V + MAX_STAGES) ? LOAD_WARPS
-                                                                                             : 1;
+      const auto is = [&](int first, int n) { return i >= first && i < first + n; };
+      const unsigned count = is(B_Q, 2) || is(B_DONE, PIECES)                     ? SOFTMAX_WARPS
+                             : is(B_P, 4)                                         ? SOFTMAX_WARPS / 2
+                             : is(B_K, MAX_STAGES) || is(B_V, MAX_STAGES)         ? LOAD_WARPS
+                             : is(B_K_FREE, MAX_STAGES) || is(B_V_FREE, MAX_STAGES) || is(B_PLAN_FREE, BATCHES) || i == B_FIN
+                                 ? 2   // the warps of the products
+                                 : 1;
       bar_init(bar(i), count);
     }
     s_abort = 0;
@@ -521,8 +525,9 @@ __global__ void __launch_bounds__(THREADS, 1) k_paged_many(const AttnArgs<T> a) 
           if (lane == 0) bar_arrive(bar(B_PLAN + batch % BATCHES));
         }
       }
-    } else if (warp == MMA_WARP) {
-      // ---------------- products ----------------
+    } else {
+      // ---------------- products of tile x ----------------
+      const int x = warp == MMA_WARP ? 0 : 1;
       // The whole warp walks the loop, so that addresses and descriptors are uniform values; one elected thread
       // issues (with a single thread in the loop each product took 100 to 150 clocks to issue, twice its own time).
       const bool leader = elect_one();
@@ -530,31 +535,32 @@ __global__ void __launch_bounds__(THREADS, 1) k_paged_many(const AttnArgs<T> a) 
       auto commit = [&](int i) {
         if (leader) mma_commit(bar(i));
       };
-      unsigned done = 0, batch = 0, tile_done[2] = {0, 0};  // blocks in all, batches, blocks of each tile
+      unsigned done = 0, batch = 0, tile_done = 0;  // blocks in all, batches, blocks of the tile
       bool ok = true;
 #pragma unroll 1
       for (unsigned k = 0; ok; k++) {
         if (!(ok = wait(B_PIECE + k % PIECES, k / PIECES))) break;
         const int n = __shfl_sync(0xffffffffu, s_pieces[k % PIECES].n, 0);
-        const int tiles = __shfl_sync(0xffffffffu, s_pieces[k % PIECES].n_rows, 0) > TILE_ROWS ? 2 : 1;
+        const bool active = x == 0 || __shfl_sync(0xffffffffu, s_pieces[k % PIECES].n_rows, 0) > TILE_ROWS;
         if (n < 0) break;
         // An operand's place is the low bits of its descriptor, in units of 16 bytes: every one is a base and a sum.
-        const uint64_t qd = sw128_desc(base + C::OFF_Q), kd = sw128_desc(base + C::OFF_K);
+        const uint64_t qd = sw128_desc(base + C::OFF_Q + x * TERMS * C::Q_TILE), kd = sw128_desc(base + C::OFF_K);
         const uint64_t vd = mn_desc(base + C::OFF_V, C::KV_PANEL);
-        auto scores = [&](int x, int buf, int st) {
-          const uint64_t q = qd + (uint32_t)(x * (TERMS * C::Q_TILE >> 4)), kk = kd + (uint32_t)(st * (C::KV_TILE >> 4));
+        auto scores = [&](int buf, int st) {
+          const uint64_t kk = kd + (uint32_t)(st * (C::KV_TILE >> 4));
           const uint32_t d = tm + x * 128 + buf * 64;
           if (leader) {
 #pragma unroll
             for (int t = TERMS - 1; t >= 0; t--)  // second terms first: their sums are small when they are truncated
 #pragma unroll
               for (int i = 0; i < HD / 16; i++)
-                mma_f16(d, q + ((t * C::Q_TILE + (i >> 2) * C::Q_PANEL + (i & 3) * 32) >> 4),
-                        kk + (((i >> 2) * C::KV_PANEL + (i & 3) * 32) >> 4), idesc_f16(TILE_ROWS, BK, false), t < TERMS - 1 || i);
+                mma_f16(d, qd + ((t * C::Q_TILE + (i >> 2) * C::Q_PANEL + (i & 3) * 32) >> 4),
+                        kk + (((i >> 2) * C::KV_PANEL + (i & 3) * 32) >> 4), idesc_f16(TILE_ROWS, BK, false),
+                        t < TERMS - 1 || i);
             mma_commit(bar(B_S + 2 * x + buf));
           }
         };
-        auto output = [&](int x, int buf, int st, bool add) {
+        auto output = [&](int buf, int st, bool add) {
           const uint64_t v = vd + (uint32_t)(st * (C::KV_TILE >> 4));
           const uint32_t d = tm + TM_O + x * 128, w = tm + x * 128 + buf * 64;
           if (leader) {
@@ -562,45 +568,40 @@ __global__ void __launch_bounds__(THREADS, 1) k_paged_many(const AttnArgs<T> a) 
             for (int t = TERMS - 1; t >= 0; t--)
 #pragma unroll
               for (int i = 0; i < BK / 16; i++)
-                mma_f16_ts(d, w + t * 32 + i * 8, v + (i * 2048 >> 4), idesc_f16(TILE_ROWS, HD, true), t < TERMS - 1 || i || add);
+                mma_f16_ts(d, w + t * 32 + i * 8, v + (i * 2048 >> 4), idesc_f16(TILE_ROWS, HD, true),
+                           t < TERMS - 1 || i || add);
             mma_commit(bar(B_PV + 2 * x + buf));
           }
         };
         if (!(ok = wait(B_Q + (k & 1), k / 2))) break;
-        // Turn i: P V of block i, then the scores of block i + 2 (turns -2 and -1: the first scores alone).
+        // Turn i: P V of block i, then the scores of block i + 2 (turns -2 and -1: the first scores alone). A tile
+        // without rows only gives its leave for each stage as it is filled.
 #pragma unroll 1
-        for (int i = -2; ok && i < n; i++) {
-          const unsigned now = done + i, ahead = now + 2;
-          const int st = now % STAGES, st2 = ahead % STAGES;
+        for (int i = -2; i < n; i++) {
+          const unsigned now = done + i, ahead = now + 2, t = tile_done + i;  // the tile's buffer t % 2, its turn t / 2
+          const int st = now % STAGES, st2 = ahead % STAGES, buf = t & 1;
           const bool more = i + 2 < n;
           // K of block i + 2 comes after V of block i + 1: one wait for both, well before it is needed
           if (!(ok = more ? wait(B_K + st2, ahead / STAGES) : i < 0 || wait(B_V + st, now / STAGES))) break;
-          fence_after();
-#pragma unroll 1
-          for (int x = 0; x < tiles; x++) {
-            const unsigned t = (x ? tile_done[1] : tile_done[0]) + i;  // of this tile: buffer t % 2, its turn t / 2
-            const int buf = t & 1;
-            if (i >= 0) {
-              if (!(ok = wait(B_P + 2 * x + buf, t / 2))) break;
-              fence_after();
-              output(x, buf, st, SPLIT ? i % MOVE : i);
-            }
-            if (more) scores(x, buf, st2);
-          }
-          if (!ok) break;
-          if (more) commit(B_K_FREE + st2);
           if (i >= 0) {
+            if (active && !(ok = wait(B_P + 2 * x + buf, t / 2))) break;
+            fence_after();
+            if (active) output(buf, st, SPLIT ? i % MOVE : i);
             commit(B_V_FREE + st);
             if (i % BATCH == BATCH - 1 || i == n - 1) commit(B_PLAN_FREE + batch++ % BATCHES);
           }
+          if (more) {
+            fence_after();
+            if (active) scores(buf, st2);
+            commit(B_K_FREE + st2);
+          }
         }
         done += n;
-        tile_done[0] += n;
-        if (tiles == 2) tile_done[1] += n;
+        if (active) tile_done += n;
       }
       // every product done before the columns are freed
       commit(B_FIN);
-      bar_drain(bar(B_FIN), 0u);
+      if (x == 0) bar_drain(bar(B_FIN), 0u);
       __syncwarp();
     }
   } else if (warp >= SOFTMAX_WARPS) {
