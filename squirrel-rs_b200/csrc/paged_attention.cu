@@ -52,6 +52,11 @@ namespace {
 constexpr int WARPS = 4, THREADS = WARPS * 32, STAGES = 2;
 constexpr int BLOCKS_PER_SM = 3;
 constexpr int MAX_BLOCKS = 160 * BLOCKS_PER_SM;  // and parts of a row tile
+// What a row tile costs besides its keys (queries, look-ups, the join of the warps), in key tiles, when the work is
+// shared out; these places hold no keys and a piece that would begin in them begins with the next row tile. 0 / 4 / 16:
+// 64 x 5 drafts in up to 1,000 positions (f32, 64 dimensions) 49.1 / 43.1 / 43.2 us, 128 x up to 300 (bf16, 128) 25.0 / 22.4 /
+// 24.0, 64 x up to 4,000 62.4 / 62.3 / 62.2, 16 x 5 drafts in up to 4,099 (f32) 37.6 / 38.7 / 42.5.
+constexpr int JOB_COST = 4;
 constexpr int MIN_TILES = WARPS;  // key tiles a block takes at least
 constexpr int FLUSH_STEPS = 16;    // f32 rows: groups of 16 keys summed on the tensor core at a stretch
 constexpr int SLOT_FLOATS = 2112;  // partial results of a row tile: 32 x 66 at most: maxima, sums, [row][head_dim]
@@ -161,7 +166,7 @@ __global__ void __launch_bounds__(THREADS, C::BLOCKS) k_paged_few(const AttnArgs
   auto tiles_of = [&](const Seq &s) -> int {
     if (!s.n || s.n * rows_of_token > a.few_rows) return 0;
     const int rt = (s.n * rows_of_token + ROWS - 1) / ROWS;
-    return key_span<TK>(s, a.window, a.sinks).n * rt * c.kv_heads;
+    return (key_span<TK>(s, a.window, a.sinks).n + JOB_COST) * rt * c.kv_heads;
   };
   // This block's piece [at, end) of the line of all tiles, and the sequence it starts in.
   const int first_n = tid < a.b.n_seqs ? tiles_of(load_seq(a.b, c, tid)) : 0;
@@ -208,9 +213,9 @@ __global__ void __launch_bounds__(THREADS, C::BLOCKS) k_paged_few(const AttnArgs
       for (int i = 0; i < 2; i++) {  // this piece's start and the next one's
         const int x = per * ((int)blockIdx.x + i);
         if (x >= start && x < run) {  // one thread at most
-          const int in_row_tile = (x - start) % n_span;
+          const int in_row_tile = (x - start) % (n_span + JOB_COST);
           s_end[i] = in_row_tile <= SNAP && in_row_tile <= n_span - in_row_tile ? x - in_row_tile
-                     : n_span - in_row_tile <= SNAP                             ? x - in_row_tile + n_span
+                     : n_span - in_row_tile <= SNAP                             ? x - in_row_tile + n_span + JOB_COST
                                                                                 : x;
           if (i == 0) {
             s_last = b;
@@ -240,8 +245,8 @@ __global__ void __launch_bounds__(THREADS, C::BLOCKS) k_paged_few(const AttnArgs
     }
     const Span span = key_span<TK>(s, a.window, a.sinks);
     const int row_tiles = (s.n * rows_of_token + ROWS - 1) / ROWS;
-    const int job = (at - b_start) / span.n, head = job / row_tiles, rt = job - head * row_tiles;
-    const int job_start = b_start + job * span.n;
+    const int slots = span.n + JOB_COST, job = (at - b_start) / slots, head = job / row_tiles, rt = job - head * row_tiles;
+    const int job_start = b_start + job * slots;
     const int t0 = at - job_start, t1 = min(span.n, end - job_start);
     const int pos0 = s.len - s.n;  // position of the first new token
 
@@ -652,7 +657,7 @@ __global__ void __launch_bounds__(THREADS, C::BLOCKS) k_paged_few(const AttnArgs
     if (!whole) {
       // The last block to arrive joins all parts, in block order: every part's factors once, to shared memory, then
       // the threads share out rows, dimensions and (when there are few of those) slices of the parts.
-      // The cuts are the multiples of `per` more than SNAP tiles inside; the part before the first is the block's before.
+      // The cuts are the multiples of `per` more than SNAP tiles inside its keys; the part before the first is the block's before.
       const int first = (job_start + SNAP) / per, parts = (job_start + span.n - SNAP - 1) / per - first + 1;
       int *count = a.count + (b * c.kv_heads + head) * a.max_row_tiles + rt;
       __syncthreads();
@@ -714,7 +719,7 @@ __global__ void __launch_bounds__(THREADS, C::BLOCKS) k_paged_few(const AttnArgs
         if (tid == 0) *count = 0;
       }
     }
-    at = job_start + t1;
+    at = t1 < span.n ? end : job_start + slots;
     __syncthreads();  // the ring is free again
   }
 }
@@ -773,7 +778,7 @@ bool countable(const Batch &b, const Cache &c, int n_heads) {
   const double keys = (double)b.table_row * c.page, tokens = b.n_tokens, seqs = b.n_seqs;
   const double few = many ? seqs * (FEW_ROWS / 4) : tokens * group / 4 + seqs;
   const double rest = many ? (tokens * group / 128 + seqs) * (keys / 64 + 16) : 0;
-  return few * c.kv_heads * (keys / 16 + 2) < 1 << 30 && rest * c.kv_heads < 1 << 30;
+  return few * c.kv_heads * (keys / 16 + 32) < 1 << 30 && rest * c.kv_heads < 1 << 30;
 }
 
 // Partial results of both kernels, then the counters of both.

@@ -56,8 +56,8 @@ constexpr int TILE_ROWS = 128, ROWS = 2 * TILE_ROWS;
 constexpr int BATCH = 8, BATCHES = 2;  // blocks of keys looked up at once, and how many such batches are held
 constexpr int MAX_BLOCKS = 160;
 // What a row tile costs besides its key blocks, in blocks (queries in, results out, the pipeline's start and end), when
-// the work is shared out. 0 / 4 / 8 / 12 (bf16, 128 dimensions): 2 x 4,096 rows of 8,000 positions 927 / 831 /
-// 774 / 772 us, 16 x 1,000 rows 348 / 294 / 270 / 271 us, 2,048 rows of 4,133 positions 182 / 173 / 167 / 169 us.
+// the work is shared out. 0 / 3 / 5 / 8 (bf16, 128 dimensions): 2 x 4,096 rows of 8,000 positions 776 / 718 /
+// 696 / 696 us, 16 x 1,000 rows 260 / 222 / 213 / 218 us, 64 x 100 rows of 300 positions 136 / 105 / 101 / 102 us.
 constexpr int TILE_COST = 5;
 constexpr int MIN_BLOCKS = 2;  // key blocks a thread block takes at least
 constexpr int MOVE = 4;        // f32 rows: blocks of keys summed in tensor memory at a stretch
