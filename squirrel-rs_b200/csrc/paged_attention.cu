@@ -760,14 +760,15 @@ cudaError_t launch_few(cudaStream_t s, AttnArgs<T> &a) {
   return cudaErrorInvalidValue;
 }
 
-// Rows a kv head up to which a sequence is this file's: beyond, the products cost more than
-// the reading of the cache. 12 x 4,096 positions at 64 rows, this kernel against the other:
-// f32 rows 72 / 77 us (64 dimensions) and 82 / 146 us (128), bf16 rows 47 / 58 and 66 / 82 us; at
-// 96 rows the other one is ahead.
-constexpr int FEW_ROWS = 64;
+// Query rows a kv head. A call of up to ALONE_ROWS is this kernel's: 12 x up to 4,096 positions, this one / the other at
+// 72 rows: f32 58 / 65 us (64 dimensions), 86 / 105 us (128), bf16 43 / 50 and 69 / 66 us; at 80 rows 73 / 65, 89 / 105,
+// 53 / 50, 72 / 66. Beyond, the other kernel takes the sequences of more than FEW_ROWS and this one the rest, one after
+// the other: where all are long FEW_ROWS would only leave work for a second launch (a ragged batch of up to 96 rows:
+// 16 or 32: 64 us, 48: 86, 64: 103), and single and drafted tokens beside prompts stay here.
+constexpr int ALONE_ROWS = 72, FEW_ROWS = 32;
 
 bool goes_many(const Cache &c, int max_new, int group) {
-  return (long long)max_new * group > FEW_ROWS && many_supported(c, group);
+  return (long long)max_new * group > ALONE_ROWS && many_supported(c, group);
 }
 
 // Whether the (row tile, key tile) pairs of a call can be numbered in 30 bits by both kernels: 128 rows or

@@ -28,8 +28,8 @@
 //   f32 rows:  weights in two terms; the O of four blocks of keys is summed in tensor memory and
 //              added to f32 registers, because the tensor core truncates its running sum
 //              (2^-25 of it a step: 500 steps would cost 1e-5). 2048 x 4,133 positions, 128
-//              dimensions: every block 371 us (error 4.5e-7 of the result), every four 348 us
-//              (7.5e-7), every eight 344 us (1.2e-6).
+//              dimensions: every block 331 us (error 4.5e-7 of the result), every four 269 us
+//              (7.5e-7), every eight 258 us (1.2e-6; the plain f32 form: 1.4e-6).
 //   bf16 rows: weights in one term (11 bits, under the output's 8); O stays in tensor memory.
 //
 // Work is split as in the few-row kernel: one line of (sequence, kv head, row tile, key
