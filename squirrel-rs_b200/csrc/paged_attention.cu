@@ -25,9 +25,10 @@
 // instruction a pair more), and V's always is: an output is an average that may be a
 // thousand times smaller than 128. The tensor core truncates its running sum (2^-25 of it a
 // step on average): the scores of the query's two terms are summed apart, and f32 rows
-// move their output sums every 16 groups of keys to f32 sums in shared memory. Measured
+// move their output sums every 8 groups of keys to f32 sums in shared memory. Measured
 // with 4 x 131,072 positions of f32 rows: the bias taken off afterwards and one sum 66 us, error
-// 1.4e-6 of the result; as it is 69 us, 1.0e-6; sums moved every 8 groups 69.4 us, 8.4e-7.
+// 1.4e-6 of the result; as it is 69.4 us, 8.4e-7; sums moved every 16 groups 68.7 us, 1.0e-6
+// (1,001 positions: 5.5e-7 and 8.1e-7, the plain f32 form 9.1e-7).
 //
 // Work is split evenly over the grid: the (sequence, kv head, row tile, key tile) space is
 // one line, every block takes an equal piece of it, the four warps of a block take its key
@@ -58,7 +59,7 @@ constexpr int MAX_BLOCKS = 160 * BLOCKS_PER_SM;  // and parts of a row tile
 // 24.0, 64 x up to 4,000 62.4 / 62.3 / 62.2, 16 x 5 drafts in up to 4,099 (f32) 37.6 / 38.7 / 42.5.
 constexpr int JOB_COST = 4;
 constexpr int MIN_TILES = WARPS;  // key tiles a block takes at least
-constexpr int FLUSH_STEPS = 16;    // f32 rows: groups of 16 keys summed on the tensor core at a stretch
+constexpr int FLUSH_STEPS = 8;     // f32 rows: groups of 16 keys summed on the tensor core at a stretch
 constexpr int SLOT_FLOATS = 2112;  // partial results of a row tile: 32 x 66 at most: maxima, sums, [row][head_dim]
 constexpr size_t PARTIAL_BYTES = (size_t)MAX_BLOCKS * 2 * SLOT_FLOATS * 4;
 constexpr float WEIGHT_EXP = 10.f;  // weights are 2^(s - max + 10)

@@ -13,7 +13,9 @@
 //               S_X = Q_X K^T (K-major operands), O_X (+)= P_X V (V read MN-major as it
 //               lies, P from tensor memory). A tile's scores have two buffers: those of
 //               block j + 2 are issued right after P V of block j, so the softmax finds
-//               the next block's scores ready
+//               the next block's scores ready (two blocks' scores in one product of 128
+//               columns take a third less tensor time, but leave no second buffer: 694
+//               -> 838 us for 2 x 4,096 rows of 8,000 positions, bf16, 128 dimensions)
 //   warp 13     walks this block's share of the work, handed out piece by piece
 //   warp 14     looks up pages and scales, eight blocks of keys at a time
 //   warps 0-7   one thread a row (= tensor-memory lane): running maximum of its scores,

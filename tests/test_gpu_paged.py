@@ -215,6 +215,14 @@ def test_attention_window(gpu_lib, case, window, sinks, kind):
 
 
 @pytest.mark.parametrize("kind", ["f32", "bf16"])
+@pytest.mark.parametrize("hd", [64, 128])
+@pytest.mark.parametrize("news", [[18, 1, 7], [19, 8, 9, 1, 0, 18], [64, 8], [65, 9]], ids=str)
+def test_attention_where_the_kernels_share_a_batch(gpu_lib, news, hd, kind):
+    """Row counts on both sides of where sequences pass from the one kernel to the other (groups of 4)."""
+    Setup(17, 2, hd, 32, news, [n + 61 * (i + 1) for i, n in enumerate(news)]).check_attention(8, kind)
+
+
+@pytest.mark.parametrize("kind", ["f32", "bf16"])
 @pytest.mark.parametrize("page", [16, 64])
 def test_attention_pages_left_behind_by_the_window(gpu_lib, page, kind):
     """Pages that no new token sees may be gone: their entries and scales are not used."""
