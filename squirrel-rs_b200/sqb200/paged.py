@@ -207,8 +207,8 @@ def read(cache, batch, first, count, dtype=torch.float32):
     kind = _KINDS.get(dtype)
     if kind is None:
         raise KernelError(_TYPE, "values are read as float32 or bfloat16")
-    like = cache.like[dtype]
-    k, v = like.new_empty((n, count, cache.row)), like.new_empty((n, count, cache.row))
+    k = cache.like[dtype].new_empty((n, count, cache.row))
+    v = torch.empty_like(k)
     st = _fn("sq_paged_read")(_raw_stream(_device()), cache.ref, batch.ref, first.data_ptr(), count, kind,
                               k.data_ptr(), v.data_ptr())
     if st:

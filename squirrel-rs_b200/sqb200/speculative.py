@@ -21,14 +21,16 @@ def _array(t, shape, dtype, what):
 
 def _probs(t, n, rows, vocab, what):
     """[n, rows, vocab] float32 whose rows lie one stride apart (a slice of wider rows)."""
-    if t.shape != (n, rows, vocab) or t.numel() and ((vocab > 1 and t.stride(2) != 1) or
-                                                    (n > 1 and t.stride(0) != rows * t.stride(1))):
+    if t.shape != (n, rows, vocab):
+        raise KernelError(_SHAPE, f"{what}: [{n}, {rows}, {vocab}] is wanted")
+    far, stride, step = t.stride()
+    if ((step != 1 and vocab > 1) or (n > 1 and far != rows * stride)) and t.numel():
         raise KernelError(_SHAPE, f"{what}: [{n}, {rows}, {vocab}] with one stride between rows is wanted")
-    if t.dtype != torch.float32:
+    if t.dtype is not torch.float32:
         raise KernelError(_TYPE, f"{what}: probabilities are float32")
     if not t.is_cuda:
         raise KernelError(_ARG, f"{what}: a CUDA tensor is wanted")
-    return t.data_ptr(), max(t.stride(1), vocab)
+    return t.data_ptr(), stride if stride > vocab else vocab
 
 
 def verify_drafts(target, draft, tokens, uniform, n_draft=None):
