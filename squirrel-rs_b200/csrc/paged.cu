@@ -291,7 +291,8 @@ __global__ void __launch_bounds__(READ_THREADS)
         scale[j][z] = 0.f;
         if (page[j] >= 0) {
           const long long slot = (long long)page[j] * c.kv_heads + g;
-          const uint32_t *src = reinterpret_cast<const uint32_t *>((z ? c.v : c.k) + (slot * c.page + ((pos0 + j) & (c.page - 1))) * c.hd + d);
+          const uint8_t *codes = (z ? c.v : c.k) + (slot * c.page + ((pos0 + j) & (c.page - 1))) * c.hd + d;
+          const uint32_t *src = reinterpret_cast<const uint32_t *>(codes);
           scale[j][z] = (z ? c.vs : c.ks)[slot];
           if constexpr (WORDS == 2) {
             const uint2 w = *reinterpret_cast<const uint2 *>(src);

@@ -300,7 +300,8 @@ __global__ void __launch_bounds__(THREADS, C::BLOCKS) k_paged_few(const AttnArgs
     const int low = a.window ? min_pos - a.window - 15 : -1;  // groups from there on are in a row's window
     auto entry_of = [&](int batch) {  // INT_MIN: no such group, or none that a row sees
       const int k = batch * BATCH + lane / NG, key = tile_key(k) + 16 * (lane % NG);
-      return k < n_tiles && key < s.len && (key > low || key < a.sinks) ? a.b.table[(long long)b * a.b.table_row + (key >> c.page_shift)] : INT_MIN;
+      if (k >= n_tiles || key >= s.len || (key <= low && key >= a.sinks)) return INT_MIN;
+      return a.b.table[(long long)b * a.b.table_row + (key >> c.page_shift)];
     };
     auto place_of = [&](int batch, int entry) {
       if ((unsigned)entry >= (unsigned)c.n_pages) {
@@ -439,32 +440,23 @@ __global__ void __launch_bounds__(THREADS, C::BLOCKS) k_paged_few(const AttnArgs
 #pragma unroll
           for (int x = 0; x < 4; x++) sc[j][nt][x] = second[nt][x] = 0.f;
         const uint32_t base = kt + j * 16 * HD;
+        auto step = [&](uint32_t u, uint32_t w, int i) {  // 16 dimensions
+          const uint32_t f[4] = {codes_02<SPLIT>(u), codes_02<SPLIT>(w), codes_13<SPLIT>(u), codes_13<SPLIT>(w)};
+#pragma unroll
+          for (int nt = 0; nt < NT; nt++)
+#pragma unroll
+            for (int y = 0; y < TERMS; y++) mma(y ? second[nt] : sc[j][nt], f, qf[nt][i][y][0], qf[nt][i][y][1]);
+        };
         if constexpr (HD >= 64) {
 #pragma unroll
           for (int ch = 0; ch < HD / 64; ch++) {
             const uint4 u = lds128(base + chunk_at<HD>(g, ch * 4 + t)), w = lds128(base + chunk_at<HD>(g + 8, ch * 4 + t));
-            const uint32_t uu[4] = {u.x, u.y, u.z, u.w}, ww[4] = {w.x, w.y, w.z, w.w};
-#pragma unroll
-            for (int x = 0; x < 4; x++) {
-              const uint32_t f[4] = {codes_02<SPLIT>(uu[x]), codes_02<SPLIT>(ww[x]), codes_13<SPLIT>(uu[x]), codes_13<SPLIT>(ww[x])};
-#pragma unroll
-              for (int nt = 0; nt < NT; nt++)
-#pragma unroll
-                for (int y = 0; y < TERMS; y++) mma(y ? second[nt] : sc[j][nt], f, qf[nt][ch * 4 + x][y][0], qf[nt][ch * 4 + x][y][1]);
-            }
+            step(u.x, w.x, ch * 4), step(u.y, w.y, ch * 4 + 1), step(u.z, w.z, ch * 4 + 2), step(u.w, w.w, ch * 4 + 3);
           }
         } else {
           const uint2 u = lds64(base + chunk_at<HD>(g, t >> 1) + (t & 1) * 8);
           const uint2 w = lds64(base + chunk_at<HD>(g + 8, t >> 1) + (t & 1) * 8);
-          const uint32_t uu[2] = {u.x, u.y}, ww[2] = {w.x, w.y};
-#pragma unroll
-          for (int x = 0; x < 2; x++) {
-            const uint32_t f[4] = {codes_02<SPLIT>(uu[x]), codes_02<SPLIT>(ww[x]), codes_13<SPLIT>(uu[x]), codes_13<SPLIT>(ww[x])};
-#pragma unroll
-            for (int nt = 0; nt < NT; nt++)
-#pragma unroll
-              for (int y = 0; y < TERMS; y++) mma(y ? second[nt] : sc[j][nt], f, qf[nt][x][y][0], qf[nt][x][y][1]);
-          }
+          step(u.x, w.x, 0), step(u.y, w.y, 1);
         }
         if constexpr (SPLIT) {
 #pragma unroll
