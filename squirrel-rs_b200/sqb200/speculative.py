@@ -20,17 +20,25 @@ def _array(t, shape, dtype, what):
 
 
 def _probs(t, n, rows, vocab, what):
-    """[n, rows, vocab] float32 whose rows lie one stride apart (a slice of wider rows)."""
+    """Address and row stride of [n, rows, vocab] float32 whose rows lie one stride apart (a slice
+    of wider rows or of more of them). Broadcast or overlapping rows are refused: the kernel
+    would read past the end of them."""
     if t.shape != (n, rows, vocab):
         raise KernelError(_SHAPE, f"{what}: [{n}, {rows}, {vocab}] is wanted")
     far, stride, step = t.stride()
-    if ((step != 1 and vocab > 1) or (n > 1 and far != rows * stride)) and t.numel():
+    if rows == 1:
+        stride = far  # the stride of a single row says nothing: rows are a sequence apart
+    if n * rows < 2:
+        stride = vocab
+    elif vocab and (stride < vocab or (n > 1 and far != rows * stride)):
         raise KernelError(_SHAPE, f"{what}: [{n}, {rows}, {vocab}] with one stride between rows is wanted")
+    if step != 1 and vocab > 1 and n * rows:
+        raise KernelError(_SHAPE, f"{what}: a row's elements must be consecutive")
     if t.dtype is not torch.float32:
         raise KernelError(_TYPE, f"{what}: probabilities are float32")
     if not t.is_cuda:
         raise KernelError(_ARG, f"{what}: a CUDA tensor is wanted")
-    return t.data_ptr(), stride if stride > vocab else vocab
+    return t.data_ptr(), stride
 
 
 def verify_drafts(target, draft, tokens, uniform, n_draft=None):
