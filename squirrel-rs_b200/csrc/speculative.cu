@@ -141,11 +141,17 @@ __device__ int find_token(const Row &r, int lo, int hi, unsigned long long befor
   return -1;  // not reached: the piece holds the goal
 }
 
+// A block's shared memory may be written by another only once the block runs: arrival when it starts, the wait
+// before the first such write (by then the others have long arrived).
+__device__ __forceinline__ void cluster_started() { asm volatile("barrier.cluster.arrive.relaxed.aligned;" ::: "memory"); }
+__device__ __forceinline__ void cluster_wait_started() { asm volatile("barrier.cluster.wait.aligned;" ::: "memory"); }
+
 __global__ void __cluster_dims__(VERIFY_CLUSTER, 1, 1) __launch_bounds__(VERIFY_THREADS, 4)
     k_verify(const VerifyArgs a) {
   __shared__ unsigned long long sums[VERIFY_WARPS], totals[2][VERIFY_CLUSTER];  // of the warps; of the cluster's blocks
   __shared__ int s_accepted;
   cg::cluster_group cluster = cg::this_cluster();
+  cluster_started();
   const int rank = cluster.block_rank(), b = blockIdx.x / VERIFY_CLUSTER;
   const int tid = threadIdx.x, lane = tid & 31, wid = tid >> 5;
   const int K = a.max_draft, V = a.vocab;
@@ -199,6 +205,7 @@ __global__ void __cluster_dims__(VERIFY_CLUSTER, 1, 1) __launch_bounds__(VERIFY_
     const unsigned long long sum = vec ? sum_piece<true>(row, lo, hi) : sum_piece<false>(row, lo, hi);
     if (lane == 0) sums[wid] = sum;
     __syncthreads();
+    if (!pass) cluster_wait_started();
     if (wid == 0) {
       const unsigned long long mine = warp_sum_u64(lane < VERIFY_WARPS ? sums[lane] : 0ull);
       if (lane < VERIFY_CLUSTER) *cluster.map_shared_rank(&totals[pass][rank], lane) = mine;

@@ -2,6 +2,7 @@
 import numpy as np
 import pytest
 
+import paged_oracle as P
 from test_gpu_speculative import case, dev
 
 pytestmark = pytest.mark.gpu
@@ -24,3 +25,20 @@ def test_verify_slices_of_the_places(gpu_lib, vocab):
     got = speculative.verify_drafts(wide[2:3, 1:3], None, tokens, dev(uniform[2:3, :2]))
     want = speculative.verify_drafts(wide[2:3, 1:3].contiguous(), None, tokens, dev(uniform[2:3, :2]))
     assert all(torch.equal(a, b) for a, b in zip(got, want))
+
+
+@pytest.mark.parametrize("vocab", [1, 3, 130])
+def test_verify_small_vocabularies(gpu_lib, vocab):
+    """Rows that leave most blocks of a cluster nothing to read: their sums are exchanged as soon as they start. Many
+    clusters, many more than run at once, on every call the same ids."""
+    from sqb200 import speculative
+    rng = np.random.default_rng(vocab)
+    n, k = 3000, 2
+    target, draft = (rng.random((n, r, vocab), np.float32) / vocab for r in (k + 1, k))
+    tokens, uniform = rng.integers(0, vocab, (n, k)).astype(np.int32), rng.random((n, k + 1), np.float32)
+    acc, out = P.verify(target, draft, tokens, [k] * n, uniform)
+    args = [dev(x) for x in (target, draft, tokens, uniform)]
+    for _ in range(5):
+        got_acc, got = speculative.verify_drafts(*args)
+        np.testing.assert_array_equal(got_acc.cpu().numpy(), acc)
+        np.testing.assert_array_equal(got.cpu().numpy(), out)
