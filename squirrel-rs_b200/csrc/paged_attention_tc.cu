@@ -84,7 +84,7 @@ struct Cfg {
   static constexpr int OFF_Q = 0, OFF_K = OFF_Q + 2 * TERMS * Q_TILE, OFF_V = OFF_K + STAGES * KV_TILE,
                        OFF_SCALE = OFF_V + STAGES * KV_TILE,
                        OFF_BAR = OFF_SCALE + BATCHES * BATCH * 96;
-  static constexpr int SMEM = 1024 + OFF_BAR + 352;
+  static constexpr int SMEM = 1024 + OFF_BAR + 368;
   static constexpr int SLOT = ROWS * (HD + 2);  // floats of a cut row tile's partial result
   static_assert(SMEM <= 232448 - 256, "shared memory of a block");
 };
@@ -104,23 +104,25 @@ static_assert(sizeof(Plan) == 96, "room in shared memory");
 constexpr int MAX_STAGES = 4;
 // A wait tells a phase from the one before it only. So every barrier is one whose phase before is known to be done
 // when a phase is waited for, and whose phase after cannot be: where a waiter may skip phases or lag behind, there
-// is one for each buffer or place.
+// is one for each buffer or place. Nothing else waits for tile 1's product warp in a piece that leaves tile 1
+// without rows, so a piece is done, and its place and B_Q used again, only with that warp's arrival too.
 enum : int {
-  B_Q = 0,        // [2] both tiles' queries of a piece written
-  B_K = 2,        // [stages] K written
-  B_K_FREE = 6,   // [stages] scores of both tiles done
-  B_V = 10,       // [stages]
-  B_V_FREE = 14,  // [stages]
-  B_S = 18,       // [2 tiles][2 buffers] scores done
-  B_P = 22,       // [2 tiles][2 buffers] weights written
-  B_PV = 26,      // [2 tiles][2 buffers] P V done
-  B_PIECE = 30,   // [4] a piece handed out
-  B_DONE = 34,    // [4] a piece's rows written
-  B_PLAN = 38,    // [2] a batch of blocks looked up
-  B_PLAN_FREE = 40,
-  B_FIN = 42,
-  N_BARS = 43
+  B_Q = 0,        // [4] both tiles' queries of a piece written
+  B_K = 4,        // [stages] K written
+  B_K_FREE = 8,   // [stages] scores of both tiles done
+  B_V = 12,       // [stages]
+  B_V_FREE = 16,  // [stages]
+  B_S = 20,       // [2 tiles][2 buffers] scores done
+  B_P = 24,       // [2 tiles][2 buffers] weights written
+  B_PV = 28,      // [2 tiles][2 buffers] P V done
+  B_PIECE = 32,   // [4] a piece handed out
+  B_DONE = 36,    // [4] a piece's rows written, and tile 1's products issued
+  B_PLAN = 40,    // [2] a batch of blocks looked up
+  B_PLAN_FREE = 42,
+  B_FIN = 44,
+  N_BARS = 45
 };
+static_assert(8 * N_BARS <= 368, "room in shared memory");
 // Columns: S, and P over it, of tile X and buffer B at 128 X + 64 B (P: first terms in 32, second terms
 // in the next 32); O at 256 + 128 X.
 constexpr uint32_t TM_O = 256, TM_COLS = 512;
@@ -420,7 +422,8 @@ __global__ void __launch_bounds__(THREADS, 1) k_paged_many(const AttnArgs<T> a) 
   if (tid == 0) {
     for (int i = 0; i < N_BARS; i++) {
       const auto is = [&](int first, int n) { return i >= first && i < first + n; };
-      const unsigned count = is(B_Q, 2) || is(B_DONE, PIECES)                     ? SOFTMAX_WARPS
+      const unsigned count = is(B_Q, PIECES)                                      ? SOFTMAX_WARPS
+                             : is(B_DONE, PIECES)                                 ? SOFTMAX_WARPS + 1
                              : is(B_P, 4)                                         ? SOFTMAX_WARPS / 2
                              : is(B_K, MAX_STAGES) || is(B_V, MAX_STAGES)         ? LOAD_WARPS
                              : is(B_K_FREE, MAX_STAGES) || is(B_V_FREE, MAX_STAGES) || is(B_PLAN_FREE, BATCHES) || i == B_FIN
@@ -575,7 +578,7 @@ __global__ void __launch_bounds__(THREADS, 1) k_paged_many(const AttnArgs<T> a) 
             mma_commit(bar(B_PV + 2 * x + buf));
           }
         };
-        if (!(ok = wait(B_Q + (k & 1), k / 2))) break;
+        if (!(ok = wait(B_Q + k % PIECES, k / PIECES))) break;
         // Turn i: P V of block i, then the scores of block i + 2 (turns -2 and -1: the first scores alone). A tile
         // without rows only gives its leave for each stage as it is filled.
 #pragma unroll 1
@@ -600,6 +603,7 @@ __global__ void __launch_bounds__(THREADS, 1) k_paged_many(const AttnArgs<T> a) 
         }
         done += n;
         if (active) tile_done += n;
+        if (ok && x == 1 && lane == 0) bar_arrive(bar(B_DONE + k % PIECES));
       }
       // every product done before the columns are freed
       commit(B_FIN);
@@ -782,7 +786,7 @@ __global__ void __launch_bounds__(THREADS, 1) k_paged_many(const AttnArgs<T> a) 
       }
       fence_proxy_async();
       __syncwarp();
-      if (lane == 0) bar_arrive(bar(B_Q + (k & 1)));
+      if (lane == 0) bar_arrive(bar(B_Q + k % PIECES));
 
       const int pos0 = piece.pos0, t0 = piece.t0, n_sink = piece.n_sink, skip = piece.skip;
       const int pos = live ? pos0 + tok : -1;
