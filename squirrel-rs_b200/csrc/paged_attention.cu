@@ -856,6 +856,8 @@ extern "C" int sq_paged_attention(void *stream, const sq_paged_cache *cache, con
   if (!paged::countable(b, c, n_heads))
     return fail(SQ_ERR_SHAPE, "paged_attention: too many query rows for so long a page table in one call");
   if (!b.n_tokens) return SQ_OK;
+  // a window that holds every position of the page table hides none; the kernels' sums with it fit 32 bits
+  if (window >= (long long)b.table_row * c.page) window = 0;
   const long long width = (long long)n_heads * c.hd;
   st = paged::check_rows(q, q_stride, width, dtype, "paged_attention: q");
   if (!st) st = paged::check_rows(out, out_stride, width, dtype, "paged_attention: out");

@@ -21,6 +21,7 @@ from .lib import KernelError, _check
 
 _KINDS = {torch.float32: lib.F32, torch.bfloat16: lib.BF16}
 _SHAPE, _TYPE, _ARG = 1, 2, 5
+_INT_MAX = 2**31 - 1
 
 
 def _need(ok, code, what):
@@ -190,6 +191,8 @@ def attention(cache, batch, q, window=0, sinks=0, scale=None, out=None):
         op, os_ = out.data_ptr(), width
     else:
         op, os_ = _rows(out, n, width, dtype, "out")
+    if window > _INT_MAX or sinks > _INT_MAX:
+        window, sinks = min(window, _INT_MAX), min(sinks, _INT_MAX)
     _, ws, ws_bytes = batch.workspace(cache, n_heads)
     st = _fn("sq_paged_attention")(_raw_stream(_device()), cache.ref, batch.ref, kind, qp, qs, n_heads,
                                    cache.scale if scale is None else scale, window, sinks, op, os_, ws, ws_bytes)
