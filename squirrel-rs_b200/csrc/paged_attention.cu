@@ -171,15 +171,13 @@ __global__ void __launch_bounds__(THREADS, C::BLOCKS) k_paged_few(const AttnArgs
   };
   // This block's piece [at, end) of the line of all tiles, and the sequence it starts in.
   const int first_n = tid < a.b.n_seqs ? tiles_of(load_seq(a.b, c, tid)) : 0;
-  int total = first_n;
-  for (int b = tid + THREADS; b < a.b.n_seqs; b += THREADS) total += tiles_of(load_seq(a.b, c, b));
-  total = __reduce_add_sync(0xffffffffu, total);
-  if (lane == 0) s_scan[wid] = total;
+  unsigned sum = first_n;
+  for (int b = tid + THREADS; b < a.b.n_seqs; b += THREADS) sum = line_add(sum, tiles_of(load_seq(a.b, c, b)));
+  sum = line_sum(sum);
+  if (lane == 0) s_scan[wid] = (int)sum;
   if (tid < 2) s_end[tid] = -1;
   __syncthreads();
-  total = 0;
-#pragma unroll
-  for (int w = 0; w < WARPS; w++) total += s_scan[w];
+  const int total = line_total<WARPS>(s_scan, a.b.err);
   const int per = max((total + (int)gridDim.x - 1) / (int)gridDim.x, MIN_TILES);
   if (per * (int)blockIdx.x >= total) return;
   {
@@ -764,7 +762,7 @@ bool goes_many(const Cache &c, int max_new, int group) {
   return (long long)max_new * group > ALONE_ROWS && many_supported(c, group);
 }
 
-// Whether the (row tile, key tile) pairs of a call can be numbered in 30 bits by both kernels: 128 rows or
+// Whether the (row tile, key tile) pairs of a call can be numbered below LINE_END by both kernels: 128 rows or
 // more a tile and 64 keys for the many-row one, 4 rows and 16 keys at least for the other.
 bool countable(const Batch &b, const Cache &c, int n_heads) {
   const int group = n_heads / c.kv_heads;
@@ -772,7 +770,7 @@ bool countable(const Batch &b, const Cache &c, int n_heads) {
   const double keys = (double)b.table_row * c.page, tokens = b.n_tokens, seqs = b.n_seqs;
   const double few = many ? seqs * (FEW_ROWS / 4) : tokens * group / 4 + seqs;
   const double rest = many ? (tokens * group / 128 + seqs) * (keys / 64 + 16) : 0;
-  return few * c.kv_heads * (keys / 16 + 32) < 1 << 30 && rest * c.kv_heads < 1 << 30;
+  return few * c.kv_heads * (keys / 16 + 32) < LINE_END && rest * c.kv_heads < LINE_END;
 }
 
 // Partial results of both kernels, then the counters of both.

@@ -27,6 +27,26 @@ struct AttnArgs {
   int max_row_tiles;
 };
 
+// Places on a line of work. The host refuses calls of LINE_END or more, taking the batch at its word; arrays that give
+// rows to several sequences can still have more. Counts stop there, and such a call is recorded and left out: past
+// 32 bits a thread block would look for its piece beyond the last sequence.
+constexpr unsigned LINE_END = 1u << 30;
+__device__ __forceinline__ unsigned line_add(unsigned a, unsigned b) { return min(a + b, LINE_END); }
+__device__ __forceinline__ unsigned line_sum(unsigned v) {  // of the warp
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) v = line_add(v, __shfl_xor_sync(0xffffffffu, v, o));
+  return v;
+}
+template <int WARPS>
+__device__ __forceinline__ int line_total(const int *warp_sums, unsigned *err) {  // 0 for a line that is too long
+  unsigned v = 0;
+#pragma unroll
+  for (int w = 0; w < WARPS; w++) v = line_add(v, (unsigned)warp_sums[w]);
+  if (v < LINE_END) return (int)v;
+  if (threadIdx.x == 0) flag(err, BAD_START);
+  return 0;
+}
+
 __device__ __forceinline__ uint32_t smem_addr(const void *p) { return (uint32_t)__cvta_generic_to_shared(p); }
 __device__ __forceinline__ void cp16(uint32_t dst, const void *src) {
   asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");

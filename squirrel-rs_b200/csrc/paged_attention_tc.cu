@@ -202,8 +202,8 @@ __device__ __forceinline__ void sts128(uint32_t a, uint32_t x, uint32_t y, uint3
   asm volatile("st.shared.v4.u32 [%0], {%1, %2, %3, %4};" ::"r"(a), "r"(x), "r"(y), "r"(z), "r"(w) : "memory");
 }
 
-// Sum over i < n of floor((a i + b) / m), by Euclid's steps. The host refuses calls whose
-// line of key blocks would not be below 2^31.
+// Sum over i < n of floor((a i + b) / m), by Euclid's steps. It fits 32 bits for the row tiles of a sequence
+// that has no more new tokens than positions: the host refuses calls whose line of key blocks would not.
 __device__ __forceinline__ int floor_sum(unsigned n, unsigned m, unsigned a, unsigned b) {
   unsigned sum = 0;
   while (n) {
@@ -227,12 +227,13 @@ __device__ __forceinline__ int floor_sum(unsigned n, unsigned m, unsigned a, uns
 }
 
 // Places of a sequence's row tiles on the line: key blocks, without a window the causal
-// count of each (a little over for the last), with one the same for all, and TILE_COST
+// count of each (a little over for the last), with one (and where there are more new tokens
+// than positions, whose first rows see nothing) the same for all, and TILE_COST
 // more; what a tile does not have of them is empty.
 template <int BK>
 struct Line {
   int row_tiles, tokens;  // tokens of a row tile
-  int flat;               // key blocks of every row tile (window), or 0
+  int flat;               // key blocks of every row tile, or 0
   int pos0, len;
   __device__ __forceinline__ void set(const Seq &s, int group, int window, int sinks, int few_rows) {
     tokens = ROWS / group;
@@ -242,6 +243,8 @@ struct Line {
     flat = 0;
     if (window && window < s.len)
       flat = min((min(sinks, s.len) + BK - 1) / BK + (window + tokens + BK - 3) / BK + 1, (s.len + BK - 1) / BK);
+    else if (s.n > s.len)
+      flat = max((s.len + BK - 1) / BK, 1);
   }
   __device__ __forceinline__ int before(int rt) const {  // key blocks of row tiles 0 .. rt - 1
     if (flat) return rt * (flat + TILE_COST);
@@ -328,7 +331,7 @@ struct Walk {
       p.len = s.len;
       int real = max(p.pos0 + toks - 1, 0) / BK + 1;
       p.n_sink = p.skip = 0;
-      if (line.flat) {
+      if (a.window && a.window < s.len) {
         const int low = max(p.pos0 - a.window + 1, 0) / BK;
         p.n_sink = min((min(a.sinks, s.len) + BK - 1) / BK, low);
         p.skip = low - p.n_sink;
@@ -375,13 +378,12 @@ __global__ void __launch_bounds__(THREADS, 1) k_paged_many(const AttnArgs<T> a) 
     l.set(load_seq(a.b, c, b), a.group, a.window, a.sinks, a.few_rows);
     return l.before(l.row_tiles) * c.kv_heads;
   };
-  int total = 0;
-  for (int b = tid; b < a.b.n_seqs; b += THREADS) total += blocks_of(b);
-  total = __reduce_add_sync(0xffffffffu, total);
-  if (lane == 0) s_scan[warp] = total;
+  unsigned sum = 0;
+  for (int b = tid; b < a.b.n_seqs; b += THREADS) sum = line_add(sum, blocks_of(b));
+  sum = line_sum(sum);
+  if (lane == 0) s_scan[warp] = (int)sum;
   __syncthreads();
-  total = 0;
-  for (int w = 0; w < WARPS; w++) total += s_scan[w];
+  const int total = line_total<WARPS>(s_scan, a.b.err);
   Walk<BK> walk;
   walk.per = max((total + (int)gridDim.x - 1) / (int)gridDim.x, MIN_BLOCKS);
   if (walk.per * (long long)blockIdx.x >= total) return;

@@ -3,7 +3,7 @@ import numpy as np
 import pytest
 
 import paged_oracle as P
-from test_gpu_paged import KINDS, Setup, dev
+from test_gpu_paged import KINDS, Setup, as_kind, dev
 
 pytestmark = pytest.mark.gpu
 
@@ -33,3 +33,42 @@ def test_windows_as_long_as_the_table_and_longer(gpu_lib, window, sinks, kind):
     pages of 16: the oracle takes the window as it is.)"""
     for heads, news, lens in ((8, [1, 3], [1, 9]), (8, [40, 90, 1, 2], [40, 100, 240, 2])):
         Setup(22, 2, 64, 16, news, lens).check_attention(heads, kind, window=window, sinks=sinks)
+
+
+@pytest.mark.parametrize("hd,news,n_seqs,pages", [(32, 2048, 4500, 256), (64, 16384, 900, 512)], ids=str)
+def test_sequences_that_claim_the_same_rows_are_recorded(gpu_lib, hd, news, n_seqs, pages):
+    """Every other sequence claims all rows and very many keys: together more (row tile, key tile) pairs than 32 bits
+    count. Nothing is looked for beyond the last sequence, the call is recorded, and the device is as usable as before."""
+    from sqb200 import lib, paged
+    s = Setup(26, 8, hd, 256, [1], [1])
+    q_start = np.int32([0, news] * (n_seqs // 2) + [0])
+    table = np.full((n_seqs, pages), s.table[0, 0], np.int32)
+    batch = paged.PagedBatch(dev(q_start), dev(np.full(n_seqs, 256 * pages, np.int32)), dev(table), news, news)
+    q = torch.randn(news, 32 * hd, device="cuda")
+    paged.status()
+    paged.attention(s.dcache, batch, q)
+    torch.cuda.synchronize()
+    with pytest.raises(lib.KernelError) as e:
+        paged.status()
+    assert "q_start" in str(e.value)
+    paged.status()
+    Setup(26, 2, hd, 16, [1, 40, 1], [50, 90, 20]).check_attention(8, "f32")
+
+
+def test_far_more_rows_than_positions(gpu_lib):
+    """A sequence of 2^22 new tokens and 100 positions: all but the last rows stand before position 0. Counted as if
+    they had keys, the row tiles' key blocks would not fit 32 bits."""
+    from sqb200 import paged
+    n, lens = 1 << 22, 100
+    s = Setup(27, 8, 64, 64, [lens], [lens])
+    tail = as_kind(s.rows(512, "bf16"), "bf16")
+    q = torch.full((n, 512), 3.0, dtype=torch.bfloat16, device="cuda")
+    q[-lens:] = dev(tail).bfloat16()
+    batch = paged.PagedBatch(dev(np.int32([0, n])), s.batch.kv_len, s.batch.page_table, n, n)
+    out = paged.attention(s.dcache, batch, q)
+    torch.cuda.synchronize()
+    paged.status()
+    assert not out[:-lens].any()
+    want, size = P.attention(s.cache, [0, lens], [lens], s.table, tail, 8)
+    over = np.abs(out[-lens:].float().cpu().numpy().reshape(want.shape) - want) / P.bound(want, size, "bf16")
+    assert over.max() <= 1
