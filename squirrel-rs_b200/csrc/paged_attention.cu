@@ -650,7 +650,7 @@ __global__ void __launch_bounds__(THREADS, C::BLOCKS) k_paged_few(const AttnArgs
       // the threads share out rows, dimensions and (when there are few of those) slices of the parts.
       // The cuts are the multiples of `per` more than SNAP tiles inside its keys; the part before the first is the block's before.
       const int first = (job_start + SNAP) / per, parts = (job_start + span.n - SNAP - 1) / per - first + 1;
-      int *count = a.count + (b * c.kv_heads + head) * a.max_row_tiles + rt;
+      int *count = a.count + (long long)(b * c.kv_heads + head) * a.max_row_tiles + rt;
       __syncthreads();
       if (tid == 0) {  // the block's stores before its arrival, the other blocks' arrivals before its loads
         __threadfence();

@@ -266,7 +266,7 @@ struct Piece {
   int slot;             // of the partial results
   int first, parts;     // thread blocks first .. first + parts - 1 share the tile
   int late;             // block `first` began another tile before this one: its second slot
-  int counter;
+  long long counter;
   __device__ __forceinline__ int block(int i) const { return t0 + i + (t0 + i < n_sink ? 0 : skip); }
 };
 constexpr int PIECES = 4;
@@ -345,7 +345,7 @@ struct Walk {
       p.parts = (tile_start + real - 1) / per - p.first + 1;
       p.late = tile_start > per * p.first;
       p.slot = 2 * blockIdx.x + (tile_start > per * (int)blockIdx.x ? 1 : 0);
-      p.counter = (b * a.c.kv_heads + head) * a.max_row_tiles + rt;
+      p.counter = (long long)(b * a.c.kv_heads + head) * a.max_row_tiles + rt;
       at = tile_start + t1;
       tile_start += slots;
       if (p.n > 0) return true;

@@ -72,3 +72,29 @@ def test_far_more_rows_than_positions(gpu_lib):
     want, size = P.attention(s.cache, [0, lens], [lens], s.table, tail, 8)
     over = np.abs(out[-lens:].float().cpu().numpy().reshape(want.shape) - want) / P.bound(want, size, "bf16")
     assert over.max() <= 1
+
+
+def test_counters_past_32_bits(gpu_lib):
+    """Many sequences beside one of many new tokens: more row tiles in the workspace than 32 bits count, and the last
+    sequence's, which are cut between thread blocks, at its far end."""
+    from sqb200 import paged
+    n_seqs, news, last, lens = 65535, 4200 * 64, 300, 1000
+    s = Setup(28, 8, 64, 64, [last], [lens])
+    q_start = np.full(n_seqs + 1, news, np.int32)
+    q_start[0], q_start[-1] = 0, news + last
+    kv_len = np.zeros(n_seqs, np.int32)
+    kv_len[-1] = lens
+    table = np.full((n_seqs, s.table.shape[1]), -1, np.int32)
+    table[-1] = s.table[0]
+    batch = paged.PagedBatch(dev(q_start), dev(kv_len), dev(table), news + last, news)
+    tail = as_kind(s.rows(2048, "bf16", 1.5), "bf16")
+    q = torch.zeros(news + last, 2048, dtype=torch.bfloat16, device="cuda")
+    q[news:] = dev(tail).bfloat16()
+    assert batch.workspace(s.dcache, 32)[2] > 4 << 31
+    for _ in range(2):
+        out = paged.attention(s.dcache, batch, q)
+        torch.cuda.synchronize()
+        paged.status()
+        want, size = P.attention(s.cache, [0, last], [lens], s.table, tail, 32)
+        over = np.abs(out[news:].float().cpu().numpy().reshape(want.shape) - want) / P.bound(want, size, "bf16")
+        assert over.max() <= 1 and not out[:news].any()
