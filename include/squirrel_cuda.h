@@ -169,7 +169,7 @@ typedef struct {
     const int32_t *page_table; /* [n_seqs][pages_per_seq] */
     int n_seqs, n_tokens;
     int max_new;               /* most new tokens of one sequence */
-    int pages_per_seq;
+    int pages_per_seq;         /* pages_per_seq * page: at most 2^30 */
 } sq_paged_batch;
 
 /* What the kernels found wrong in a batch's arrays on the current device since the

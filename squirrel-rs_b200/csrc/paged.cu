@@ -52,7 +52,7 @@ int check_cache(const sq_paged_cache *c, Cache *out, const char *what) {
   return SQ_OK;
 }
 
-int check_batch(const sq_paged_batch *b, Batch *out, const char *what) {
+int check_batch(const sq_paged_batch *b, const Cache &c, Batch *out, const char *what) {
   auto fail = [&](int code, const char *msg) { return sq::fail(code, std::string(what) + ": " + msg); };
   if (!b || !b->q_start || !b->kv_len || !b->page_table) return fail(SQ_ERR_ARG, "null batch pointer");
   if (b->n_seqs <= 0 || b->n_seqs > 65535) return fail(SQ_ERR_SHAPE, "1 to 65535 sequences");
@@ -60,6 +60,8 @@ int check_batch(const sq_paged_batch *b, Batch *out, const char *what) {
       (long long)b->max_new * b->n_seqs < b->n_tokens)
     return fail(SQ_ERR_SHAPE, "max_new must be the most new tokens of one sequence");
   if (b->pages_per_seq <= 0) return fail(SQ_ERR_SHAPE, "a page table has columns");
+  if ((long long)b->pages_per_seq * c.page > MAX_POSITIONS)
+    return fail(SQ_ERR_SHAPE, "a page table names at most 2^30 positions of a sequence");
   if (((uintptr_t)b->q_start | (uintptr_t)b->kv_len | (uintptr_t)b->page_table) & 3)
     return fail(SQ_ERR_ALIGN, "batch arrays must be 4-byte aligned");
   *out = {b->q_start, b->kv_len, b->page_table, b->n_seqs, b->n_tokens, b->max_new, b->pages_per_seq, nullptr};
@@ -194,8 +196,9 @@ __global__ void __launch_bounds__(256) k_paged_append(const AppendArgs<T> a) {
   const int pos0 = s.len - s.n;  // position of the first new token
   const int end = min(s.len, a.rope_rows);
   if (tid == 0 && s.n && (pos0 < 0 || s.len > a.rope_rows)) flag(a.b.err, BAD_POSITION);
-  const int from = max(pos0, 0), p = (from >> c.page_shift) + blk % a.touches, start = p << c.page_shift;
-  if (!s.n || start >= end) return;
+  const int from = max(pos0, 0), p = (from >> c.page_shift) + blk % a.touches;
+  if (!s.n || p > (end - 1) >> c.page_shift) return;
+  const int start = p << c.page_shift;
   const int lo = max(start, from), rows = min(start + c.page, end) - lo, held = lo - start;
   const long long stride = is_v ? a.vs : a.ks;
   const T *src = (is_v ? a.v : a.k) + (s.first + (lo - pos0)) * stride + g * c.hd;
@@ -369,7 +372,7 @@ extern "C" int sq_paged_append(void *stream, const sq_paged_cache *cache, const 
   paged::Cache c;
   paged::Batch b;
   int st = paged::check_cache(cache, &c, "paged_append");
-  if (!st) st = paged::check_batch(batch, &b, "paged_append");
+  if (!st) st = paged::check_batch(batch, c, &b, "paged_append");
   if (st) return st;
   if (dtype != SQ_F32 && dtype != SQ_BF16) return fail(SQ_ERR_INVALID_TYPE, "paged_append: rows must be F32 or BF16");
   if (!b.n_tokens) return SQ_OK;
@@ -398,7 +401,7 @@ extern "C" int sq_paged_read(void *stream, const sq_paged_cache *cache, const sq
   paged::Cache c;
   paged::Batch b;
   int st = paged::check_cache(cache, &c, "paged_read");
-  if (!st) st = paged::check_batch(batch, &b, "paged_read");
+  if (!st) st = paged::check_batch(batch, c, &b, "paged_read");
   if (st) return st;
   if (dtype != SQ_F32 && dtype != SQ_BF16) return fail(SQ_ERR_INVALID_TYPE, "paged_read: rows must be F32 or BF16");
   if (count < 0) return fail(SQ_ERR_SHAPE, "paged_read: negative count");

@@ -91,11 +91,13 @@ __device__ __forceinline__ void store4(__nv_bfloat16 *p, float4 v) {
       make_uint2(*reinterpret_cast<const uint32_t *>(&a), *reinterpret_cast<const uint32_t *>(&b));
 }
 
+constexpr long long MAX_POSITIONS = 1 << 30;  // of a page table's row: sums of positions, tiles and pages fit 32 bits
+
 unsigned *err_ptr();  // device address of the current device's word (null: no such device)
 // Checked copies of the caller's structs (Batch::err left to the caller, who sets it to
 // err_ptr() once every check that needs no GPU has passed); SQ_OK or the status.
 int check_cache(const sq_paged_cache *c, Cache *out, const char *what);
-int check_batch(const sq_paged_batch *b, Batch *out, const char *what);
+int check_batch(const sq_paged_batch *b, const Cache &c, Batch *out, const char *what);
 // Rows [n][width] of `dtype` at p with `stride` elements between them: 16-byte aligned throughout.
 int check_rows(const void *p, long long stride, long long width, int dtype, const char *what);
 

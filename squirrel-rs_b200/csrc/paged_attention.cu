@@ -831,7 +831,7 @@ extern "C" int sq_paged_attention_workspace(const sq_paged_cache *cache, const s
   paged::Cache c;
   int st = paged::check_cache(cache, &c, "paged_attention_workspace");
   paged::Batch b;
-  if (!st) st = paged::check_batch(batch, &b, "paged_attention_workspace");
+  if (!st) st = paged::check_batch(batch, c, &b, "paged_attention_workspace");
   if (!st && !bytes) st = fail(SQ_ERR_ARG, "paged_attention_workspace: null pointer");
   if (!st) st = paged::check_heads(c, n_heads, "paged_attention_workspace");
   if (st) return st;
@@ -845,7 +845,7 @@ extern "C" int sq_paged_attention(void *stream, const sq_paged_cache *cache, con
   paged::Cache c;
   paged::Batch b;
   int st = paged::check_cache(cache, &c, "paged_attention");
-  if (!st) st = paged::check_batch(batch, &b, "paged_attention");
+  if (!st) st = paged::check_batch(batch, c, &b, "paged_attention");
   if (!st) st = paged::check_heads(c, n_heads, "paged_attention");
   if (st) return st;
   if (dtype != SQ_F32 && dtype != SQ_BF16)
