@@ -174,7 +174,7 @@ typedef struct {
 
 /* What the kernels found wrong in a batch's arrays on the current device since the
  * record was last cleared (a page id outside the cache, lengths beyond the page table,
- * rows out of order, positions outside the rotation table; such entries are skipped,
+ * rows out of order or of no sequence, positions outside the rotation table; such entries are skipped,
  * never read through): SQ_OK, SQ_ERR_ARG with a message that says what, or
  * SQ_ERR_TIMEOUT when a bounded wait expired. Call after synchronizing the stream;
  * `clear` != 0 resets the record. */

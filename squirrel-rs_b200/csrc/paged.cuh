@@ -21,7 +21,7 @@ namespace paged {
 enum : unsigned {
   BAD_PAGE = 1,      // page id outside the cache: its positions count as masked
   BAD_LENGTH = 2,    // kv_len negative or beyond the page table's row
-  BAD_START = 4,     // q_start not ascending, outside [0, n_tokens], or more than max_new tokens
+  BAD_START = 4,     // q_start not ascending from 0 to n_tokens, or more than max_new tokens of a sequence
   BAD_POSITION = 8,  // a new token before position 0 or past the rotation table
   BAD_WAIT = 16,     // a bounded wait gave up
 };
@@ -51,7 +51,8 @@ __device__ __forceinline__ Seq load_seq(const Batch &b, const Cache &c, int i) {
   s.first = min(max(a, 0), b.n_tokens);
   s.n = min(max(min(e, b.n_tokens) - s.first, 0), b.max_new);
   s.len = (int)min((long long)max(l, 0), (long long)b.table_row << c.page_shift);
-  if (s.first != a || s.n != e - a) flag(b.err, BAD_START);
+  // rows before the first sequence's or after the last one's would stay as they are
+  if (s.first != a || s.n != e - a || (i == 0 && a != 0) || (i + 1 == b.n_seqs && e != b.n_tokens)) flag(b.err, BAD_START);
   if (s.len != l) flag(b.err, BAD_LENGTH);
   return s;
 }

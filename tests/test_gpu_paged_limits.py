@@ -35,6 +35,33 @@ def test_windows_as_long_as_the_table_and_longer(gpu_lib, window, sinks, kind):
         Setup(22, 2, 64, 16, news, lens).check_attention(heads, kind, window=window, sinks=sinks)
 
 
+@pytest.mark.parametrize("what", ["begins_late", "ends_early", "none"])
+@pytest.mark.parametrize("news", [[1, 2, 1], [40, 40, 40]], ids=str)
+def test_rows_of_no_sequence_are_recorded(gpu_lib, news, what):
+    """q_start has to run from 0 to n_tokens: rows outside it would be left as they were."""
+    from sqb200 import lib, paged
+    s = Setup(24, 2, 64, 16, news, [50, 90, 60])
+    q_start = s.batch.q_start.clone()
+    if what == "begins_late":
+        q_start[0] = 1
+    elif what == "ends_early":
+        q_start[3] -= 1
+    else:
+        q_start[:] = 0
+    batch = paged.PagedBatch(q_start, s.batch.kv_len, s.batch.page_table, sum(news), max(news))
+    q, k = dev(s.rows(512, "f32")), dev(s.rows(128, "f32"))
+    cos, sin = (dev(x) for x in P.rotation(128, 64))
+    paged.status()
+    for call in (lambda: paged.attention(s.dcache, batch, q), lambda: paged.append(s.dcache, batch, k, k, cos, sin, q=q),
+                 lambda: paged.read(s.dcache, batch, dev(np.int32([0, 0, 0])), 90)):
+        call()
+        torch.cuda.synchronize()
+        with pytest.raises(lib.KernelError) as e:
+            paged.status()
+        assert e.value.kind == "InvalidArgument" and "q_start" in str(e.value)
+        paged.status()  # cleared
+
+
 @pytest.mark.parametrize("hd,news,n_seqs,pages", [(32, 2048, 4500, 256), (64, 16384, 900, 512)], ids=str)
 def test_sequences_that_claim_the_same_rows_are_recorded(gpu_lib, hd, news, n_seqs, pages):
     """Every other sequence claims all rows and very many keys: together more (row tile, key tile) pairs than 32 bits
