@@ -17,8 +17,9 @@
 // Precision. Codes are whole numbers up to 127: exact in f16. Query rows are scaled by a
 // power of two; an f32 row takes two f16 terms (22 bits) and so two products, a bf16 row is
 // exact in one. Weights, at most 2^10 (the maximum's), likewise: two terms for f32
-// rows, one (11 bits, under the output's 8) for bf16 rows. The V scale of a page goes
-// into the weights relative to the largest met so far, so f16 never overflows. With bf16
+// rows, one (11 bits, under the output's 8) for bf16 rows. The exponent of a page's V scale goes
+// into its scores, the rest of it into the weights, so f16 neither overflows nor loses the
+// weights of a page with small values beside one with large ones. With bf16
 // rows K's codes enter as the f16 numbers code * 2^-24 (denormal, exact; one instruction a
 // pair) and their bias leaves with the sum of the row, 128 sum(q): that costs a score two
 // bits of 24 at most. With f32 rows the bias is taken off before the product (one
@@ -252,7 +253,7 @@ __global__ void __launch_bounds__(THREADS, C::BLOCKS) k_paged_few(const AttnArgs
     const int last_row = min((rt + 1) * ROWS, s.n * rows_of_token) - 1;
     const int min_pos = pos0 + rt * ROWS / rows_of_token, max_pos = pos0 + last_row / rows_of_token;
 
-    float o[MT][NT][4], m[NT][2], l[NT][2], unit = 0.f;
+    float o[MT][NT][4], m[NT][2], l[NT][2];
 #pragma unroll
     for (int nt = 0; nt < NT; nt++) {
 #pragma unroll
@@ -331,8 +332,8 @@ __global__ void __launch_bounds__(THREADS, C::BLOCKS) k_paged_few(const AttnArgs
       cp_commit();
     };
     int place = place_of(0, entry_of(0)), entry = entry_of(1), next_place = -1;
-    float ks = scale_of(c.ks, place), vs = scale_of(c.vs, place), next_ks = 0.f, next_vs = 0.f, share = 0.f;
-    int st = 0;
+    float ks = scale_of(c.ks, place), vs = scale_of(c.vs, place), next_ks = 0.f, next_vs = 0.f, v_inv = 0.f, v_man = 0.f;
+    int st = 0, v_top = V_EXP_MIN;
     if constexpr (BATCH >= STAGES) {
 #pragma unroll
       for (int k = 0; k < STAGES; k++) load_tile(k, place, k);
@@ -401,22 +402,10 @@ __global__ void __launch_bounds__(THREADS, C::BLOCKS) k_paged_few(const AttnArgs
       const int in_batch = k % BATCH;
       if (in_batch == 0) {
         if (k) place = next_place, ks = next_ks, vs = next_vs, entry = entry_of(k / BATCH + 1);
-        // the largest V scale so far: earlier results move to it
-        const float top = __uint_as_float(__reduce_max_sync(0xffffffffu, __float_as_uint(fmaxf(vs, 0.f))));
-        const float new_unit = fmaxf(unit, top), per_unit = new_unit > 0.f ? 1.f / new_unit : 0.f;
-        const float move = unit * per_unit;
-        if (k && move != 1.f) {
-#pragma unroll
-          for (int nt = 0; nt < NT; nt++) {
-            if (SPLIT) late[nt][0] *= move, late[nt][1] *= move;
-#pragma unroll
-            for (int mt = 0; mt < MT; mt++)
-#pragma unroll
-              for (int i = 0; i < 4; i++) o[mt][nt][i] *= move;
-          }
-        }
-        unit = new_unit;
-        share = vs * per_unit;
+        const int e = v_exp(vs);
+        v_top = max(v_top, __reduce_max_sync(0xffffffffu, e));
+        v_inv = exp_inv(max(e, v_top - V_EXP_SPAN));
+        v_man = vs * v_inv;
       }
       if (in_batch == BATCH / 2) {
         next_place = place_of(k / BATCH + 1, entry);
@@ -463,13 +452,17 @@ __global__ void __launch_bounds__(THREADS, C::BLOCKS) k_paged_few(const AttnArgs
             for (int x = 0; x < 4; x++) sc[j][nt][x] += second[nt][x];
         }
       }
-      // in log2 units
+      // in log2 units, with the exponents of the V scales
+      float g_inv[NG];
 #pragma unroll
       for (int j = 0; j < NG; j++) {
         const float gks = __shfl_sync(0xffffffffu, ks, in_batch * NG + j);
+        g_inv[j] = __shfl_sync(0xffffffffu, v_inv, in_batch * NG + j);
+        const float e = (float)(127 - (int)(__float_as_uint(g_inv[j]) >> 23));
 #pragma unroll
         for (int nt = 0; nt < NT; nt++) {
-          const float f0 = cf[nt][0] * gks, f1 = cf[nt][1] * gks, b0 = cb[nt][0] * gks, b1 = cb[nt][1] * gks;
+          const float f0 = cf[nt][0] * gks, f1 = cf[nt][1] * gks;
+          const float b0 = SPLIT ? e : fmaf(cb[nt][0], gks, e), b1 = SPLIT ? e : fmaf(cb[nt][1], gks, e);
 #pragma unroll
           for (int x = 0; x < 4; x++) sc[j][nt][x] = fmaf(sc[j][nt][x], x & 1 ? f1 : f0, x & 1 ? b1 : b0);
         }
@@ -503,15 +496,15 @@ __global__ void __launch_bounds__(THREADS, C::BLOCKS) k_paged_few(const AttnArgs
 #pragma unroll
           for (int x = 4; x < 32; x <<= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, x));
           ref[nt][j] = mx == -INFINITY ? 0.f : mx - WEIGHT_EXP;
-          corr[nt][j] = mx == m[nt][j] ? 1.f : ex2(m[nt][j] - mx);  // 0 while nothing was seen
-          moved |= corr[nt][j] != 1.f;
+          corr[nt][j] = mx == m[nt][j] ? 0.f : m[nt][j] - mx;  // as an exponent
+          moved |= corr[nt][j] != 0.f;
           m[nt][j] = mx;
         }
       if (__any_sync(0xffffffffu, moved)) {
 #pragma unroll
         for (int nt = 0; nt < NT; nt++) {
-          const float f0 = corr[nt][0], f1 = corr[nt][1];
-          l[nt][0] *= f0, l[nt][1] *= f1;
+          const float f0 = ex2(corr[nt][0]), f1 = ex2(corr[nt][1]);  // 0 while nothing was seen
+          l[nt][0] = scaled(l[nt][0], corr[nt][0]), l[nt][1] = scaled(l[nt][1], corr[nt][1]);
           if (SPLIT) late[nt][0] *= f0, late[nt][1] *= f1;
 #pragma unroll
           for (int mt = 0; mt < MT; mt++) {
@@ -523,16 +516,16 @@ __global__ void __launch_bounds__(THREADS, C::BLOCKS) k_paged_few(const AttnArgs
       uint32_t pf[NG][NT][TERMS][2];
 #pragma unroll
       for (int j = 0; j < NG; j++) {
-        const float gshare = __shfl_sync(0xffffffffu, share, in_batch * NG + j);
+        const float g_man = __shfl_sync(0xffffffffu, v_man, in_batch * NG + j);
 #pragma unroll
         for (int nt = 0; nt < NT; nt++)
 #pragma unroll
           for (int x = 0; x < 2; x++) {
             float u = ex2(sc[j][nt][2 * x] - ref[nt][0]), v = ex2(sc[j][nt][2 * x + 1] - ref[nt][1]);
-            l[nt][0] += u;
-            l[nt][1] += v;
-            u *= gshare;
-            v *= gshare;
+            l[nt][0] = fmaf(u, g_inv[j], l[nt][0]);
+            l[nt][1] = fmaf(v, g_inv[j], l[nt][1]);
+            u *= g_man;
+            v *= g_man;
             const uint32_t f = pack(u, v);
             pf[j][nt][0][x] = transpose8x8(f);
             if constexpr (SPLIT) {
@@ -604,7 +597,7 @@ __global__ void __launch_bounds__(THREADS, C::BLOCKS) k_paged_few(const AttnArgs
           const float *sm = sums + ((mt * NT + nt) * 4 + j) * 32;
           const float2 v = SPLIT ? make_float2(sm[0], sm[64]) : make_float2(o[mt][nt][j], o[mt][nt][2 + j]);
           const int d = HD >= 128 ? (mt / 8) * 128 + g * 16 + (mt % 8) * 2 : g * (HD / 8) + mt * 2;
-          *reinterpret_cast<float2 *>(dst + 2 + d) = make_float2(v.x * unit, v.y * unit);
+          *reinterpret_cast<float2 *>(dst + 2 + d) = v;
         }
       }
     __syncthreads();
@@ -630,7 +623,7 @@ __global__ void __launch_bounds__(THREADS, C::BLOCKS) k_paged_few(const AttnArgs
       for (int w = 0; w < WARPS; w++) {
         const float *x = src + w * ROWS * (HD + 2);
         const float f = ex2(x[0] - at0);
-        sum = fmaf(x[1], f, sum);
+        sum += scaled(x[1], x[0] - at0);
         v.x = fmaf(x[2 + d], f, v.x), v.y = fmaf(x[3 + d], f, v.y);
         v.z = fmaf(x[4 + d], f, v.z), v.w = fmaf(x[5 + d], f, v.w);
       }
@@ -672,9 +665,9 @@ __global__ void __launch_bounds__(THREADS, C::BLOCKS) k_paged_few(const AttnArgs
             top = warp_max(top);
             const float at0 = top == -INFINITY ? 0.f : top;
             for (int i = lane; i < parts; i += 32) {
-              const float x = ex2(f[i] - at0);
-              f[i] = x;
-              sum = fmaf(__ldcg(part(i) + ROWS + r0 + r), x, sum);
+              const float x = f[i] - at0;
+              f[i] = ex2(x);
+              sum += scaled(__ldcg(part(i) + ROWS + r0 + r), x);
             }
             sum = warp_sum(sum);
             if (lane == 0) s_sum[r] = sum;

@@ -85,6 +85,18 @@ __device__ __forceinline__ float row_factor(int e, bool finite) {
   return finite ? __uint_as_float((uint32_t)(e + 127) << 23) : __int_as_float(0x7fffffff);
 }
 
+// The exponent e of a page's V scale goes into its keys' scores: weights are 2^(s + e - max(s + e)), in f16's range where
+// they count for the result, and the sum of the weights takes them times 2^-e. A key's exponent is not taken lower than
+// V_EXP_SPAN below the largest met so far, so that no weight of the sum's first 50 bits vanishes, and at least
+// V_EXP_MIN, so that the sum has room for 2^30 positions: what remains of such a scale counts as far as f16 goes.
+constexpr int V_EXP_MIN = -80, V_EXP_SPAN = 80;
+__device__ __forceinline__ int v_exp(float vs) {
+  return min(max((int)(__float_as_uint(vs) >> 23 & 255) - 127, V_EXP_MIN), 126);
+}
+__device__ __forceinline__ float exp_inv(int e) { return __uint_as_float((uint32_t)(127 - e) << 23); }  // 2^-e
+// v 2^x for a sum of weights: x may be below f32's exponents where v makes up for it.
+__device__ __forceinline__ float scaled(float v, float x) { return v * ex2(fmaxf(x, -126.f)) * ex2(fminf(x + 126.f, 0.f)); }
+
 // The many-row kernel (paged_attention_tc.cu).
 bool many_supported(const Cache &c, int group);
 template <typename T>

@@ -24,9 +24,9 @@
 // KB) every role spent its time waiting for instructions.
 //
 // Precision, as in the few-row kernel: query rows scaled by powers of two, two f16 terms
-// for f32 rows, one (exact) for bf16 rows. Weights are 2^(s - ref + 3); ref follows the
-// maximum only when it is passed by 2^6, and the V scales go into the weights relative to
-// a unit, so that f16 never overflows and outputs are seldom rescaled.
+// for f32 rows, one (exact) for bf16 rows. Scores s take the V scales' exponents on, weights are
+// 2^(s - ref + 3), and ref follows the maximum only when it is passed by 2^6, so that f16 never overflows, loses
+// no page with small values beside one with large ones, and outputs are seldom rescaled.
 //   f32 rows:  weights in two terms; the O of four blocks of keys is summed in tensor memory and
 //              added to f32 registers, because the tensor core truncates its running sum
 //              (2^-25 of it a step: 500 steps would cost 1e-5). 2048 x 4,133 positions, 128
@@ -56,6 +56,7 @@ constexpr int WARPS = 16;  // whole warpgroups: registers are shared out by them
 constexpr int THREADS = WARPS * 32, LOADERS = LOAD_WARPS * 32;
 constexpr int TILE_ROWS = 128, ROWS = 2 * TILE_ROWS;
 constexpr int BATCH = 8, BATCHES = 2;  // blocks of keys looked up at once, and how many such batches are held
+constexpr int PLAN_BYTES = 96;
 constexpr int MAX_BLOCKS = 160;
 // What a row tile costs besides its key blocks, in blocks (queries in, results out, the pipeline's start and end), when
 // the work is shared out. 0 / 3 / 5 / 8 (bf16, 128 dimensions): 2 x 4,096 rows of 8,000 positions 776 / 718 /
@@ -63,7 +64,7 @@ constexpr int MAX_BLOCKS = 160;
 constexpr int TILE_COST = 5;
 constexpr int MIN_BLOCKS = 2;  // key blocks a thread block takes at least
 constexpr int MOVE = 4;        // f32 rows: blocks of keys summed in tensor memory at a stretch
-constexpr float WEIGHT_EXP = 3.f, REF_LAG = 6.f, UNIT_LAG = 64.f;
+constexpr float WEIGHT_EXP = 3.f, REF_LAG = 6.f;
 // Registers a thread: launched with 128 (512 x 128 = 65,536), then 256 x 184 + 128 x 80 + 128 x 64.
 constexpr int SOFTMAX_REGS = 184, LOAD_REGS = 80, MMA_REGS = 64;
 
@@ -83,23 +84,22 @@ struct Cfg {
   static constexpr int STEPS = BK / STEP_ROWS;
   static constexpr int OFF_Q = 0, OFF_K = OFF_Q + 2 * TERMS * Q_TILE, OFF_V = OFF_K + STAGES * KV_TILE,
                        OFF_SCALE = OFF_V + STAGES * KV_TILE,
-                       OFF_BAR = OFF_SCALE + BATCHES * BATCH * 96;
+                       OFF_BAR = OFF_SCALE + BATCHES * BATCH * PLAN_BYTES;
   static constexpr int SMEM = 1024 + OFF_BAR + 368;
   static constexpr int SLOT = ROWS * (HD + 2);  // floats of a cut row tile's partial result
   static_assert(SMEM <= 232448 - 256, "shared memory of a block");
 };
 
 // What is looked up for a block of 64 keys: of its four groups of 16 the place in the
-// codes (in groups of 16 keys; -1: none), the K scale, the V scale relative to the unit
-// (f32 rows: the ratio; bf16 rows: its log2, and 1 / ratio).
+// codes (in groups of 16 keys; -1: none), the K scale, the V scale 2^exp * man (f32 rows: exp is a whole
+// number; bf16 rows: man is 1) and 2^-exp.
 struct Plan {
   int place[4];
-  float ks[4], share[4], inv[4];
-  uint32_t present, with_v;  // bit masks of groups: there at all; with a V scale that is not 0
-  float unit;
-  float pad[5];
+  float ks[4], exp[4], inv[4], man[4];
+  uint32_t present, with_v;  // bit masks of groups: there at all; with a V scale that counts
+  uint32_t pad[2];
 };
-static_assert(sizeof(Plan) == 96, "room in shared memory");
+static_assert(sizeof(Plan) == PLAN_BYTES, "room in shared memory");
 
 constexpr int MAX_STAGES = 4;
 // A wait tells a phase from the one before it only. So every barrier is one whose phase before is known to be done
@@ -485,7 +485,7 @@ __global__ void __launch_bounds__(THREADS, 1) k_paged_many(const AttnArgs<T> a) 
         if (!(ok = wait(B_PIECE + k % PIECES, k / PIECES))) break;
         const Piece p = s_pieces[k % PIECES];
         if (p.n < 0) break;
-        float unit = 0.f;
+        int v_top = V_EXP_MIN;
         const int j = lane & 3;  // lane: group j of block i
 #pragma unroll 1
         for (int i0 = 0; i0 < p.n; i0 += BATCH, batch++) {
@@ -499,34 +499,28 @@ __global__ void __launch_bounds__(THREADS, 1) k_paged_many(const AttnArgs<T> a) 
             ks = c.ks[(long long)page * c.kv_heads + p.head];
             vs = c.vs[(long long)page * c.kv_heads + p.head];
           }
-          float top = fmaxf(vs, __shfl_xor_sync(0xffffffffu, vs, 1));
-          top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
-          float my_unit = 0.f;
-          // outputs stay in the unit of the first block (of the stretch) until a much larger scale comes
-#pragma unroll 1
-          for (int q = 0; q < BATCH; q++) {
-            const float t = __shfl_sync(0xffffffffu, top, 4 * q);
-            if (t > unit * UNIT_LAG || unit == 0.f || (SPLIT && q % MOVE == 0)) unit = t;
-            if (lane >> 2 == q) my_unit = unit;
-          }
           const uint32_t present = __ballot_sync(0xffffffffu, page >= 0) >> (lane & 28) & 15;
-          const uint32_t with_v = __ballot_sync(0xffffffffu, vs > 0.f) >> (lane & 28) & 15;
+          const int e = v_exp(vs);
+          v_top = max(v_top, __reduce_max_sync(0xffffffffu, e));
+          const int floor = max(v_top - V_EXP_SPAN, V_EXP_MIN);
+          const uint32_t with_v = __ballot_sync(0xffffffffu, e > floor) >> (lane & 28) & 15;
           if (batch >= BATCHES && !(ok = wait(B_PLAN_FREE + batch % BATCHES, batch / BATCHES - 1))) break;
           Plan &plan = plans[batch % BATCHES * BATCH + (lane >> 2)];
-          const float share = vs > 0.f ? vs / my_unit : 0.f;
           plan.place[j] = page < 0 ? -1 : ((page * c.kv_heads + p.head) << (c.page_shift - 4)) + ((key & (c.page - 1)) >> 4);
           plan.ks[j] = ks;
           if (SPLIT) {
-            plan.share[j] = share;
-          } else {  // as an exponent; below 2^-100 of the unit: as good as none
-            const float e = share > 0.f ? fmaxf(log2f(share), -100.f) : 0.f;
-            plan.share[j] = e;
-            plan.inv[j] = share > 0.f ? exp2f(-e) : 1.f;
+            const int x = max(e, floor);
+            plan.exp[j] = (float)x;
+            plan.inv[j] = exp_inv(x);
+            plan.man[j] = vs * exp_inv(x);
+          } else {
+            const float x = e > floor ? log2f(vs) : (float)floor;
+            plan.exp[j] = x;
+            plan.inv[j] = exp2f(-x);
           }
           if (j == 0) {
             plan.present = present;
             plan.with_v = with_v;
-            plan.unit = my_unit;
           }
           __syncwarp();
           if (lane == 0) bar_arrive(bar(B_PLAN + batch % BATCHES));
@@ -795,13 +789,13 @@ __global__ void __launch_bounds__(THREADS, 1) k_paged_many(const AttnArgs<T> a) 
       const int low = a.window ? pos - a.window : -1;  // seen: low < key <= pos, or key < sinks
       const int sinks = a.window ? a.sinks : 0;
       const int min_pos = pos0 + warp_row / a.group, max_pos = pos0 + (warp_row + 31) / a.group;
-      float o[SPLIT ? HD : 1], ref = -INFINITY, l = 0.f, unit = 0.f;
+      float o[SPLIT ? HD : 1], ref = -INFINITY, l = 0.f;
       if constexpr (SPLIT) {
 #pragma unroll
         for (int d = 0; d < HD; d++) o[d] = 0.f;
       }
-      // f32 rows: o += unit * O
-      auto add_output = [&](float unit) {
+      // f32 rows: o += O
+      auto add_output = [&]() {
         if constexpr (SPLIT) {
 #pragma unroll
           for (int d = 0; d < HD; d += 32) {
@@ -809,7 +803,7 @@ __global__ void __launch_bounds__(THREADS, 1) k_paged_many(const AttnArgs<T> a) 
             tmem_ld32(o_col + d, v);
             tmem_ready<32>(v);
 #pragma unroll
-            for (int j = 0; j < 32; j++) o[d + j] = fmaf(v[j], unit, o[d + j]);
+            for (int j = 0; j < 32; j++) o[d + j] += v[j];
           }
         }
       };
@@ -821,7 +815,7 @@ __global__ void __launch_bounds__(THREADS, 1) k_paged_many(const AttnArgs<T> a) 
         if (i == n) {
           ok = products_done(tile_done + n - 1);
           fence_after();
-          if (ok) add_output(unit);
+          if (ok) add_output();
           break;
         }
         const unsigned t = tile_done + i, bt = batch + i / BATCH;
@@ -835,12 +829,11 @@ __global__ void __launch_bounds__(THREADS, 1) k_paged_many(const AttnArgs<T> a) 
         tmem_ld32(s_col + 32, v + 32);
         const int key0 = (t0 + i + (t0 + i < n_sink ? 0 : skip)) * BK;
         const uint32_t present = plan.present;
-        const float4 ks = *reinterpret_cast<const float4 *>(plan.ks), share4 = *reinterpret_cast<const float4 *>(plan.share);
+        const float4 ks = *reinterpret_cast<const float4 *>(plan.ks), exp4 = *reinterpret_cast<const float4 *>(plan.exp);
         // the factors of the groups' scores; not 0, because hidden scores are -infinity
         const float f[4] = {fmaxf(cf * ks.x, FLT_MIN), fmaxf(cf * ks.y, FLT_MIN), fmaxf(cf * ks.z, FLT_MIN),
                             fmaxf(cf * ks.w, FLT_MIN)};
-        const float share[4] = {share4.x, share4.y, share4.z, share4.w};
-        const float new_unit = plan.unit;
+        const float exp[4] = {exp4.x, exp4.y, exp4.z, exp4.w};
         tmem_ready<64>(v);
         if (key0 + BK - 1 > min_pos || (a.window && key0 <= max_pos - a.window && key0 + BK > a.sinks) ||
             present != (1u << NG) - 1) {
@@ -868,13 +861,16 @@ __global__ void __launch_bounds__(THREADS, 1) k_paged_many(const AttnArgs<T> a) 
             m1 = max3(m1, v[16 * g + j], v[16 * g + j + 1]);
             m2 = max3(m2, v[16 * g + j + 2], v[16 * g + j + 3]);
           }
-          mx = fmaxf(mx, fmaxf(m1, m2) * f[g]);
+          mx = fmaxf(mx, fmaf(fmaxf(m1, m2), f[g], exp[g]));
         }
-        // the reference follows the maximum, the unit the block's: earlier results move along
+        // the reference follows the maximum: earlier results move along. A whole number, so that an f32 row's page
+        // exponents are added to it exactly
         float alpha = 1.f;
         if (mx > ref + REF_LAG) {  // also the first key that a row sees: alpha = 0
-          alpha = ex2(ref - mx);
-          ref = mx;
+          const float to = rintf(mx);
+          alpha = ex2(ref - to);
+          l = scaled(l, ref - to);
+          ref = to;
         }
         const float shift = ref == -INFINITY ? 0.f : WEIGHT_EXP - ref;
         // weights, over the scores
@@ -882,15 +878,15 @@ __global__ void __launch_bounds__(THREADS, 1) k_paged_many(const AttnArgs<T> a) 
         uint32_t hi[32], lo[SPLIT ? 32 : 1];
 #pragma unroll
         for (int g = 0; g < NG; g++) {
-          const float sh = SPLIT ? shift : shift + share[g];
-          const f2x f2 = pk2(f[g], f[g]), sh2 = pk2(sh, sh), share2 = pk2(share[g], share[g]);
+          const float sh = shift + exp[g], man = SPLIT ? plan.man[g] : 1.f;
+          const f2x f2 = pk2(f[g], f[g]), sh2 = pk2(sh, sh), man2 = pk2(man, man);
           f2x gs = 0ull;
 #pragma unroll
           for (int j = 0; j < 8; j++) {
             const float2 y = up2(ffma2(pk2(v[16 * g + 2 * j], v[16 * g + 2 * j + 1]), f2, sh2));
             f2x w = pk2(ex2(y.x), ex2(y.y));
             gs = fadd2(gs, w);
-            if constexpr (SPLIT) w = fmul2(w, share2);
+            if constexpr (SPLIT) w = fmul2(w, man2);
             const float2 z = up2(w);
             hi[8 * g + j] = pack(z.x, z.y);
             if constexpr (SPLIT) {
@@ -899,21 +895,18 @@ __global__ void __launch_bounds__(THREADS, 1) k_paged_many(const AttnArgs<T> a) 
             }
           }
           const float2 z = up2(gs);
-          if constexpr (SPLIT) sum += z.x + z.y;
-          else sum = fmaf(z.x + z.y, plan.inv[g], sum);
+          sum = fmaf(z.x + z.y, plan.inv[g], sum);
         }
         tmem_st32(s_col, hi);
         if constexpr (SPLIT) tmem_st32(s_col + 32, lo);
-        l = fmaf(l, alpha, sum);
-        float move = alpha;
-        if (unit != new_unit) move *= new_unit > 0.f ? unit / new_unit : 0.f;
+        l += sum;
         const bool take = SPLIT && i % MOVE == 0;  // the output so far is taken, this block's starts anew
-        const bool any = i && __any_sync(0xffffffffu, move != 1.f);
+        const bool any = i && __any_sync(0xffffffffu, alpha != 1.f);
         if (i && (take || any)) {  // the last block's P V is done before its output is read or moved
           if (!(ok = products_done(t - 1))) break;
           fence_after();
           if (take) {
-            add_output(unit);
+            add_output();
           } else {
 #pragma unroll 1
             for (int d = 0; d < HD; d += 32) {
@@ -922,7 +915,7 @@ __global__ void __launch_bounds__(THREADS, 1) k_paged_many(const AttnArgs<T> a) 
               tmem_ready<32>(y);
               uint32_t u[32];
 #pragma unroll
-              for (int j = 0; j < 32; j++) u[j] = __float_as_uint(y[j] * move);
+              for (int j = 0; j < 32; j++) u[j] = __float_as_uint(y[j] * alpha);
               tmem_st32(o_col + d, u);
             }
           }
@@ -933,7 +926,6 @@ __global__ void __launch_bounds__(THREADS, 1) k_paged_many(const AttnArgs<T> a) 
             }
           }
         }
-        unit = new_unit;
         tmem_wait_st();
         fence_before();
         __syncwarp();
@@ -988,7 +980,7 @@ __global__ void __launch_bounds__(THREADS, 1) k_paged_many(const AttnArgs<T> a) 
           tmem_ld32(o_col + d, v);
           tmem_ready<32>(v);
 #pragma unroll
-          for (int j = 0; j < 32; j++) v[j] = none ? 0.f : v[j] * unit;
+          for (int j = 0; j < 32; j++) v[j] = none ? 0.f : v[j];
           put(d, v);
         }
       }
@@ -1012,7 +1004,7 @@ __global__ void __launch_bounds__(THREADS, 1) k_paged_many(const AttnArgs<T> a) 
           const float at0 = top == -INFINITY ? 0.f : top;
 #pragma unroll 1
           for (int i = 0; i < parts; i++)
-            sum = fmaf(__ldcg(part(i) + (HD + 1) * ROWS), ex2(__ldcg(part(i) + HD * ROWS) - at0), sum);
+            sum += scaled(__ldcg(part(i) + (HD + 1) * ROWS), __ldcg(part(i) + HD * ROWS) - at0);
           const float all_inv = sum == 0.f ? 0.f : 1.f / sum;
 #pragma unroll 1
           for (int d = 0; d < HD; d += 32) {

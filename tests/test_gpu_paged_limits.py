@@ -35,6 +35,42 @@ def test_windows_as_long_as_the_table_and_longer(gpu_lib, window, sinks, kind):
         Setup(22, 2, 64, 16, news, lens).check_attention(heads, kind, window=window, sinks=sinks)
 
 
+BIG = [  # news, lens: rows of the one kernel, of the other, of both
+    [1, 2], [300, 190],
+    [200, 90], [420, 300],
+    [150, 1], [400, 260],
+]
+
+
+@pytest.mark.parametrize("kind", ["f32", "bf16"])
+@pytest.mark.parametrize("hd", [64, 128])
+@pytest.mark.parametrize("ratio", [1e6, 1e10, 1e20])
+@pytest.mark.parametrize("where", [0, 3, 10])
+@pytest.mark.parametrize("news,lens", list(zip(BIG[0::2], BIG[1::2])), ids=str)
+def test_values_beside_far_larger_ones_without_weight(gpu_lib, news, lens, where, ratio, hd, kind):
+    """One page has V scales `ratio` times the others', and keys that every query scores about 290 octaves below the
+    others: the result is that of the small values alone, to the bound that goes by the largest of those."""
+    from sqb200 import paged
+    s = Setup(23, 2, hd, 16, news, lens)
+    s.cache["vs"] /= np.float32(ratio)
+    for b, n in enumerate(lens):
+        s.cache["vs"][s.table[b, where]] *= np.float32(ratio)
+        s.cache["k"][s.table[b, where]] = 1  # -127 in every dimension
+        s.cache["ks"][s.table[b, where]] = 0.05
+    for n, t in (("k", s.dcache.k), ("ks", s.dcache.k_scale), ("vs", s.dcache.v_scale)):
+        t.copy_(dev(s.cache[n]))
+    q = np.full((sum(news), 8 * hd), 4, np.float32)
+    got = paged.attention(s.dcache, s.batch, dev(q).to(KINDS[kind]))
+    torch.cuda.synchronize()
+    paged.status()
+    want, size = P.attention(s.cache, s.q_start, lens, s.table, q, 8)
+    # what the far larger page adds is below 2^-200 of the rest; every row sees another page before or after it
+    size[..., 1] = 127 * 1.5 / 60 / ratio
+    seen = np.concatenate([(np.arange(n - k, n) >= 16) | (where > 0) for k, n in zip(news, lens)])
+    over = np.abs(got.float().cpu().numpy().reshape(want.shape) - want) / (P.bound(want, size, kind))
+    assert over[seen].max() <= 1
+
+
 @pytest.mark.parametrize("what", ["begins_late", "ends_early", "none"])
 @pytest.mark.parametrize("news", [[1, 2, 1], [40, 40, 40]], ids=str)
 def test_rows_of_no_sequence_are_recorded(gpu_lib, news, what):
