@@ -177,7 +177,8 @@ typedef struct {
  * rows out of order or of no sequence, positions outside the rotation table; such entries are skipped,
  * never read through): SQ_OK, SQ_ERR_ARG with a message that says what, or
  * SQ_ERR_TIMEOUT when a bounded wait expired. Call after synchronizing the stream;
- * `clear` != 0 resets the record. */
+ * `clear` != 0 resets the record. After SQ_ERR_TIMEOUT the attention's workspaces that were in
+ * use on the device must be zero-filled again: a block that gave up leaves its counters short. */
 int sq_paged_status(int clear);
 
 /* Rotate and append. k and v rows (n_kv_heads * head_dim elements of dtype SQ_F32 or
@@ -201,7 +202,7 @@ int sq_paged_append(void *stream, const sq_paged_cache *c, const sq_paged_batch 
  * n_heads * head_dim elements of dtype. ws: sq_paged_attention_workspace() bytes of
  * device memory, 256-byte aligned, zero-filled once before its first use and again
  * before it serves another cache shape, n_seqs, max_new or n_heads (its counters' places
- * follow from them); calls that share it must be ordered on the device. SQ_ERR_SHAPE
+ * follow from them), and after SQ_ERR_TIMEOUT from sq_paged_status; calls that share it must be ordered on the device. SQ_ERR_SHAPE
  * also when the step's rows times the page table's positions are too many to count in
  * 31 bits. */
 int sq_paged_attention(void *stream, const sq_paged_cache *c, const sq_paged_batch *b, int dtype,

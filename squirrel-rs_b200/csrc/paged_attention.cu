@@ -789,7 +789,7 @@ cudaError_t attention(cudaStream_t s, const Cache &c, const Batch &b, const void
   const Workspace w = workspace(b, c, n_heads);
   uint8_t *p = (uint8_t *)ws;
   AttnArgs<T> a = {c,      b,     (const T *)q, (T *)out,  qs,      os, n_heads, n_heads / c.kv_heads, scale * LOG2E,
-                   window, sinks, INT32_MAX,    (float *)p, (int *)(p + w.few_count), 0};
+                   window, sinks, INT32_MAX,    (float *)p, (int *)(p + w.few_count), 0, 0};
   if (goes_many(c, b.max_new, a.group)) {
     AttnArgs<T> m = a;
     a.few_rows = m.few_rows = FEW_ROWS;

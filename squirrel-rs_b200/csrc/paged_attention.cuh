@@ -25,6 +25,7 @@ struct AttnArgs {
   float *part;
   int *count;  // blocks that have left their part of a row tile; zero between calls
   int max_row_tiles;
+  int withhold;  // failure-detection tests only: the many-row kernel's first block never gets its first piece
 };
 
 // Places on a line of work. The host refuses calls of LINE_END or more, taking the batch at its word; arrays that give

@@ -40,6 +40,9 @@
 // copies finish, frees its tensor memory and returns.
 #include <cuda.h>
 #include <float.h>
+#include <stdlib.h>
+
+#include <atomic>
 
 #include "ops.cuh"
 #include "paged_attention.cuh"
@@ -470,7 +473,7 @@ __global__ void __launch_bounds__(THREADS, 1) k_paged_many(const AttnArgs<T> a) 
         more = walk.next(a, p);
         if (!more) p.n = -1;
         if (k >= PIECES && !wait(B_DONE + k % PIECES, k / PIECES - 1)) break;  // its place is free
-        if (lane == 0) {
+        if (lane == 0 && !(a.withhold && blockIdx.x == 0 && k == 0)) {
           s_pieces[k % PIECES] = p;
           bar_arrive(bar(B_PIECE + k % PIECES));
         }
@@ -1038,6 +1041,18 @@ __global__ void __launch_bounds__(THREADS, 1) k_paged_many(const AttnArgs<T> a) 
   }
 }
 
+// Failure-detection tests only: SQ_TEST_WITHHOLD_PIECE=n (read at the process's first launch of this kernel) makes its
+// n-th launch leave the first block's first piece unsaid, so that every wait of that block for it expires and the
+// next status check reports a timeout.
+int test_withhold() {
+  static const long n = [] {
+    const char *v = getenv("SQ_TEST_WITHHOLD_PIECE");
+    return v ? strtol(v, nullptr, 10) : 0L;
+  }();
+  static std::atomic<long> launches{0};
+  return n > 0 && ++launches == n ? 1 : 0;
+}
+
 template <class C, typename T>
 cudaError_t launch(cudaStream_t s, AttnArgs<T> &a) {
   static int blocks[64] = {};
@@ -1054,6 +1069,7 @@ cudaError_t launch(cudaStream_t s, AttnArgs<T> &a) {
     blocks[dev] = min(sms, MAX_BLOCKS);
   }
   a.max_row_tiles = many_row_tiles(a.b.max_new, a.group);
+  a.withhold = test_withhold();
   return launch_ex(k_paged_many<C, T>, dim3(blocks[dev]), dim3(THREADS), C::SMEM, s, pdl_enabled(), a);
 }
 

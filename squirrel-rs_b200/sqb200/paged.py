@@ -13,6 +13,7 @@ outside the cache, a length beyond the page table, ...) is recorded on the devic
 status() raises it after a synchronization.
 """
 import ctypes as C
+import weakref
 
 import torch
 
@@ -105,6 +106,9 @@ class PagedCache:
         return cls(*codes, *(torch.zeros((n_pages, n_kv_heads), device=device) for _ in range(2)))
 
 
+_batches = weakref.WeakSet()  # those that hold a workspace
+
+
 class PagedBatch:
     """One step: sequence b has rows q_start[b] .. q_start[b + 1] - 1 of the step's tensors,
     the last of the kv_len[b] positions that it holds with them; page_table [n_seqs,
@@ -140,6 +144,7 @@ class PagedBatch:
                                                            C.byref(size)))
             t = torch.zeros(size.value, dtype=torch.uint8, device=cache.k.device)
             ws = self._workspaces[key] = (t, t.data_ptr(), size.value)
+            _batches.add(self)
         return ws
 
 
@@ -221,5 +226,15 @@ def read(cache, batch, first, count, dtype=torch.float32):
 
 def status(clear=True):
     """sq_paged_status: raise what the kernels found wrong in a batch's arrays (call after
-    synchronizing)."""
-    _check(_fn("sq_paged_status")(int(clear)))
+    synchronizing). After a Timeout the device's workspaces are made as new: a block that
+    gave up leaves its counters short."""
+    try:
+        _check(_fn("sq_paged_status")(int(clear)))
+    except KernelError as e:
+        if e.kind == "Timeout":
+            for batch in list(_batches):
+                for t, _, _ in batch._workspaces.values():
+                    if t.device.index == _device():
+                        t.zero_()
+            torch.cuda.current_stream().synchronize()  # before calls on any stream
+        raise
