@@ -33,12 +33,14 @@ def _child(q, kind):
             got = e.kind
         took = time.monotonic() - t0
         same = []
-        for _ in range(2):  # the same batch and workspace, after the error was cleared
+        fresh = paged.PagedBatch(s.batch.q_start, s.batch.kv_len, s.batch.page_table, 300, 300)
+        for length in (2500, 6000):  # the same batch and workspace; row tiles cut into fewer parts, then as many as before
+            s.batch.kv_len.fill_(length)
             out.zero_()
             paged.attention(s.dcache, s.batch, x, out=out)
+            same.append(bool(torch.equal(out, paged.attention(s.dcache, fresh, x))))
             torch.cuda.synchronize()
             paged.status()
-            same.append(bool(torch.equal(out, first)))
         with torch.cuda.graph(graph):
             paged.attention(s.dcache, s.batch, x, out=out)
         graph.replay()
@@ -64,4 +66,4 @@ def test_an_expired_wait_is_reported_and_the_batch_stays_usable(gpu_lib, kind):
             p.kill()
     assert got == "Timeout", got
     assert 0.5 < took < 60, took
-    assert same == [True, True, True]
+    assert same == [True] * 3
