@@ -116,8 +116,8 @@ class PagedBatch:
     those of pages that no new token sees, are not read). The arrays are int32
     CUDA tensors and are read by the kernels: their contents may change between calls
     within what n_tokens (rows in all) and max_new (most of one sequence) say. The
-    attention's workspace is kept here, so calls with one batch must be ordered on the
-    device."""
+    attention's workspace is kept here from the first call on, so calls with one batch must be
+    ordered on the device (a graph captured before any other call gets workspaces of its own)."""
 
     def __init__(self, q_start, kv_len, page_table, n_tokens, max_new):
         for t in (q_start, kv_len, page_table):
@@ -143,8 +143,10 @@ class PagedBatch:
             _check(lib.load().sq_paged_attention_workspace(C.pointer(cache.desc), C.pointer(self.desc), n_heads,
                                                            C.byref(size)))
             t = torch.zeros(size.value, dtype=torch.uint8, device=cache.k.device)
-            ws = self._workspaces[key] = (t, t.data_ptr(), size.value)
-            _batches.add(self)
+            ws = (t, t.data_ptr(), size.value)
+            if not torch.cuda.is_current_stream_capturing():  # zeros that a graph writes are its own calls' alone
+                self._workspaces[key] = ws
+                _batches.add(self)
         return ws
 
 

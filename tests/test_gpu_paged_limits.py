@@ -98,6 +98,30 @@ def test_rows_of_no_sequence_are_recorded(gpu_lib, news, what):
         paged.status()  # cleared
 
 
+def test_a_batch_first_used_in_a_capture(gpu_lib):
+    """The captured call must not leave the batch a workspace that only its replay fills with zeros."""
+    from sqb200 import paged
+    s = Setup(25, 2, 64, 64, [1, 1], [9000, 7000])
+    q = s.rows(512, "f32")
+    x = dev(q)
+    other = paged.PagedBatch(s.batch.q_start, s.batch.kv_len, s.batch.page_table, 2, 1)
+    want = paged.attention(s.dcache, other, x)
+    torch.cuda.synchronize()
+    dirty, graph = torch.cuda.CUDAGraph(), torch.cuda.CUDAGraph()
+    with torch.cuda.graph(dirty):  # memory that later captures in the same pool are given
+        torch.full((64 << 20,), 255, dtype=torch.uint8, device="cuda")
+    dirty.replay()
+    with torch.cuda.graph(graph, pool=dirty.pool()):
+        out = paged.attention(s.dcache, s.batch, x)
+    torch.cuda.synchronize()
+    assert torch.equal(paged.attention(s.dcache, s.batch, x), want)
+    for _ in range(3):
+        out.zero_()
+        graph.replay()
+        assert torch.equal(out, want)
+    assert torch.equal(paged.attention(s.dcache, s.batch, x), want)
+
+
 @pytest.mark.parametrize("hd,news,n_seqs,pages", [(32, 2048, 4500, 256), (64, 16384, 900, 512)], ids=str)
 def test_sequences_that_claim_the_same_rows_are_recorded(gpu_lib, hd, news, n_seqs, pages):
     """Every other sequence claims all rows and very many keys: together more (row tile, key tile) pairs than 32 bits
