@@ -134,8 +134,11 @@ class PagedBatch:
         self.ref = C.addressof(self.desc)
         self._workspaces = {}
 
-    def workspace(self, cache, n_heads):
-        """(tensor, address, bytes) for attention over caches of this shape."""
+    def workspace(self, cache, n_heads, stream=None):
+        """(tensor, address, bytes, raw stream it was made on) for attention over caches of this
+        shape, on the current stream (whose raw value may be given)."""
+        if stream is None:
+            stream = _raw_stream(_device())
         key = (cache.shape_key, n_heads)
         ws = self._workspaces.get(key)
         if ws is None:
@@ -143,10 +146,12 @@ class PagedBatch:
             _check(lib.load().sq_paged_attention_workspace(C.pointer(cache.desc), C.pointer(self.desc), n_heads,
                                                            C.byref(size)))
             t = torch.zeros(size.value, dtype=torch.uint8, device=cache.k.device)
-            ws = (t, t.data_ptr(), size.value)
+            ws = (t, t.data_ptr(), size.value, stream)
             if not torch.cuda.is_current_stream_capturing():  # zeros that a graph writes are its own calls' alone
                 self._workspaces[key] = ws
                 _batches.add(self)
+        elif ws[3] != stream and not torch.cuda.is_current_stream_capturing():
+            ws[0].record_stream(torch.cuda.current_stream())  # the memory outlives the batch until that stream is done
         return ws
 
 
@@ -200,8 +205,9 @@ def attention(cache, batch, q, window=0, sinks=0, scale=None, out=None):
         op, os_ = _rows(out, n, width, dtype, "out")
     if window > _INT_MAX or sinks > _INT_MAX:
         window, sinks = min(window, _INT_MAX), min(sinks, _INT_MAX)
-    _, ws, ws_bytes = batch.workspace(cache, n_heads)
-    st = _fn("sq_paged_attention")(_raw_stream(_device()), cache.ref, batch.ref, kind, qp, qs, n_heads,
+    stream = _raw_stream(_device())
+    held, ws, ws_bytes, _ = batch.workspace(cache, n_heads, stream)
+    st = _fn("sq_paged_attention")(stream, cache.ref, batch.ref, kind, qp, qs, n_heads,
                                    cache.scale if scale is None else scale, window, sinks, op, os_, ws, ws_bytes)
     if st:
         _check(st)
@@ -235,7 +241,7 @@ def status(clear=True):
     except KernelError as e:
         if e.kind == "Timeout":
             for batch in list(_batches):
-                for t, _, _ in batch._workspaces.values():
+                for t, *_ in batch._workspaces.values():
                     if t.device.index == _device():
                         t.zero_()
             torch.cuda.current_stream().synchronize()  # before calls on any stream

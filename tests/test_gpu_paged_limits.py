@@ -185,3 +185,27 @@ def test_counters_past_32_bits(gpu_lib):
         want, size = P.attention(s.cache, [0, last], [lens], s.table, tail, 32)
         over = np.abs(out[news:].float().cpu().numpy().reshape(want.shape) - want) / P.bound(want, size, "bf16")
         assert over.max() <= 1 and not out[:news].any()
+
+
+def test_the_workspace_outlives_its_batch_on_other_streams(gpu_lib):
+    """A call on another stream than the workspace's, which is still to run when the batch goes: its memory is not given
+    to the first stream's next tensor."""
+    from sqb200 import paged
+    s = Setup(29, 2, 64, 64, [1, 1], [9000, 7000])
+    x = dev(s.rows(512, "f32"))
+    want = paged.attention(s.dcache, s.batch, x)
+    size = s.batch.workspace(s.dcache, 8)[2]
+    torch.cuda.synchronize()
+    for _ in range(3):
+        batch = paged.PagedBatch(s.batch.q_start, s.batch.kv_len, s.batch.page_table, 2, 1)
+        paged.attention(s.dcache, batch, x)
+        side = torch.cuda.Stream()
+        side.wait_stream(torch.cuda.current_stream())
+        with torch.cuda.stream(side):
+            torch.cuda._sleep(100_000_000)  # some 50 ms
+            out = paged.attention(s.dcache, batch, x)
+        del batch
+        other = torch.empty(size, dtype=torch.uint8, device="cuda").fill_(255)
+        side.synchronize()
+        assert torch.equal(out, want)
+        del other
