@@ -179,15 +179,27 @@ def probabilities(logits, temperature):
     return torch.softmax(logits / temperature, -1)
 
 
+def spread(rows, counts):
+    """[n, max(counts), vocab] from rows [sum(counts), vocab] of n sequences, zeros behind the shorter ones."""
+    n, most, vocab = len(counts), max(counts), rows.shape[1]
+    if min(counts) == most:
+        return rows.view(n, most, vocab)
+    out = rows.new_zeros((n * most, vocab))
+    out[[b * most + i for b, c in enumerate(counts) for i in range(c)]] = rows
+    return out.view(n, most, vocab)
+
+
 def generate(model, prompts, max_tokens, draft=4, draft_blocks=1, temperature=1.0, generator=None):
     """max_tokens new tokens of each prompt: in every round the first draft_blocks blocks
-    draft `draft` tokens one after the other, the whole model scores them in one pass, and
-    the accepted ones and one more are kept. With draft=0 a plain batched decode. Returns
-    (token lists, share of drafted tokens accepted)."""
+    draft `draft` tokens one after the other (fewer where a sequence wants fewer), the whole
+    model scores them in one pass, and the accepted ones and one more are kept. A sequence
+    leaves the rounds with its last token, and never holds more than len(prompt) + max_tokens - 1
+    positions. With draft=0 a plain batched decode. Returns (token lists, share of
+    drafted tokens accepted)."""
     seqs = [Sequence(p) for p in prompts]
-    n, vocab = len(seqs), model.config.vocab_size
-    uniform = lambda k: torch.rand(n, k, device=model.device, generator=generator)  # noqa: E731
-    none = torch.zeros((n, 0), dtype=torch.int32, device=model.device)
+    vocab = model.config.vocab_size
+    uniform = lambda n, k: torch.rand(n, k, device=model.device, generator=generator)  # noqa: E731
+    ints = lambda v: torch.tensor(v, dtype=torch.int32, device=model.device)  # noqa: E731
     # the prompts but their last tokens, which every round starts with
     news = [len(s.tokens) - 1 for s in seqs]
     if max(news):
@@ -196,25 +208,35 @@ def generate(model, prompts, max_tokens, draft=4, draft_blocks=1, temperature=1.
             s.held += k
     want = [len(s.tokens) + max_tokens for s in seqs]
     drafted = taken = 0
-    while any(len(s.tokens) < w for s, w in zip(seqs, want)):
+    while True:
+        live = [(s, w - len(s.tokens)) for s, w in zip(seqs, want) if len(s.tokens) < w]
+        if not live:
+            break
+        left = [k for _, k in live]
+        live = [s for s, _ in live]
+        n, most = len(live), [min(draft, k - 1) for k in left]  # one token is drawn after the drafts
         probs = []
-        for i in range(draft):
-            p = probabilities(model.forward(seqs, [i + 1] * n, draft_blocks).view(n, i + 1, vocab)[:, -1:], temperature)
-            _, token = speculative.verify_drafts(p, None, none, uniform(1))  # no draft: drawn from p
-            for s, t in zip(seqs, token[:, 0].tolist()):
+        for i in range(max(most)):
+            on = [s for s, k in zip(live, most) if k > i]
+            p = probabilities(model.forward(on, [i + 1] * len(on), draft_blocks).view(len(on), i + 1, vocab)[:, -1],
+                              temperature)
+            _, token = speculative.verify_drafts(p[:, None], None, ints([[]] * len(on)), uniform(len(on), 1))  # drawn from p
+            for s, t in zip(on, token[:, 0].tolist()):
                 s.tokens.append(t)
-            probs.append(p)
-        target = probabilities(model.forward(seqs, [draft + 1] * n).view(n, draft + 1, vocab), temperature)
-        tokens = torch.tensor([s.tokens[s.held + 1:] for s in seqs], dtype=torch.int32, device=model.device).view(n, draft)
-        accepted, out = speculative.verify_drafts(target, torch.cat(probs, 1) if probs else None, tokens,
-                                                  uniform(draft + 1))
-        for s, k, row in zip(seqs, accepted.tolist(), out.tolist()):
+            probs.append(p.new_zeros((n, vocab)).index_copy_(0, ints([b for b, k in enumerate(most) if k > i]).long(), p)
+                         if len(on) < n else p)
+        target = probabilities(model.forward(live, [k + 1 for k in most]), temperature)
+        tokens = ints([s.tokens[s.held + 1:] + [0] * (max(most) - k) for s, k in zip(live, most)])
+        accepted, out = speculative.verify_drafts(spread(target, [k + 1 for k in most]),
+                                                  torch.stack(probs, 1) if probs else None, tokens,
+                                                  uniform(n, max(most) + 1), ints(most))
+        for s, k, m, row in zip(live, accepted.tolist(), most, out.tolist()):
             s.tokens[s.held + 1:] = row[:k + 1]  # the accepted drafts and the drawn token
             s.held += k + 1
-            drafted, taken = drafted + draft, taken + k
+            drafted, taken = drafted + m, taken + k
     for s in seqs:
         model.release(s)
-    return [s.tokens[:w] for s, w in zip(seqs, want)], taken / max(drafted, 1)
+    return [s.tokens for s in seqs], taken / max(drafted, 1)
 
 
 def main():
