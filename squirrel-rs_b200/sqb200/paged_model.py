@@ -200,42 +200,44 @@ def generate(model, prompts, max_tokens, draft=4, draft_blocks=1, temperature=1.
     vocab = model.config.vocab_size
     uniform = lambda n, k: torch.rand(n, k, device=model.device, generator=generator)  # noqa: E731
     ints = lambda v: torch.tensor(v, dtype=torch.int32, device=model.device)  # noqa: E731
-    # the prompts but their last tokens, which every round starts with
-    news = [len(s.tokens) - 1 for s in seqs]
-    if max(news):
-        model.forward(seqs, news)
-        for s, k in zip(seqs, news):
-            s.held += k
-    want = [len(s.tokens) + max_tokens for s in seqs]
-    drafted = taken = 0
-    while True:
-        live = [(s, w - len(s.tokens)) for s, w in zip(seqs, want) if len(s.tokens) < w]
-        if not live:
-            break
-        left = [k for _, k in live]
-        live = [s for s, _ in live]
-        n, most = len(live), [min(draft, k - 1) for k in left]  # one token is drawn after the drafts
-        probs = []
-        for i in range(max(most)):
-            on = [s for s, k in zip(live, most) if k > i]
-            p = probabilities(model.forward(on, [i + 1] * len(on), draft_blocks).view(len(on), i + 1, vocab)[:, -1],
-                              temperature)
-            _, token = speculative.verify_drafts(p[:, None], None, ints([[]] * len(on)), uniform(len(on), 1))  # drawn from p
-            for s, t in zip(on, token[:, 0].tolist()):
-                s.tokens.append(t)
-            probs.append(p.new_zeros((n, vocab)).index_copy_(0, ints([b for b, k in enumerate(most) if k > i]).long(), p)
-                         if len(on) < n else p)
-        target = probabilities(model.forward(live, [k + 1 for k in most]), temperature)
-        tokens = ints([s.tokens[s.held + 1:] + [0] * (max(most) - k) for s, k in zip(live, most)])
-        accepted, out = speculative.verify_drafts(spread(target, [k + 1 for k in most]),
-                                                  torch.stack(probs, 1) if probs else None, tokens,
-                                                  uniform(n, max(most) + 1), ints(most))
-        for s, k, m, row in zip(live, accepted.tolist(), most, out.tolist()):
-            s.tokens[s.held + 1:] = row[:k + 1]  # the accepted drafts and the drawn token
-            s.held += k + 1
-            drafted, taken = drafted + m, taken + k
-    for s in seqs:
-        model.release(s)
+    try:
+        # the prompts but their last tokens, which every round starts with
+        news = [len(s.tokens) - 1 for s in seqs]
+        if max(news):
+            model.forward(seqs, news)
+            for s, k in zip(seqs, news):
+                s.held += k
+        want = [len(s.tokens) + max_tokens for s in seqs]
+        drafted = taken = 0
+        while True:
+            live = [(s, w - len(s.tokens)) for s, w in zip(seqs, want) if len(s.tokens) < w]
+            if not live:
+                break
+            left = [k for _, k in live]
+            live = [s for s, _ in live]
+            n, most = len(live), [min(draft, k - 1) for k in left]  # one token is drawn after the drafts
+            probs = []
+            for i in range(max(most)):
+                on = [s for s, k in zip(live, most) if k > i]
+                p = probabilities(model.forward(on, [i + 1] * len(on), draft_blocks).view(len(on), i + 1, vocab)[:, -1],
+                                  temperature)
+                _, token = speculative.verify_drafts(p[:, None], None, ints([[]] * len(on)), uniform(len(on), 1))  # drawn from p
+                for s, t in zip(on, token[:, 0].tolist()):
+                    s.tokens.append(t)
+                probs.append(p.new_zeros((n, vocab)).index_copy_(0, ints([b for b, k in enumerate(most) if k > i]).long(), p)
+                             if len(on) < n else p)
+            target = probabilities(model.forward(live, [k + 1 for k in most]), temperature)
+            tokens = ints([s.tokens[s.held + 1:] + [0] * (max(most) - k) for s, k in zip(live, most)])
+            accepted, out = speculative.verify_drafts(spread(target, [k + 1 for k in most]),
+                                                      torch.stack(probs, 1) if probs else None, tokens,
+                                                      uniform(n, max(most) + 1), ints(most))
+            for s, k, m, row in zip(live, accepted.tolist(), most, out.tolist()):
+                s.tokens[s.held + 1:] = row[:k + 1]  # the accepted drafts and the drawn token
+                s.held += k + 1
+                drafted, taken = drafted + m, taken + k
+    finally:
+        for s in seqs:
+            model.release(s)
     return [s.tokens for s in seqs], taken / max(drafted, 1)
 
 

@@ -70,3 +70,25 @@ def test_sequences_that_are_done_leave_the_rounds(world, draft, max_tokens):
             left -= min(draft, left - 1) + 1
         odd = sum(min(draft, left - 1) for left in range(1, max_tokens + 1))
         assert share == pytest.approx(even / (even + odd))
+
+
+@pytest.mark.parametrize("call", [0, 1, 3])
+def test_pages_come_back_from_a_call_that_fails(world, call):
+    """Whatever raises: no page, a drafting pass, a scoring pass."""
+    from sqb200.lib import KernelError
+
+    class Failing(world.Model):
+        def forward(self, *a):
+            out = super().forward(*a)
+            if len(self.rows) > call:
+                raise RuntimeError("as told")
+            return out
+
+    model = Failing(20)
+    with pytest.raises(RuntimeError):
+        world.generate(model, [[2] * 7, [3] * 9], 5, draft=2, temperature=0)
+    assert sorted(model.free) == list(range(20))
+    model = world.Model(3)
+    with pytest.raises(KernelError) as e:
+        world.generate(model, [[2] * 7, [3] * 9], 5, draft=2, temperature=0)
+    assert e.value.kind == "CacheFull" and sorted(model.free) == list(range(3))
