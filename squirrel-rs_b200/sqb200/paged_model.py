@@ -123,6 +123,8 @@ class PagedLlama:
 
     def _step(self, seqs, news):
         """The batch of the next news[i] tokens of each sequence, with pages for them."""
+        if max(s.held + n for s, n in zip(seqs, news)) > self.cos.shape[0]:
+            raise lib.KernelError(19, f"a sequence would pass the rotation table's {self.cos.shape[0]} positions")
         for s, n in zip(seqs, news):
             while len(s.pages) * self.page < s.held + n:
                 if not self.free:
@@ -195,7 +197,8 @@ def generate(model, prompts, max_tokens, draft=4, draft_blocks=1, temperature=1.
     model scores them in one pass, and the accepted ones and one more are kept. A sequence
     leaves the rounds with its last token, and never holds more than len(prompt) + max_tokens - 1
     positions. With draft=0 a plain batched decode. Returns (token lists, share of
-    drafted tokens accepted)."""
+    drafted tokens accepted); raises CacheFull without pages or positions for them, and what
+    the kernels recorded (paged.status)."""
     seqs = [Sequence(p) for p in prompts]
     vocab = model.config.vocab_size
     uniform = lambda n, k: torch.rand(n, k, device=model.device, generator=generator)  # noqa: E731
@@ -235,6 +238,7 @@ def generate(model, prompts, max_tokens, draft=4, draft_blocks=1, temperature=1.
                 s.tokens[s.held + 1:] = row[:k + 1]  # the accepted drafts and the drawn token
                 s.held += k + 1
                 drafted, taken = drafted + m, taken + k
+        paged.status()  # the last round's results are on the host: every kernel of the call has run
     finally:
         for s in seqs:
             model.release(s)

@@ -92,3 +92,27 @@ def test_pages_come_back_from_a_call_that_fails(world, call):
     with pytest.raises(KernelError) as e:
         world.generate(model, [[2] * 7, [3] * 9], 5, draft=2, temperature=0)
     assert e.value.kind == "CacheFull" and sorted(model.free) == list(range(3))
+
+
+def test_positions_past_the_rotation_table_are_an_error(world):
+    """Their keys would be left out of the cache. As many positions as there are is taken."""
+    from sqb200.lib import KernelError
+    out, _ = world.generate(world.Model(20, positions=11), [[2] * 7], 5, draft=3, temperature=0)
+    assert out == [[2] * 12]
+    model = world.Model(20, positions=10)
+    with pytest.raises(KernelError) as e:
+        world.generate(model, [[2] * 7], 5, draft=3, temperature=0)
+    assert e.value.kind == "CacheFull" and "10 positions" in str(e.value) and len(model.free) == 20
+
+
+def test_what_the_kernels_recorded_is_asked_for(world, monkeypatch):
+    from sqb200 import paged
+    world.generate(world.Model(20), [[2] * 7], 5, temperature=0)
+    assert world.calls == ["status"]
+
+    def raises(clear=True):
+        raise RuntimeError("recorded")
+
+    monkeypatch.setattr(paged, "status", raises)
+    with pytest.raises(RuntimeError, match="recorded"):
+        world.generate(world.Model(20), [[2] * 7], 5, temperature=0)
