@@ -198,7 +198,7 @@ def generate(model, prompts, max_tokens, draft=4, draft_blocks=1, temperature=1.
     leaves the rounds with its last token, and never holds more than len(prompt) + max_tokens - 1
     positions. With draft=0 a plain batched decode. Returns (token lists, share of
     drafted tokens accepted); raises CacheFull without pages or positions for them, and what
-    the kernels recorded (paged.status)."""
+    the kernels recorded (paged.status, lib.wait_status)."""
     seqs = [Sequence(p) for p in prompts]
     vocab = model.config.vocab_size
     uniform = lambda n, k: torch.rand(n, k, device=model.device, generator=generator)  # noqa: E731
@@ -238,7 +238,9 @@ def generate(model, prompts, max_tokens, draft=4, draft_blocks=1, temperature=1.
                 s.tokens[s.held + 1:] = row[:k + 1]  # the accepted drafts and the drawn token
                 s.held += k + 1
                 drafted, taken = drafted + m, taken + k
-        paged.status()  # the last round's results are on the host: every kernel of the call has run
+        # the last round's results are on the host: every kernel of the call has run
+        paged.status()
+        lib.wait_status()
     finally:
         for s in seqs:
             model.release(s)

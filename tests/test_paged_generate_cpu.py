@@ -14,7 +14,7 @@ VOCAB = 8
 
 @pytest.fixture
 def world(monkeypatch):
-    from sqb200 import paged, paged_model, speculative
+    from sqb200 import lib, paged, paged_model, speculative
 
     def verify(target, draft, tokens, uniform, n_draft=None):
         n, k = tokens.shape
@@ -26,6 +26,7 @@ def world(monkeypatch):
     monkeypatch.setattr(speculative, "verify_drafts", verify)
     monkeypatch.setattr(paged, "PagedBatch", lambda *a: a)
     monkeypatch.setattr(paged, "status", lambda clear=True: calls.append("status"))
+    monkeypatch.setattr(lib, "wait_status", lambda clear=True: calls.append("wait_status"))
 
     class Model(paged_model.PagedLlama):
         """The next token is the same again; drafting says so of even tokens alone."""
@@ -108,7 +109,7 @@ def test_positions_past_the_rotation_table_are_an_error(world):
 def test_what_the_kernels_recorded_is_asked_for(world, monkeypatch):
     from sqb200 import paged
     world.generate(world.Model(20), [[2] * 7], 5, temperature=0)
-    assert world.calls == ["status"]
+    assert world.calls == ["status", "wait_status"]
 
     def raises(clear=True):
         raise RuntimeError("recorded")
