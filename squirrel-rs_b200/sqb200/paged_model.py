@@ -200,13 +200,15 @@ def generate(model, prompts, max_tokens, draft=4, draft_blocks=1, temperature=1.
     drafted tokens accepted); raises CacheFull without pages or positions for them, and what
     the kernels recorded (paged.status, lib.wait_status)."""
     seqs = [Sequence(p) for p in prompts]
+    if not all(s.tokens for s in seqs):
+        raise lib.KernelError(3, "a prompt without tokens")
     vocab = model.config.vocab_size
     uniform = lambda n, k: torch.rand(n, k, device=model.device, generator=generator)  # noqa: E731
     ints = lambda v: torch.tensor(v, dtype=torch.int32, device=model.device)  # noqa: E731
     try:
         # the prompts but their last tokens, which every round starts with
         news = [len(s.tokens) - 1 for s in seqs]
-        if max(news):
+        if max(news, default=0):
             model.forward(seqs, news)
             for s, k in zip(seqs, news):
                 s.held += k

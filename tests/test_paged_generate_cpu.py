@@ -117,3 +117,12 @@ def test_what_the_kernels_recorded_is_asked_for(world, monkeypatch):
     monkeypatch.setattr(paged, "status", raises)
     with pytest.raises(RuntimeError, match="recorded"):
         world.generate(world.Model(20), [[2] * 7], 5, temperature=0)
+
+
+def test_empty_prompts_are_refused_and_no_prompts_are_none(world):
+    from sqb200.lib import KernelError
+    model = world.Model(20)
+    with pytest.raises(KernelError) as e:
+        world.generate(model, [[2, 2], []], 5, temperature=0)
+    assert e.value.kind == "EmptyInput" and len(model.free) == 20 and not model.rows
+    assert world.generate(model, [], 5, temperature=0) == ([], 0)
