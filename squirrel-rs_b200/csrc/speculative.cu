@@ -243,7 +243,8 @@ extern "C" int sq_verify_drafts(void *stream, const float *target, long long tar
                                 long long draft_stride, const int32_t *tokens, const int32_t *n_draft,
                                 const float *uniform, int n_seqs, int max_draft, int vocab, int32_t *n_accepted,
                                 int32_t *out_tokens) {
-  if (!target || !uniform || !n_accepted || !out_tokens || (max_draft > 0 && !tokens))
+  // without sequences the arrays are empty, and an empty array may have no address
+  if (n_seqs && (!target || !uniform || !n_accepted || !out_tokens || (max_draft > 0 && !tokens)))
     return fail(SQ_ERR_ARG, "verify_drafts: null pointer");
   if (n_seqs < 0 || n_seqs > INT32_MAX / VERIFY_CLUSTER || max_draft < 0 || max_draft == INT32_MAX || vocab <= 0 ||
       vocab > INT32_MAX - 4096)

@@ -42,3 +42,13 @@ def test_verify_small_vocabularies(gpu_lib, vocab):
         got_acc, got = speculative.verify_drafts(*args)
         np.testing.assert_array_equal(got_acc.cpu().numpy(), acc)
         np.testing.assert_array_equal(got.cpu().numpy(), out)
+
+
+@pytest.mark.parametrize("k", [0, 3])
+def test_verify_no_sequences(gpu_lib, k):
+    from sqb200 import speculative
+    z = lambda *s, **kw: torch.zeros(s, device="cuda", **kw)  # noqa: E731
+    for draft in (None, z(0, k, 50)):
+        acc, out = speculative.verify_drafts(z(0, k + 1, 50), draft, z(0, k, dtype=torch.int32), z(0, k + 1),
+                                             z(0, dtype=torch.int32))
+        assert acc.shape == (0,) and out.shape == (0, k + 1)

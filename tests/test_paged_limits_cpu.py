@@ -1,7 +1,7 @@
 """Refusals at the limits of what the paged cache's entry points count with, from the host's checks."""
 import pytest
 
-from test_paged_cpu import append, attention, read
+from test_paged_cpu import append, attention, read, verify
 
 
 @pytest.mark.parametrize("call", [append, attention, read])
@@ -14,3 +14,9 @@ def test_page_tables_of_more_than_a_billion_positions(call, page, pages):
     assert call(cache=dict(page=page), batch=dict(empty, pages_per_seq=pages), **nothing) == "Ok"
     assert call(cache=dict(page=page), batch=dict(empty, pages_per_seq=pages + 1), **nothing) == "ShapeMismatch"
     assert call(cache=dict(page=page), batch=dict(pages_per_seq=2**31 - 1)) == "ShapeMismatch"
+
+
+def test_no_sequences_need_no_arrays():
+    assert verify(seqs=0, target=None, draft=None, ds=0, tokens=None, u=None, acc=None, out=None) == "Ok"
+    assert verify(seqs=0, target=None, vocab=0) == "ShapeMismatch"
+    assert verify(seqs=1, u=None) == "InvalidArgument"
