@@ -63,10 +63,11 @@ _entries = {}
 
 
 def _bind(name):
-    """The library's entry point `name`: structs are passed as addresses, and the interpreter
-    lock is kept, for the calls only queue work."""
+    """The library's entry point `name`: structs are passed as addresses. The interpreter lock is
+    given up meanwhile: a status copy, or a launch into a full queue, waits for the GPU
+    (0.1 us a call: append_one's two calls 19.6 with the lock kept, 19.75 us)."""
     lib.load()
-    f = getattr(C.PyDLL(lib.LIB_PATH), name)
+    f = getattr(C.CDLL(lib.LIB_PATH), name)
     f.restype, types = lib.SIGNATURES[name]
     f.argtypes = [C.c_void_p if issubclass(t, C._Pointer) else t for t in types]
     _entries[name] = f
