@@ -37,9 +37,9 @@ def _kind(t):
     return kind
 
 
-def _rows(t, rows, width, dtype, what):
-    """Address and row stride of a [rows, width] tensor of dtype whose rows may be a slice of
-    wider ones."""
+def _rows(t, rows, width, dtype, device, what):
+    """Address and row stride of a [rows, width] tensor of dtype on the device whose rows may be
+    a slice of wider ones."""
     if t.dtype is not dtype:
         raise KernelError(_TYPE, f"{what}: {dtype} is wanted")
     if t.shape != (rows, width):
@@ -47,9 +47,17 @@ def _rows(t, rows, width, dtype, what):
     stride, step = t.stride()
     if step != 1 and width > 1:
         raise KernelError(_SHAPE, f"{what}: a row's elements must be consecutive")
-    if not t.is_cuda:
-        raise KernelError(_ARG, f"{what}: a CUDA tensor is wanted")
+    if t.get_device() != device:
+        raise KernelError(_ARG, f"{what}: a CUDA tensor of the current device is wanted")
     return t.data_ptr(), stride if rows > 1 else width  # one row: its stride says nothing
+
+
+def _device_of(cache, batch):
+    """The current device, which has to be the cache's and the batch's."""
+    device = _device()
+    if cache.device != device or batch.device != device:
+        raise KernelError(_ARG, "cache and batch have to be on the current CUDA device")
+    return device
 
 
 # The smallest calls take a few microseconds of GPU time, so the binding spends as little as
@@ -93,6 +101,7 @@ class PagedCache:
         _need(all(t.is_cuda and t.device == k.device for t in (k, v, k_scale, v_scale)), _ARG,
               "a cache is CUDA tensors of one device")
         self.k, self.v, self.k_scale, self.v_scale = k, v, k_scale, v_scale
+        self.device = k.get_device()
         self.n_pages, self.n_kv_heads, self.page, self.head_dim = k.shape
         self.shape_key = (self.n_kv_heads, self.page, self.head_dim)
         self.row, self.half, self.scale = self.n_kv_heads * self.head_dim, self.head_dim // 2, self.head_dim ** -0.5
@@ -124,11 +133,11 @@ class PagedBatch:
         for t in (q_start, kv_len, page_table):
             _need(t.dtype == torch.int32, _TYPE, "batch arrays are int32")
             _need(t.is_contiguous(), _SHAPE, "batch arrays are contiguous")
-            _need(t.is_cuda, _ARG, "batch arrays are CUDA tensors")
+            _need(t.is_cuda and t.device == q_start.device, _ARG, "batch arrays are CUDA tensors of one device")
         _need(page_table.dim() == 2 and kv_len.shape == page_table.shape[:1] and
               q_start.shape == (kv_len.shape[0] + 1,), _SHAPE,
               "q_start [n_seqs + 1], kv_len [n_seqs], page_table [n_seqs, pages_per_seq]")
-        self.q_start, self.kv_len, self.page_table = q_start, kv_len, page_table
+        self.q_start, self.kv_len, self.page_table, self.device = q_start, kv_len, page_table, q_start.get_device()
         self.n_seqs, self.n_tokens, self.max_new = kv_len.shape[0], n_tokens, max_new
         self.desc = lib.PagedBatchDesc(q_start.data_ptr(), kv_len.data_ptr(), page_table.data_ptr(), self.n_seqs,
                                        n_tokens, max_new, page_table.shape[1])
@@ -160,13 +169,14 @@ def append(cache, batch, k, v, cos, sin, q=None, q_out=None):
     """Rotate k [n_tokens, n_kv_heads * head_dim] to its positions and store it and v in the
     pages; rotate q [n_tokens, n_heads * head_dim], if given, and return it (in q_out, which
     may be q, or a new tensor). cos, sin: [positions, head_dim / 2] float32."""
-    n, width, dtype = batch.n_tokens, cache.row, k.dtype
+    n, width, dtype, device = batch.n_tokens, cache.row, k.dtype, _device_of(cache, batch)
     kind = _kind(k)
-    kp, ks = _rows(k, n, width, dtype, "k")
-    vp, vs = _rows(v, n, width, dtype, "v")
+    kp, ks = _rows(k, n, width, dtype, device, "k")
+    vp, vs = _rows(v, n, width, dtype, device, "v")
     positions = cos.shape[0]
     for t in (cos, sin):
-        if t.shape != (positions, cache.half) or t.dtype is not torch.float32 or not t.is_contiguous() or not t.is_cuda:
+        if (t.shape != (positions, cache.half) or t.dtype is not torch.float32 or not t.is_contiguous() or
+                t.get_device() != device):
             raise KernelError(_SHAPE, "rotation tables are contiguous float32 [positions, head_dim / 2] on the GPU")
     qp = qop = None
     qs = qos = n_heads = 0
@@ -175,13 +185,13 @@ def append(cache, batch, k, v, cos, sin, q=None, q_out=None):
         n_heads = q_width // cache.head_dim
         if n_heads * cache.head_dim != q_width or not n_heads:
             raise KernelError(_SHAPE, "q: rows of whole heads are wanted")
-        qp, qs = _rows(q, n, q_width, dtype, "q")
+        qp, qs = _rows(q, n, q_width, dtype, device, "q")
         if q_out is None:
             q_out = torch.empty_like(q)
             qop, qos = q_out.data_ptr(), q_width
         else:
-            qop, qos = _rows(q_out, n, q_width, dtype, "q_out")
-    st = _fn("sq_paged_append")(_raw_stream(_device()), cache.ref, batch.ref, kind, kp, ks, vp, vs, cos.data_ptr(),
+            qop, qos = _rows(q_out, n, q_width, dtype, device, "q_out")
+    st = _fn("sq_paged_append")(_raw_stream(device), cache.ref, batch.ref, kind, kp, ks, vp, vs, cos.data_ptr(),
                                 sin.data_ptr(), positions, qp, qs, n_heads, qop, qos)
     if st:
         _check(st)
@@ -192,21 +202,21 @@ def attention(cache, batch, q, window=0, sinks=0, scale=None, out=None):
     """Causal grouped attention of q [n_tokens, n_heads * head_dim] over the cache: the query
     at position p sees the positions <= p, with window > 0 only the last `window` of them
     and the first `sinks` ones. scale: head_dim ** -0.5 unless given."""
-    n, dtype = batch.n_tokens, q.dtype
+    n, dtype, device = batch.n_tokens, q.dtype, _device_of(cache, batch)
     width = q.shape[1] if q.dim() == 2 else 0
     n_heads = width // cache.head_dim
     if n_heads * cache.head_dim != width or not n_heads:
         raise KernelError(_SHAPE, "q: rows of whole heads are wanted")
     kind = _kind(q)
-    qp, qs = _rows(q, n, width, dtype, "q")
+    qp, qs = _rows(q, n, width, dtype, device, "q")
     if out is None:
         out = torch.empty_like(q)
         op, os_ = out.data_ptr(), width
     else:
-        op, os_ = _rows(out, n, width, dtype, "out")
+        op, os_ = _rows(out, n, width, dtype, device, "out")
     if window > _INT_MAX or sinks > _INT_MAX:
         window, sinks = min(window, _INT_MAX), min(sinks, _INT_MAX)
-    stream = _raw_stream(_device())
+    stream = _raw_stream(device)
     held, ws, ws_bytes, _ = batch.workspace(cache, n_heads, stream)
     st = _fn("sq_paged_attention")(stream, cache.ref, batch.ref, kind, qp, qs, n_heads,
                                    cache.scale if scale is None else scale, window, sinks, op, os_, ws, ws_bytes)
@@ -218,15 +228,16 @@ def attention(cache, batch, q, window=0, sinks=0, scale=None, out=None):
 def read(cache, batch, first, count, dtype=torch.float32):
     """The values of `count` positions of each sequence from first[b] (int32 CUDA tensor) on:
     k, v [n_seqs, count, n_kv_heads * head_dim], zeros past kv_len[b]."""
-    n = batch.n_seqs
-    if first.shape != (n,) or first.dtype is not torch.int32 or not first.is_cuda or not first.is_contiguous():
+    n, device = batch.n_seqs, _device_of(cache, batch)
+    if (first.shape != (n,) or first.dtype is not torch.int32 or first.get_device() != device or
+            not first.is_contiguous()):
         raise KernelError(_SHAPE, "first: one int32 position of each sequence on the GPU")
     kind = _KINDS.get(dtype)
     if kind is None:
         raise KernelError(_TYPE, "values are read as float32 or bfloat16")
     k = cache.like[dtype].new_empty((n, count, cache.row))
     v = torch.empty_like(k)
-    st = _fn("sq_paged_read")(_raw_stream(_device()), cache.ref, batch.ref, first.data_ptr(), count, kind,
+    st = _fn("sq_paged_read")(_raw_stream(device), cache.ref, batch.ref, first.data_ptr(), count, kind,
                               k.data_ptr(), v.data_ptr())
     if st:
         _check(st)

@@ -9,17 +9,17 @@ from .paged import _device, _fn, _raw_stream
 _SHAPE, _TYPE, _ARG = 1, 2, 5
 
 
-def _array(t, shape, dtype, what):
+def _array(t, shape, dtype, device, what):
     if t.shape != shape or not t.is_contiguous():
         raise KernelError(_SHAPE, f"{what}: a contiguous {shape} tensor is wanted")
     if t.dtype is not dtype:
         raise KernelError(_TYPE, f"{what}: {dtype} is wanted")
-    if not t.is_cuda:
-        raise KernelError(_ARG, f"{what}: a CUDA tensor is wanted")
+    if t.get_device() != device:
+        raise KernelError(_ARG, f"{what}: a CUDA tensor of the current device is wanted")
     return t.data_ptr()
 
 
-def _probs(t, n, rows, vocab, what):
+def _probs(t, n, rows, vocab, device, what):
     """Address and row stride of [n, rows, vocab] float32 whose rows lie one stride apart (a slice
     of wider rows or of more of them). Broadcast or overlapping rows are refused: the kernel
     would read past the end of them."""
@@ -36,8 +36,8 @@ def _probs(t, n, rows, vocab, what):
         raise KernelError(_SHAPE, f"{what}: a row's elements must be consecutive")
     if t.dtype is not torch.float32:
         raise KernelError(_TYPE, f"{what}: probabilities are float32")
-    if not t.is_cuda:
-        raise KernelError(_ARG, f"{what}: a CUDA tensor is wanted")
+    if t.get_device() != device:
+        raise KernelError(_ARG, f"{what}: a CUDA tensor of the current device is wanted")
     return t.data_ptr(), stride
 
 
@@ -50,14 +50,14 @@ def verify_drafts(target, draft, tokens, uniform, n_draft=None):
     if tokens.dim() != 2 or target.dim() != 3:
         raise KernelError(_SHAPE, "tokens are [n, K], target is [n, K + 1, vocab]")
     n, k = tokens.shape
-    vocab = target.shape[2]
-    tp, ts = _probs(target, n, k + 1, vocab, "target")
-    dp, ds = _probs(draft, n, k, vocab, "draft") if draft is not None else (None, 0)
+    vocab, device = target.shape[2], _device()
+    tp, ts = _probs(target, n, k + 1, vocab, device, "target")
+    dp, ds = _probs(draft, n, k, vocab, device, "draft") if draft is not None else (None, 0)
     accepted, out = tokens.new_empty(n), tokens.new_empty((n, k + 1))
     st = _fn("sq_verify_drafts")(
-        _raw_stream(_device()), tp, ts, dp, ds, _array(tokens, (n, k), torch.int32, "tokens"),
-        _array(n_draft, (n,), torch.int32, "n_draft") if n_draft is not None else None,
-        _array(uniform, (n, k + 1), torch.float32, "uniform"), n, k, vocab, accepted.data_ptr(), out.data_ptr())
+        _raw_stream(device), tp, ts, dp, ds, _array(tokens, (n, k), torch.int32, device, "tokens"),
+        _array(n_draft, (n,), torch.int32, device, "n_draft") if n_draft is not None else None,
+        _array(uniform, (n, k + 1), torch.float32, device, "uniform"), n, k, vocab, accepted.data_ptr(), out.data_ptr())
     if st:
         _check(st)
     return accepted, out

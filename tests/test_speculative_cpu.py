@@ -14,7 +14,7 @@ def outcome(t, n, rows, vocab):
     from sqb200 import speculative
     from sqb200.lib import KernelError
     with pytest.raises(KernelError) as e:
-        speculative._probs(t, n, rows, vocab, "draft")
+        speculative._probs(t, n, rows, vocab, 0, "draft")
     return "taken" if "CUDA tensor" in str(e.value) else (e.value.kind, str(e.value))
 
 
