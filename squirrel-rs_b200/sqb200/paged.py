@@ -232,6 +232,8 @@ def read(cache, batch, first, count, dtype=torch.float32):
     if (first.shape != (n,) or first.dtype is not torch.int32 or first.get_device() != device or
             not first.is_contiguous()):
         raise KernelError(_SHAPE, "first: one int32 position of each sequence on the GPU")
+    if not 0 <= count <= _INT_MAX:
+        raise KernelError(_SHAPE, "count: 0 to 2^31 - 1 positions")
     kind = _KINDS.get(dtype)
     if kind is None:
         raise KernelError(_TYPE, "values are read as float32 or bfloat16")

@@ -61,3 +61,13 @@ def test_tensors_of_another_device_are_refused(monkeypatch):
     assert refused(paged.read, *world(0, 0), Elsewhere(2, dtype=torch.int32), 4)[0] == "ShapeMismatch"
     args = [Elsewhere(2, 4, 50), None, Elsewhere(2, 3, dtype=torch.int32), Elsewhere(2, 4)]
     assert refused(speculative.verify_drafts, *args)[0] == "InvalidArgument"
+
+
+@pytest.mark.parametrize("count", [-1, 2**31])
+def test_read_refuses_counts_out_of_range(monkeypatch, count):
+    from sqb200 import paged
+    monkeypatch.setattr(paged, "_device", lambda: 1)
+    first = Elsewhere(2, dtype=torch.int32)
+    world = SimpleNamespace(device=1, row=128, half=32, head_dim=64, like={torch.float32: torch.zeros(0)}), SimpleNamespace(
+        device=1, n_tokens=3, n_seqs=2)
+    assert refused(paged.read, *world, first, count)[0] == "ShapeMismatch"
