@@ -340,7 +340,7 @@ __global__ void __launch_bounds__(THREADS, C::BLOCKS) k_paged_few(const AttnArgs
     }
     // ---- query fragments (the first tiles are on their way): column g of tile nt = row 8 nt + g
     uint32_t qf[NT][KS][TERMS][2];
-    float cf[NT][2], cb[NT][2];  // factor and offset of the scores of the lane's columns 2t, 2t + 1
+    float cf[NT][2], cb[NT][2];  // factor of the scores of the lane's columns 2t, 2t + 1, offset before it
     int pos[NT][2];              // and their rows' positions (-1: no such row)
     float4 qx[NT][KS];           // the lane's dimensions: 16 consecutive ones of each 64 (8 of 32)
 #pragma unroll
@@ -392,8 +392,8 @@ __global__ void __launch_bounds__(THREADS, C::BLOCKS) k_paged_few(const AttnArgs
       for (int j = 0; j < 2; j++) {  // row 2t + j is held by the lanes of g = 2t + j
         const int from = (2 * t + j) * 4;
         const float d = __shfl_sync(0xffffffffu, down, from), q = __shfl_sync(0xffffffffu, sum, from);
-        cf[nt][j] = SPLIT ? d : d * 16777216.f;
-        cb[nt][j] = SPLIT ? 0.f : -128.f * q * d;
+        cf[nt][j] = d;
+        cb[nt][j] = SPLIT ? 0.f : -128.f * q;
         pos[nt][j] = __shfl_sync(0xffffffffu, ok ? pos0 + tok : -1, from);
       }
     }
@@ -461,8 +461,9 @@ __global__ void __launch_bounds__(THREADS, C::BLOCKS) k_paged_few(const AttnArgs
         const float e = (float)(127 - (int)(__float_as_uint(g_inv[j]) >> 23));
 #pragma unroll
         for (int nt = 0; nt < NT; nt++) {
-          const float f0 = cf[nt][0] * gks, f1 = cf[nt][1] * gks;
-          const float b0 = SPLIT ? e : fmaf(cb[nt][0], gks, e), b1 = SPLIT ? e : fmaf(cb[nt][1], gks, e);
+          float f0 = cf[nt][0] * gks, f1 = cf[nt][1] * gks;
+          const float b0 = SPLIT ? e : fmaf(cb[nt][0], f0, e), b1 = SPLIT ? e : fmaf(cb[nt][1], f1, e);
+          if (!SPLIT) f0 *= 16777216.f, f1 *= 16777216.f;  // after the K scale: large rows have finite scores too
 #pragma unroll
           for (int x = 0; x < 4; x++) sc[j][nt][x] = fmaf(sc[j][nt][x], x & 1 ? f1 : f0, x & 1 ? b1 : b0);
         }

@@ -209,3 +209,29 @@ def test_the_workspace_outlives_its_batch_on_other_streams(gpu_lib):
         side.synchronize()
         assert torch.equal(out, want)
         del other
+
+
+@pytest.mark.parametrize("kind", ["f32", "bf16"])
+@pytest.mark.parametrize("news", [3])
+@pytest.mark.parametrize("power", [-120, -60, 14, 16, 18, 20, 24, 34, 90, 114, 118, 120])
+def test_query_rows_of_any_size(gpu_lib, power, news, kind):
+    """Rows of 2^power in one dimension, K scales of 2^-7: scores of about 2^(power - 3). Large rows leave the key with the
+    largest code there all the weight, tiny ones weight all keys alike."""
+    from sqb200 import paged
+    s = Setup(30, 2, 64, 16, [news], [200])
+    s.cache["ks"][:] = 2.0**-7
+    s.cache["k"][:, :, :, 5] = 100 + s.rng.integers(0, 2, s.cache["k"].shape[:3])
+    best = s.rng.integers(0, 200 - news, 2)
+    for g in range(2):
+        s.cache["k"][s.table[0, best[g] // 16], g, best[g] % 16, 5] = 102
+    for n, t in (("k", s.dcache.k), ("ks", s.dcache.k_scale)):
+        t.copy_(dev(s.cache[n]))
+    q = np.zeros((news, 8, 64), np.float32)
+    q[:, :, 5] = 2.0**power
+    got = paged.attention(s.dcache, s.batch, dev(q.reshape(news, 512)).to(KINDS[kind])).float().cpu().numpy()
+    paged.status()
+    want, size = P.attention(s.cache, s.q_start, s.lens, s.table, q.reshape(news, 512), 8)
+    if power > 0:
+        size[..., 0] = 0  # the other keys' weights are below 2^-20: an error of scores moves nothing
+    over = np.abs(got.reshape(q.shape) - want) / P.bound(want, size, kind)
+    assert over.max() <= 1
