@@ -67,7 +67,7 @@ constexpr int MAX_BLOCKS = 160;
 constexpr int TILE_COST = 5;
 constexpr int MIN_BLOCKS = 2;  // key blocks a thread block takes at least
 constexpr int MOVE = 4;        // f32 rows: blocks of keys summed in tensor memory at a stretch
-constexpr float WEIGHT_EXP = 3.f, REF_LAG = 6.f;
+constexpr float WEIGHT_EXP = 3.f, REF_LAG = 6.f, LARGE_SCORE = 4194304.f;
 // Registers a thread: launched with 128 (512 x 128 = 65,536), then 256 x 184 + 128 x 80 + 128 x 64.
 constexpr int SOFTMAX_REGS = 184, LOAD_REGS = 80, MMA_REGS = 64;
 
@@ -834,9 +834,9 @@ __global__ void __launch_bounds__(THREADS, 1) k_paged_many(const AttnArgs<T> a) 
         const uint32_t present = plan.present;
         const float4 ks = *reinterpret_cast<const float4 *>(plan.ks), exp4 = *reinterpret_cast<const float4 *>(plan.exp);
         // the factors of the groups' scores; not 0, because hidden scores are -infinity
-        const float f[4] = {fmaxf(cf * ks.x, FLT_MIN), fmaxf(cf * ks.y, FLT_MIN), fmaxf(cf * ks.z, FLT_MIN),
+        float f[4] = {fmaxf(cf * ks.x, FLT_MIN), fmaxf(cf * ks.y, FLT_MIN), fmaxf(cf * ks.z, FLT_MIN),
                             fmaxf(cf * ks.w, FLT_MIN)};
-        const float exp[4] = {exp4.x, exp4.y, exp4.z, exp4.w};
+        float exp[4] = {exp4.x, exp4.y, exp4.z, exp4.w};
         tmem_ready<64>(v);
         if (key0 + BK - 1 > min_pos || (a.window && key0 <= max_pos - a.window && key0 + BK > a.sinks) ||
             present != (1u << NG) - 1) {
@@ -876,6 +876,16 @@ __global__ void __launch_bounds__(THREADS, 1) k_paged_many(const AttnArgs<T> a) 
           ref = to;
         }
         const float shift = ref == -INFINITY ? 0.f : WEIGHT_EXP - ref;
+        // The reference is a rounded score. Where a score's rounding is some octaves, they are all rounded before it is
+        // taken off, or the largest weights would be off by as many.
+        if (__any_sync(0xffffffffu, fabsf(shift) > LARGE_SCORE)) {
+#pragma unroll
+          for (int g = 0; g < NG; g++) {
+#pragma unroll
+            for (int j = 16 * g; j < 16 * g + 16; j++) v[j] = fmaf(v[j], f[g], exp[g]);
+            f[g] = 1.f, exp[g] = 0.f;
+          }
+        }
         // weights, over the scores
         float sum = 0.f;
         uint32_t hi[32], lo[SPLIT ? 32 : 1];

@@ -212,7 +212,7 @@ def test_the_workspace_outlives_its_batch_on_other_streams(gpu_lib):
 
 
 @pytest.mark.parametrize("kind", ["f32", "bf16"])
-@pytest.mark.parametrize("news", [3])
+@pytest.mark.parametrize("news", [3, 100])
 @pytest.mark.parametrize("power", [-120, -60, 14, 16, 18, 20, 24, 34, 90, 114, 118, 120])
 def test_query_rows_of_any_size(gpu_lib, power, news, kind):
     """Rows of 2^power in one dimension, K scales of 2^-7: scores of about 2^(power - 3). Large rows leave the key with the
