@@ -162,7 +162,7 @@ typedef struct {
  * the page of each `page` positions; entries past kv_len, and with a window those of pages
  * that no new token sees, are not read (such pages may be given away). The arrays are
  * device memory and are read by the kernels (a captured graph replays with new
- * contents); n_tokens and max_new bound what they may say. */
+ * contents, of as many rows in all and at most max_new a sequence). */
 typedef struct {
     const int32_t *q_start;    /* [n_seqs + 1], ascending from 0 to n_tokens */
     const int32_t *kv_len;     /* [n_seqs] */
@@ -197,14 +197,16 @@ int sq_paged_append(void *stream, const sq_paged_cache *c, const sq_paged_batch 
 
 /* Causal grouped attention of the new tokens over the cache (the step appended before):
  * head h reads kv head h / (n_heads / n_kv_heads); the query at position p sees the
- * positions <= p, with window > 0 only those > p - window and the first `sinks` ones.
+ * positions <= p, with window > 0 only those > p - window and the first `sinks` ones (a
+ * window of pages_per_seq * page or more hides nothing).
  * out = softmax(scale * q.k) v; a query that sees nothing gets zeros. q, out: rows of
  * n_heads * head_dim elements of dtype. ws: sq_paged_attention_workspace() bytes of
  * device memory, 256-byte aligned, zero-filled once before its first use and again
  * before it serves another cache shape, n_seqs, max_new or n_heads (its counters' places
- * follow from them), and after SQ_ERR_TIMEOUT from sq_paged_status; calls that share it must be ordered on the device. SQ_ERR_SHAPE
- * also when the step's rows times the page table's positions are too many to count in
- * 31 bits. */
+ * follow from them), and after SQ_ERR_TIMEOUT from sq_paged_status; calls that share it must
+ * be ordered on the device. V scales below 2^-80, or below 2^-80 of the largest met, lose bits
+ * and then count as none. SQ_ERR_SHAPE also when the step's row tiles and the page table's
+ * positions make more than 2^30 pairs of tiles. */
 int sq_paged_attention(void *stream, const sq_paged_cache *c, const sq_paged_batch *b, int dtype,
                        const void *q, long long q_stride, int n_heads, float scale, int window, int sinks,
                        void *out, long long out_stride, void *ws, size_t ws_bytes);

@@ -79,10 +79,11 @@ int check_rows(const void *p, long long stride, long long width, int dtype, cons
 
 namespace {
 
-// Append moves 2 x (4 or 2) + 1 bytes an element and is bound by that. Threads take eight
+// Append moves 2 x (4 or 2) bytes an element of q, (4 or 2) + 1 of k and v. Threads take eight
 // elements (16 or 32 bytes) at a time; a page block keeps HELD such chunks a thread in
-// registers from the maximum to the codes, so that rows are read once (read twice, in
-// chunks of four: 64 x 64 bf16 pages 34.1 us for 18,000 tokens, 2.2 TB/s).
+// registers from the maximum to the codes, so that rows are read once. 24,465 tokens of 32
+// and 8 heads of 64: f32 85.5 us, 6.2 TB/s, bound by that; bf16 85.8 us, 3.3 TB/s, bound by the
+// instructions an element (rotation, maximum, rounding to a code), which are the same.
 constexpr int HELD = 4;
 constexpr int Q_CHUNKS = 4;  // chunks a thread of a query block takes
 

@@ -28,7 +28,7 @@
 // step on average): the scores of the query's two terms are summed apart, and f32 rows
 // move their output sums every 8 groups of keys to f32 sums in shared memory. Measured
 // with 4 x 131,072 positions of f32 rows: the bias taken off afterwards and one sum 66 us, error
-// 1.4e-6 of the result; as it is 69.4 us, 8.4e-7; sums moved every 16 groups 68.7 us, 1.0e-6
+// 1.4e-6 of the result; as it is 69 us, 8.2e-7; sums moved every 16 groups 0.7 us less, 1.0e-6
 // (1,001 positions: 5.5e-7 and 8.1e-7, the plain f32 form 9.1e-7).
 //
 // Work is split evenly over the grid: the (sequence, kv head, row tile, key tile) space is
@@ -747,7 +747,7 @@ cudaError_t launch_few(cudaStream_t s, AttnArgs<T> &a) {
 
 // Query rows a kv head. A call of up to ALONE_ROWS is this kernel's: 12 x up to 4,096 positions, this one / the other at
 // 72 rows: f32 58 / 65 us (64 dimensions), 86 / 105 us (128), bf16 43 / 50 and 69 / 66 us; at 80 rows 73 / 65, 89 / 105,
-// 53 / 50, 72 / 66. Beyond, the other kernel takes the sequences of more than FEW_ROWS and this one the rest, one after
+// 53 / 50, 72 / 66: one number for all, 3 us late for bf16 of 128 dimensions, 16 us early for f32 of 128. Beyond, the other kernel takes the sequences of more than FEW_ROWS and this one the rest, one after
 // the other: where all are long FEW_ROWS would only leave work for a second launch (a ragged batch of up to 96 rows:
 // 16 or 32: 64 us, 48: 86, 64: 103), and single and drafted tokens beside prompts stay here.
 constexpr int ALONE_ROWS = 72, FEW_ROWS = 32;

@@ -31,7 +31,9 @@
 //              added to f32 registers, because the tensor core truncates its running sum
 //              (2^-25 of it a step: 500 steps would cost 1e-5). 2048 x 4,133 positions, 128
 //              dimensions: every block 331 us (error 4.5e-7 of the result), every four 269 us
-//              (7.5e-7), every eight 258 us (1.2e-6; the plain f32 form: 1.4e-6).
+//              (7.5e-7), every eight 258 us (1.2e-6; the plain f32 form: 1.4e-6). With the V scales'
+//              exponents in the scores every four takes 275 us (8.0e-7); a row's 128 sums leave too few
+//              registers there (288 bytes of a thread's spill, 24 and less in the other forms).
 //   bf16 rows: weights in one term (11 bits, under the output's 8); O stays in tensor memory.
 //
 // Work is split as in the few-row kernel: one line of (sequence, kv head, row tile, key

@@ -124,8 +124,8 @@ class PagedBatch:
     the last of the kv_len[b] positions that it holds with them; page_table [n_seqs,
     pages_per_seq] names its pages (entries past kv_len, and with a window
     those of pages that no new token sees, are not read). The arrays are int32
-    CUDA tensors and are read by the kernels: their contents may change between calls
-    within what n_tokens (rows in all) and max_new (most of one sequence) say. The
+    CUDA tensors and are read by the kernels: their contents may change between calls, with
+    n_tokens rows in all and at most max_new of one sequence. The
     attention's workspace is kept here from the first call on, so calls with one batch must be
     ordered on the device (a graph captured before any other call gets workspaces of its own)."""
 
